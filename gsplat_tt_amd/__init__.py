@@ -3,7 +3,8 @@
 Drop-in for the reference's render path: `gsplat_tt_amd.render_clean` is the
 `render_clean` pybind module (render_view & co.), `gsplat_tt_amd._lib` binds
 the C ABI of include/gsplat_hip.h, `gsplat_tt_amd.scenes` builds the seeded
-benchmark workloads.
+benchmark workloads, `gsplat_tt_amd.field` holds the operators for learned
+features on splats (torch tensors on the GPU).
 """
 from __future__ import annotations
 
@@ -12,7 +13,7 @@ import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 
-__all__ = ["build", "render_clean_module", "Context"]
+__all__ = ["build", "render_clean_module", "Context", "FieldOps"]
 
 
 def build(arch: str = "gfx950", jobs: int = 8) -> None:
@@ -30,4 +31,7 @@ def __getattr__(name):
     if name == "Context":
         from ._lib import Context
         return Context
+    if name == "FieldOps":
+        from .field import FieldOps
+        return FieldOps
     raise AttributeError(name)

@@ -40,6 +40,9 @@ EXPORTED = (
     "gs_graph_counts",
     "gs_sort_tile_depth_dev", "gs_sort_tile_depth_ids_dev", "gs_last_ranges_ms",
     "gs_sort_tile_depth_noalloc",
+    "gs_stream", "gs_lookup_dev", "gs_lookup_grad_workspace", "gs_lookup_grad_dev",
+    "gs_group_norm_workspace", "gs_group_norm_dev", "gs_group_norm_grad_dev",
+    "gs_label_loss_workspace", "gs_label_loss_dev", "gs_label_loss_grad_dev",
 )
 TRAIN_PARAMS = ("means", "log_scales", "quats", "opacity_logits", "sh")
 
@@ -117,6 +120,40 @@ class GsTrainProj(ctypes.Structure):
                                                 "valid", "visible")]
 
 
+class GsGroupNorm(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int64), ("pixels", ctypes.c_int64),
+                ("channels", ctypes.c_int), ("groups", ctypes.c_int), ("act", ctypes.c_int),
+                ("dtype", ctypes.c_int), ("eps", ctypes.c_float), ("reserved", ctypes.c_int),
+                ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p)]
+
+
+class GsLabelLoss(ctypes.Structure):
+    _fields_ = [("feat", ctypes.c_void_p), ("table", ctypes.c_void_p),
+                ("labels", ctypes.c_void_p), ("n", ctypes.c_int64), ("rows", ctypes.c_int64),
+                ("feat_stride", ctypes.c_int64), ("table_stride", ctypes.c_int64),
+                ("dim", ctypes.c_int), ("dtype", ctypes.c_int), ("labels64", ctypes.c_int),
+                ("scale", ctypes.c_float)]
+
+
+def _field_argtypes(L):
+    """Argument types of the feature operators (they are called often: typed
+    arguments need no wrapping per call)."""
+    p, q, i, f = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
+    L.gs_stream.argtypes = [p, ctypes.POINTER(p)]
+    L.gs_lookup_dev.argtypes = [p, p, q, q, i, p, i, q, i, f, p, q, i, p, p]
+    L.gs_lookup_grad_workspace.argtypes = [q, q, i]
+    L.gs_lookup_grad_dev.argtypes = [p, p, q, i, p, i, q, i, f, i, p, q, q, i, p, q, p, p]
+    L.gs_group_norm_workspace.argtypes = [q, q, i]
+    norm, loss = ctypes.POINTER(GsGroupNorm), ctypes.POINTER(GsLabelLoss)
+    L.gs_group_norm_dev.argtypes = [p, norm, p, q, q, p, q, q, p, p, p, q, p]
+    L.gs_group_norm_grad_dev.argtypes = [p, norm, p, q, q, p, q, q, p, p, p, q, q, p, p, p, q, p]
+    L.gs_label_loss_workspace.argtypes = [q, q, i, i, i]
+    L.gs_label_loss_dev.argtypes = [p, loss, p, p, p, q, p, p]
+    L.gs_label_loss_grad_dev.argtypes = [p, loss, p, p, p, p, q, p, q, p, q, p, p]
+    for name in ("gs_lookup_grad_workspace", "gs_group_norm_workspace", "gs_label_loss_workspace"):
+        getattr(L, name).restype = q
+
+
 def make_train_cfg(near=0.2, lowpass=0.3, alpha_max=0.99, alpha_min=1.0 / 255.0, t_min=1e-4,
                    background=(0.0, 0.0, 0.0), loss_scale=1.0, lr=None, betas=(0.9, 0.999),
                    eps=1e-15, lambda_dssim=0.0) -> GsTrainCfg:
@@ -162,6 +199,7 @@ def load_library():
         L.gs_overflow_next_floor.argtypes = [ctypes.c_float, ctypes.c_uint32, ctypes.c_uint32]
         L.gs_last_ranges_ms.restype = ctypes.c_float
         L.gs_last_ranges_ms.argtypes = [ctypes.c_void_p]
+        _field_argtypes(L)
         for name in EXPORTED:
             getattr(L, name)  # every declared symbol must resolve
         _LIB = L
@@ -235,6 +273,7 @@ class Context:
         the blend's evaluation counters (gs_set_timing)."""
         self._L = load_library()
         self._c = ctypes.c_void_p()
+        self.device_index = int(device)
         _check(self._L.gs_create(int(device), ctypes.byref(self._c)))
         if timing:
             _check(self._L.gs_set_timing(self._c, int(timing)))

@@ -1,0 +1,90 @@
+// field_device.h - device helpers of the feature operators: element types, vector
+// loads and stores, checked ids, workgroup scans, workspace layout.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "field.h"
+
+namespace gs {
+
+using bf16 = __bf16;
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(bf16 v) { return (float)v; }
+// to bf16: round to nearest even, NaN kept
+template <typename T>
+__device__ __forceinline__ T from_float(float v) { return (T)v; }
+
+// VEC elements at an address aligned to VEC * sizeof(T) bytes.
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) VecOf {
+    T v[VEC];
+};
+template <int VEC, typename T>
+__device__ __forceinline__ void load_vec(const T* p, float* out) {
+    const VecOf<T, VEC> u = *reinterpret_cast<const VecOf<T, VEC>*>(p);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) out[j] = to_float(u.v[j]);
+}
+template <int VEC, typename T>
+__device__ __forceinline__ void store_vec(T* p, const float* in) {
+    VecOf<T, VEC> u;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) u.v[j] = from_float<T>(in[j]);
+    *reinterpret_cast<VecOf<T, VEC>*>(p) = u;
+}
+
+// Whether rows at `stride` elements apart can be read VEC elements at a time.
+template <typename T>
+inline bool aligned_rows(const void* p, int64_t stride, int vec) {
+    return reinterpret_cast<uintptr_t>(p) % (sizeof(T) * vec) == 0 && stride % vec == 0;
+}
+
+// Id i, or -1 where it is masked (below 0) or past the table; the latter is
+// reported in *flags.
+__device__ __forceinline__ int32_t load_id(const void* ids, int ids64, int64_t i, int64_t rows,
+                                           uint32_t* flags) {
+    const int64_t v = ids64 ? static_cast<const int64_t*>(ids)[i]
+                            : (int64_t) static_cast<const int32_t*>(ids)[i];
+    if (v >= rows) {
+        if (flags != nullptr) atomicOr(flags, kFlagIdRange);
+        return -1;
+    }
+    return v < 0 ? -1 : (int32_t)v;
+}
+
+// Exclusive prefix of one value per thread over the workgroup, and the total.
+template <int THREADS>
+__device__ __forceinline__ uint32_t block_excl_scan(uint32_t v, uint32_t* lds, uint32_t* total) {
+    const int t = threadIdx.x;
+    __syncthreads();
+    lds[t] = v;
+    __syncthreads();
+    for (int o = 1; o < THREADS; o <<= 1) {
+        const uint32_t u = t >= o ? lds[t - o] : 0u;
+        __syncthreads();
+        lds[t] += u;
+        __syncthreads();
+    }
+    *total = lds[THREADS - 1];
+    return lds[t] - v;
+}
+
+// Consecutive 256-byte aligned arrays of a workspace; a null base only counts.
+struct Carve {
+    uintptr_t base;
+    size_t at = 0;
+    explicit Carve(void* p) : base(reinterpret_cast<uintptr_t>(p)) {}
+    template <typename T>
+    T* take(size_t n) {
+        T* p = reinterpret_cast<T*>(base + at);
+        at += (n * sizeof(T) + 255) & ~size_t(255);
+        return p;
+    }
+    size_t bytes() const { return at; }
+};
+
+}  // namespace gs

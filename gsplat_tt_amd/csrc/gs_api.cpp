@@ -25,45 +25,17 @@
 #include <vector>
 
 #include "../../include/gsplat_hip.h"
+#include "field.h"
+#include "gs_error.h"
 #include "gs_internal.h"
 #include "host_threads.h"
 #include "out_ring.h"
 
 namespace {
 
-thread_local std::string g_err;
-
-struct GsError : std::runtime_error {
-    int code;
-    GsError(int c, const std::string& m) : std::runtime_error(m), code(c) {}
-};
-
-#define HIPCHK(x)                                                                        \
-    do {                                                                                 \
-        hipError_t e_ = (x);                                                             \
-        if (e_ != hipSuccess)                                                            \
-            throw GsError(GS_E_DEVICE, std::string(#x) + ": " + hipGetErrorString(e_)); \
-    } while (0)
-
-#define REQUIRE(cond, msg)                                  \
-    do {                                                    \
-        if (!(cond)) throw GsError(GS_E_INVALID, (msg));    \
-    } while (0)
-
-template <class F>
-int guard(F&& f) {
-    try {
-        f();
-        return GS_OK;
-    } catch (const GsError& e) {
-        g_err = e.what();
-        return e.code;
-    } catch (const std::exception& e) {
-        g_err = e.what();
-        return GS_E_DEVICE;
-    }
-}
-
+using gs::g_err;
+using gs::GsError;
+using gs::guard;
 
 struct DevBuf {
     void* p = nullptr;
@@ -2032,6 +2004,11 @@ struct gs_ctx {
 
 gs::CtxInfo gs::ctx_info(const gs_ctx* ctx) { return gs::CtxInfo{ctx->device, ctx->st}; }
 void gs::set_last_error(const char* msg) { g_err = msg ? msg : ""; }
+
+namespace gs {
+int ctx_device(const gs_ctx* ctx) { return ctx->device; }
+hipStream_t ctx_stream(const gs_ctx* ctx) { return ctx->st; }
+}  // namespace gs
 
 extern "C" {
 

@@ -412,6 +412,114 @@ int gs_train_step(gs_ctx* ctx, const gs_view* view, const gs_train_cfg* cfg,
 int gs_train_loss(gs_ctx* ctx, const float* image, const float* target, int height, int width,
                   float lambda_dssim, float loss_scale, float* dimage, double* loss3);
 
+/* ---- feature operators (learned features on splats) --------------------
+ * Device pointers, on the stream the caller names. They have no counterpart in
+ * the reference. Rules that hold for all of them:
+ *
+ * - `stream` is a hipStream_t (NULL: HIP's default stream); gs_stream gives the
+ *   context's own. Every call only enqueues kernels: it neither waits, nor
+ *   allocates, nor copies, nor keeps anything in the context, so calls may be
+ *   captured into a HIP graph and calls on several streams may overlap when
+ *   each has a workspace of its own.
+ * - dtype: GS_F32 or GS_BF16. Sums, statistics and exponentials are fp32; a bf16
+ *   result is rounded once, to nearest even.
+ * - strides are in elements, between rows (or images, pixels); the values of a
+ *   row are contiguous. Inputs may overlap each other and themselves (a stride
+ *   of 0 repeats a row); an output overlaps nothing, except that gs_group_norm_dev's y may be x and
+ *   gs_group_norm_grad_dev's dx may be x or dy, with the same strides.
+ * - ids and labels: int32 (ids64 0) or int64 (1). One below 0 is masked. One at
+ *   or past `rows` is treated as masked too, and bit GS_FLAG_ID_RANGE is set in
+ *   *flags (a device word that the caller clears and reads; NULL: not wanted).
+ *   Values in masked rows are not used, whatever they hold.
+ * - `workspace`: device memory of at least the bytes the matching
+ *   gs_*_workspace says, 256-byte aligned; its contents are not kept between
+ *   calls. A size past the limits gives -1 there.
+ * - results are the same from run to run: no sum's order depends on timing.
+ * - bad arguments give GS_E_INVALID, sizes past the limits GS_E_CAPACITY, and
+ *   nothing is enqueued then. Sizes of 0 are valid. */
+#define GS_F32 0
+#define GS_BF16 1
+#define GS_FLAG_ID_RANGE 1u
+#define GS_ACT_NONE 0
+#define GS_ACT_RELU 1
+#define GS_ACT_SILU 2
+#define GS_ACT_GELU 3  /* z Phi(z), with the error function */
+
+/* The context's own stream (a hipStream_t). */
+int gs_stream(gs_ctx* ctx, void** stream);
+
+/* out[i] = scale * table[ids[i]] for n ids, dim values a row (at most 65536);
+ * masked rows are zeros. table (rows, dim), out (n, dim), each with a type of
+ * its own. */
+int gs_lookup_dev(gs_ctx* ctx, const void* table, int64_t rows, int64_t table_stride,
+                  int table_dtype, const void* ids, int ids64, int64_t n, int dim, float scale,
+                  void* out, int64_t out_stride, int out_dtype, uint32_t* flags, void* stream);
+/* Its gradient: dtable[v] = scale * sum of dout[i] over ids[i] = v, every row
+ * written (zeros where no id names it); with accumulate the sums are added to
+ * what dtable holds. The ids are sorted (stable), and each row's sum runs in
+ * that order. n below 2^31 - 1, rows below 2^30. */
+int64_t gs_lookup_grad_workspace(int64_t n, int64_t rows, int dim);
+int gs_lookup_grad_dev(gs_ctx* ctx, const void* dout, int64_t dout_stride, int dout_dtype,
+                       const void* ids, int ids64, int64_t n, int dim, float scale,
+                       int accumulate, void* dtable, int64_t rows, int64_t dtable_stride,
+                       int dtable_dtype, void* workspace, int64_t workspace_bytes,
+                       uint32_t* flags, void* stream);
+
+/* Group norm with an activation over channels-last images: x (batch, pixels,
+ * channels) with strides between images and pixels, `groups` equal groups of
+ * consecutive channels, statistics over a group's channels and the image's
+ * pixels (variance by count). y = act((x - mean) rstd weight + bias), rstd =
+ * 1 / sqrt(var + eps); weight and bias (channels) fp32 or NULL (1 and 0). mean
+ * and rstd (batch, groups) fp32 are written for the gradient. */
+typedef struct gs_group_norm {
+    int64_t batch, pixels;
+    int channels, groups;
+    int act;   /* GS_ACT_* */
+    int dtype; /* of x, y, dy, dx */
+    float eps; /* > 0 */
+    int reserved;
+    const float* weight;
+    const float* bias;
+} gs_group_norm;
+int64_t gs_group_norm_workspace(int64_t batch, int64_t pixels, int channels);
+int gs_group_norm_dev(gs_ctx* ctx, const gs_group_norm* norm, const void* x, int64_t x_batch,
+                      int64_t x_pixel, void* y, int64_t y_batch, int64_t y_pixel, float* mean,
+                      float* rstd, void* workspace, int64_t workspace_bytes, void* stream);
+/* Its gradients from dy, x and the forward's mean and rstd: dx, and dweight and
+ * dbias (channels) fp32 summed over images and pixels (each may be NULL). */
+int gs_group_norm_grad_dev(gs_ctx* ctx, const gs_group_norm* norm, const void* dy,
+                           int64_t dy_batch, int64_t dy_pixel, const void* x, int64_t x_batch,
+                           int64_t x_pixel, const float* mean, const float* rstd, void* dx,
+                           int64_t dx_batch, int64_t dx_pixel, float* dweight, float* dbias,
+                           void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Softmax cross entropy of n features against a table of labels: scores
+ * l_iv = scale <feat_i, table_v>, lse_i = log sum_v exp(l_iv), loss_i = lse_i -
+ * l_i,label(i); 0 and 0 for a masked label. feat (n, dim) and table (rows, dim)
+ * of one dtype, dim at most 65536, rows 1 .. 2^22. The scores are made in pieces
+ * and never kept. loss and lse (n) fp32, each may be NULL. */
+typedef struct gs_label_loss {
+    const void* feat;
+    const void* table;
+    const void* labels;
+    int64_t n, rows;
+    int64_t feat_stride, table_stride;
+    int dim, dtype;
+    int labels64;
+    float scale;
+} gs_label_loss;
+int64_t gs_label_loss_workspace(int64_t n, int64_t rows, int dim, int dtype, int grad);
+int gs_label_loss_dev(gs_ctx* ctx, const gs_label_loss* in, float* loss, float* lse,
+                      void* workspace, int64_t workspace_bytes, uint32_t* flags, void* stream);
+/* The losses and the gradients of sum_i row_weight[i] loss_i (row_weight (n) fp32,
+ * NULL: 1): dfeat (n, dim) and dtable (rows, dim) of the inputs' dtype; masked
+ * rows of dfeat are zeros. For bf16 inputs the scores' gradients are rounded to
+ * bf16 before they are multiplied, as operands of the matrix cores. */
+int gs_label_loss_grad_dev(gs_ctx* ctx, const gs_label_loss* in, const float* row_weight,
+                           float* loss, float* lse, void* dfeat, int64_t dfeat_stride,
+                           void* dtable, int64_t dtable_stride, void* workspace,
+                           int64_t workspace_bytes, uint32_t* flags, void* stream);
+
 /* ---- device memory helpers (for callers without a GPU framework) ------ */
 int gs_dev_alloc(gs_ctx* ctx, int64_t bytes, void** ptr);
 int gs_dev_free(gs_ctx* ctx, void* ptr);
