@@ -26,6 +26,7 @@ namespace {
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(4))) uint32_t quad;  // 16 bytes: one lane's operand
 
 constexpr int kThreads = 256;
 constexpr int kTile = 128;  // rows and columns of a workgroup's tile
@@ -33,24 +34,48 @@ constexpr int kStep = 64;   // summed index per step
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // Part p of a value: the leading 8 significant bits, the next 8, the rest.
-// Cutting off (not rounding) leaves exact remainders; a value that is not
-// finite stays whole in part 0.
+// Cutting off (not rounding) leaves exact remainders.
 __device__ __forceinline__ float cut_bf16(float v) {
     return __uint_as_float(__float_as_uint(v) & 0xFFFF0000u);
 }
+// An input is made canonical first: one that is not finite has parts that are not.
+template <int NP>
+__device__ __forceinline__ float plain_input(float v) {
+    if (NP > 1 && v != v) return __uint_as_float(0x7FC00000u);
+    return v;
+}
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+// Parts of two values, each pair in one word.
+template <int NP>
+__device__ __forceinline__ void split2(float v0, float v1, uint32_t* out) {
+    if (NP == 1) {
+        out[0] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{v0, v1}, bf16x2));
+    } else {
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            // the high halves of both
+            out[p] = __builtin_amdgcn_perm(__float_as_uint(v1), __float_as_uint(v0), 0x07060302u);
+            v0 -= cut_bf16(v0);
+            v1 -= cut_bf16(v1);
+        }
+    }
+}
+// Parts of eight values, as operands.
+template <int NP>
+__device__ __forceinline__ void split8(const float* v, quad* out) {
+    uint32_t w[4][NP];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) split2<NP>(v[2 * k], v[2 * k + 1], w[k]);
+#pragma unroll
+    for (int p = 0; p < NP; ++p) out[p] = quad{w[0][p], w[1][p], w[2][p], w[3][p]};
+}
 template <int NP>
 __device__ __forceinline__ void split(float v, bf16* out) {
-    if (NP == 1) {
-        out[0] = (bf16)v;
-    } else {
-        const float a = cut_bf16(v);
-        float r = v - a;
-        if (!(fabsf(v) <= 3.402823466e38f)) r = 0.0f;
-        const float b = cut_bf16(r), c = cut_bf16(r - b);
-        out[0] = (v != v) ? (bf16)v : (bf16)a;
-        out[1] = (bf16)b;
-        out[2] = (bf16)c;
-    }
+    uint32_t w[NP];
+    split2<NP>(v, 0.0f, w);
+#pragma unroll
+    for (int p = 0; p < NP; ++p) out[p] = __builtin_bit_cast(bf16x2, w[p])[0];
 }
 // The products of parts: (0,0) for one part; for three, all with p + q <= 2.
 template <int NP>
@@ -93,7 +118,7 @@ __global__ __launch_bounds__(kThreads) void k_parts(const T* src, int64_t rows, 
         const int c = (int)(e - r * kd);
         float v = 0.0f;
         if (r < rows && c < dim && (label == nullptr || label[r] >= 0))
-            v = to_float(src[r * stride + c]);
+            v = plain_input<NP>(to_float(src[r * stride + c]));
         bf16 part[NP];
         split<NP>(v, part);
 #pragma unroll
@@ -114,7 +139,7 @@ __global__ __launch_bounds__(kThreads) void k_parts_t(const T* src, int64_t rows
         const int c = c0 + tx;
         float v = 0.0f;
         if (r < rows && c < dim && (label == nullptr || label[r] >= 0))
-            v = to_float(src[r * stride + c]);
+            v = plain_input<NP>(to_float(src[r * stride + c]));
         tile[k][tx] = v;
     }
     __syncthreads();
@@ -139,13 +164,13 @@ struct Mat {
 // touch all banks once.
 template <int NP>
 __device__ __forceinline__ void tile_product(const Mat& A, const Mat& B, int64_t m0, int64_t n0,
-                                             int64_t k0, int64_t k1, uint4 (*lds)[2][kTile * 8],
+                                             int64_t k0, int64_t k1, quad (*lds)[2][kTile * 8],
                                              f32x4 acc[4][4]) {
     const int t = threadIdx.x, lane = t & 63, w = t >> 6;
     const int wm = (w >> 1) * 64, wn = (w & 1) * 64;
     const int steps_k = (int)((k1 - k0) / kStep);
     const int steps = steps_k * Products<NP>::kCount;
-    uint4 ra[4], rb[4];
+    quad ra[4], rb[4];
     auto fetch = [&](int s) {
         const int q = s / steps_k;
         const int64_t k = k0 + (int64_t)(s - q * steps_k) * kStep;
@@ -154,8 +179,8 @@ __device__ __forceinline__ void tile_product(const Mat& A, const Mat& B, int64_t
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int e = t + j * kThreads, r = e >> 3, c = e & 7;
-            ra[j] = *reinterpret_cast<const uint4*>(pa + r * A.ld + c * 8);
-            rb[j] = *reinterpret_cast<const uint4*>(pb + r * B.ld + c * 8);
+            ra[j] = *reinterpret_cast<const quad*>(pa + r * A.ld + c * 8);
+            rb[j] = *reinterpret_cast<const quad*>(pb + r * B.ld + c * 8);
         }
     };
     auto keep = [&](int buf) {
@@ -175,7 +200,7 @@ __device__ __forceinline__ void tile_product(const Mat& A, const Mat& B, int64_t
         if (s + 1 < steps) fetch(s + 1);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            uint4 fa[4], fb[4];
+            quad fa[4], fb[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int c = h * 4 + (lane >> 4);
@@ -196,7 +221,7 @@ __device__ __forceinline__ void tile_product(const Mat& A, const Mat& B, int64_t
     }
 }
 
-#define GS_TILE_LDS __shared__ uint4 lds[2][2][kTile * 8]
+#define GS_TILE_LDS __shared__ quad lds[2][2][kTile * 8]
 #define GS_TILE_ACC                    \
     f32x4 acc[4][4];                   \
     for (int i = 0; i < 4; ++i)        \
@@ -353,6 +378,391 @@ __global__ __launch_bounds__(kThreads) void k_loss_fold(const float* slices, int
     }
 }
 
+// ---------------------------------------------------------------- streaming
+// For rows short enough that a wave keeps its own in registers: a workgroup
+// holds 4 x 64 "queries", the other side's rows ("keys") stream through LDS, 32
+// a tile, and neither scores nor G ever leave the registers.
+//
+// The scores of a tile are made transposed, keys by queries: a lane then holds
+// 16 keys' scores of one query, the sums over keys need no other lane until the
+// end, and the same registers, as they are, are the left operand of the second
+// product (queries by keys times keys by dim). The keys' order within that
+// product is the lane's own: slot (h, e) of a half tile f is key
+// 16 f + 4 h + e (e < 4) or 16 f + 4 h + 4 + e (e >= 4), h = lane / 32.
+//
+// Keys are laid out once as whole matrix-instruction operands (1 KB each, 16
+// bytes a lane), so that LDS is filled and read in order: per tile the operands
+// of the scores, [part][dim / 16], then those of the second product,
+// [part][dim / 32][f].
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+
+enum { kScores = 0, kGradFeat = 1, kGradTable = 2 };
+
+struct StreamArgs {
+    const void* q;  // queries (nq, dim)
+    int64_t nq, q_stride;
+    const quad* keys;  // tiles of 32 keys
+    int64_t nk;         // keys that are there
+    int tiles, share;   // tiles in all, and of a share
+    int tile_stride;    // quad from tile to tile
+    int dim;
+    float scale2;  // scale * log2(e)
+    // of the samples, whichever side they are: label, weight * scale, lse in log2 units
+    const int32_t* label;
+    const float *weight, *lse2;
+    // kScores
+    const void* labels;
+    int labels64;
+    float2* part;
+    float *label_score, *loss, *lse, *lse2_out;
+    uint32_t* flags;
+    int64_t table_rows;
+    // gradients: into out where there is one share, else into (share, padded, KD) sums
+    void* out;
+    int64_t out_stride;
+    float* sums;
+    int64_t padded;
+};
+
+// exp2 of a gradient's exponent. The bare instruction gives 0 below 2^-126, which
+// fp32 gradients, times weight * scale, would show; for bf16 ones it is left so.
+template <int NP>
+__device__ __forceinline__ float grad_exp2(float x) {
+    return NP == 1 ? __builtin_amdgcn_exp2f(x) : exp2f(x);
+}
+
+// Key of register r of a lane in half h.
+__device__ __forceinline__ constexpr int key_of(int r) { return (r & 3) + 8 * (r >> 2); }
+
+// A row's 8 values from column c, cut into parts; zeros past the row.
+template <typename T, int NP>
+__device__ __forceinline__ void load_parts(const T* row, int dim, int c, bool on, quad* out) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        v[e] = on && c + e < dim ? plain_input<NP>(to_float(row[c + e])) : 0.0f;
+    split8<NP>(v, out);
+}
+
+// (rows, dim) as tiles of operands, one workgroup a tile; of samples (label) the
+// masked ones are zeros, and label and weight are written for the gradients.
+template <typename T, int NP, int KD, bool SECOND>
+__global__ __launch_bounds__(kThreads) void k_operands(const T* src, int64_t rows, int64_t stride,
+                                                       int dim, LossArgs a, int32_t* label,
+                                                       float* weight, float* lse2, quad* out) {
+    __shared__ float tile[32][KD + 1];
+    __shared__ int32_t lab[32];
+    const int64_t r0 = (int64_t)blockIdx.x * 32;
+    if (threadIdx.x < 32) {
+        int32_t l = 0;
+        if (label != nullptr) {
+            const int64_t i = r0 + threadIdx.x;
+            l = i < rows ? load_id(a.labels, a.labels64, i, a.rows, nullptr) : -1;
+            label[i] = l;
+            weight[i] = l < 0 ? 0.0f : a.scale * (a.row_weight != nullptr ? a.row_weight[i] : 1.0f);
+            if (i >= rows) lse2[i] = 0.0f;  // the others' come from the scores
+        }
+        lab[threadIdx.x] = l;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < 32 * KD; e += kThreads) {
+        const int r = e / KD, c = e % KD;
+        float v = 0.0f;
+        if (r0 + r < rows && c < dim && lab[r] >= 0) v = plain_input<NP>(to_float(src[(r0 + r) * stride + c]));
+        tile[r][c] = v;
+    }
+    __syncthreads();
+    constexpr int kFirst = KD / 16 * 64, kSecond = SECOND ? KD / 32 * 2 * 64 : 0;
+    quad* to = out + (size_t)blockIdx.x * NP * (kFirst + kSecond);
+    for (int e = threadIdx.x; e < kFirst + kSecond; e += kThreads) {
+        const int lane = e & 63, h = lane >> 5;
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (e < kFirst) {
+                v[k] = tile[lane & 31][(e >> 6) * 16 + 8 * h + k];
+            } else {
+                const int b = (e - kFirst) >> 6;  // dim / 32, f
+                v[k] = tile[16 * (b & 1) + 4 * h + k + (k < 4 ? 0 : 4)][(b >> 1) * 32 + (lane & 31)];
+            }
+        }
+        quad piece[NP];
+        split8<NP>(v, piece);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const size_t at = e < kFirst ? p * kFirst + e : NP * kFirst + p * kSecond + (e - kFirst);
+            to[at] = piece[p];
+        }
+    }
+}
+
+template <typename T, int NP, int KD, int ROLE>
+struct StreamShape {
+    static constexpr int kPieces = NP * KD / 16 * 64 * (ROLE == kScores ? 1 : 2);  // quad a tile
+    // tiles per step: about 16 KB
+    static constexpr int kTiles = kPieces * 16 >= 16384 ? 1 : (kPieces * 16 >= 8192 ? 2 : 4);
+    static constexpr int kStage = kPieces * kTiles;
+    static constexpr size_t kLds = 2 * kStage * 16 + (ROLE == kGradTable ? 2 * kTiles * 32 * 12 : 0);
+};
+
+template <typename T, int NP, int KD, int ROLE>
+__global__ __launch_bounds__(kThreads, (NP * KD >= (ROLE == kScores ? 256 : 128) ? 1 : 2)) void k_stream(StreamArgs a) {
+    using Shape = StreamShape<T, NP, KD, ROLE>;
+    constexpr int KJ = KD / 16, DB = KD / 32, TS = Shape::kTiles, STAGE = Shape::kStage;
+    constexpr int PER = STAGE / kThreads;
+    static_assert(STAGE % kThreads == 0, "a stage is whole rounds of loads");
+    extern __shared__ quad lds[];
+    float* info = reinterpret_cast<float*>(lds + 2 * STAGE);  // kGradTable: lse2, weight, label
+    const int t = threadIdx.x, lane = t & 63, h = lane >> 5, col = lane & 31;
+    const int64_t q0 = ((int64_t)blockIdx.x * 4 + (t >> 6)) * 64;
+
+    // the wave's own queries, as right operands of the scores
+    quad q[2][KJ][NP];
+    int32_t y[2];
+    float lse2[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        const int64_t i = q0 + b * 32 + col;
+        bool on = i < a.nq;
+        y[b] = -1;
+        lse2[b] = 0.0f;
+        if (ROLE == kScores) {
+            if (on) y[b] = load_id(a.labels, a.labels64, i, a.table_rows,
+                                   blockIdx.y == 0 && h == 0 ? a.flags : nullptr);
+            on = y[b] >= 0;
+        }
+        if (ROLE == kGradFeat) {
+            if (on) {
+                y[b] = a.label[i];
+                lse2[b] = a.lse2[i];
+            }
+            on = y[b] >= 0;
+        }
+        if (ROLE == kGradTable) y[b] = (int32_t)min(i, (int64_t)0x7FFFFFFF);
+        const T* row = static_cast<const T*>(a.q) + i * a.q_stride;
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) load_parts<T, NP>(row, a.dim, 16 * j + 8 * h, on, q[b][j]);
+    }
+
+    f32x16 acc[2][ROLE == kScores ? 1 : DB];
+    float m[2], sum[2], own[2];
+    if (ROLE == kScores) {
+        m[0] = m[1] = -1e30f;
+        sum[0] = sum[1] = own[0] = own[1] = 0.0f;
+    } else {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[b][d][r] = 0.0f;
+    }
+
+    const int t0 = blockIdx.y * a.share, t1 = min(a.tiles, t0 + a.share);
+    const int steps = (t1 - t0 + TS - 1) / TS;
+    quad pre[PER];
+    // a step past the last tile reads on into the padding behind the tiles
+    auto fetch = [&](int s) {
+        const quad* from = a.keys + ((size_t)t0 + (size_t)s * TS) * a.tile_stride;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int e = k * kThreads + t;
+            pre[k] = from[(size_t)(e / Shape::kPieces) * a.tile_stride + e % Shape::kPieces];
+        }
+    };
+    auto keep = [&](int s) {
+        quad* to = lds + (s & 1) * STAGE + t;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) to[k * kThreads] = pre[k];
+        if (ROLE == kGradTable) {
+            float* f = info + (s & 1) * TS * 96;
+            for (int k = t; k < TS * 32; k += kThreads) {
+                const int64_t i = ((int64_t)t0 + (int64_t)s * TS) * 32 + k;
+                f[k] = a.lse2[i];
+                f[TS * 32 + k] = a.weight[i];
+                f[2 * TS * 32 + k] = __int_as_float(a.label[i]);
+            }
+        }
+    };
+    fetch(0);
+    keep(0);
+    __syncthreads();
+    for (int s = 0; s < steps; ++s) {
+        if (s + 1 < steps) fetch(s + 1);
+        const quad* stage = lds + (s & 1) * STAGE;
+#pragma unroll 1
+        for (int u = 0; u < TS; ++u) {
+            const int tile = t0 + s * TS + u;
+            if (tile >= t1) break;
+            const quad* kf = stage + u * Shape::kPieces + lane;
+            f32x16 sc[2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sc[b][r] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < KJ; ++j) {
+                bf16x8 k[NP];
+#pragma unroll
+                for (int p = 0; p < NP; ++p)
+                    k[p] = __builtin_bit_cast(bf16x8, kf[(p * KJ + j) * 64]);
+#pragma unroll
+                for (int i = 0; i < Products<NP>::kCount; ++i)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+                        sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                            k[Products<NP>::a(i)],
+                            __builtin_bit_cast(bf16x8, q[b][j][Products<NP>::b(i)]), sc[b], 0, 0, 0);
+            }
+            const int64_t k0 = (int64_t)tile * 32;
+            if (ROLE == kScores) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sc[b][r] *= a.scale2;
+                    if (k0 + 32 > a.nk) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            if (k0 + key_of(r) + 4 * h >= a.nk) sc[b][r] = -INFINITY;
+                    }
+                    const int64_t yl = y[b] - k0;
+                    if (__any(yl >= 0 && yl < 32)) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            if (yl == key_of(r) + 4 * h) own[b] = sc[b][r];
+                    }
+                    float mt = m[b];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) mt = fmaxf(mt, sc[b][r]);
+                    // an infinite largest counts as 0: the sum is infinite too then
+                    const float base = mt < INFINITY ? mt : 0.0f;
+                    const float was = m[b] < INFINITY ? m[b] : 0.0f;
+                    float add = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        add += __builtin_amdgcn_exp2f(sc[b][r] - base);
+                    sum[b] = sum[b] * __builtin_amdgcn_exp2f(was - base) + add;
+                    m[b] = mt;
+                }
+                continue;
+            }
+            quad g[2][2][NP];
+            const float* f = info + (s & 1) * TS * 96 + u * 32;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                float v[16];
+                if (ROLE == kGradFeat) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        v[r] = grad_exp2<NP>(fmaf(sc[b][r], a.scale2, -lse2[b]));
+                    const int64_t yl = y[b] - k0;
+                    if (__any(yl >= 0 && yl < 32)) {
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            if (yl == key_of(r) + 4 * h) v[r] -= 1.0f;
+                    }
+                } else {
+                    const int yk = __float_as_int(f[2 * TS * 32 + col]);
+                    const bool any = __any(yk >= q0 + b * 32 && yk < q0 + b * 32 + 32);
+#pragma unroll
+                    for (int g4 = 0; g4 < 4; ++g4) {
+                        const float4 l4 = *reinterpret_cast<const float4*>(f + g4 * 8 + 4 * h);
+                        const float4 w4 =
+                            *reinterpret_cast<const float4*>(f + TS * 32 + g4 * 8 + 4 * h);
+                        const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+                        const float w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            v[g4 * 4 + e] =
+                                grad_exp2<NP>(fmaf(sc[b][g4 * 4 + e], a.scale2, -l[e]));
+                        if (any) {
+                            const float4 y4 = *reinterpret_cast<const float4*>(
+                                f + 2 * TS * 32 + g4 * 8 + 4 * h);
+                            const float yy[4] = {y4.x, y4.y, y4.z, y4.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (__float_as_int(yy[e]) == y[b]) v[g4 * 4 + e] -= 1.0f;
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[g4 * 4 + e] *= w[e];
+                    }
+                }
+                split8<NP>(v, g[b][0]);
+                split8<NP>(v + 8, g[b][1]);
+            }
+            const quad* kt = kf + NP * KJ * 64;
+#pragma unroll
+            for (int d = 0; d < (ROLE == kScores ? 1 : DB); ++d)
+#pragma unroll
+                for (int f2 = 0; f2 < 2; ++f2) {
+                    bf16x8 k[NP];
+#pragma unroll
+                    for (int p = 0; p < NP; ++p)
+                        k[p] = __builtin_bit_cast(bf16x8, kt[(p * DB * 2 + d * 2 + f2) * 64]);
+#pragma unroll
+                    for (int i = 0; i < Products<NP>::kCount; ++i)
+#pragma unroll
+                        for (int b = 0; b < 2; ++b)
+                            acc[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                                __builtin_bit_cast(bf16x8, g[b][f2][Products<NP>::a(i)]),
+                                k[Products<NP>::b(i)], acc[b][d], 0, 0, 0);
+                }
+        }
+        if (s + 1 < steps) keep(s + 1);
+        __syncthreads();
+    }
+
+    if (ROLE == kScores) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int64_t i = q0 + b * 32 + col;
+            const float m2 = __shfl_xor(m[b], 32, 64), s2 = __shfl_xor(sum[b], 32, 64);
+            const float mm = fmaxf(m[b], m2), base = mm < INFINITY ? mm : 0.0f;
+            const float total =
+                sum[b] * __builtin_amdgcn_exp2f((m[b] < INFINITY ? m[b] : 0.0f) - base) +
+                s2 * __builtin_amdgcn_exp2f((m2 < INFINITY ? m2 : 0.0f) - base);
+            // the half that holds the label's score gives it to the other
+            const bool here = y[b] >= 0 && ((y[b] >> 2) & 1) == h;
+            const float o2 = __shfl_xor(own[b], 32, 64);
+            const float mine = here ? own[b] : o2;
+            if (h != 0 || i >= a.nq) continue;
+            if (gridDim.y == 1) {
+                const float l = base + log2f(total);
+                const bool on = y[b] >= 0;
+                if (a.loss != nullptr) a.loss[i] = on ? (l - mine) * kLn2 : 0.0f;
+                if (a.lse != nullptr) a.lse[i] = on ? l * kLn2 : 0.0f;
+                if (a.lse2_out != nullptr) a.lse2_out[i] = on ? l : 0.0f;
+            } else {
+                a.part[blockIdx.y * a.padded + i] = make_float2(mm, total);
+                if (y[b] >= (int64_t)t0 * 32 && y[b] < (int64_t)t1 * 32) a.label_score[i] = mine;
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int64_t i = q0 + b * 32 + key_of(r) + 4 * h;
+            if (i >= a.nq) continue;
+            float w = 1.0f;
+            bool on = true;
+            if (ROLE == kGradFeat) {
+                on = a.label[i] >= 0;
+                w = a.weight[i];
+            }
+#pragma unroll
+            for (int d = 0; d < (ROLE == kScores ? 1 : DB); ++d) {
+                const int c = d * 32 + col;
+                const float v = on ? acc[b][d][r] * w : 0.0f;
+                if (gridDim.y > 1)
+                    a.sums[((size_t)blockIdx.y * a.padded + i) * KD + c] = v;
+                else if (c < a.dim)
+                    static_cast<T*>(a.out)[i * a.out_stride + c] = from_float<T>(v);
+            }
+        }
+}
+
 // ---------------------------------------------------------------- pieces
 int64_t pad_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
@@ -413,6 +823,173 @@ unsigned blocks_for(int64_t items) {
     return (unsigned)(b < 65536 ? b : 65536);
 }
 
+// Joins the shares' partials of a row's scores.
+__global__ __launch_bounds__(kThreads) void k_stream_join(StreamArgs a, int shares) {
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (i >= a.nq) return;
+    const bool on = load_id(a.labels, a.labels64, i, a.table_rows, nullptr) >= 0;
+    float m = -INFINITY;
+    for (int k = 0; k < shares; ++k) m = fmaxf(m, a.part[k * a.padded + i].x);
+    const float base = m < INFINITY ? m : 0.0f;
+    float sum = 0.0f;
+    for (int k = 0; k < shares; ++k) {
+        const float2 p = a.part[k * a.padded + i];
+        sum += p.y * __builtin_amdgcn_exp2f((p.x < INFINITY ? p.x : 0.0f) - base);
+    }
+    const float l = base + log2f(sum);
+    if (a.loss != nullptr) a.loss[i] = on ? (l - a.label_score[i]) * kLn2 : 0.0f;
+    if (a.lse != nullptr) a.lse[i] = on ? l * kLn2 : 0.0f;
+    if (a.lse2_out != nullptr) a.lse2_out[i] = on ? l : 0.0f;
+}
+
+// Shares of the streamed side: enough workgroups for the chip (two a compute
+// unit), at least `least` tiles each, at most `most` of them.
+struct Shares {
+    int count, tiles;
+    Shares(int64_t queries, int64_t tiles_all, int least, int64_t most) {
+        const int64_t groups = (queries + 255) / 256;
+        int64_t want = groups >= 512 ? 1 : (512 + groups - 1) / std::max<int64_t>(groups, 1);
+        want = std::min(want, std::max<int64_t>(1, tiles_all / least));
+        want = std::max<int64_t>(1, std::min(want, most));
+        tiles = (int)((tiles_all + want - 1) / want);
+        count = (int)((tiles_all + tiles - 1) / tiles);
+    }
+};
+
+// Workspace of the streaming kernels.
+struct StreamPlan {
+    int64_t tf, tt;  // tiles of the samples and of the table
+    Shares scores, by_feat, by_table;
+    quad *F, *T;
+    int32_t* label;
+    float *weight, *lse2, *score, *sums;
+    float2* part;
+    size_t bytes;
+    // partial sums of the gradients: at most 64 MB a side
+    static int64_t most(int64_t rows, int kd) {
+        return std::max<int64_t>(1, ((int64_t)1 << 24) / std::max<int64_t>(1, rows * kd));
+    }
+    StreamPlan(void* base, int64_t n, int64_t rows, int np, int kd, bool grad)
+        : tf((n + 31) / 32), tt((rows + 31) / 32), scores(n, tt, 4, 512),
+          by_feat(n, tt, 8, most(n, kd)), by_table(rows, tf, 8, most(rows, kd)) {
+        Carve c(base);
+        const size_t first = (size_t)np * kd / 16 * 64, tile = grad ? 2 * first : first;
+        T = c.take<quad>((tt + 4) * tile);
+        part = c.take<float2>(scores.count > 1 ? (size_t)scores.count * n : 0);
+        score = c.take<float>(scores.count > 1 ? (size_t)n : 0);
+        F = nullptr;
+        label = nullptr;
+        weight = lse2 = sums = nullptr;
+        if (grad) {
+            F = c.take<quad>((tf + 4) * tile);
+            label = c.take<int32_t>((tf + 4) * 32);
+            weight = c.take<float>((tf + 4) * 32);
+            lse2 = c.take<float>((tf + 4) * 32);
+            const size_t sf = by_feat.count > 1 ? (size_t)by_feat.count * n * kd : 0;
+            const size_t sr = by_table.count > 1 ? (size_t)by_table.count * rows * kd : 0;
+            sums = c.take<float>(std::max(sf, sr));
+        }
+        bytes = c.bytes();
+    }
+};
+
+template <typename T, int NP, int KD, int ROLE>
+hipError_t launch_stream(const StreamArgs& a, const Shares& sh, hipStream_t st) {
+    constexpr size_t lds = StreamShape<T, NP, KD, ROLE>::kLds;
+    if (lds > 65536) {  // above the default limit of a launch
+        const hipError_t e =
+            hipFuncSetAttribute(reinterpret_cast<const void*>(&k_stream<T, NP, KD, ROLE>),
+                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+    }
+    k_stream<T, NP, KD, ROLE>
+        <<<dim3((unsigned)((a.nq + 255) / 256), (unsigned)sh.count), kThreads, lds, st>>>(a);
+    return hipGetLastError();
+}
+
+template <typename T, int NP, int KD>
+hipError_t stream_run(const LossArgs& a, bool grad, hipStream_t st) {
+    const StreamPlan w(a.ws, a.n, a.rows, NP, KD, grad);
+    const T* feat = static_cast<const T*>(a.feat);
+    const T* table = static_cast<const T*>(a.table);
+    if (grad)
+        k_operands<T, NP, KD, true><<<(unsigned)w.tt, kThreads, 0, st>>>(
+            table, a.rows, a.table_stride, a.dim, a, nullptr, nullptr, nullptr, w.T);
+    else
+        k_operands<T, NP, KD, false><<<(unsigned)w.tt, kThreads, 0, st>>>(
+            table, a.rows, a.table_stride, a.dim, a, nullptr, nullptr, nullptr, w.T);
+    StreamArgs s{};
+    s.q = feat;
+    s.nq = a.n;
+    s.q_stride = a.feat_stride;
+    s.keys = w.T;
+    s.nk = a.rows;
+    s.tiles = (int)w.tt;
+    s.dim = a.dim;
+    s.scale2 = a.scale * kLog2e;
+    s.labels = a.labels;
+    s.labels64 = a.labels64;
+    s.flags = a.flags;
+    s.table_rows = a.rows;
+    s.label = w.label;
+    s.weight = w.weight;
+    s.lse2 = w.lse2;
+    s.share = w.scores.tiles;
+    s.part = w.part;
+    s.label_score = w.score;
+    s.loss = a.loss;
+    s.lse = a.lse;
+    s.lse2_out = w.lse2;
+    s.padded = a.n;
+    hipError_t e;
+    // the gradients' tiles hold both products' operands, the scores take the first
+    constexpr int kFirst = NP * KD / 16 * 64;
+    s.tile_stride = grad ? 2 * kFirst : kFirst;
+    e = launch_stream<T, NP, KD, kScores>(s, w.scores, st);
+    if (e != hipSuccess) return e;
+    if (w.scores.count > 1)
+        k_stream_join<<<(unsigned)((a.n + kThreads - 1) / kThreads), kThreads, 0, st>>>(
+            s, w.scores.count);
+    if (!grad) return hipGetLastError();
+    k_operands<T, NP, KD, true><<<(unsigned)w.tf, kThreads, 0, st>>>(
+        feat, a.n, a.feat_stride, a.dim, a, w.label, w.weight, w.lse2, w.F);
+    s.share = w.by_feat.tiles;
+    s.out = a.dfeat;
+    s.out_stride = a.dfeat_stride;
+    s.sums = w.sums;
+    e = launch_stream<T, NP, KD, kGradFeat>(s, w.by_feat, st);
+    if (e != hipSuccess) return e;
+    if (w.by_feat.count > 1)
+        k_loss_fold<T><<<blocks_for(a.n * KD), kThreads, 0, st>>>(
+            w.sums, w.by_feat.count, a.n, KD, nullptr, 1, 1, static_cast<T*>(a.dfeat), a.n,
+            a.dfeat_stride, a.dim, w.label);
+    s.q = table;
+    s.nq = a.rows;
+    s.q_stride = a.table_stride;
+    s.keys = w.F;
+    s.nk = a.n;
+    s.tiles = (int)w.tf;
+    s.share = w.by_table.tiles;
+    s.out = a.dtable;
+    s.out_stride = a.dtable_stride;
+    s.padded = a.rows;
+    e = launch_stream<T, NP, KD, kGradTable>(s, w.by_table, st);
+    if (e != hipSuccess) return e;
+    if (w.by_table.count > 1)
+        k_loss_fold<T><<<blocks_for(a.rows * KD), kThreads, 0, st>>>(
+            w.sums, w.by_table.count, a.rows, KD, nullptr, 1, 1, static_cast<T*>(a.dtable), a.rows,
+            a.dtable_stride, a.dim, nullptr);
+    return hipGetLastError();
+}
+
+// Padded row length that the streaming kernels take, 0: none. Past it a wave's
+// own rows and sums no longer fit its registers.
+int stream_kd(int dim, int dtype) {
+    for (int kd : {32, 64, 128, 256})
+        if (dim <= kd) return dtype == 0 && kd > 128 ? 0 : kd;
+    return 0;
+}
+
 template <typename T, int NP>
 hipError_t loss_run(const LossArgs& a, bool grad, hipStream_t st) {
     const LossPlan w(a.ws, a.n, a.rows, a.dim, a.dtype, grad);
@@ -467,6 +1044,8 @@ hipError_t loss_run(const LossArgs& a, bool grad, hipStream_t st) {
 }  // namespace
 
 size_t label_loss_ws(int64_t n, int64_t rows, int dim, int dtype, bool grad) {
+    const int kd = stream_kd(dim, dtype);
+    if (kd != 0) return StreamPlan(nullptr, n, rows, dtype == 0 ? 3 : 1, kd, grad).bytes;
     return LossPlan(nullptr, n, rows, dim, dtype, grad).bytes;
 }
 
@@ -484,7 +1063,15 @@ hipError_t launch_label_loss(const LossArgs& a, bool grad, hipStream_t st) {
                                                       a.dtable_stride, a.dim, nullptr);
         return hipGetLastError();
     }
-    return a.dtype == 0 ? loss_run<float, 3>(a, grad, st) : loss_run<bf16, 1>(a, grad, st);
+    const bool f = a.dtype == 0;
+    switch (stream_kd(a.dim, a.dtype)) {
+        case 32: return f ? stream_run<float, 3, 32>(a, grad, st) : stream_run<bf16, 1, 32>(a, grad, st);
+        case 64: return f ? stream_run<float, 3, 64>(a, grad, st) : stream_run<bf16, 1, 64>(a, grad, st);
+        case 128:
+            return f ? stream_run<float, 3, 128>(a, grad, st) : stream_run<bf16, 1, 128>(a, grad, st);
+        case 256: return stream_run<bf16, 1, 256>(a, grad, st);
+        default: return f ? loss_run<float, 3>(a, grad, st) : loss_run<bf16, 1>(a, grad, st);
+    }
 }
 
 }  // namespace gs
