@@ -19,37 +19,91 @@ namespace {
 constexpr int kThreads = 256;
 enum { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3 };
 
+// The normal distribution's Phi(z), and exp(-z^2 / 2) on the way: Abramowitz and
+// Stegun's 7.1.26 in its complementary form, Phi(-|z|) = exp(-z^2 / 2) P(t) / 2,
+// t = 1 / (1 + 0.3275911 |z| / sqrt 2), off by at most 7.5e-8 (fp32's own last
+// place near 1) and by less in the tail. The library's erff takes several times
+// the instructions, which made the gelu passes bound by arithmetic.
+__device__ __forceinline__ float normal_cdf(float z, float* pdf_exp) {
+    const float e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
+    const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(z), 0.23164190f, 1.0f));
+    float p = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+    p = fmaf(t, p, 0.5f * 1.421413741f);
+    p = fmaf(t, p, 0.5f * -0.284496736f);
+    p = fmaf(t, p, 0.5f * 0.254829592f);
+    const float q = p * t * e;
+    *pdf_exp = e;
+    return z >= 0.0f ? 1.0f - q : q;
+}
+__device__ __forceinline__ float logistic(float z) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
+}
+
 template <int ACT>
 __device__ __forceinline__ float act(float z) {
     if (ACT == kActRelu) return z > 0.0f ? z : (z != z ? z : 0.0f);
-    if (ACT == kActSilu) return z / (1.0f + __expf(-z));
-    if (ACT == kActGelu) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    if (ACT == kActSilu) return z * logistic(z);
+    if (ACT == kActGelu) {
+        float e;
+        return z * normal_cdf(z, &e);
+    }
     return z;
 }
 template <int ACT>
 __device__ __forceinline__ float act_slope(float z) {
     if (ACT == kActRelu) return z > 0.0f ? 1.0f : 0.0f;
     if (ACT == kActSilu) {
-        const float s = 1.0f / (1.0f + __expf(-z));
-        return s * (1.0f + z * (1.0f - s));
+        const float s = logistic(z);
+        return s * fmaf(z, 1.0f - s, 1.0f);
     }
-    if (ACT == kActGelu)
-        return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) +
-               z * 0.39894228040143268f * __expf(-0.5f * z * z);
+    if (ACT == kActGelu) {
+        float e;
+        const float c = normal_cdf(z, &e);
+        return fmaf(z * 0.39894228040143268f, e, c);
+    }
     return 1.0f;
 }
 
-// Count, mean and sum of squared distances from the mean, joined pairwise, so
-// that a mean far from 0 costs no digits.
+// Count, mean and sum of squared distances from the mean. Pieces are joined by
+// their means' difference, so that a mean far from 0 costs no digits.
 struct Moments {
     float n, mean, m2;
 };
 __device__ __forceinline__ Moments join(const Moments& a, const Moments& b) {
-    if (b.n == 0.0f) return a;
-    if (a.n == 0.0f) return b;
-    const float n = a.n + b.n, d = b.mean - a.mean, f = b.n / n;
-    return {n, a.mean + d * f, a.m2 + b.m2 + d * d * a.n * f};
+    const float n = a.n + b.n, d = b.mean - a.mean;
+    const float f = n > 0.0f ? b.n * __builtin_amdgcn_rcpf(n) : 0.0f;
+    return {n, fmaf(d, f, a.mean), a.m2 + fmaf(d * d, a.n * f, b.m2)};
 }
+
+// A wave's and then the workgroup's sum, the same order every time.
+template <int THREADS>
+__device__ __forceinline__ float block_sum(float v, float* lds) {
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float s = lds[0];
+#pragma unroll
+    for (int k = 1; k < THREADS / 64; ++k) s += lds[k];
+    return s;
+}
+
+// Parameters of VEC channels from c of image b.
+template <int VEC>
+struct Channels {
+    float mean[VEC], rstd[VEC], w[VEC], bias[VEC];
+    __device__ __forceinline__ Channels(const NormArgs& a, int64_t b, int c) {
+        const int per_group = a.channels / a.groups;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const int64_t g = b * a.groups + (c + j) / per_group;
+            mean[j] = a.mean[g];
+            rstd[j] = a.rstd[g];
+            w[j] = a.weight != nullptr ? a.weight[c + j] : 1.0f;
+            bias[j] = a.bias != nullptr ? a.bias[c + j] : 0.0f;
+        }
+    }
+};
 
 // A workgroup's place: image b, chunk of pixels, channel vectors from cv0; a
 // thread's channels and its first pixel.
@@ -76,34 +130,73 @@ __device__ __forceinline__ Place place_of(int64_t pixels, int channels, int chun
     return p;
 }
 
+// Pixels that a thread loads before it uses them.
+constexpr int kAhead = 4;
+
 // ---------------------------------------------------------------- statistics
 // Partials (batch, chunks, channels) of a chunk's mean and squared distances.
+// Four pixels at a time get a mean of their own, then their distances from it:
+// 3 operations a value, against 10 for a running mean.
 template <typename T, int VEC>
 __global__ __launch_bounds__(kThreads) void k_norm_stats(NormArgs a, int chunks, float2* part) {
     __shared__ Moments lds[kThreads * VEC];
     const Place p = place_of<VEC>(a.pixels, a.channels, chunks);
     const T* x = static_cast<const T*>(a.x) + p.b * a.x_batch + p.c;
-    Moments m[VEC];
+    float n = 0.0f, mean[VEC], m2[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) m[j] = {0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < VEC; ++j) mean[j] = m2[j] = 0.0f;
     if (p.on) {
-        for (int64_t q = p.p0 + p.slot; q < p.p1; q += p.slots) {
+        int64_t q = p.p0 + p.slot;
+        for (; q + (kAhead - 1) * p.slots < p.p1; q += kAhead * p.slots) {
+            float v[kAhead][VEC];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) load_vec<VEC>(x + (q + k * p.slots) * a.x_pixel, v[k]);
+            const float total = n + kAhead, f = kAhead * __builtin_amdgcn_rcpf(total), nf = n * f;
+            n = total;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                float s = 0.0f, d2 = 0.0f;
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) s += v[k][j];
+                s *= 1.0f / kAhead;
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) d2 = fmaf(v[k][j] - s, v[k][j] - s, d2);
+                const float d = s - mean[j];
+                mean[j] = fmaf(d, f, mean[j]);
+                m2[j] += fmaf(d * d, nf, d2);
+            }
+        }
+        for (; q < p.p1; q += p.slots) {
             float v[VEC];
             load_vec<VEC>(x + q * a.x_pixel, v);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) m[j] = join(m[j], {1.0f, v[j], 0.0f});
+            for (int j = 0; j < VEC; ++j) {
+                const Moments m = join({n, mean[j], m2[j]}, {1.0f, v[j], 0.0f});
+                mean[j] = m.mean;
+                m2[j] = m.m2;
+            }
+            n += 1.0f;
         }
     }
+    const int at = threadIdx.x;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) lds[threadIdx.x * VEC + j] = m[j];
-    __syncthreads();
-    if (p.slot == 0) {
-        for (int j = 0; j < VEC; ++j) {
-            Moments s = m[j];
-            for (int k = 1; k < p.slots; ++k) s = join(s, lds[(threadIdx.x + k * p.cols) * VEC + j]);
-            part[p.part * a.channels + p.c + j] = make_float2(s.mean, s.m2);
-        }
+    for (int j = 0; j < VEC; ++j) lds[j * kThreads + at] = {n, mean[j], m2[j]};
+    // halve the slots until one is left
+    for (int len = p.slots; len > 1;) {
+        const int half = (len + 1) / 2;
+        __syncthreads();
+        if (p.slot < len - half)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                lds[j * kThreads + at] =
+                    join(lds[j * kThreads + at], lds[j * kThreads + at + half * p.cols]);
+        len = half;
     }
+    if (p.slot == 0)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            part[p.part * a.channels + p.c + j] =
+                make_float2(lds[j * kThreads + at].mean, lds[j * kThreads + at].m2);
 }
 
 // One workgroup per (image, group): joins its channels' chunks.
@@ -113,12 +206,24 @@ __global__ __launch_bounds__(kThreads) void k_norm_finish(NormArgs a, int chunks
     const int64_t b = blockIdx.x / a.groups;
     const int g = blockIdx.x % a.groups, per_group = a.channels / a.groups;
     const int64_t per = (a.pixels + chunks - 1) / chunks;
+    const float2* from = part + b * chunks * a.channels + (int64_t)g * per_group;
     Moments m = {0.0f, 0.0f, 0.0f};
-    for (int i = threadIdx.x; i < chunks * per_group; i += kThreads) {
-        const int k = i / per_group, c = g * per_group + i % per_group;
-        const int64_t p0 = min(a.pixels, per * k), p1 = min(a.pixels, p0 + per);
-        const float2 v = part[(b * chunks + k) * a.channels + c];
-        m = join(m, {(float)(p1 - p0), v.x, v.y});
+    const int all = chunks * per_group;
+    for (int i0 = threadIdx.x; i0 < all; i0 += kThreads * 8) {
+        float2 v[8];
+        float n[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int i = min(i0 + u * kThreads, all - 1);
+            const int k = i / per_group, c = i - k * per_group;
+            const bool on = i0 + u * kThreads < all;
+            v[u] = from[(int64_t)k * a.channels + c];
+            if (!on) v[u] = make_float2(0.0f, 0.0f);
+            const int64_t p0 = min(a.pixels, per * k);
+            n[u] = on ? (float)(min(a.pixels, p0 + per) - p0) : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) m = join(m, {n[u], v[u].x, v[u].y});
     }
     lds[threadIdx.x] = m;
     __syncthreads();
@@ -138,108 +243,147 @@ template <typename T, int VEC, int ACT>
 __global__ __launch_bounds__(kThreads) void k_norm_apply(NormArgs a, int chunks) {
     const Place p = place_of<VEC>(a.pixels, a.channels, chunks);
     if (!p.on) return;
-    const int per_group = a.channels / a.groups;
-    float mean[VEC], k[VEC], bias[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-        const int64_t g = p.b * a.groups + (p.c + j) / per_group;
-        mean[j] = a.mean[g];
-        k[j] = a.rstd[g] * (a.weight != nullptr ? a.weight[p.c + j] : 1.0f);
-        bias[j] = a.bias != nullptr ? a.bias[p.c + j] : 0.0f;
-    }
+    const Channels<VEC> ch(a, p.b, p.c);
     const T* x = static_cast<const T*>(a.x) + p.b * a.x_batch + p.c;
     T* y = static_cast<T*>(a.y) + p.b * a.y_batch + p.c;
-    for (int64_t q = p.p0 + p.slot; q < p.p1; q += p.slots) {
+    auto one = [&](float* v) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            v[j] = act<ACT>(fmaf((v[j] - ch.mean[j]) * ch.rstd[j], ch.w[j], ch.bias[j]));
+    };
+    int64_t q = p.p0 + p.slot;
+    for (; q + (kAhead - 1) * p.slots < p.p1; q += kAhead * p.slots) {
+        float v[kAhead][VEC];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) load_vec<VEC>(x + (q + k * p.slots) * a.x_pixel, v[k]);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            one(v[k]);
+            store_vec<VEC>(y + (q + k * p.slots) * a.y_pixel, v[k]);
+        }
+    }
+    for (; q < p.p1; q += p.slots) {
         float v[VEC];
         load_vec<VEC>(x + q * a.x_pixel, v);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] = act<ACT>(fmaf(v[j] - mean[j], k[j], bias[j]));
+        one(v);
         store_vec<VEC>(y + q * a.y_pixel, v);
     }
 }
 
 // ---------------------------------------------------------------- gradient
+// Adds the slots' channel sums, halving; slot 0 ends with the total.
+template <int VEC, int THREADS>
+__device__ __forceinline__ void slots_sum(float2* lds, int at, int slot, int slots, int cols,
+                                          float* s1, float* s2) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) lds[j * THREADS + at] = make_float2(s1[j], s2[j]);
+    for (int len = slots; len > 1;) {
+        const int half = (len + 1) / 2;
+        __syncthreads();
+        if (slot < len - half)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const float2 u = lds[j * THREADS + at + half * cols];
+                s1[j] += u.x;
+                s2[j] += u.y;
+                lds[j * THREADS + at] = make_float2(s1[j], s2[j]);
+            }
+        len = half;
+    }
+}
+
 // Partials (batch, chunks, channels) of sum dz and sum dz xh.
 template <typename T, int VEC, int ACT>
 __global__ __launch_bounds__(kThreads) void k_norm_grad_sums(NormArgs a, int chunks, float2* part) {
     __shared__ float2 lds[kThreads * VEC];
+    constexpr int AHEAD = kAhead / 2;  // of x and of dy
     const Place p = place_of<VEC>(a.pixels, a.channels, chunks);
-    const int per_group = a.channels / a.groups;
     float s1[VEC], s2[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) s1[j] = s2[j] = 0.0f;
     if (p.on) {
-        float mean[VEC], rstd[VEC], w[VEC], bias[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            const int64_t g = p.b * a.groups + (p.c + j) / per_group;
-            mean[j] = a.mean[g];
-            rstd[j] = a.rstd[g];
-            w[j] = a.weight != nullptr ? a.weight[p.c + j] : 1.0f;
-            bias[j] = a.bias != nullptr ? a.bias[p.c + j] : 0.0f;
-        }
+        const Channels<VEC> ch(a, p.b, p.c);
         const T* x = static_cast<const T*>(a.x) + p.b * a.x_batch + p.c;
         const T* dy = static_cast<const T*>(a.dy) + p.b * a.dy_batch + p.c;
-        for (int64_t q = p.p0 + p.slot; q < p.p1; q += p.slots) {
-            float v[VEC], d[VEC];
-            load_vec<VEC>(x + q * a.x_pixel, v);
-            load_vec<VEC>(dy + q * a.dy_pixel, d);
+        auto one = [&](const float* v, const float* d) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                const float xh = (v[j] - mean[j]) * rstd[j];
-                const float dz = d[j] * act_slope<ACT>(fmaf(xh, w[j], bias[j]));
+                const float xh = (v[j] - ch.mean[j]) * ch.rstd[j];
+                const float dz = d[j] * act_slope<ACT>(fmaf(xh, ch.w[j], ch.bias[j]));
                 s1[j] += dz;
                 s2[j] = fmaf(dz, xh, s2[j]);
             }
-        }
-    }
+        };
+        int64_t q = p.p0 + p.slot;
+        for (; q + (AHEAD - 1) * p.slots < p.p1; q += AHEAD * p.slots) {
+            float v[AHEAD][VEC], d[AHEAD][VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) lds[threadIdx.x * VEC + j] = make_float2(s1[j], s2[j]);
-    __syncthreads();
-    if (p.slot == 0) {
-        for (int j = 0; j < VEC; ++j) {
-            for (int k = 1; k < p.slots; ++k) {
-                const float2 u = lds[(threadIdx.x + k * p.cols) * VEC + j];
-                s1[j] += u.x;
-                s2[j] += u.y;
+            for (int k = 0; k < AHEAD; ++k) {
+                load_vec<VEC>(x + (q + k * p.slots) * a.x_pixel, v[k]);
+                load_vec<VEC>(dy + (q + k * p.slots) * a.dy_pixel, d[k]);
             }
-            part[p.part * a.channels + p.c + j] = make_float2(s1[j], s2[j]);
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) one(v[k], d[k]);
+        }
+        for (; q < p.p1; q += p.slots) {
+            float v[VEC], d[VEC];
+            load_vec<VEC>(x + q * a.x_pixel, v);
+            load_vec<VEC>(dy + q * a.dy_pixel, d);
+            one(v, d);
         }
     }
+    slots_sum<VEC, kThreads>(lds, threadIdx.x, p.slot, p.slots, p.cols, s1, s2);
+    if (p.slot == 0)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            part[p.part * a.channels + p.c + j] = make_float2(s1[j], s2[j]);
 }
 
-// One workgroup per (image, group): the group's channel sums over the chunks, and m1, m2.
+// One workgroup per (image, group): the group's channel sums over the chunks, and
+// m1, m2. Threads of one channel stand `per_group` apart (or walk over channels
+// when a group has more than the workgroup has threads).
 __global__ __launch_bounds__(kThreads) void k_norm_grad_finish(NormArgs a, int chunks,
                                                                const float2* part, float2* sums,
                                                                float2* means) {
     __shared__ float2 lds[kThreads];
+    __shared__ float red[kThreads / 64];
     const int64_t b = blockIdx.x / a.groups;
     const int g = blockIdx.x % a.groups, per_group = a.channels / a.groups;
     float m1 = 0.0f, m2 = 0.0f;
-    for (int c = g * per_group; c < (g + 1) * per_group; ++c) {
-        float2 s = make_float2(0.0f, 0.0f);
-        for (int k = threadIdx.x; k < chunks; k += kThreads) {
-            const float2 v = part[(b * chunks + k) * a.channels + c];
-            s.x += v.x;
-            s.y += v.y;
-        }
-        __syncthreads();
-        lds[threadIdx.x] = s;
-        __syncthreads();
-        for (int o = kThreads / 2; o > 0; o >>= 1) {
-            if ((int)threadIdx.x < o) {
-                lds[threadIdx.x].x += lds[threadIdx.x + o].x;
-                lds[threadIdx.x].y += lds[threadIdx.x + o].y;
+    const int cols = min(per_group, kThreads), rows = kThreads / cols;
+    const int row = threadIdx.x / cols, col = threadIdx.x % cols;
+    for (int c0 = 0; c0 < per_group; c0 += cols) {
+        const bool on = row < rows && c0 + col < per_group;
+        const int c = g * per_group + c0 + col;
+        float s1[1] = {0.0f}, s2[1] = {0.0f};
+        if (on) {
+            const float2* from = part + b * chunks * a.channels + c;
+            for (int k0 = row; k0 < chunks; k0 += rows * 8) {
+                float2 v[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int k = k0 + u * rows;
+                    v[u] = from[(int64_t)min(k, chunks - 1) * a.channels];
+                    if (k >= chunks) v[u] = make_float2(0.0f, 0.0f);
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    s1[0] += v[u].x;
+                    s2[0] += v[u].y;
+                }
             }
-            __syncthreads();
         }
-        if (threadIdx.x == 0) {
+        __syncthreads();
+        slots_sum<1, kThreads>(lds, threadIdx.x, row, rows, cols, s1, s2);
+        if (on && row == 0) {
             const float w = a.weight != nullptr ? a.weight[c] : 1.0f;
-            sums[b * a.channels + c] = lds[0];
-            m1 += w * lds[0].x;
-            m2 += w * lds[0].y;
+            sums[b * a.channels + c] = make_float2(s1[0], s2[0]);
+            m1 = fmaf(w, s1[0], m1);
+            m2 = fmaf(w, s2[0], m2);
         }
     }
+    m1 = block_sum<kThreads>(m1, red);
+    m2 = block_sum<kThreads>(m2, red);
     if (threadIdx.x == 0) {
         const float count = (float)a.pixels * (float)per_group;
         means[blockIdx.x] = make_float2(m1 / count, m2 / count);
@@ -259,45 +403,205 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_params(NormArgs a, const
     if (a.dweight != nullptr) a.dweight[c] = dw;
 }
 
+template <int ACT, int VEC>
+__device__ __forceinline__ void grad_of(const Channels<VEC>& ch, const float* m1, const float* m2,
+                                        float* v, const float* d) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        const float xh = (v[j] - ch.mean[j]) * ch.rstd[j];
+        const float dz = d[j] * act_slope<ACT>(fmaf(xh, ch.w[j], ch.bias[j]));
+        v[j] = ch.rstd[j] * (fmaf(ch.w[j], dz, -m1[j]) - xh * m2[j]);
+    }
+}
+
 template <typename T, int VEC, int ACT>
 __global__ __launch_bounds__(kThreads) void k_norm_grad_apply(NormArgs a, int chunks,
                                                               const float2* means) {
+    constexpr int AHEAD = kAhead / 2;
     const Place p = place_of<VEC>(a.pixels, a.channels, chunks);
     if (!p.on) return;
-    const int per_group = a.channels / a.groups;
-    float mean[VEC], rstd[VEC], w[VEC], bias[VEC], m1[VEC], m2[VEC];
+    const Channels<VEC> ch(a, p.b, p.c);
+    float m1[VEC], m2[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-        const int64_t g = p.b * a.groups + (p.c + j) / per_group;
-        mean[j] = a.mean[g];
-        rstd[j] = a.rstd[g];
-        w[j] = a.weight != nullptr ? a.weight[p.c + j] : 1.0f;
-        bias[j] = a.bias != nullptr ? a.bias[p.c + j] : 0.0f;
-        const float2 m = means[g];
+        const float2 m = means[p.b * a.groups + (p.c + j) / (a.channels / a.groups)];
         m1[j] = m.x;
         m2[j] = m.y;
     }
     const T* x = static_cast<const T*>(a.x) + p.b * a.x_batch + p.c;
     const T* dy = static_cast<const T*>(a.dy) + p.b * a.dy_batch + p.c;
     T* dx = static_cast<T*>(a.dx) + p.b * a.dx_batch + p.c;
-    for (int64_t q = p.p0 + p.slot; q < p.p1; q += p.slots) {
+    int64_t q = p.p0 + p.slot;
+    for (; q + (AHEAD - 1) * p.slots < p.p1; q += AHEAD * p.slots) {
+        float v[AHEAD][VEC], d[AHEAD][VEC];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            load_vec<VEC>(x + (q + k * p.slots) * a.x_pixel, v[k]);
+            load_vec<VEC>(dy + (q + k * p.slots) * a.dy_pixel, d[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            grad_of<ACT, VEC>(ch, m1, m2, v[k], d[k]);
+            store_vec<VEC>(dx + (q + k * p.slots) * a.dx_pixel, v[k]);
+        }
+    }
+    for (; q < p.p1; q += p.slots) {
         float v[VEC], d[VEC];
         load_vec<VEC>(x + q * a.x_pixel, v);
         load_vec<VEC>(dy + q * a.dy_pixel, d);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            const float xh = (v[j] - mean[j]) * rstd[j];
-            const float dz = d[j] * act_slope<ACT>(fmaf(xh, w[j], bias[j]));
-            v[j] = rstd[j] * (fmaf(w[j], dz, -m1[j]) - xh * m2[j]);
-        }
+        grad_of<ACT, VEC>(ch, m1, m2, v, d);
         store_vec<VEC>(dx + q * a.dx_pixel, v);
     }
 }
 
-// Chunks of an image's pixels: enough workgroups for the chip, at least 64
-// pixels each.
+// ---------------------------------------------------------------- small groups
+// A group of an image that fits one workgroup's registers: one workgroup per (image, group) reads it once, in one launch.
+constexpr int kSmallThreads = 1024;
+// Vectors of a thread: 32 values, or 4 single ones where a group's channels do
+// not make vectors.
+template <int VEC>
+constexpr int kSmallVectors = VEC > 1 ? 32 / VEC : 4;
+
+struct SmallPlace {
+    int cols, slots, slot, c;
+    bool on;
+};
+template <int VEC>
+__device__ __forceinline__ SmallPlace small_place(int per_group) {
+    SmallPlace p;
+    p.cols = per_group / VEC;
+    p.slots = kSmallThreads / p.cols;
+    p.slot = threadIdx.x / p.cols;
+    p.c = (blockIdx.x * p.cols + (int)threadIdx.x % p.cols) * VEC;
+    p.on = p.slot < p.slots;
+    return p;
+}
+
+template <typename T, int VEC, int ACT>
+__global__ __launch_bounds__(kSmallThreads) void k_norm_small(NormArgs a) {
+    constexpr int K = kSmallVectors<VEC>;
+    __shared__ float red[kSmallThreads / 64];
+    const int per_group = a.channels / a.groups;
+    const SmallPlace p = small_place<VEC>(per_group);
+    const int64_t b = blockIdx.y;
+    const T* x = static_cast<const T*>(a.x) + b * a.x_batch + p.c;
+    const int pixels = (int)a.pixels;
+    float v[K][VEC], sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int q = p.slot + k * p.slots;
+        if (p.on && q < pixels) load_vec<VEC>(x + q * a.x_pixel, v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (p.on && p.slot + k * p.slots < pixels)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) sum += v[k][j];
+    const float count = (float)pixels * (float)per_group;
+    const float mean = block_sum<kSmallThreads>(sum, red) / count;
+    float m2 = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (p.on && p.slot + k * p.slots < pixels)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) m2 = fmaf(v[k][j] - mean, v[k][j] - mean, m2);
+    const float rstd = 1.0f / sqrtf(block_sum<kSmallThreads>(m2, red) / count + a.eps);
+    if (threadIdx.x == 0) {
+        a.mean[b * a.groups + blockIdx.x] = mean;
+        a.rstd[b * a.groups + blockIdx.x] = rstd;
+    }
+    if (!p.on) return;
+    float w[VEC], bias[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        w[j] = a.weight != nullptr ? a.weight[p.c + j] : 1.0f;
+        bias[j] = a.bias != nullptr ? a.bias[p.c + j] : 0.0f;
+    }
+    T* y = static_cast<T*>(a.y) + b * a.y_batch + p.c;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int q = p.slot + k * p.slots;
+        if (q < pixels) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                v[k][j] = act<ACT>(fmaf((v[k][j] - mean) * rstd, w[j], bias[j]));
+            store_vec<VEC>(y + q * a.y_pixel, v[k]);
+        }
+    }
+}
+
+template <typename T, int VEC, int ACT>
+__global__ __launch_bounds__(kSmallThreads) void k_norm_small_grad(NormArgs a, float2* sums) {
+    constexpr int K = kSmallVectors<VEC>;
+    __shared__ float2 lds[kSmallThreads * VEC];
+    __shared__ float red[kSmallThreads / 64];
+    const int per_group = a.channels / a.groups;
+    const SmallPlace p = small_place<VEC>(per_group);
+    const int64_t b = blockIdx.y;
+    const int pixels = (int)a.pixels;
+    const T* x = static_cast<const T*>(a.x) + b * a.x_batch + p.c;
+    const T* dy = static_cast<const T*>(a.dy) + b * a.dy_batch + p.c;
+    float v[K][VEC], d[K][VEC], s1[VEC], s2[VEC], w[VEC], bias[VEC];
+    const float mean = a.mean[b * a.groups + blockIdx.x], rstd = a.rstd[b * a.groups + blockIdx.x];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        s1[j] = s2[j] = 0.0f;
+        w[j] = a.weight != nullptr && p.on ? a.weight[p.c + j] : 1.0f;
+        bias[j] = a.bias != nullptr && p.on ? a.bias[p.c + j] : 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int q = p.slot + k * p.slots;
+        if (p.on && q < pixels) {
+            load_vec<VEC>(x + q * a.x_pixel, v[k]);
+            load_vec<VEC>(dy + q * a.dy_pixel, d[k]);
+        }
+    }
+    // v and d become xh and dz
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (p.on && p.slot + k * p.slots < pixels)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                v[k][j] = (v[k][j] - mean) * rstd;
+                d[k][j] *= act_slope<ACT>(fmaf(v[k][j], w[j], bias[j]));
+                s1[j] += d[k][j];
+                s2[j] = fmaf(d[k][j], v[k][j], s2[j]);
+            }
+    slots_sum<VEC, kSmallThreads>(lds, threadIdx.x, p.slot, p.slots, p.cols, s1, s2);
+    float m1 = 0.0f, m2 = 0.0f;
+    if (p.slot == 0)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            m1 = fmaf(w[j], s1[j], m1);
+            m2 = fmaf(w[j], s2[j], m2);
+            if (a.batch > 1) {
+                sums[b * a.channels + p.c + j] = make_float2(s1[j], s2[j]);
+            } else {
+                if (a.dbias != nullptr) a.dbias[p.c + j] = s1[j];
+                if (a.dweight != nullptr) a.dweight[p.c + j] = s2[j];
+            }
+        }
+    const float count = (float)pixels * (float)per_group;
+    m1 = block_sum<kSmallThreads>(m1, red) / count;
+    m2 = block_sum<kSmallThreads>(m2, red) / count;
+    if (!p.on) return;
+    T* dx = static_cast<T*>(a.dx) + b * a.dx_batch + p.c;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int q = p.slot + k * p.slots;
+        if (q < pixels) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                v[k][j] = rstd * (fmaf(w[j], d[k][j], -m1) - v[k][j] * m2);
+            store_vec<VEC>(dx + q * a.dx_pixel, v[k]);
+        }
+    }
+}
+
+// Chunks of an image's pixels: four workgroups a compute unit, at least 64 pixels each.
 int chunks_of(int64_t batch, int64_t pixels) {
-    int64_t k = batch < 1 ? 1 : (2048 + batch - 1) / batch;
+    int64_t k = batch < 1 ? 1 : (1024 + batch - 1) / batch;
     if (k > (pixels + 63) / 64) k = (pixels + 63) / 64;
     return k < 1 ? 1 : (int)k;
 }
@@ -314,6 +618,15 @@ struct NormWs {
     }
 };
 
+// Whether a group is one workgroup's work: it fits the registers in whole vectors
+// (or is so small that reading by single values costs nothing).
+template <int VEC>
+bool small_group(const NormArgs& a) {
+    const int per_group = a.channels / a.groups;
+    if (a.batch > 65535 || per_group % VEC != 0 || per_group / VEC > kSmallThreads) return false;
+    return a.pixels <= kSmallThreads / (per_group / VEC) * kSmallVectors<VEC>;
+}
+
 template <typename T, int VEC, int ACT>
 hipError_t norm_run(const NormArgs& a, bool grad, hipStream_t st) {
     const NormWs w(a.ws, a.batch, a.pixels, a.channels);
@@ -321,6 +634,18 @@ hipError_t norm_run(const NormArgs& a, bool grad, hipStream_t st) {
     const int cols = (a.channels + VEC - 1) / VEC;
     const dim3 grid((unsigned)(chunks * a.batch), (unsigned)((cols + kThreads - 1) / kThreads));
     const unsigned groups = (unsigned)(a.batch * a.groups);
+    if (small_group<VEC>(a)) {
+        const dim3 small((unsigned)a.groups, (unsigned)a.batch);
+        if (!grad) {
+            k_norm_small<T, VEC, ACT><<<small, kSmallThreads, 0, st>>>(a);
+        } else {
+            k_norm_small_grad<T, VEC, ACT><<<small, kSmallThreads, 0, st>>>(a, w.sums);
+            if (a.batch > 1)
+                k_norm_grad_params<<<(unsigned)((a.channels + kThreads - 1) / kThreads), kThreads,
+                                     0, st>>>(a, w.sums);
+        }
+        return hipGetLastError();
+    }
     if (!grad) {
         k_norm_stats<T, VEC><<<grid, kThreads, 0, st>>>(a, chunks, w.part);
         k_norm_finish<<<groups, kThreads, 0, st>>>(a, chunks, w.part);
