@@ -71,7 +71,7 @@ struct NormArgs {
     int64_t dx_batch, dx_pixel;
     float *dweight, *dbias;
 };
-size_t group_norm_ws(int64_t batch, int64_t pixels, int channels);
+size_t group_norm_ws(int64_t batch, int channels);
 hipError_t launch_group_norm(const NormArgs& a, hipStream_t st);
 hipError_t launch_group_norm_grad(const NormArgs& a, hipStream_t st);
 

@@ -231,7 +231,7 @@ int64_t gs_group_norm_workspace(int64_t batch, int64_t pixels, int channels) {
     if (batch < 0 || batch > kMaxImages || pixels < 0 || pixels > kMaxPixels || channels < 1 ||
         channels > kMaxDim)
         return -1;
-    return (int64_t)gs::group_norm_ws(batch, pixels, channels);
+    return (int64_t)gs::group_norm_ws(batch, channels);
 }
 
 int gs_group_norm_dev(gs_ctx* ctx, const gs_group_norm* norm, const void* x, int64_t x_batch,
@@ -247,7 +247,7 @@ int gs_group_norm_dev(gs_ctx* ctx, const gs_group_norm* norm, const void* x, int
         check_words(mean, "group_norm: mean");
         check_words(rstd, "group_norm: rstd");
         check_ws(workspace, workspace_bytes,
-                 gs::group_norm_ws(norm->batch, norm->pixels, norm->channels), "group_norm");
+                 gs::group_norm_ws(norm->batch, norm->channels), "group_norm");
         gs::NormArgs a = norm_args(norm);
         a.x = x;
         a.x_batch = x_batch;
@@ -281,7 +281,7 @@ int gs_group_norm_grad_dev(gs_ctx* ctx, const gs_group_norm* norm, const void* d
         check_words(dweight, "group_norm_grad: dweight");
         check_words(dbias, "group_norm_grad: dbias");
         check_ws(workspace, workspace_bytes,
-                 gs::group_norm_ws(norm->batch, norm->pixels, norm->channels), "group_norm_grad");
+                 gs::group_norm_ws(norm->batch, norm->channels), "group_norm_grad");
         gs::NormArgs a = norm_args(norm);
         a.x = x;
         a.x_batch = x_batch;

@@ -37,6 +37,20 @@ __device__ __forceinline__ void store_vec(T* p, const float* in) {
     *reinterpret_cast<VecOf<T, VEC>*>(p) = u;
 }
 
+// The same past the caches, for outputs that are not read again soon.
+template <int VEC, typename T>
+__device__ __forceinline__ void store_nt(T* p, const float* in) {
+    VecOf<T, VEC> u;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) u.v[j] = from_float<T>(in[j]);
+    if constexpr (sizeof(u) % 4 == 0) {
+        typedef __attribute__((ext_vector_type(sizeof(u) / 4))) uint32_t words;
+        __builtin_nontemporal_store(__builtin_bit_cast(words, u), reinterpret_cast<words*>(p));
+    } else {
+        *reinterpret_cast<VecOf<T, VEC>*>(p) = u;
+    }
+}
+
 // Whether rows at `stride` elements apart can be read VEC elements at a time.
 template <typename T>
 inline bool aligned_rows(const void* p, int64_t stride, int vec) {

@@ -88,21 +88,25 @@ __device__ __forceinline__ float block_sum(float v, float* lds) {
     return s;
 }
 
-// Parameters of VEC channels from c of image b.
+// What VEC channels from c of image b need, folded to one fused multiply-add a
+// step: xh = x r + o, z = xh w + bias. (The offset's rounding is that of a mean's
+// last place, which the mean itself has.)
 template <int VEC>
 struct Channels {
-    float mean[VEC], rstd[VEC], w[VEC], bias[VEC];
+    float r[VEC], o[VEC], w[VEC], bias[VEC];
     __device__ __forceinline__ Channels(const NormArgs& a, int64_t b, int c) {
         const int per_group = a.channels / a.groups;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
             const int64_t g = b * a.groups + (c + j) / per_group;
-            mean[j] = a.mean[g];
-            rstd[j] = a.rstd[g];
+            r[j] = a.rstd[g];
+            o[j] = -a.mean[g] * r[j];
             w[j] = a.weight != nullptr ? a.weight[c + j] : 1.0f;
             bias[j] = a.bias != nullptr ? a.bias[c + j] : 0.0f;
         }
     }
+    __device__ __forceinline__ float xh(float x, int j) const { return fmaf(x, r[j], o[j]); }
+    __device__ __forceinline__ float z(float h, int j) const { return fmaf(h, w[j], bias[j]); }
 };
 
 // A workgroup's place: image b, chunk of pixels, channel vectors from cv0; a
@@ -243,13 +247,18 @@ template <typename T, int VEC, int ACT>
 __global__ __launch_bounds__(kThreads) void k_norm_apply(NormArgs a, int chunks) {
     const Place p = place_of<VEC>(a.pixels, a.channels, chunks);
     if (!p.on) return;
-    const Channels<VEC> ch(a, p.b, p.c);
+    Channels<VEC> ch(a, p.b, p.c);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {  // xh is not needed: z = x k + c
+        ch.bias[j] = fmaf(ch.o[j], ch.w[j], ch.bias[j]);
+        ch.w[j] *= ch.r[j];
+    }
     const T* x = static_cast<const T*>(a.x) + p.b * a.x_batch + p.c;
     T* y = static_cast<T*>(a.y) + p.b * a.y_batch + p.c;
     auto one = [&](float* v) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j)
-            v[j] = act<ACT>(fmaf((v[j] - ch.mean[j]) * ch.rstd[j], ch.w[j], ch.bias[j]));
+            v[j] = act<ACT>(ch.z(v[j], j));
     };
     int64_t q = p.p0 + p.slot;
     for (; q + (kAhead - 1) * p.slots < p.p1; q += kAhead * p.slots) {
@@ -259,7 +268,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_apply(NormArgs a, int chunks)
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
             one(v[k]);
-            store_vec<VEC>(y + (q + k * p.slots) * a.y_pixel, v[k]);
+            store_nt<VEC>(y + (q + k * p.slots) * a.y_pixel, v[k]);
         }
     }
     for (; q < p.p1; q += p.slots) {
@@ -308,8 +317,8 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_sums(NormArgs a, int chu
         auto one = [&](const float* v, const float* d) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                const float xh = (v[j] - ch.mean[j]) * ch.rstd[j];
-                const float dz = d[j] * act_slope<ACT>(fmaf(xh, ch.w[j], ch.bias[j]));
+                const float xh = ch.xh(v[j], j);
+                const float dz = d[j] * act_slope<ACT>(ch.z(xh, j));
                 s1[j] += dz;
                 s2[j] = fmaf(dz, xh, s2[j]);
             }
@@ -403,14 +412,15 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_params(NormArgs a, const
     if (a.dweight != nullptr) a.dweight[c] = dw;
 }
 
+// dx = rstd w dz - rstd m1 - xh rstd m2
 template <int ACT, int VEC>
-__device__ __forceinline__ void grad_of(const Channels<VEC>& ch, const float* m1, const float* m2,
-                                        float* v, const float* d) {
+__device__ __forceinline__ void grad_of(const Channels<VEC>& ch, const float* rw, const float* m1,
+                                        const float* m2, float* v, const float* d) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-        const float xh = (v[j] - ch.mean[j]) * ch.rstd[j];
-        const float dz = d[j] * act_slope<ACT>(fmaf(xh, ch.w[j], ch.bias[j]));
-        v[j] = ch.rstd[j] * (fmaf(ch.w[j], dz, -m1[j]) - xh * m2[j]);
+        const float xh = ch.xh(v[j], j);
+        const float dz = d[j] * act_slope<ACT>(ch.z(xh, j));
+        v[j] = fmaf(-xh, m2[j], fmaf(rw[j], dz, -m1[j]));
     }
 }
 
@@ -421,12 +431,13 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_apply(NormArgs a, int ch
     const Place p = place_of<VEC>(a.pixels, a.channels, chunks);
     if (!p.on) return;
     const Channels<VEC> ch(a, p.b, p.c);
-    float m1[VEC], m2[VEC];
+    float rw[VEC], m1[VEC], m2[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
         const float2 m = means[p.b * a.groups + (p.c + j) / (a.channels / a.groups)];
-        m1[j] = m.x;
-        m2[j] = m.y;
+        rw[j] = ch.r[j] * ch.w[j];
+        m1[j] = ch.r[j] * m.x;
+        m2[j] = ch.r[j] * m.y;
     }
     const T* x = static_cast<const T*>(a.x) + p.b * a.x_batch + p.c;
     const T* dy = static_cast<const T*>(a.dy) + p.b * a.dy_batch + p.c;
@@ -441,15 +452,15 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_apply(NormArgs a, int ch
         }
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
-            grad_of<ACT, VEC>(ch, m1, m2, v[k], d[k]);
-            store_vec<VEC>(dx + (q + k * p.slots) * a.dx_pixel, v[k]);
+            grad_of<ACT, VEC>(ch, rw, m1, m2, v[k], d[k]);
+            store_nt<VEC>(dx + (q + k * p.slots) * a.dx_pixel, v[k]);
         }
     }
     for (; q < p.p1; q += p.slots) {
         float v[VEC], d[VEC];
         load_vec<VEC>(x + q * a.x_pixel, v);
         load_vec<VEC>(dy + q * a.dy_pixel, d);
-        grad_of<ACT, VEC>(ch, m1, m2, v, d);
+        grad_of<ACT, VEC>(ch, rw, m1, m2, v, d);
         store_vec<VEC>(dx + q * a.dx_pixel, v);
     }
 }
@@ -600,8 +611,9 @@ __global__ __launch_bounds__(kSmallThreads) void k_norm_small_grad(NormArgs a, f
 }
 
 // Chunks of an image's pixels: four workgroups a compute unit, at least 64 pixels each.
+constexpr int kGroups = 1024;
 int chunks_of(int64_t batch, int64_t pixels) {
-    int64_t k = batch < 1 ? 1 : (1024 + batch - 1) / batch;
+    int64_t k = (kGroups + batch - 1) / batch;
     if (k > (pixels + 63) / 64) k = (pixels + 63) / 64;
     return k < 1 ? 1 : (int)k;
 }
@@ -609,9 +621,9 @@ int chunks_of(int64_t batch, int64_t pixels) {
 struct NormWs {
     float2 *part, *sums, *means;
     size_t bytes;
-    NormWs(void* base, int64_t batch, int64_t pixels, int channels) {
+    NormWs(void* base, int64_t batch, int channels) {
         Carve c(base);
-        part = c.take<float2>((size_t)batch * chunks_of(batch, pixels) * channels);
+        part = c.take<float2>((size_t)(kGroups + batch) * channels);  // at least batch * chunks
         sums = c.take<float2>((size_t)batch * channels);
         means = c.take<float2>((size_t)batch * channels);
         bytes = c.bytes();
@@ -629,11 +641,9 @@ bool small_group(const NormArgs& a) {
 
 template <typename T, int VEC, int ACT>
 hipError_t norm_run(const NormArgs& a, bool grad, hipStream_t st) {
-    const NormWs w(a.ws, a.batch, a.pixels, a.channels);
+    const NormWs w(a.ws, a.batch, a.channels);
     const int chunks = chunks_of(a.batch, a.pixels);
     const int cols = (a.channels + VEC - 1) / VEC;
-    const dim3 grid((unsigned)(chunks * a.batch), (unsigned)((cols + kThreads - 1) / kThreads));
-    const unsigned groups = (unsigned)(a.batch * a.groups);
     if (small_group<VEC>(a)) {
         const dim3 small((unsigned)a.groups, (unsigned)a.batch);
         if (!grad) {
@@ -646,6 +656,8 @@ hipError_t norm_run(const NormArgs& a, bool grad, hipStream_t st) {
         }
         return hipGetLastError();
     }
+    const dim3 grid((unsigned)(chunks * a.batch), (unsigned)((cols + kThreads - 1) / kThreads));
+    const unsigned groups = (unsigned)(a.batch * a.groups);
     if (!grad) {
         k_norm_stats<T, VEC><<<grid, kThreads, 0, st>>>(a, chunks, w.part);
         k_norm_finish<<<groups, kThreads, 0, st>>>(a, chunks, w.part);
@@ -684,8 +696,8 @@ hipError_t norm_typed(const NormArgs& a, bool grad, hipStream_t st) {
 
 }  // namespace
 
-size_t group_norm_ws(int64_t batch, int64_t pixels, int channels) {
-    return NormWs(nullptr, batch, pixels, channels).bytes;
+size_t group_norm_ws(int64_t batch, int channels) {
+    return NormWs(nullptr, batch, channels).bytes;
 }
 
 hipError_t launch_group_norm(const NormArgs& a, hipStream_t st) {
