@@ -6,6 +6,8 @@
 // The gradient is by sorted ids: a stable radix sort of (id, position), then
 // each id's run of rows is summed in position order, so the result does not
 // depend on timing. Sums are held in fp32.
+#include <type_traits>
+
 #include "field.h"
 
 #include "field_device.h"
@@ -17,118 +19,150 @@ namespace {
 constexpr int kThreads = 256;
 
 // ---------------------------------------------------------------- lookup
-// A workgroup takes R consecutive ids, stages their rows' numbers in LDS and
-// writes the R * dim values in memory order, VEC at a time.
+// A workgroup takes R consecutive ids, stages where their rows begin in LDS and
+// writes the rows in memory order, a unit of VEC values a lane, so that reads
+// and writes of a wave are contiguous whatever the row length. A thread's next
+// unit lies kThreads further: its row and column follow by addition, where a
+// division a unit took longer than the memory.
 constexpr int kLookupRows = 1024;  // most ids of a workgroup
+constexpr int kLookupUnits = 8;    // units that a thread loads before it stores
 
-template <typename TT, typename TO, int VEC, bool VLOAD, bool VSTORE>
+template <typename TT, typename TO, int VEC>
 __global__ __launch_bounds__(kThreads) void k_lookup(LookupArgs a, int R) {
-    __shared__ int32_t row_of[kLookupRows];
+    __shared__ int64_t start[kLookupRows];
     const TT* table = static_cast<const TT*>(a.table);
     TO* out = static_cast<TO*>(a.out);
-    const uint32_t dim = (uint32_t)a.dim;
+    const uint32_t units = (uint32_t)a.dim / VEC;
+    const uint32_t step_r = kThreads / units, step_c = kThreads % units;
+    const bool flat = a.out_stride == a.dim;
     for (int64_t r0 = (int64_t)blockIdx.x * R; r0 < a.n; r0 += (int64_t)gridDim.x * R) {
         const int nr = (int)min((int64_t)R, a.n - r0);
         __syncthreads();
-        for (int i = threadIdx.x; i < nr; i += kThreads)
-            row_of[i] = load_id(a.ids, a.ids64, r0 + i, a.rows, a.flags);
+        for (int i = threadIdx.x; i < nr; i += kThreads) {
+            const int32_t t = load_id(a.ids, a.ids64, r0 + i, a.rows, a.flags);
+            start[i] = t >= 0 ? t * a.table_stride : -1;
+        }
         __syncthreads();
-        const uint32_t total = (uint32_t)nr * dim;
-        for (uint32_t l = threadIdx.x * VEC; l < total; l += kThreads * VEC) {
-            uint32_t r = l / dim, c = l - r * dim;
-            float v[VEC];
-            if (VLOAD) {
-                const int32_t t = row_of[r];
-                if (t >= 0) {
-                    load_vec<VEC>(table + t * a.table_stride + c, v);
+        uint32_t r = threadIdx.x / units, c = threadIdx.x % units;
+        const uint32_t total = (uint32_t)nr * units;
+        TO* to = out + r0 * a.out_stride;
+        for (uint32_t u0 = threadIdx.x; u0 < total; u0 += kThreads * kLookupUnits) {
+            float v[kLookupUnits][VEC];
+            uint32_t rk = r, ck = c;
+#pragma unroll
+            for (int k = 0; k < kLookupUnits; ++k) {
+                const int64_t from = u0 + k * kThreads < total ? start[rk] : -1;
+                if (from >= 0) {
+                    load_vec<VEC>(table + from + ck * VEC, v[k]);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) v[j] = 0.0f;
+                    for (int j = 0; j < VEC; ++j) v[k][j] = 0.0f;
                 }
-            } else {
-                uint32_t rr = r, cc = c;
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const int32_t t = l + j < total ? row_of[rr] : -1;
-                    v[j] = t >= 0 ? to_float(table[t * a.table_stride + cc]) : 0.0f;
-                    if (++cc == dim) {
-                        cc = 0;
-                        ++rr;
-                    }
+                rk += step_r;
+                ck += step_c;
+                if (ck >= units) {
+                    ck -= units;
+                    ++rk;
                 }
             }
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[j] *= a.scale;
-            if (VSTORE && l + VEC <= total) {
-                if (VLOAD)
-                    store_vec<VEC>(out + (r0 + r) * a.out_stride + c, v);
-                else  // rows without gaps: out_stride == dim
-                    store_vec<VEC>(out + r0 * (int64_t)dim + l, v);
-            } else {
-                uint32_t rr = r, cc = c;
+            for (int k = 0; k < kLookupUnits; ++k) {
+                if (u0 + k * kThreads < total) {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    if (l + j < total) out[(r0 + rr) * a.out_stride + cc] = from_float<TO>(v[j]);
-                    if (++cc == dim) {
-                        cc = 0;
-                        ++rr;
-                    }
+                    for (int j = 0; j < VEC; ++j) v[k][j] *= a.scale;
+                    if (flat)
+                        store_vec<VEC>(to + (uint64_t)(u0 + k * kThreads) * VEC, v[k]);
+                    else
+                        store_vec<VEC>(to + r * a.out_stride + c * VEC, v[k]);
+                }
+                r += step_r;
+                c += step_c;
+                if (c >= units) {
+                    c -= units;
+                    ++r;
                 }
             }
         }
     }
 }
 
-template <typename TT, typename TO>
-hipError_t lookup_typed(const LookupArgs& a, hipStream_t st) {
-    constexpr int VEC = (sizeof(TT) == 2 && sizeof(TO) == 2) ? 8 : 4;
-    const int64_t want = (int64_t)kThreads * VEC * 4;
-    int64_t R = (want + a.dim - 1) / a.dim;
-    R = ((R + 7) / 8) * 8;
-    if (R > kLookupRows) R = kLookupRows;
+template <typename TT, typename TO, int VEC>
+hipError_t lookup_run(const LookupArgs& a, hipStream_t st) {
+    // about kLookupUnits units a thread, whole groups of 8 rows
+    const int64_t want = (int64_t)kThreads * kLookupUnits * VEC;
+    int64_t R = (want / a.dim + 7) / 8 * 8;
+    R = R < 8 ? 8 : (R > kLookupRows ? kLookupRows : R);
+    // fewer where that leaves compute units idle
+    while (R > 8 && a.n / R < 1024) R = R / 2 / 8 * 8 < 8 ? 8 : R / 2 / 8 * 8;
     const int64_t blocks = (a.n + R - 1) / R;
     const dim3 grid((unsigned)(blocks < (1 << 30) ? blocks : (1 << 30)));
-    const bool vload = a.dim % VEC == 0 && aligned_rows<TT>(a.table, a.table_stride, VEC) &&
-                       aligned_rows<TO>(a.out, a.out_stride, VEC);
-    const bool flat = a.out_stride == a.dim && aligned_rows<TO>(a.out, 0, VEC);
-    if (vload)
-        k_lookup<TT, TO, VEC, true, true><<<grid, kThreads, 0, st>>>(a, (int)R);
-    else if (flat)
-        k_lookup<TT, TO, VEC, false, true><<<grid, kThreads, 0, st>>>(a, (int)R);
-    else
-        k_lookup<TT, TO, VEC, false, false><<<grid, kThreads, 0, st>>>(a, (int)R);
+    k_lookup<TT, TO, VEC><<<grid, kThreads, 0, st>>>(a, (int)R);
     return hipGetLastError();
+}
+
+// The widest unit that divides a row and every row's address, on both sides.
+template <typename TT, typename TO>
+hipError_t lookup_typed(const LookupArgs& a, hipStream_t st) {
+    auto fits = [&](int v) {
+        return a.dim % v == 0 && aligned_rows<TT>(a.table, a.table_stride, v) &&
+               aligned_rows<TO>(a.out, a.out_stride, v);
+    };
+    if constexpr (sizeof(TT) == 2 && sizeof(TO) == 2)
+        if (fits(8)) return lookup_run<TT, TO, 8>(a, st);
+    if (fits(4)) return lookup_run<TT, TO, 4>(a, st);
+    if (fits(2)) return lookup_run<TT, TO, 2>(a, st);
+    return lookup_run<TT, TO, 1>(a, st);
 }
 
 // ---------------------------------------------------------------- sort
 // Stable LSD radix sort of (id, position), 8 bits a pass at most: per block the
-// digits' counts, per digit the blocks' offsets, then the scatter. Ids outside
-// the table get the key `rows` and end last.
-constexpr int kSortItems = 16;                      // keys of a thread
-constexpr int kSortTile = kThreads * kSortItems;    // keys of a workgroup
+// digits' counts, per digit the blocks' offsets, then the scatter. The first
+// pass reads the caller's ids; those outside the table get the key `rows` and
+// end last.
+__device__ __forceinline__ uint32_t sort_key(const LookupGradArgs& a, const uint32_t* keys,
+                                             int64_t i, uint32_t* flags) {
+    if (keys != nullptr) return keys[i];
+    const int32_t t = load_id(a.ids, a.ids64, i, a.rows, flags);
+    return t >= 0 ? (uint32_t)t : (uint32_t)a.rows;
+}
 
+// Rank of a wave's keys among its earlier ones of the same digit, 64 keys a call
+// in order: the lanes of equal digit are found with one ballot a bit; `seen` (LDS,
+// this wave's) counts each digit so far.
+__device__ __forceinline__ uint32_t wave_rank(uint32_t digit, bool on, int bits, uint32_t* seen) {
+    uint64_t same = __ballot(on);
+    for (int b = 0; b < bits; ++b) {
+        const uint64_t m = __ballot((digit >> b) & 1u);
+        same &= ((digit >> b) & 1u) ? m : ~m;
+    }
+    const uint32_t before = __popcll(same & ((1ull << (threadIdx.x & 63)) - 1ull));
+    volatile uint32_t* mine = seen + digit;  // other lanes of the wave write it
+    const uint32_t n = on ? *mine : 0u;
+    __builtin_amdgcn_wave_barrier();
+    if (on && before == 0) *mine = n + (uint32_t)__popcll(same);
+    __builtin_amdgcn_wave_barrier();
+    return n + before;
+}
+
+// Also clears the ids' runs, which k_run_sums fills in.
+template <int ITEMS>
 __global__ __launch_bounds__(kThreads) void k_sort_count(LookupGradArgs a, const uint32_t* keys,
-                                                         uint32_t* first, int shift, int bits,
-                                                         uint32_t* counts) {
+                                                         int shift, int bits, uint32_t* counts,
+                                                         uint2* runs) {
     __shared__ uint32_t hist[256];
     hist[threadIdx.x] = 0u;
     __syncthreads();
-    const int64_t base = (int64_t)blockIdx.x * kSortTile;
+    const int64_t base = (int64_t)blockIdx.x * (kThreads * ITEMS);
     const uint32_t mask = (1u << bits) - 1u;
-    for (int k = 0; k < kSortItems; ++k) {
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
         const int64_t i = base + k * kThreads + threadIdx.x;
-        if (i < a.n) {
-            uint32_t key;
-            if (first != nullptr) {  // the first pass reads the caller's ids
-                const int32_t t = load_id(a.ids, a.ids64, i, a.rows, a.flags);
-                key = t >= 0 ? (uint32_t)t : (uint32_t)a.rows;
-                first[i] = key;
-            } else {
-                key = keys[i];
-            }
-            atomicAdd(&hist[(key >> shift) & mask], 1u);
-        }
+        if (i < a.n) atomicAdd(&hist[(sort_key(a, keys, i, a.flags) >> shift) & mask], 1u);
     }
+    if (runs != nullptr)
+        for (int64_t v = (int64_t)blockIdx.x * kThreads + threadIdx.x; v < a.rows;
+             v += (int64_t)gridDim.x * kThreads)
+            runs[v] = make_uint2(0u, 0u);
     __syncthreads();
     if (threadIdx.x < (1u << bits))
         counts[(size_t)threadIdx.x * gridDim.x + blockIdx.x] = hist[threadIdx.x];
@@ -139,29 +173,33 @@ __global__ __launch_bounds__(kThreads) void k_sort_scan(uint32_t* counts, int bl
                                                         uint32_t* totals) {
     __shared__ uint32_t part[kThreads];
     uint32_t* row = counts + (size_t)blockIdx.x * blocks;
-    const int per = (blocks + kThreads - 1) / kThreads;
-    const int lo = min((int)threadIdx.x * per, blocks), hi = min(lo + per, blocks);
-    uint32_t sum = 0;
-    for (int i = lo; i < hi; ++i) sum += row[i];
-    uint32_t total;
-    uint32_t at = block_excl_scan<kThreads>(sum, part, &total);
-    for (int i = lo; i < hi; ++i) {
-        const uint32_t c = row[i];
-        row[i] = at;
-        at += c;
+    uint32_t base = 0;
+    for (int i0 = 0; i0 < blocks; i0 += kThreads * 4) {
+        uint32_t c[4], sum = 0;
+        const int i = i0 + threadIdx.x * 4;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            c[k] = i + k < blocks ? row[i + k] : 0u;
+            sum += c[k];
+        }
+        uint32_t total;
+        uint32_t at = base + block_excl_scan<kThreads>(sum, part, &total);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (i + k < blocks) row[i + k] = at;
+            at += c[k];
+        }
+        base += total;
     }
-    if (threadIdx.x == 0) totals[blockIdx.x] = total;
+    if (threadIdx.x == 0) totals[blockIdx.x] = base;
 }
 
-// A wave ranks its keys in order, 64 at a time: the lanes of equal digit are
-// found with one ballot per digit bit, and the wave's count of each digit so far
-// is kept in LDS.
-__global__ __launch_bounds__(kThreads) void k_sort_scatter(const uint32_t* keys,
-                                                           const uint32_t* vals, int64_t n,
-                                                           int shift, int bits,
-                                                           const uint32_t* counts,
-                                                           const uint32_t* totals, uint32_t* keys_o,
-                                                           uint32_t* vals_o) {
+template <int ITEMS>
+__global__ __launch_bounds__(kThreads) void k_sort_scatter(LookupGradArgs a, const uint32_t* keys,
+                                                           const uint32_t* vals, int shift,
+                                                           int bits, const uint32_t* counts,
+                                                           const uint32_t* totals,
+                                                           uint32_t* keys_o, uint32_t* vals_o) {
     constexpr int kWaves = kThreads / 64;
     __shared__ uint32_t cnt[kWaves][256];
     __shared__ uint32_t part[kThreads];
@@ -169,29 +207,18 @@ __global__ __launch_bounds__(kThreads) void k_sort_scatter(const uint32_t* keys,
     const int digits = 1 << bits;
     const uint32_t mask = digits - 1u;
     for (int k = 0; k < kWaves; ++k) cnt[k][t] = 0u;
-    __syncthreads();
-    const int64_t base = (int64_t)blockIdx.x * kSortTile + (int64_t)w * 64 * kSortItems;
-    uint32_t key[kSortItems], rank[kSortItems];
+    const int64_t base = (int64_t)blockIdx.x * (kThreads * ITEMS) + (int64_t)w * 64 * ITEMS;
+    uint32_t key[ITEMS], val[ITEMS], rank[ITEMS];
 #pragma unroll
-    for (int k = 0; k < kSortItems; ++k) {
+    for (int k = 0; k < ITEMS; ++k) {
         const int64_t i = base + k * 64 + lane;
-        const bool on = i < n;
-        key[k] = on ? keys[i] : 0u;
-        const uint32_t d = (key[k] >> shift) & mask;
-        uint64_t same = __ballot(on);
-        for (int b = 0; b < bits; ++b) {
-            const uint64_t m = __ballot((d >> b) & 1u);
-            same &= ((d >> b) & 1u) ? m : ~m;
-        }
-        const uint32_t before = __popcll(same & ((1ull << lane) - 1ull));
-        uint32_t seen = 0;
-        volatile uint32_t* mine = &cnt[w][d];  // other lanes of the wave write it
-        if (on) seen = *mine;
-        rank[k] = seen + before;
-        __builtin_amdgcn_wave_barrier();
-        if (on && before == 0) *mine = seen + (uint32_t)__popcll(same);
-        __builtin_amdgcn_wave_barrier();
+        key[k] = i < a.n ? sort_key(a, keys, i, nullptr) : 0u;
+        val[k] = i < a.n && vals != nullptr ? vals[i] : (uint32_t)i;
     }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+        rank[k] = wave_rank((key[k] >> shift) & mask, base + k * 64 + lane < a.n, bits, cnt[w]);
     __syncthreads();
     // digit starts: all smaller digits' totals, this block's offset, earlier waves
     const uint32_t mine = t < digits ? totals[t] : 0u;
@@ -207,149 +234,300 @@ __global__ __launch_bounds__(kThreads) void k_sort_scatter(const uint32_t* keys,
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kSortItems; ++k) {
-        const int64_t i = base + k * 64 + lane;
-        if (i < n) {
+    for (int k = 0; k < ITEMS; ++k)
+        if (base + k * 64 + lane < a.n) {
             const uint32_t to = cnt[w][(key[k] >> shift) & mask] + rank[k];
             keys_o[to] = key[k];
-            vals_o[to] = vals != nullptr ? vals[i] : (uint32_t)i;
+            vals_o[to] = val[k];
         }
-    }
-}
-
-// Run of every id in the sorted keys; [0, 0) for ids without one.
-__global__ __launch_bounds__(kThreads) void k_run_clear(uint2* runs, int64_t rows) {
-    const int64_t v = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (v < rows) runs[v] = make_uint2(0u, 0u);
-}
-__global__ __launch_bounds__(kThreads) void k_run_bounds(const uint32_t* keys, int64_t n,
-                                                         int64_t rows, uint2* runs) {
-    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (i >= n) return;
-    const uint32_t k = keys[i];
-    if (k >= (uint32_t)rows) return;
-    if (i == 0 || keys[i - 1] != k) runs[k].x = (uint32_t)i;
-    if (i == n - 1 || keys[i + 1] != k) runs[k].y = (uint32_t)(i + 1);
 }
 
 // ---------------------------------------------------------------- run sums
-// The sorted list is cut into stretches of S entries; a slot of LPR lanes sums
-// one, VEC columns a lane. A run inside one stretch is written at once; the
-// pieces of a longer one go to `part` (two rows a stretch: the run that holds
-// its first entry, and the last run) and k_run_join adds them in order.
+// A workgroup takes a span of (id, position) in id order, its slots of `lpr` lanes
+// (VEC columns a lane) equal stretches of it. Runs inside a stretch are finished
+// at once; each stretch's first and last run are joined over the slots in LDS,
+// in order.
+//
+// Two uses. Where ids have to be sorted over the whole list (LOCAL false), spans
+// follow that order: a run inside a span is a row's whole sum, and a span's first
+// and last run, where they go on in its neighbours, are added up by k_run_join
+// from `part` (span, 2, dim). With few rows (LOCAL) no such sort is needed: a span
+// is kLocal consecutive ids that the workgroup sorts itself, and each row's sum
+// over it goes to `part` (span, rows, dim). That reads dout almost in order, in 2
+// launches instead of 5.
+constexpr int kSpan = 1024;      // most entries of a span, and those of a LOCAL one
+constexpr int kLocalRows = 128;  // most rows for LOCAL: an eighth of the span
+
 template <typename TD, int VEC>
-__device__ __forceinline__ void put_row(TD* out, const float* acc, float scale, int accumulate,
-                                        int nvalid) {
+__device__ __forceinline__ void put_row(TD* out, const float* acc, float scale, int accumulate) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j)
-        if (j < nvalid) {
-            float s = acc[j] * scale;
-            if (accumulate) s += to_float(out[j]);
-            out[j] = from_float<TD>(s);
-        }
+    for (int j = 0; j < VEC; ++j) {
+        float s = acc[j] * scale;
+        if (accumulate) s += to_float(out[j]);
+        out[j] = from_float<TD>(s);
+    }
 }
 
-template <typename TI, typename TD, int VEC>
+template <typename TI, typename TD, int VEC, bool LOCAL>
 __global__ __launch_bounds__(kThreads) void k_run_sums(LookupGradArgs a, const uint32_t* keys,
-                                                       const uint32_t* pos, int S, int lpr,
-                                                       float* part) {
+                                                       const uint32_t* pos, int span, int lpr,
+                                                       int bits, float* part, uint2* runs) {
+    constexpr int kWaves = kThreads / 64;
+    constexpr uint32_t kNone = 0xFFFFFFFFu;
+    __shared__ uint32_t skey[kSpan], spos[kSpan];
+    __shared__ float ends[kThreads * 2 * VEC];  // (slot, first or last, column)
+    __shared__ uint32_t end_key[kThreads * 2];
     const TI* dout = static_cast<const TI*>(a.dout);
     TD* dtable = static_cast<TD*>(a.dtable);
-    const int slots = kThreads / lpr;
-    const int lane = threadIdx.x % lpr;
-    const int64_t s = (int64_t)blockIdx.x * slots + threadIdx.x / lpr;
-    const int c = (blockIdx.y * lpr + lane) * VEC;
-    const int64_t lo = s * S;
-    if (lo >= a.n || c >= a.dim) return;
-    const int64_t hi = min(lo + S, a.n);
-    const int nv = min(VEC, a.dim - c);
+    const int t = threadIdx.x, cols = lpr * VEC, c0 = blockIdx.y * cols;
+    const int slots = kThreads / lpr, slot = t / lpr, lane = t % lpr;
+    const int c = c0 + lane * VEC;
     const uint32_t rows = (uint32_t)a.rows;
+    const int64_t base = (int64_t)blockIdx.x * span;
+    const int m = (int)min((int64_t)span, a.n - base);
+    uint32_t before = kNone, after = kNone;  // the neighbours' keys
+    if (LOCAL) {
+        __shared__ uint32_t cnt[kWaves][kLocalRows + 1];
+        __shared__ uint32_t scan[kThreads];
+        for (int k = t; k < kWaves * (kLocalRows + 1); k += kThreads) (&cnt[0][0])[k] = 0u;
+        __syncthreads();
+        const int w = t >> 6, l = t & 63;
+        uint32_t key[kSpan / kThreads], rank[kSpan / kThreads];
+#pragma unroll
+        for (int k = 0; k < kSpan / kThreads; ++k) {
+            const int i = w * (kSpan / kWaves) + k * 64 + l;
+            key[k] = i < m ? sort_key(a, nullptr, base + i, blockIdx.y == 0 ? a.flags : nullptr) : 0u;
+            rank[k] = wave_rank(key[k], i < m, bits, cnt[w]);
+        }
+        __syncthreads();
+        uint32_t mine = 0, all;
+        if (t <= (int)rows)
+            for (int k = 0; k < kWaves; ++k) mine += cnt[k][t];
+        uint32_t at = block_excl_scan<kThreads>(mine, scan, &all);
+        if (t <= (int)rows)
+            for (int k = 0; k < kWaves; ++k) {
+                const uint32_t n = cnt[k][t];
+                cnt[k][t] = at;
+                at += n;
+            }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kSpan / kThreads; ++k) {
+            const int i = w * (kSpan / kWaves) + k * 64 + l;
+            if (i < m) {
+                const uint32_t to = cnt[w][key[k]] + rank[k];
+                skey[to] = key[k];
+                spos[to] = (uint32_t)(base + i);
+            }
+        }
+        __syncthreads();
+        // rows that no id of the span names
+        float* row0 = part + (size_t)blockIdx.x * rows * a.dim;
+        for (uint32_t v = slot; v < rows; v += slots) {
+            const uint32_t lo = cnt[0][v];
+            if (lo < (uint32_t)m && skey[lo] == v) continue;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (c + j < a.dim) row0[(size_t)v * a.dim + c + j] = 0.0f;
+        }
+    } else {
+        for (int i = t; i < m; i += kThreads) {
+            const uint32_t k = keys[base + i];
+            skey[i] = k;
+            spos[i] = pos[base + i];
+        }
+        if (base > 0) before = keys[base - 1];
+        if (base + m < a.n) after = keys[base + m];
+        __syncthreads();
+        if (blockIdx.y == 0)
+            for (int i = t; i < m; i += kThreads) {
+                const uint32_t k = skey[i];
+                if (k >= rows) continue;
+                if ((i > 0 ? skey[i - 1] : before) != k) runs[k].x = (uint32_t)(base + i);
+                if ((i + 1 < m ? skey[i + 1] : after) != k) runs[k].y = (uint32_t)(base + i + 1);
+            }
+    }
+    // a run's sum over the span; `which`: 0 it holds the span's first entry, 1 only
+    // its last, 2 neither
+    auto finish = [&](uint32_t key, const float* acc, int at, int which, auto width) {
+        constexpr int W = decltype(width)::value;
+        if (key >= rows) return;
+        if (LOCAL) {
+            float* p = part + ((size_t)blockIdx.x * rows + key) * a.dim + at;
+#pragma unroll
+            for (int j = 0; j < W; ++j) p[j] = acc[j];
+        } else if (which < 2) {
+            float* p = part + ((size_t)blockIdx.x * 2 + which) * a.dim + at;
+#pragma unroll
+            for (int j = 0; j < W; ++j) p[j] = acc[j];
+        } else {
+            put_row<TD, W>(dtable + (int64_t)key * a.dtable_stride + at, acc, a.scale,
+                           a.accumulate);
+        }
+    };
+
+    const int per = span / slots, lo = min(m, slot * per), hi = min(m, lo + per);
     float acc[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
-    uint32_t cur = keys[lo];
-    int64_t from = lo;
-    auto flush = [&](int64_t end) {
-        if (cur >= rows) return;
-        const bool starts = from > lo || lo == 0 || keys[lo - 1] != cur;
-        const bool ends = end < hi || hi == a.n || keys[hi] != cur;
-        if (starts && ends) {
-            put_row<TD, VEC>(dtable + (int64_t)cur * a.dtable_stride + c, acc, a.scale,
-                             a.accumulate, nv);
-        } else {
-            float* p = part + ((size_t)s * 2 + (from == lo ? 0 : 1)) * a.dim + c;
+    uint32_t cur = lo < hi ? skey[lo] : kNone, first = cur;
+    bool single = true;
+    const bool col_on = c < a.dim;
+    constexpr int U = 8;  // rows in flight
+    for (int i0 = lo; i0 < hi; i0 += U) {
+        float v[U][VEC];
+        uint32_t k[U];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                if (j < nv) p[j] = acc[j];
-        }
-    };
-    for (int64_t i = lo; i < hi; ++i) {
-        const uint32_t k = keys[i];
-        if (k != cur) {
-            flush(i);
-            cur = k;
-            from = i;
+        for (int u = 0; u < U; ++u) {
+            k[u] = i0 + u < hi ? skey[i0 + u] : kNone;
+            if (k[u] < rows && col_on) {
+                load_vec<VEC>(dout + (int64_t)spos[i0 + u] * a.dout_stride + c, v[u]);
+            } else {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
-        }
-        if (k >= rows) break;
-        const TI* src = dout + (int64_t)pos[i] * a.dout_stride + c;
-        float v[VEC];
-        if (nv == VEC && VEC > 1) {
-            load_vec<VEC>(src, v);
-        } else {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) v[j] = j < nv ? to_float(src[j]) : 0.0f;
+                for (int j = 0; j < VEC; ++j) v[u][j] = 0.0f;
+            }
         }
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) acc[j] += v[j];
+        for (int u = 0; u < U; ++u) {
+            if (k[u] == kNone) continue;
+            if (k[u] != cur) {
+                if (single) {
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) ends[(slot * 2) * cols + lane * VEC + j] = acc[j];
+                    single = false;
+                } else if (col_on) {
+                    finish(cur, acc, c, 2, std::integral_constant<int, VEC>());
+                }
+                cur = k[u];
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) acc[j] += v[u][j];
+        }
     }
-    flush(hi);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+        ends[(slot * 2 + (single ? 0 : 1)) * cols + lane * VEC + j] = acc[j];
+    if (lane == 0) {
+        end_key[slot * 2] = first;
+        end_key[slot * 2 + 1] = single ? kNone : cur;
+    }
+    __syncthreads();
+    for (int j = t; j < cols && c0 + j < a.dim; j += kThreads) {
+        uint32_t key = end_key[0];
+        const uint32_t span_first = key;
+        float sum = 0.0f;
+        bool begin = true;  // the run holds the span's first entry
+        for (int e = 0; e < slots * 2; ++e) {
+            const uint32_t k = end_key[e];
+            if (k == kNone) continue;
+            if (k != key) {
+                finish(key, &sum, c0 + j, begin && before == span_first ? 0 : 2,
+                       std::integral_constant<int, 1>());
+                begin = false;
+                key = k;
+                sum = 0.0f;
+            }
+            sum += ends[e * cols + j];
+        }
+        const bool more = after == key;
+        const int which = begin ? (before == span_first || more ? 0 : 2) : (more ? 1 : 2);
+        finish(key, &sum, c0 + j, which, std::integral_constant<int, 1>());
+    }
 }
 
-// One workgroup per table row: zeros for a row no id names, the sum of the
-// pieces for a run of several stretches (each slot of lanes adds every slots-th
-// piece, then the slots' sums are added in order).
+// Rows whose run crosses spans: the sum of the spans' pieces in order; zeros for
+// rows that no id names. A wave a row; a row of many pieces takes the workgroup,
+// each wave every fourth piece.
+constexpr int kWavePieces = 32;
+
 template <typename TD>
-__global__ __launch_bounds__(kThreads) void k_run_join(LookupGradArgs a, const uint2* runs, int S,
-                                                       const float* part) {
+__global__ __launch_bounds__(kThreads) void k_run_join(LookupGradArgs a, const uint2* runs,
+                                                       int span, const float* part) {
     __shared__ float sums[kThreads];
     TD* dtable = static_cast<TD*>(a.dtable);
-    for (int64_t v = blockIdx.x; v < a.rows; v += gridDim.x) {
-        const uint2 run = runs[v];
-        TD* out = dtable + v * a.dtable_stride;
-        if (run.x == run.y) {
-            if (!a.accumulate)
-                for (int c = threadIdx.x; c < a.dim; c += kThreads) out[c] = from_float<TD>(0.0f);
-            continue;
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    // sum of pieces s0 + k, s0 + k + by, .. of column c
+    auto pieces = [&](uint2 run, uint32_t k, uint32_t by, int c) {
+        const uint32_t s0 = run.x / (uint32_t)span, s1 = (run.y - 1u) / (uint32_t)span;
+        float acc = 0.0f;
+        for (uint32_t s = s0 + k; s <= s1; s += by * 4) {
+            float v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const uint32_t q = s + u * by;
+                const int which = q == s0 && run.x % (uint32_t)span != 0u ? 1 : 0;
+                v[u] = q <= s1 ? part[((size_t)q * 2 + which) * a.dim + c] : 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) acc += v[u];
         }
-        const uint32_t s0 = run.x / (uint32_t)S, s1 = (run.y - 1u) / (uint32_t)S;
-        if (s0 == s1) continue;
-        const int w = min(a.dim, kThreads), slots = kThreads / w;
-        const int slot = threadIdx.x / w, lane = threadIdx.x % w;
-        for (int c0 = 0; c0 < a.dim; c0 += w) {
-            const int c = c0 + lane;
-            float acc = 0.0f;
-            if (slot < slots && c < a.dim)
-                for (uint32_t s = s0 + slot; s <= s1; s += slots) {
-                    const int which = s == s0 && run.x % (uint32_t)S != 0u ? 1 : 0;
-                    acc += part[((size_t)s * 2 + which) * a.dim + c];
+        return acc;
+    };
+    auto count = [&](uint2 run) {
+        return run.x == run.y ? 0u : (run.y - 1u) / (uint32_t)span - run.x / (uint32_t)span + 1u;
+    };
+    for (int64_t v0 = (int64_t)blockIdx.x * 4; v0 < a.rows; v0 += (int64_t)gridDim.x * 4) {
+        const int64_t v = v0 + w;
+        if (v < a.rows) {
+            const uint2 run = runs[v];
+            const uint32_t n = count(run);
+            TD* out = dtable + v * a.dtable_stride;
+            if (n == 0 && !a.accumulate)
+                for (int c = lane; c < a.dim; c += 64) out[c] = from_float<TD>(0.0f);
+            if (n > 1 && n <= kWavePieces)
+                for (int c = lane; c < a.dim; c += 64) {
+                    const float acc = pieces(run, 0, 1, c);
+                    put_row<TD, 1>(out + c, &acc, a.scale, a.accumulate);
                 }
-            __syncthreads();
-            sums[threadIdx.x] = acc;
-            __syncthreads();
-            if (slot == 0 && c < a.dim) {
-                for (int k = 1; k < slots; ++k) acc += sums[k * w + lane];
-                put_row<TD, 1>(out + c, &acc, a.scale, a.accumulate, 1);
+        }
+        for (int k = 0; k < 4 && v0 + k < a.rows; ++k) {
+            const uint2 run = runs[v0 + k];
+            if (count(run) <= kWavePieces) continue;
+            for (int cb = 0; cb < a.dim; cb += 64) {
+                const int c = cb + lane;
+                float acc = c < a.dim ? pieces(run, w, kThreads / 64, c) : 0.0f;
+                __syncthreads();
+                sums[threadIdx.x] = acc;
+                __syncthreads();
+                if (w == 0 && c < a.dim) {
+                    for (int q = 1; q < kThreads / 64; ++q) acc += sums[q * 64 + lane];
+                    put_row<TD, 1>(dtable + (v0 + k) * a.dtable_stride + c, &acc, a.scale,
+                                   a.accumulate);
+                }
             }
         }
     }
 }
 
-int stretch_of(int64_t n) {
-    int S = 16;
-    while (S < 1024 && n / S > 16384) S *= 2;
-    return S;
+// LOCAL's join: a workgroup per row and 16 columns, 16 slots over the spans.
+template <typename TD>
+__global__ __launch_bounds__(kThreads) void k_local_join(LookupGradArgs a, int spans,
+                                                         const float* part) {
+    __shared__ float sums[16][17];
+    const int slot = threadIdx.x >> 4, j = threadIdx.x & 15;
+    const int64_t v = blockIdx.x;
+    const int c = blockIdx.y * 16 + j;
+    float acc = 0.0f;
+    if (c < a.dim)
+        for (int s0 = slot; s0 < spans; s0 += 16 * 8) {
+            float x[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int s = s0 + u * 16;
+                x[u] = s < spans ? part[((size_t)s * a.rows + v) * a.dim + c] : 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) acc += x[u];
+        }
+    sums[slot][j] = acc;
+    __syncthreads();
+    if (slot == 0 && c < a.dim) {
+        for (int q = 1; q < 16; ++q) acc += sums[q][j];
+        put_row<TD, 1>(static_cast<TD*>(a.dtable) + v * a.dtable_stride + c, &acc, a.scale,
+                       a.accumulate);
+    }
 }
 
 int key_bits(int64_t rows) {  // keys 0 .. rows
@@ -358,6 +536,19 @@ int key_bits(int64_t rows) {  // keys 0 .. rows
     return b;
 }
 
+bool is_local(int64_t n, int64_t rows) { return rows <= kLocalRows && n > 0; }
+
+// Entries of a span of the sorted list: at most 4096 spans while spans can grow,
+// so that one row's pieces stay few.
+int span_of(int64_t n) {
+    int s = 256;
+    while (s < kSpan && n / s > 4096) s *= 2;
+    return s;
+}
+
+// Keys of a sort block's thread: fewer where that fills the chip.
+int sort_items(int64_t n) { return n <= (1 << 21) ? 4 : 16; }
+
 struct GradWs {
     uint32_t *key[2], *val[2], *counts, *totals;
     uint2* runs;
@@ -365,42 +556,83 @@ struct GradWs {
     size_t bytes;
     GradWs(void* base, int64_t n, int64_t rows, int dim) {
         Carve c(base);
-        const size_t blocks = (size_t)((n + kSortTile - 1) / kSortTile);
-        for (int k = 0; k < 2; ++k) {
-            key[k] = c.take<uint32_t>((size_t)n);
-            val[k] = c.take<uint32_t>((size_t)n);
+        if (is_local(n, rows)) {
+            part = c.take<float>((size_t)((n + kSpan - 1) / kSpan) * rows * dim);
+        } else {
+            const int64_t tile = (int64_t)kThreads * sort_items(n);
+            for (int k = 0; k < 2; ++k) {
+                key[k] = c.take<uint32_t>((size_t)n);
+                val[k] = c.take<uint32_t>((size_t)n);
+            }
+            counts = c.take<uint32_t>((size_t)((n + tile - 1) / tile) * 256);
+            totals = c.take<uint32_t>(256);
+            runs = c.take<uint2>((size_t)rows);
+            const int span = span_of(n);
+            part = c.take<float>((size_t)((n + span - 1) / span) * 2 * dim);
         }
-        counts = c.take<uint32_t>(blocks * 256);
-        totals = c.take<uint32_t>(256);
-        runs = c.take<uint2>((size_t)rows);
-        const int S = stretch_of(n);
-        part = c.take<float>((size_t)((n + S - 1) / S) * 2 * dim);
         bytes = c.bytes();
     }
 };
+
+template <typename TI, typename TD, int VEC>
+hipError_t grad_run(const LookupGradArgs& a, const GradWs& w, const uint32_t* keys,
+                    const uint32_t* vals, hipStream_t st) {
+    const int units = (a.dim + VEC - 1) / VEC;
+    int lpr = 1;
+    while (lpr < 64 && lpr < units) lpr *= 2;
+    const unsigned cols = (unsigned)((units + lpr - 1) / lpr);
+    if (is_local(a.n, a.rows)) {
+        const int spans = (int)((a.n + kSpan - 1) / kSpan);
+        k_run_sums<TI, TD, VEC, true><<<dim3((unsigned)spans, cols), kThreads, 0, st>>>(
+            a, nullptr, nullptr, kSpan, lpr, key_bits(a.rows), w.part, nullptr);
+        k_local_join<TD><<<dim3((unsigned)a.rows, (unsigned)((a.dim + 15) / 16)), kThreads, 0, st>>>(
+            a, spans, w.part);
+        return hipGetLastError();
+    }
+    const int span = span_of(a.n);
+    if (a.n > 0)
+        k_run_sums<TI, TD, VEC, false>
+            <<<dim3((unsigned)((a.n + span - 1) / span), cols), kThreads, 0, st>>>(
+                a, keys, vals, span, lpr, 0, w.part, w.runs);
+    const int64_t joins = (a.rows + 3) / 4;
+    k_run_join<TD><<<(unsigned)(joins < 65536 ? joins : 65536), kThreads, 0, st>>>(a, w.runs, span,
+                                                                                w.part);
+    return hipGetLastError();
+}
 
 template <typename TI, typename TD>
 hipError_t grad_typed(const LookupGradArgs& a, const GradWs& w, const uint32_t* keys,
                       const uint32_t* vals, hipStream_t st) {
     constexpr int VEC = 16 / sizeof(TI);
-    const int S = stretch_of(a.n);
-    const bool vec = a.dim % VEC == 0 && aligned_rows<TI>(a.dout, a.dout_stride, VEC);
-    const int cols = vec ? a.dim / VEC : a.dim;
-    int lpr = 1;
-    while (lpr < 64 && lpr < cols) lpr *= 2;
-    const int64_t stretches = (a.n + S - 1) / S;
-    const int slots = kThreads / lpr;
-    if (stretches > 0) {
-        const dim3 grid((unsigned)((stretches + slots - 1) / slots),
-                        (unsigned)((cols + lpr - 1) / lpr));
-        if (vec)
-            k_run_sums<TI, TD, VEC><<<grid, kThreads, 0, st>>>(a, keys, vals, S, lpr, w.part);
-        else
-            k_run_sums<TI, TD, 1><<<grid, kThreads, 0, st>>>(a, keys, vals, S, lpr, w.part);
+    if (a.dim % VEC == 0 && aligned_rows<TI>(a.dout, a.dout_stride, VEC))
+        return grad_run<TI, TD, VEC>(a, w, keys, vals, st);
+    if (a.dim % 2 == 0 && aligned_rows<TI>(a.dout, a.dout_stride, 2))
+        return grad_run<TI, TD, 2>(a, w, keys, vals, st);
+    return grad_run<TI, TD, 1>(a, w, keys, vals, st);
+}
+
+template <int ITEMS>
+void sort_ids(const LookupGradArgs& a, const GradWs& w, const uint32_t** keys,
+              const uint32_t** vals, hipStream_t st) {
+    const int bits = key_bits(a.rows), passes = (bits + 7) / 8;
+    const unsigned blocks = (unsigned)((a.n + kThreads * ITEMS - 1) / (kThreads * ITEMS));
+    *keys = *vals = nullptr;
+    for (int p = 0, done = 0; p < passes; ++p) {
+        const int b = (bits - done + passes - p - 1) / (passes - p);
+        k_sort_count<ITEMS><<<blocks, kThreads, 0, st>>>(a, *keys, done, b, w.counts,
+                                                         p == 0 ? w.runs : nullptr);
+        k_sort_scan<<<1u << b, kThreads, 0, st>>>(w.counts, (int)blocks, w.totals);
+        k_sort_scatter<ITEMS><<<blocks, kThreads, 0, st>>>(a, *keys, *vals, done, b, w.counts,
+                                                           w.totals, w.key[p & 1], w.val[p & 1]);
+        *keys = w.key[p & 1];
+        *vals = w.val[p & 1];
+        done += b;
     }
-    const unsigned joins = (unsigned)(a.rows < 65536 ? a.rows : 65536);
-    k_run_join<TD><<<joins, kThreads, 0, st>>>(a, w.runs, S, w.part);
-    return hipGetLastError();
+}
+
+__global__ __launch_bounds__(kThreads) void k_run_clear(uint2* runs, int64_t rows) {
+    const int64_t v = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (v < rows) runs[v] = make_uint2(0u, 0u);
 }
 
 }  // namespace
@@ -419,27 +651,17 @@ size_t lookup_grad_ws(int64_t n, int64_t rows, int dim) {
 
 hipError_t launch_lookup_grad(const LookupGradArgs& a, hipStream_t st) {
     if (a.rows == 0) return hipSuccess;
-    GradWs w(a.ws, a.n, a.rows, a.dim);
-    const int bits = key_bits(a.rows), passes = (bits + 7) / 8;
-    const unsigned blocks = (unsigned)((a.n + kSortTile - 1) / kSortTile);
-    const uint32_t *keys = w.key[0], *vals = nullptr;
-    int cur = 0, done = 0;
-    for (int p = 0; p < passes && a.n > 0; ++p) {
-        const int b = (bits - done + passes - p - 1) / (passes - p);
-        k_sort_count<<<blocks, kThreads, 0, st>>>(a, keys, p == 0 ? w.key[0] : nullptr, done, b,
-                                                  w.counts);
-        k_sort_scan<<<1u << b, kThreads, 0, st>>>(w.counts, (int)blocks, w.totals);
-        k_sort_scatter<<<blocks, kThreads, 0, st>>>(keys, vals, a.n, done, b, w.counts, w.totals,
-                                                    w.key[cur ^ 1], w.val[cur ^ 1]);
-        cur ^= 1;
-        keys = w.key[cur];
-        vals = w.val[cur];
-        done += b;
+    const GradWs w(a.ws, a.n, a.rows, a.dim);
+    const uint32_t *keys = nullptr, *vals = nullptr;
+    if (a.n == 0) {
+        k_run_clear<<<(unsigned)((a.rows + kThreads - 1) / kThreads), kThreads, 0, st>>>(w.runs,
+                                                                                      a.rows);
+    } else if (!is_local(a.n, a.rows)) {
+        if (sort_items(a.n) == 4)
+            sort_ids<4>(a, w, &keys, &vals, st);
+        else
+            sort_ids<16>(a, w, &keys, &vals, st);
     }
-    k_run_clear<<<(unsigned)((a.rows + kThreads - 1) / kThreads), kThreads, 0, st>>>(w.runs, a.rows);
-    if (a.n > 0)
-        k_run_bounds<<<(unsigned)((a.n + kThreads - 1) / kThreads), kThreads, 0, st>>>(
-            keys, a.n, a.rows, w.runs);
     if (a.dout_dtype == 0)
         return a.dtable_dtype == 0 ? grad_typed<float, float>(a, w, keys, vals, st)
                                    : grad_typed<float, bf16>(a, w, keys, vals, st);
