@@ -29,6 +29,14 @@ __device__ __forceinline__ void load_vec(const T* p, float* out) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) out[j] = to_float(u.v[j]);
 }
+// The same at any address of a T.
+template <int VEC, typename T>
+__device__ __forceinline__ void load_any(const T* p, float* out) {
+    T u[VEC];
+    __builtin_memcpy(u, p, sizeof(u));
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) out[j] = to_float(u[j]);
+}
 template <int VEC, typename T>
 __device__ __forceinline__ void store_vec(T* p, const float* in) {
     VecOf<T, VEC> u;
@@ -70,21 +78,28 @@ __device__ __forceinline__ int32_t load_id(const void* ids, int ids64, int64_t i
     return v < 0 ? -1 : (int32_t)v;
 }
 
-// Exclusive prefix of one value per thread over the workgroup, and the total.
+// Exclusive prefix of one value per thread over the workgroup, and the total; lds:
+// a word per wave.
 template <int THREADS>
 __device__ __forceinline__ uint32_t block_excl_scan(uint32_t v, uint32_t* lds, uint32_t* total) {
-    const int t = threadIdx.x;
-    __syncthreads();
-    lds[t] = v;
-    __syncthreads();
-    for (int o = 1; o < THREADS; o <<= 1) {
-        const uint32_t u = t >= o ? lds[t - o] : 0u;
-        __syncthreads();
-        lds[t] += u;
-        __syncthreads();
+    const int t = threadIdx.x, lane = t & 63;
+    uint32_t s = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t u = __shfl_up(s, o, 64);
+        if (lane >= o) s += u;
     }
-    *total = lds[THREADS - 1];
-    return lds[t] - v;
+    __syncthreads();
+    if (lane == 63) lds[t >> 6] = s;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+#pragma unroll
+    for (int k = 0; k < THREADS / 64; ++k) {
+        if (k == (t >> 6)) before = all;
+        all += lds[k];
+    }
+    *total = all;
+    return before + s - v;
 }
 
 // Consecutive 256-byte aligned arrays of a workspace; a null base only counts.

@@ -24,17 +24,21 @@ constexpr int kThreads = 256;
 // and writes of a wave are contiguous whatever the row length. A thread's next
 // unit lies kThreads further: its row and column follow by addition, where a
 // division a unit took longer than the memory.
+//
+// FLAT: the output has no gaps, so a unit is 16 aligned bytes of it whatever the
+// row length, read in one (unaligned) load; only the units that hold a row's end
+// are read value by value. Else a unit is a divisor of a row. Outputs are stored
+// past the caches, which are left to the table.
 constexpr int kLookupRows = 1024;  // most ids of a workgroup
-constexpr int kLookupUnits = 8;    // units that a thread loads before it stores
+constexpr int kLookupUnits = 4;    // units that a thread loads before it stores
 
-template <typename TT, typename TO, int VEC>
+template <typename TT, typename TO, int VEC, bool FLAT>
 __global__ __launch_bounds__(kThreads) void k_lookup(LookupArgs a, int R) {
     __shared__ int64_t start[kLookupRows];
     const TT* table = static_cast<const TT*>(a.table);
     TO* out = static_cast<TO*>(a.out);
-    const uint32_t units = (uint32_t)a.dim / VEC;
-    const uint32_t step_r = kThreads / units, step_c = kThreads % units;
-    const bool flat = a.out_stride == a.dim;
+    const uint32_t dim = (uint32_t)a.dim;
+    const uint32_t step_r = kThreads * VEC / dim, step_c = kThreads * VEC % dim;
     for (int64_t r0 = (int64_t)blockIdx.x * R; r0 < a.n; r0 += (int64_t)gridDim.x * R) {
         const int nr = (int)min((int64_t)R, a.n - r0);
         __syncthreads();
@@ -43,42 +47,62 @@ __global__ __launch_bounds__(kThreads) void k_lookup(LookupArgs a, int R) {
             start[i] = t >= 0 ? t * a.table_stride : -1;
         }
         __syncthreads();
-        uint32_t r = threadIdx.x / units, c = threadIdx.x % units;
-        const uint32_t total = (uint32_t)nr * units;
+        uint32_t r = threadIdx.x * VEC / dim, c = threadIdx.x * VEC % dim;
+        const uint32_t total = (uint32_t)nr * dim;
         TO* to = out + r0 * a.out_stride;
-        for (uint32_t u0 = threadIdx.x; u0 < total; u0 += kThreads * kLookupUnits) {
+        for (uint32_t e0 = threadIdx.x * VEC; e0 < total; e0 += kThreads * kLookupUnits * VEC) {
             float v[kLookupUnits][VEC];
             uint32_t rk = r, ck = c;
 #pragma unroll
             for (int k = 0; k < kLookupUnits; ++k) {
-                const int64_t from = u0 + k * kThreads < total ? start[rk] : -1;
-                if (from >= 0) {
-                    load_vec<VEC>(table + from + ck * VEC, v[k]);
-                } else {
+                const uint32_t e = e0 + k * kThreads * VEC;
+                if (!FLAT || ck + VEC <= dim) {
+                    const int64_t from = e < total ? start[rk] : -1;
+                    if (from >= 0) {
+                        load_any<VEC>(table + from + ck, v[k]);
+                    } else {
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) v[k][j] = 0.0f;
+                        for (int j = 0; j < VEC; ++j) v[k][j] = 0.0f;
+                    }
+                } else {
+                    uint32_t rj = rk, cj = ck;
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) {
+                        const int64_t from = e + j < total ? start[rj] : -1;
+                        v[k][j] = from >= 0 ? to_float(table[from + cj]) : 0.0f;
+                        if (++cj == dim) {
+                            cj = 0;
+                            ++rj;
+                        }
+                    }
                 }
                 rk += step_r;
                 ck += step_c;
-                if (ck >= units) {
-                    ck -= units;
+                if (ck >= dim) {
+                    ck -= dim;
                     ++rk;
                 }
             }
 #pragma unroll
             for (int k = 0; k < kLookupUnits; ++k) {
-                if (u0 + k * kThreads < total) {
+                const uint32_t e = e0 + k * kThreads * VEC;
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) v[k][j] *= a.scale;
-                    if (flat)
-                        store_vec<VEC>(to + (uint64_t)(u0 + k * kThreads) * VEC, v[k]);
-                    else
-                        store_vec<VEC>(to + r * a.out_stride + c * VEC, v[k]);
+                for (int j = 0; j < VEC; ++j) v[k][j] *= a.scale;
+                if (FLAT) {
+                    if (e + VEC <= total) {
+                        store_nt<VEC>(to + e, v[k]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j)
+                            if (e + j < total) to[e + j] = from_float<TO>(v[k][j]);
+                    }
+                } else if (e < total) {
+                    store_nt<VEC>(to + r * a.out_stride + c, v[k]);
                 }
                 r += step_r;
                 c += step_c;
-                if (c >= units) {
-                    c -= units;
+                if (c >= dim) {
+                    c -= dim;
                     ++r;
                 }
             }
@@ -86,9 +110,9 @@ __global__ __launch_bounds__(kThreads) void k_lookup(LookupArgs a, int R) {
     }
 }
 
-template <typename TT, typename TO, int VEC>
+template <typename TT, typename TO, int VEC, bool FLAT>
 hipError_t lookup_run(const LookupArgs& a, hipStream_t st) {
-    // about kLookupUnits units a thread, whole groups of 8 rows
+    // about kLookupUnits units a thread, whole groups of 8 rows (16-byte multiples)
     const int64_t want = (int64_t)kThreads * kLookupUnits * VEC;
     int64_t R = (want / a.dim + 7) / 8 * 8;
     R = R < 8 ? 8 : (R > kLookupRows ? kLookupRows : R);
@@ -96,22 +120,21 @@ hipError_t lookup_run(const LookupArgs& a, hipStream_t st) {
     while (R > 8 && a.n / R < 1024) R = R / 2 / 8 * 8 < 8 ? 8 : R / 2 / 8 * 8;
     const int64_t blocks = (a.n + R - 1) / R;
     const dim3 grid((unsigned)(blocks < (1 << 30) ? blocks : (1 << 30)));
-    k_lookup<TT, TO, VEC><<<grid, kThreads, 0, st>>>(a, (int)R);
+    k_lookup<TT, TO, VEC, FLAT><<<grid, kThreads, 0, st>>>(a, (int)R);
     return hipGetLastError();
 }
 
-// The widest unit that divides a row and every row's address, on both sides.
+// Gapless aligned outputs by 16 bytes; else the widest unit that divides a row and
+// every output row's address.
 template <typename TT, typename TO>
 hipError_t lookup_typed(const LookupArgs& a, hipStream_t st) {
-    auto fits = [&](int v) {
-        return a.dim % v == 0 && aligned_rows<TT>(a.table, a.table_stride, v) &&
-               aligned_rows<TO>(a.out, a.out_stride, v);
-    };
-    if constexpr (sizeof(TT) == 2 && sizeof(TO) == 2)
-        if (fits(8)) return lookup_run<TT, TO, 8>(a, st);
-    if (fits(4)) return lookup_run<TT, TO, 4>(a, st);
-    if (fits(2)) return lookup_run<TT, TO, 2>(a, st);
-    return lookup_run<TT, TO, 1>(a, st);
+    constexpr int VEC = 16 / sizeof(TO);
+    if ((a.out_stride == a.dim || a.n == 1) && aligned_rows<TO>(a.out, 0, VEC))
+        return lookup_run<TT, TO, VEC, true>(a, st);
+    auto fits = [&](int v) { return a.dim % v == 0 && aligned_rows<TO>(a.out, a.out_stride, v); };
+    if (fits(4)) return lookup_run<TT, TO, 4, false>(a, st);
+    if (fits(2)) return lookup_run<TT, TO, 2, false>(a, st);
+    return lookup_run<TT, TO, 1, false>(a, st);
 }
 
 // ---------------------------------------------------------------- sort
@@ -119,9 +142,9 @@ hipError_t lookup_typed(const LookupArgs& a, hipStream_t st) {
 // digits' counts, per digit the blocks' offsets, then the scatter. The first
 // pass reads the caller's ids; those outside the table get the key `rows` and
 // end last.
-__device__ __forceinline__ uint32_t sort_key(const LookupGradArgs& a, const uint32_t* keys,
+__device__ __forceinline__ uint32_t sort_key(const LookupGradArgs& a, const uint2* pairs,
                                              int64_t i, uint32_t* flags) {
-    if (keys != nullptr) return keys[i];
+    if (pairs != nullptr) return pairs[i].x;
     const int32_t t = load_id(a.ids, a.ids64, i, a.rows, flags);
     return t >= 0 ? (uint32_t)t : (uint32_t)a.rows;
 }
@@ -146,7 +169,7 @@ __device__ __forceinline__ uint32_t wave_rank(uint32_t digit, bool on, int bits,
 
 // Also clears the ids' runs, which k_run_sums fills in.
 template <int ITEMS>
-__global__ __launch_bounds__(kThreads) void k_sort_count(LookupGradArgs a, const uint32_t* keys,
+__global__ __launch_bounds__(kThreads) void k_sort_count(LookupGradArgs a, const uint2* pairs,
                                                          int shift, int bits, uint32_t* counts,
                                                          uint2* runs) {
     __shared__ uint32_t hist[256];
@@ -157,7 +180,7 @@ __global__ __launch_bounds__(kThreads) void k_sort_count(LookupGradArgs a, const
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
         const int64_t i = base + k * kThreads + threadIdx.x;
-        if (i < a.n) atomicAdd(&hist[(sort_key(a, keys, i, a.flags) >> shift) & mask], 1u);
+        if (i < a.n) atomicAdd(&hist[(sort_key(a, pairs, i, a.flags) >> shift) & mask], 1u);
     }
     if (runs != nullptr)
         for (int64_t v = (int64_t)blockIdx.x * kThreads + threadIdx.x; v < a.rows;
@@ -171,7 +194,7 @@ __global__ __launch_bounds__(kThreads) void k_sort_count(LookupGradArgs a, const
 // One workgroup per digit: exclusive prefix of its blocks' counts, and its total.
 __global__ __launch_bounds__(kThreads) void k_sort_scan(uint32_t* counts, int blocks,
                                                         uint32_t* totals) {
-    __shared__ uint32_t part[kThreads];
+    __shared__ uint32_t part[kThreads / 64];
     uint32_t* row = counts + (size_t)blockIdx.x * blocks;
     uint32_t base = 0;
     for (int i0 = 0; i0 < blocks; i0 += kThreads * 4) {
@@ -195,51 +218,51 @@ __global__ __launch_bounds__(kThreads) void k_sort_scan(uint32_t* counts, int bl
 }
 
 template <int ITEMS>
-__global__ __launch_bounds__(kThreads) void k_sort_scatter(LookupGradArgs a, const uint32_t* keys,
-                                                           const uint32_t* vals, int shift,
-                                                           int bits, const uint32_t* counts,
-                                                           const uint32_t* totals,
-                                                           uint32_t* keys_o, uint32_t* vals_o) {
+__global__ __launch_bounds__(kThreads) void k_sort_scatter(LookupGradArgs a, const uint2* pairs,
+                                                           int shift, int bits,
+                                                           const uint32_t* counts,
+                                                           const uint32_t* totals, uint2* out) {
     constexpr int kWaves = kThreads / 64;
     __shared__ uint32_t cnt[kWaves][256];
-    __shared__ uint32_t part[kThreads];
+    __shared__ uint32_t part[kWaves];
     const int t = threadIdx.x, w = t >> 6, lane = t & 63;
     const int digits = 1 << bits;
     const uint32_t mask = digits - 1u;
+    const uint32_t mine = t < digits ? totals[t] : 0u;
+    const uint32_t offset = t < digits ? counts[(size_t)t * gridDim.x + blockIdx.x] : 0u;
     for (int k = 0; k < kWaves; ++k) cnt[k][t] = 0u;
     const int64_t base = (int64_t)blockIdx.x * (kThreads * ITEMS) + (int64_t)w * 64 * ITEMS;
-    uint32_t key[ITEMS], val[ITEMS], rank[ITEMS];
+    uint2 pair[ITEMS];
+    uint32_t rank[ITEMS];
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
         const int64_t i = base + k * 64 + lane;
-        key[k] = i < a.n ? sort_key(a, keys, i, nullptr) : 0u;
-        val[k] = i < a.n && vals != nullptr ? vals[i] : (uint32_t)i;
+        pair[k] = make_uint2(0u, (uint32_t)i);
+        if (i < a.n) {
+            if (pairs != nullptr)
+                pair[k] = pairs[i];
+            else
+                pair[k].x = sort_key(a, nullptr, i, nullptr);
+        }
     }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k)
-        rank[k] = wave_rank((key[k] >> shift) & mask, base + k * 64 + lane < a.n, bits, cnt[w]);
-    __syncthreads();
+        rank[k] = wave_rank((pair[k].x >> shift) & mask, base + k * 64 + lane < a.n, bits, cnt[w]);
     // digit starts: all smaller digits' totals, this block's offset, earlier waves
-    const uint32_t mine = t < digits ? totals[t] : 0u;
     uint32_t all;
-    uint32_t at = block_excl_scan<kThreads>(mine, part, &all);
-    if (t < digits) {
-        at += counts[(size_t)t * gridDim.x + blockIdx.x];
+    uint32_t at = block_excl_scan<kThreads>(mine, part, &all) + offset;
+    if (t < digits)
         for (int k = 0; k < kWaves; ++k) {
             const uint32_t c = cnt[k][t];
             cnt[k][t] = at;
             at += c;
         }
-    }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k)
-        if (base + k * 64 + lane < a.n) {
-            const uint32_t to = cnt[w][(key[k] >> shift) & mask] + rank[k];
-            keys_o[to] = key[k];
-            vals_o[to] = val[k];
-        }
+        if (base + k * 64 + lane < a.n)
+            out[cnt[w][(pair[k].x >> shift) & mask] + rank[k]] = pair[k];
 }
 
 // ---------------------------------------------------------------- run sums
@@ -252,26 +275,28 @@ __global__ __launch_bounds__(kThreads) void k_sort_scatter(LookupGradArgs a, con
 // follow that order: a run inside a span is a row's whole sum, and a span's first
 // and last run, where they go on in its neighbours, are added up by k_run_join
 // from `part` (span, 2, dim). With few rows (LOCAL) no such sort is needed: a span
-// is kLocal consecutive ids that the workgroup sorts itself, and each row's sum
+// is some consecutive ids that the workgroup sorts itself, and each row's sum
 // over it goes to `part` (span, rows, dim). That reads dout almost in order, in 2
 // launches instead of 5.
-constexpr int kSpan = 1024;      // most entries of a span, and those of a LOCAL one
-constexpr int kLocalRows = 128;  // most rows for LOCAL: an eighth of the span
+constexpr int kSpan = 1024;      // most entries of a span
+constexpr int kLocalRows = 128;  // most rows for LOCAL: an eighth or a quarter of the span
 
 template <typename TD, int VEC>
-__device__ __forceinline__ void put_row(TD* out, const float* acc, float scale, int accumulate) {
+__device__ __forceinline__ void put_row(TD* out, const float* acc, float scale, int accumulate,
+                                        int n = VEC) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-        float s = acc[j] * scale;
-        if (accumulate) s += to_float(out[j]);
-        out[j] = from_float<TD>(s);
-    }
+    for (int j = 0; j < VEC; ++j)
+        if (j < n) {
+            float s = acc[j] * scale;
+            if (accumulate) s += to_float(out[j]);
+            out[j] = from_float<TD>(s);
+        }
 }
 
 template <typename TI, typename TD, int VEC, bool LOCAL>
-__global__ __launch_bounds__(kThreads) void k_run_sums(LookupGradArgs a, const uint32_t* keys,
-                                                       const uint32_t* pos, int span, int lpr,
-                                                       int bits, float* part, uint2* runs) {
+__global__ __launch_bounds__(kThreads) void k_run_sums(LookupGradArgs a, const uint2* pairs,
+                                                       int span, int lpr, int bits, float* part,
+                                                       uint2* runs) {
     constexpr int kWaves = kThreads / 64;
     constexpr uint32_t kNone = 0xFFFFFFFFu;
     __shared__ uint32_t skey[kSpan], spos[kSpan];
@@ -288,14 +313,15 @@ __global__ __launch_bounds__(kThreads) void k_run_sums(LookupGradArgs a, const u
     uint32_t before = kNone, after = kNone;  // the neighbours' keys
     if (LOCAL) {
         __shared__ uint32_t cnt[kWaves][kLocalRows + 1];
-        __shared__ uint32_t scan[kThreads];
+        __shared__ uint32_t scan[kWaves];
         for (int k = t; k < kWaves * (kLocalRows + 1); k += kThreads) (&cnt[0][0])[k] = 0u;
         __syncthreads();
         const int w = t >> 6, l = t & 63;
         uint32_t key[kSpan / kThreads], rank[kSpan / kThreads];
 #pragma unroll
         for (int k = 0; k < kSpan / kThreads; ++k) {
-            const int i = w * (kSpan / kWaves) + k * 64 + l;
+            if (k >= span / kThreads) break;
+            const int i = w * (span / kWaves) + k * 64 + l;
             key[k] = i < m ? sort_key(a, nullptr, base + i, blockIdx.y == 0 ? a.flags : nullptr) : 0u;
             rank[k] = wave_rank(key[k], i < m, bits, cnt[w]);
         }
@@ -313,8 +339,8 @@ __global__ __launch_bounds__(kThreads) void k_run_sums(LookupGradArgs a, const u
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < kSpan / kThreads; ++k) {
-            const int i = w * (kSpan / kWaves) + k * 64 + l;
-            if (i < m) {
+            const int i = w * (span / kWaves) + k * 64 + l;
+            if (k < span / kThreads && i < m) {
                 const uint32_t to = cnt[w][key[k]] + rank[k];
                 skey[to] = key[k];
                 spos[to] = (uint32_t)(base + i);
@@ -332,12 +358,12 @@ __global__ __launch_bounds__(kThreads) void k_run_sums(LookupGradArgs a, const u
         }
     } else {
         for (int i = t; i < m; i += kThreads) {
-            const uint32_t k = keys[base + i];
-            skey[i] = k;
-            spos[i] = pos[base + i];
+            const uint2 p = pairs[base + i];
+            skey[i] = p.x;
+            spos[i] = p.y;
         }
-        if (base > 0) before = keys[base - 1];
-        if (base + m < a.n) after = keys[base + m];
+        if (base > 0) before = pairs[base - 1].x;
+        if (base + m < a.n) after = pairs[base + m].x;
         __syncthreads();
         if (blockIdx.y == 0)
             for (int i = t; i < m; i += kThreads) {
@@ -352,17 +378,16 @@ __global__ __launch_bounds__(kThreads) void k_run_sums(LookupGradArgs a, const u
     auto finish = [&](uint32_t key, const float* acc, int at, int which, auto width) {
         constexpr int W = decltype(width)::value;
         if (key >= rows) return;
-        if (LOCAL) {
-            float* p = part + ((size_t)blockIdx.x * rows + key) * a.dim + at;
+        const int n = min(W, a.dim - at);
+        if (LOCAL || which < 2) {
+            const size_t row = LOCAL ? (size_t)blockIdx.x * rows + key
+                                     : (size_t)blockIdx.x * 2 + which;
 #pragma unroll
-            for (int j = 0; j < W; ++j) p[j] = acc[j];
-        } else if (which < 2) {
-            float* p = part + ((size_t)blockIdx.x * 2 + which) * a.dim + at;
-#pragma unroll
-            for (int j = 0; j < W; ++j) p[j] = acc[j];
+            for (int j = 0; j < W; ++j)
+                if (j < n) part[row * a.dim + at + j] = acc[j];
         } else {
             put_row<TD, W>(dtable + (int64_t)key * a.dtable_stride + at, acc, a.scale,
-                           a.accumulate);
+                           a.accumulate, n);
         }
     };
 
@@ -372,7 +397,7 @@ __global__ __launch_bounds__(kThreads) void k_run_sums(LookupGradArgs a, const u
     for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
     uint32_t cur = lo < hi ? skey[lo] : kNone, first = cur;
     bool single = true;
-    const bool col_on = c < a.dim;
+    const bool col_on = c < a.dim, whole = c + VEC <= a.dim;
     constexpr int U = 8;  // rows in flight
     for (int i0 = lo; i0 < hi; i0 += U) {
         float v[U][VEC];
@@ -380,11 +405,14 @@ __global__ __launch_bounds__(kThreads) void k_run_sums(LookupGradArgs a, const u
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             k[u] = i0 + u < hi ? skey[i0 + u] : kNone;
-            if (k[u] < rows && col_on) {
-                load_vec<VEC>(dout + (int64_t)spos[i0 + u] * a.dout_stride + c, v[u]);
+            const bool on = k[u] < rows && col_on;
+            const TI* src = dout + (on ? (int64_t)spos[i0 + u] * a.dout_stride + c : 0);
+            if (on && whole) {
+                load_any<VEC>(src, v[u]);
             } else {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) v[u][j] = 0.0f;
+                for (int j = 0; j < VEC; ++j)
+                    v[u][j] = on && c + j < a.dim ? to_float(src[j]) : 0.0f;
             }
         }
 #pragma unroll
@@ -419,17 +447,28 @@ __global__ __launch_bounds__(kThreads) void k_run_sums(LookupGradArgs a, const u
         const uint32_t span_first = key;
         float sum = 0.0f;
         bool begin = true;  // the run holds the span's first entry
-        for (int e = 0; e < slots * 2; ++e) {
-            const uint32_t k = end_key[e];
-            if (k == kNone) continue;
-            if (k != key) {
-                finish(key, &sum, c0 + j, begin && before == span_first ? 0 : 2,
-                       std::integral_constant<int, 1>());
-                begin = false;
-                key = k;
-                sum = 0.0f;
+        constexpr int E = 8;
+        for (int e0 = 0; e0 < slots * 2; e0 += E) {
+            uint32_t k[E];
+            float v[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const bool on = e0 + e < slots * 2;
+                k[e] = on ? end_key[e0 + e] : kNone;
+                v[e] = on ? ends[(e0 + e) * cols + j] : 0.0f;
             }
-            sum += ends[e * cols + j];
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                if (k[e] == kNone) continue;
+                if (k[e] != key) {
+                    finish(key, &sum, c0 + j, begin && before == span_first ? 0 : 2,
+                           std::integral_constant<int, 1>());
+                    begin = false;
+                    key = k[e];
+                    sum = 0.0f;
+                }
+                sum += v[e];
+            }
         }
         const bool more = after == key;
         const int which = begin ? (before == span_first || more ? 0 : 2) : (more ? 1 : 2);
@@ -536,6 +575,9 @@ int key_bits(int64_t rows) {  // keys 0 .. rows
     return b;
 }
 
+// Consecutive ids of a LOCAL span: fewer where that fills the chip.
+int local_span(int64_t n) { return n <= (1 << 19) ? kSpan / 2 : kSpan; }
+
 bool is_local(int64_t n, int64_t rows) { return rows <= kLocalRows && n > 0; }
 
 // Entries of a span of the sorted list: at most 4096 spans while spans can grow,
@@ -550,20 +592,18 @@ int span_of(int64_t n) {
 int sort_items(int64_t n) { return n <= (1 << 21) ? 4 : 16; }
 
 struct GradWs {
-    uint32_t *key[2], *val[2], *counts, *totals;
-    uint2* runs;
+    uint2 *pairs[2], *runs;
+    uint32_t *counts, *totals;
     float* part;
     size_t bytes;
     GradWs(void* base, int64_t n, int64_t rows, int dim) {
         Carve c(base);
         if (is_local(n, rows)) {
-            part = c.take<float>((size_t)((n + kSpan - 1) / kSpan) * rows * dim);
+            const int span = local_span(n);
+            part = c.take<float>((size_t)((n + span - 1) / span) * rows * dim);
         } else {
             const int64_t tile = (int64_t)kThreads * sort_items(n);
-            for (int k = 0; k < 2; ++k) {
-                key[k] = c.take<uint32_t>((size_t)n);
-                val[k] = c.take<uint32_t>((size_t)n);
-            }
+            for (int k = 0; k < 2; ++k) pairs[k] = c.take<uint2>((size_t)n);
             counts = c.take<uint32_t>((size_t)((n + tile - 1) / tile) * 256);
             totals = c.take<uint32_t>(256);
             runs = c.take<uint2>((size_t)rows);
@@ -574,17 +614,18 @@ struct GradWs {
     }
 };
 
-template <typename TI, typename TD, int VEC>
-hipError_t grad_run(const LookupGradArgs& a, const GradWs& w, const uint32_t* keys,
-                    const uint32_t* vals, hipStream_t st) {
+template <typename TI, typename TD>
+hipError_t grad_typed(const LookupGradArgs& a, const GradWs& w, const uint2* pairs,
+                      hipStream_t st) {
+    constexpr int VEC = 16 / sizeof(TI);
     const int units = (a.dim + VEC - 1) / VEC;
     int lpr = 1;
     while (lpr < 64 && lpr < units) lpr *= 2;
     const unsigned cols = (unsigned)((units + lpr - 1) / lpr);
     if (is_local(a.n, a.rows)) {
-        const int spans = (int)((a.n + kSpan - 1) / kSpan);
+        const int span = local_span(a.n), spans = (int)((a.n + span - 1) / span);
         k_run_sums<TI, TD, VEC, true><<<dim3((unsigned)spans, cols), kThreads, 0, st>>>(
-            a, nullptr, nullptr, kSpan, lpr, key_bits(a.rows), w.part, nullptr);
+            a, nullptr, span, lpr, key_bits(a.rows), w.part, nullptr);
         k_local_join<TD><<<dim3((unsigned)a.rows, (unsigned)((a.dim + 15) / 16)), kThreads, 0, st>>>(
             a, spans, w.part);
         return hipGetLastError();
@@ -593,41 +634,29 @@ hipError_t grad_run(const LookupGradArgs& a, const GradWs& w, const uint32_t* ke
     if (a.n > 0)
         k_run_sums<TI, TD, VEC, false>
             <<<dim3((unsigned)((a.n + span - 1) / span), cols), kThreads, 0, st>>>(
-                a, keys, vals, span, lpr, 0, w.part, w.runs);
+                a, pairs, span, lpr, 0, w.part, w.runs);
     const int64_t joins = (a.rows + 3) / 4;
     k_run_join<TD><<<(unsigned)(joins < 65536 ? joins : 65536), kThreads, 0, st>>>(a, w.runs, span,
                                                                                 w.part);
     return hipGetLastError();
 }
 
-template <typename TI, typename TD>
-hipError_t grad_typed(const LookupGradArgs& a, const GradWs& w, const uint32_t* keys,
-                      const uint32_t* vals, hipStream_t st) {
-    constexpr int VEC = 16 / sizeof(TI);
-    if (a.dim % VEC == 0 && aligned_rows<TI>(a.dout, a.dout_stride, VEC))
-        return grad_run<TI, TD, VEC>(a, w, keys, vals, st);
-    if (a.dim % 2 == 0 && aligned_rows<TI>(a.dout, a.dout_stride, 2))
-        return grad_run<TI, TD, 2>(a, w, keys, vals, st);
-    return grad_run<TI, TD, 1>(a, w, keys, vals, st);
-}
-
 template <int ITEMS>
-void sort_ids(const LookupGradArgs& a, const GradWs& w, const uint32_t** keys,
-              const uint32_t** vals, hipStream_t st) {
+const uint2* sort_ids(const LookupGradArgs& a, const GradWs& w, hipStream_t st) {
     const int bits = key_bits(a.rows), passes = (bits + 7) / 8;
     const unsigned blocks = (unsigned)((a.n + kThreads * ITEMS - 1) / (kThreads * ITEMS));
-    *keys = *vals = nullptr;
+    const uint2* pairs = nullptr;
     for (int p = 0, done = 0; p < passes; ++p) {
         const int b = (bits - done + passes - p - 1) / (passes - p);
-        k_sort_count<ITEMS><<<blocks, kThreads, 0, st>>>(a, *keys, done, b, w.counts,
+        k_sort_count<ITEMS><<<blocks, kThreads, 0, st>>>(a, pairs, done, b, w.counts,
                                                          p == 0 ? w.runs : nullptr);
         k_sort_scan<<<1u << b, kThreads, 0, st>>>(w.counts, (int)blocks, w.totals);
-        k_sort_scatter<ITEMS><<<blocks, kThreads, 0, st>>>(a, *keys, *vals, done, b, w.counts,
-                                                           w.totals, w.key[p & 1], w.val[p & 1]);
-        *keys = w.key[p & 1];
-        *vals = w.val[p & 1];
+        k_sort_scatter<ITEMS><<<blocks, kThreads, 0, st>>>(a, pairs, done, b, w.counts, w.totals,
+                                                           w.pairs[p & 1]);
+        pairs = w.pairs[p & 1];
         done += b;
     }
+    return pairs;
 }
 
 __global__ __launch_bounds__(kThreads) void k_run_clear(uint2* runs, int64_t rows) {
@@ -652,21 +681,17 @@ size_t lookup_grad_ws(int64_t n, int64_t rows, int dim) {
 hipError_t launch_lookup_grad(const LookupGradArgs& a, hipStream_t st) {
     if (a.rows == 0) return hipSuccess;
     const GradWs w(a.ws, a.n, a.rows, a.dim);
-    const uint32_t *keys = nullptr, *vals = nullptr;
-    if (a.n == 0) {
+    const uint2* pairs = nullptr;
+    if (a.n == 0)
         k_run_clear<<<(unsigned)((a.rows + kThreads - 1) / kThreads), kThreads, 0, st>>>(w.runs,
                                                                                       a.rows);
-    } else if (!is_local(a.n, a.rows)) {
-        if (sort_items(a.n) == 4)
-            sort_ids<4>(a, w, &keys, &vals, st);
-        else
-            sort_ids<16>(a, w, &keys, &vals, st);
-    }
+    else if (!is_local(a.n, a.rows))
+        pairs = sort_items(a.n) == 4 ? sort_ids<4>(a, w, st) : sort_ids<16>(a, w, st);
     if (a.dout_dtype == 0)
-        return a.dtable_dtype == 0 ? grad_typed<float, float>(a, w, keys, vals, st)
-                                   : grad_typed<float, bf16>(a, w, keys, vals, st);
-    return a.dtable_dtype == 0 ? grad_typed<bf16, float>(a, w, keys, vals, st)
-                               : grad_typed<bf16, bf16>(a, w, keys, vals, st);
+        return a.dtable_dtype == 0 ? grad_typed<float, float>(a, w, pairs, st)
+                                   : grad_typed<float, bf16>(a, w, pairs, st);
+    return a.dtable_dtype == 0 ? grad_typed<bf16, float>(a, w, pairs, st)
+                               : grad_typed<bf16, bf16>(a, w, pairs, st);
 }
 
 }  // namespace gs
