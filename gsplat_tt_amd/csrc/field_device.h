@@ -45,6 +45,13 @@ __device__ __forceinline__ void store_vec(T* p, const float* in) {
     *reinterpret_cast<VecOf<T, VEC>*>(p) = u;
 }
 
+template <int VEC, typename T>
+__device__ __forceinline__ void store_any(T* p, const float* in) {
+    T u[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) u[j] = from_float<T>(in[j]);
+    __builtin_memcpy(p, u, sizeof(u));
+}
 // The same past the caches, for outputs that are not read again soon.
 template <int VEC, typename T>
 __device__ __forceinline__ void store_nt(T* p, const float* in) {

@@ -6,7 +6,7 @@
 // The gradient is by sorted ids: a stable radix sort of (id, position), then
 // each id's run of rows is summed in position order, so the result does not
 // depend on timing. Sums are held in fp32.
-#include <type_traits>
+#include <algorithm>
 
 #include "field.h"
 
@@ -265,11 +265,67 @@ __global__ __launch_bounds__(kThreads) void k_sort_scatter(LookupGradArgs a, con
             out[cnt[w][(pair[k].x >> shift) & mask] + rank[k]] = pair[k];
 }
 
+// The whole sort of a short list in one workgroup's LDS.
+constexpr int kShortThreads = 1024;
+constexpr int kShort = 4096;
+
+__global__ __launch_bounds__(kShortThreads) void k_sort_short(LookupGradArgs a, int bits_all,
+                                                              uint2* out, uint2* runs) {
+    constexpr int kWaves = kShortThreads / 64, kItems = kShort / kShortThreads;
+    __shared__ uint2 list[kShort];
+    __shared__ uint32_t cnt[kWaves][256];
+    __shared__ uint32_t part[kWaves];
+    const int t = threadIdx.x, w = t >> 6, lane = t & 63, n = (int)a.n;
+    const int base = w * 64 * kItems;
+    for (int64_t v = t; v < a.rows; v += kShortThreads) runs[v] = make_uint2(0u, 0u);
+    uint2 pair[kItems];
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+        const int i = base + k * 64 + lane;
+        pair[k] = make_uint2(i < n ? sort_key(a, nullptr, i, a.flags) : 0u, (uint32_t)i);
+    }
+    const int passes = (bits_all + 7) / 8;
+    for (int p = 0, done = 0; p < passes; ++p) {
+        const int bits = (bits_all - done + passes - p - 1) / (passes - p), digits = 1 << bits;
+        for (int k = t; k < kWaves * 256; k += kShortThreads) (&cnt[0][0])[k] = 0u;
+        __syncthreads();
+        uint32_t rank[kItems];
+#pragma unroll
+        for (int k = 0; k < kItems; ++k)
+            rank[k] = wave_rank((pair[k].x >> done) & (digits - 1u), base + k * 64 + lane < n, bits,
+                                cnt[w]);
+        __syncthreads();
+        uint32_t mine = 0, all;
+        if (t < digits)
+            for (int k = 0; k < kWaves; ++k) mine += cnt[k][t];
+        uint32_t at = block_excl_scan<kShortThreads>(mine, part, &all);
+        if (t < digits)
+            for (int k = 0; k < kWaves; ++k) {
+                const uint32_t c = cnt[k][t];
+                cnt[k][t] = at;
+                at += c;
+            }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kItems; ++k)
+            if (base + k * 64 + lane < n)
+                list[cnt[w][(pair[k].x >> done) & (digits - 1u)] + rank[k]] = pair[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kItems; ++k)
+            if (base + k * 64 + lane < n) pair[k] = list[base + k * 64 + lane];
+        done += bits;
+    }
+#pragma unroll
+    for (int k = 0; k < kItems; ++k)
+        if (base + k * 64 + lane < n) out[base + k * 64 + lane] = pair[k];
+}
+
 // ---------------------------------------------------------------- run sums
 // A workgroup takes a span of (id, position) in id order, its slots of `lpr` lanes
 // (VEC columns a lane) equal stretches of it. Runs inside a stretch are finished
-// at once; each stretch's first and last run are joined over the slots in LDS,
-// in order.
+// at once; runs over several stretches are joined by a segmented scan over the
+// slots, in a fixed order.
 //
 // Two uses. Where ids have to be sorted over the whole list (LOCAL false), spans
 // follow that order: a run inside a span is a row's whole sum, and a span's first
@@ -278,18 +334,33 @@ __global__ __launch_bounds__(kThreads) void k_sort_scatter(LookupGradArgs a, con
 // is some consecutive ids that the workgroup sorts itself, and each row's sum
 // over it goes to `part` (span, rows, dim). That reads dout almost in order, in 2
 // launches instead of 5.
-constexpr int kSpan = 1024;      // most entries of a span
-constexpr int kLocalRows = 128;  // most rows for LOCAL: an eighth or a quarter of the span
+constexpr int kSpan = 4096;      // most entries of a span
+constexpr int kLocalRows = 128;  // most rows for LOCAL: a quarter of the least span
 
+// scale * acc into (or onto) values lo .. hi - 1 of VEC ones of a row, at once where
+// that is all of them.
 template <typename TD, int VEC>
 __device__ __forceinline__ void put_row(TD* out, const float* acc, float scale, int accumulate,
-                                        int n = VEC) {
+                                        int lo = 0, int hi = VEC) {
+    float s[VEC];
+    if (lo == 0 && hi == VEC) {
+        if (accumulate) {
+            load_any<VEC>(out, s);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) s[j] += acc[j] * scale;
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) s[j] = acc[j] * scale;
+        }
+        store_any<VEC>(out, s);
+        return;
+    }
 #pragma unroll
     for (int j = 0; j < VEC; ++j)
-        if (j < n) {
-            float s = acc[j] * scale;
-            if (accumulate) s += to_float(out[j]);
-            out[j] = from_float<TD>(s);
+        if (j >= lo && j < hi) {
+            float v = acc[j] * scale;
+            if (accumulate) v += to_float(out[j]);
+            out[j] = from_float<TD>(v);
         }
 }
 
@@ -299,14 +370,20 @@ __global__ __launch_bounds__(kThreads) void k_run_sums(LookupGradArgs a, const u
                                                        uint2* runs) {
     constexpr int kWaves = kThreads / 64;
     constexpr uint32_t kNone = 0xFFFFFFFFu;
-    __shared__ uint32_t skey[kSpan], spos[kSpan];
-    __shared__ float ends[kThreads * 2 * VEC];  // (slot, first or last, column)
-    __shared__ uint32_t end_key[kThreads * 2];
+    extern __shared__ uint32_t entries[];
+    uint32_t *skey = entries, *spos = entries + span;
+    __shared__ float carry[kThreads / 64][64 * VEC];     // the waves' last runs
+    __shared__ uint32_t carry_flags[kThreads / 64];
+    __shared__ uint32_t first_key[kThreads], last_key[kThreads];
     const TI* dout = static_cast<const TI*>(a.dout);
     TD* dtable = static_cast<TD*>(a.dtable);
     const int t = threadIdx.x, cols = lpr * VEC, c0 = blockIdx.y * cols;
     const int slots = kThreads / lpr, slot = t / lpr, lane = t % lpr;
-    const int c = c0 + lane * VEC;
+    // the lane's columns: of a row's last ones that make no vector, a vector that ends
+    // with the row is read, and its first values, the lane before's, are not written
+    const bool col_on = c0 + lane * VEC < a.dim, whole = a.dim >= VEC;
+    const int c = whole ? min(c0 + lane * VEC, a.dim - VEC) : 0;
+    const int c_lo = c0 + lane * VEC - c, c_hi = whole ? VEC : a.dim;
     const uint32_t rows = (uint32_t)a.rows;
     const int64_t base = (int64_t)blockIdx.x * span;
     const int m = (int)min((int64_t)span, a.n - base);
@@ -320,10 +397,12 @@ __global__ __launch_bounds__(kThreads) void k_run_sums(LookupGradArgs a, const u
         uint32_t key[kSpan / kThreads], rank[kSpan / kThreads];
 #pragma unroll
         for (int k = 0; k < kSpan / kThreads; ++k) {
-            if (k >= span / kThreads) break;
             const int i = w * (span / kWaves) + k * 64 + l;
-            key[k] = i < m ? sort_key(a, nullptr, base + i, blockIdx.y == 0 ? a.flags : nullptr) : 0u;
-            rank[k] = wave_rank(key[k], i < m, bits, cnt[w]);
+            if (k < span / kThreads) {
+                key[k] = i < m ? sort_key(a, nullptr, base + i, blockIdx.y == 0 ? a.flags : nullptr)
+                               : 0u;
+                rank[k] = wave_rank(key[k], i < m, bits, cnt[w]);
+            }
         }
         __syncthreads();
         uint32_t mine = 0, all;
@@ -352,9 +431,8 @@ __global__ __launch_bounds__(kThreads) void k_run_sums(LookupGradArgs a, const u
         for (uint32_t v = slot; v < rows; v += slots) {
             const uint32_t lo = cnt[0][v];
             if (lo < (uint32_t)m && skey[lo] == v) continue;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                if (c + j < a.dim) row0[(size_t)v * a.dim + c + j] = 0.0f;
+            const float zero[VEC] = {};
+            if (col_on) put_row<float, VEC>(row0 + (size_t)v * a.dim + c, zero, 1.0f, 0, c_lo, c_hi);
         }
     } else {
         for (int i = t; i < m; i += kThreads) {
@@ -375,29 +453,25 @@ __global__ __launch_bounds__(kThreads) void k_run_sums(LookupGradArgs a, const u
     }
     // a run's sum over the span; `which`: 0 it holds the span's first entry, 1 only
     // its last, 2 neither
-    auto finish = [&](uint32_t key, const float* acc, int at, int which, auto width) {
-        constexpr int W = decltype(width)::value;
+    auto finish = [&](uint32_t key, const float* acc, int which) {
         if (key >= rows) return;
-        const int n = min(W, a.dim - at);
         if (LOCAL || which < 2) {
             const size_t row = LOCAL ? (size_t)blockIdx.x * rows + key
                                      : (size_t)blockIdx.x * 2 + which;
-#pragma unroll
-            for (int j = 0; j < W; ++j)
-                if (j < n) part[row * a.dim + at + j] = acc[j];
+            put_row<float, VEC>(part + row * a.dim + c, acc, 1.0f, 0, c_lo, c_hi);
         } else {
-            put_row<TD, W>(dtable + (int64_t)key * a.dtable_stride + at, acc, a.scale,
-                           a.accumulate, n);
+            put_row<TD, VEC>(dtable + (int64_t)key * a.dtable_stride + c, acc, a.scale,
+                             a.accumulate, c_lo, c_hi);
         }
     };
 
-    const int per = span / slots, lo = min(m, slot * per), hi = min(m, lo + per);
-    float acc[VEC];
+    const int per = (span + slots - 1) / slots, lo = min(m, slot * per), hi = min(m, lo + per);
+    float acc[VEC], head[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
-    uint32_t cur = lo < hi ? skey[lo] : kNone, first = cur;
+    for (int j = 0; j < VEC; ++j) acc[j] = head[j] = 0.0f;
+    uint32_t cur = lo < hi ? skey[lo] : kNone;
+    const uint32_t first = cur;
     bool single = true;
-    const bool col_on = c < a.dim, whole = c + VEC <= a.dim;
     constexpr int U = 8;  // rows in flight
     for (int i0 = lo; i0 < hi; i0 += U) {
         float v[U][VEC];
@@ -421,10 +495,10 @@ __global__ __launch_bounds__(kThreads) void k_run_sums(LookupGradArgs a, const u
             if (k[u] != cur) {
                 if (single) {
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) ends[(slot * 2) * cols + lane * VEC + j] = acc[j];
+                    for (int j = 0; j < VEC; ++j) head[j] = acc[j];
                     single = false;
                 } else if (col_on) {
-                    finish(cur, acc, c, 2, std::integral_constant<int, VEC>());
+                    finish(cur, acc, 2);
                 }
                 cur = k[u];
 #pragma unroll
@@ -434,109 +508,160 @@ __global__ __launch_bounds__(kThreads) void k_run_sums(LookupGradArgs a, const u
             for (int j = 0; j < VEC; ++j) acc[j] += v[u][j];
         }
     }
-#pragma unroll
-    for (int j = 0; j < VEC; ++j)
-        ends[(slot * 2 + (single ? 0 : 1)) * cols + lane * VEC + j] = acc[j];
     if (lane == 0) {
-        end_key[slot * 2] = first;
-        end_key[slot * 2 + 1] = single ? kNone : cur;
+        first_key[slot] = first;
+        last_key[slot] = cur;
     }
     __syncthreads();
-    for (int j = t; j < cols && c0 + j < a.dim; j += kThreads) {
-        uint32_t key = end_key[0];
-        const uint32_t span_first = key;
-        float sum = 0.0f;
-        bool begin = true;  // the run holds the span's first entry
-        constexpr int E = 8;
-        for (int e0 = 0; e0 < slots * 2; e0 += E) {
-            uint32_t k[E];
-            float v[E];
+    const uint32_t prev = slot > 0 ? last_key[slot - 1] : kNone;
+    uint32_t next = slot + 1 < slots ? first_key[slot + 1] : kNone;
+    // Segmented inclusive scan of the slots' last runs: `cut`: the run starts in
+    // this slot (or the scan has met such a one); `begin`: it holds the span's
+    // first entry.
+    bool cut = !single || first != prev || first == kNone;
+    bool begin = slot == 0 && single;
+    for (int o = lpr; o < 64; o <<= 1) {
+        const bool in = (t & 63) >= o;
+        const bool ucut = __shfl_up((int)cut, o, 64), ubegin = __shfl_up((int)begin, o, 64);
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const bool on = e0 + e < slots * 2;
-                k[e] = on ? end_key[e0 + e] : kNone;
-                v[e] = on ? ends[(e0 + e) * cols + j] : 0.0f;
-            }
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                if (k[e] == kNone) continue;
-                if (k[e] != key) {
-                    finish(key, &sum, c0 + j, begin && before == span_first ? 0 : 2,
-                           std::integral_constant<int, 1>());
-                    begin = false;
-                    key = k[e];
-                    sum = 0.0f;
-                }
-                sum += v[e];
-            }
+        for (int j = 0; j < VEC; ++j) {
+            const float u = __shfl_up(acc[j], o, 64);
+            if (in && !cut) acc[j] += u;
         }
-        const bool more = after == key;
-        const int which = begin ? (before == span_first || more ? 0 : 2) : (more ? 1 : 2);
-        finish(key, &sum, c0 + j, which, std::integral_constant<int, 1>());
+        if (in && !cut) {
+            begin = ubegin;
+            cut = ucut;
+        }
     }
+    const int w = t >> 6, in_wave = t & 63;
+    if (in_wave >= 64 - lpr) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) carry[w][(in_wave - (64 - lpr)) * VEC + j] = acc[j];
+        if (in_wave == 63) carry_flags[w] = (cut ? 1u : 0u) | (begin ? 2u : 0u);
+    }
+    __syncthreads();
+    // what the earlier waves bring to this one
+    float in[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) in[j] = 0.0f;
+    bool in_begin = false;
+    for (int k = 0; k < w; ++k) {
+        const bool kcut = carry_flags[k] & 1u;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            in[j] = (kcut ? 0.0f : in[j]) + carry[k][(in_wave % lpr) * VEC + j];
+        in_begin = kcut ? (carry_flags[k] & 2u) != 0u : in_begin;
+    }
+    if (!cut) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[j] += in[j];
+        begin = in_begin;
+    }
+    // the previous slot's run, which this slot's first one may continue
+    float before_sum[VEC];
+    bool before_begin = __shfl_up((int)begin, lpr, 64);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) before_sum[j] = __shfl_up(acc[j], lpr, 64);
+    if (in_wave < lpr) {
+        before_begin = in_begin;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) before_sum[j] = in[j];
+    }
+    if (!col_on || first == kNone) return;
+    if (!single) {
+        const bool joins = prev == first;
+        if (joins)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) head[j] += before_sum[j];
+        const bool from_begin = slot == 0 || (joins && before_begin);
+        finish(first, head, from_begin && before == first ? 0 : 2);
+    }
+    if (next == kNone) next = after;  // the last slot with entries
+    else if (next == cur) return;
+    const bool more = next == cur;
+    finish(cur, acc, begin ? (before == cur || more ? 0 : 2) : (more ? 1 : 2));
 }
 
 // Rows whose run crosses spans: the sum of the spans' pieces in order; zeros for
-// rows that no id names. A wave a row; a row of many pieces takes the workgroup,
-// each wave every fourth piece.
-constexpr int kWavePieces = 32;
+// rows that no id names. `lpr` lanes a row, 4 columns a lane; a row of many pieces
+// takes the workgroup, whose slots share the pieces out.
+constexpr uint32_t kSlotPieces = 32;
 
 template <typename TD>
 __global__ __launch_bounds__(kThreads) void k_run_join(LookupGradArgs a, const uint2* runs,
-                                                       int span, const float* part) {
-    __shared__ float sums[kThreads];
+                                                       int span, int lpr, const float* part) {
+    __shared__ float sums[kThreads][4];
+    __shared__ uint32_t many[kThreads], n_many;
     TD* dtable = static_cast<TD*>(a.dtable);
-    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    // sum of pieces s0 + k, s0 + k + by, .. of column c
-    auto pieces = [&](uint2 run, uint32_t k, uint32_t by, int c) {
-        const uint32_t s0 = run.x / (uint32_t)span, s1 = (run.y - 1u) / (uint32_t)span;
-        float acc = 0.0f;
-        for (uint32_t s = s0 + k; s <= s1; s += by * 4) {
-            float v[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const uint32_t q = s + u * by;
-                const int which = q == s0 && run.x % (uint32_t)span != 0u ? 1 : 0;
-                v[u] = q <= s1 ? part[((size_t)q * 2 + which) * a.dim + c] : 0.0f;
-            }
-#pragma unroll
-            for (int u = 0; u < 4; ++u) acc += v[u];
-        }
-        return acc;
-    };
-    auto count = [&](uint2 run) {
+    const int slots = kThreads / lpr, slot = threadIdx.x / lpr, lane = threadIdx.x % lpr;
+    auto pieces_of = [&](uint2 run) {
         return run.x == run.y ? 0u : (run.y - 1u) / (uint32_t)span - run.x / (uint32_t)span + 1u;
     };
-    for (int64_t v0 = (int64_t)blockIdx.x * 4; v0 < a.rows; v0 += (int64_t)gridDim.x * 4) {
-        const int64_t v = v0 + w;
+    // pieces k, k + by, .. of columns c.. c + 3
+    auto add = [&](uint2 run, uint32_t n, uint32_t k, uint32_t by, int c, float* acc) {
+        const uint32_t s0 = run.x / (uint32_t)span;
+        const uint32_t from = run.x % (uint32_t)span != 0u ? 1u : 0u;  // the first piece's place
+        const int nv = min(4, a.dim - c);
+        for (; k < n; k += by * 4) {
+            float v[4][4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const uint32_t q = k + u * by;
+                const float* p = part + ((size_t)(s0 + q) * 2 + (q == 0 ? from : 0)) * a.dim + c;
+                if (q < n && nv == 4) {
+                    load_any<4>(p, v[u]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[u][j] = q < n && j < nv ? p[j] : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j] += v[u][j];
+        }
+    };
+    for (int64_t v0 = (int64_t)blockIdx.x * slots; v0 < a.rows; v0 += (int64_t)gridDim.x * slots) {
+        if (threadIdx.x == 0) n_many = 0u;
+        __syncthreads();
+        const int64_t v = v0 + slot;
         if (v < a.rows) {
             const uint2 run = runs[v];
-            const uint32_t n = count(run);
-            TD* out = dtable + v * a.dtable_stride;
-            if (n == 0 && !a.accumulate)
-                for (int c = lane; c < a.dim; c += 64) out[c] = from_float<TD>(0.0f);
-            if (n > 1 && n <= kWavePieces)
-                for (int c = lane; c < a.dim; c += 64) {
-                    const float acc = pieces(run, 0, 1, c);
-                    put_row<TD, 1>(out + c, &acc, a.scale, a.accumulate);
-                }
-        }
-        for (int k = 0; k < 4 && v0 + k < a.rows; ++k) {
-            const uint2 run = runs[v0 + k];
-            if (count(run) <= kWavePieces) continue;
-            for (int cb = 0; cb < a.dim; cb += 64) {
-                const int c = cb + lane;
-                float acc = c < a.dim ? pieces(run, w, kThreads / 64, c) : 0.0f;
-                __syncthreads();
-                sums[threadIdx.x] = acc;
-                __syncthreads();
-                if (w == 0 && c < a.dim) {
-                    for (int q = 1; q < kThreads / 64; ++q) acc += sums[q * 64 + lane];
-                    put_row<TD, 1>(dtable + (v0 + k) * a.dtable_stride + c, &acc, a.scale,
-                                   a.accumulate);
+            const uint32_t n = pieces_of(run);
+            if (n > kSlotPieces) {
+                if (lane == 0) many[atomicAdd(&n_many, 1u)] = (uint32_t)slot;
+            } else if (n > 1 || (n == 0 && !a.accumulate)) {
+                for (int c = lane * 4; c < a.dim; c += lpr * 4) {
+                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    add(run, n, 0, 1, c, acc);
+                    put_row<TD, 4>(dtable + v * a.dtable_stride + c, acc, a.scale, a.accumulate,
+                                   0, min(4, a.dim - c));
                 }
             }
         }
+        __syncthreads();
+        for (uint32_t k = 0; k < n_many; ++k) {
+            const int64_t row = v0 + many[k];
+            const uint2 run = runs[row];
+            const uint32_t n = pieces_of(run);
+            for (int c0 = 0; c0 < a.dim; c0 += lpr * 4) {
+                const int c = c0 + lane * 4;
+                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (c < a.dim) add(run, n, slot, slots, c, acc);
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sums[threadIdx.x][j] = acc[j];
+                __syncthreads();
+                if (slot == 0 && c < a.dim) {
+                    for (int q = 1; q < slots; ++q)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) acc[j] += sums[q * lpr + lane][j];
+                    put_row<TD, 4>(dtable + row * a.dtable_stride + c, acc, a.scale, a.accumulate,
+                                   0, min(4, a.dim - c));
+                }
+            }
+        }
+        __syncthreads();
     }
 }
 
@@ -575,16 +700,25 @@ int key_bits(int64_t rows) {  // keys 0 .. rows
     return b;
 }
 
-// Consecutive ids of a LOCAL span: fewer where that fills the chip.
-int local_span(int64_t n) { return n <= (1 << 19) ? kSpan / 2 : kSpan; }
+// Consecutive ids of a LOCAL span: as many as leave two workgroups a compute unit.
+int local_span(int64_t n) {
+    int s = 512;
+    while (s < kSpan && n / (2 * s) >= 512) s *= 2;
+    return s;
+}
 
 bool is_local(int64_t n, int64_t rows) { return rows <= kLocalRows && n > 0; }
+
+// A list for one workgroup, which also clears the rows' runs.
+bool is_short(int64_t n, int64_t rows) {
+    return n <= kShort && rows <= 65536 && !is_local(n, rows);
+}
 
 // Entries of a span of the sorted list: at most 4096 spans while spans can grow,
 // so that one row's pieces stay few.
 int span_of(int64_t n) {
     int s = 256;
-    while (s < kSpan && n / s > 4096) s *= 2;
+    while (s < 1024 && n / s > 4096) s *= 2;
     return s;
 }
 
@@ -607,7 +741,7 @@ struct GradWs {
             counts = c.take<uint32_t>((size_t)((n + tile - 1) / tile) * 256);
             totals = c.take<uint32_t>(256);
             runs = c.take<uint2>((size_t)rows);
-            const int span = span_of(n);
+            const int span = span_of(n);  // or longer, with fewer pieces
             part = c.take<float>((size_t)((n + span - 1) / span) * 2 * dim);
         }
         bytes = c.bytes();
@@ -624,20 +758,23 @@ hipError_t grad_typed(const LookupGradArgs& a, const GradWs& w, const uint2* pai
     const unsigned cols = (unsigned)((units + lpr - 1) / lpr);
     if (is_local(a.n, a.rows)) {
         const int span = local_span(a.n), spans = (int)((a.n + span - 1) / span);
-        k_run_sums<TI, TD, VEC, true><<<dim3((unsigned)spans, cols), kThreads, 0, st>>>(
+        k_run_sums<TI, TD, VEC, true><<<dim3((unsigned)spans, cols), kThreads, span * 8, st>>>(
             a, nullptr, span, lpr, key_bits(a.rows), w.part, nullptr);
         k_local_join<TD><<<dim3((unsigned)a.rows, (unsigned)((a.dim + 15) / 16)), kThreads, 0, st>>>(
             a, spans, w.part);
         return hipGetLastError();
     }
-    const int span = span_of(a.n);
+    // a slot's stretch holds the 8 rows that it loads at a time
+    const int span = std::max(span_of(a.n), std::min(kSpan, kThreads / lpr * 8));
     if (a.n > 0)
         k_run_sums<TI, TD, VEC, false>
-            <<<dim3((unsigned)((a.n + span - 1) / span), cols), kThreads, 0, st>>>(
+            <<<dim3((unsigned)((a.n + span - 1) / span), cols), kThreads, span * 8, st>>>(
                 a, pairs, span, lpr, 0, w.part, w.runs);
-    const int64_t joins = (a.rows + 3) / 4;
-    k_run_join<TD><<<(unsigned)(joins < 65536 ? joins : 65536), kThreads, 0, st>>>(a, w.runs, span,
-                                                                                w.part);
+    int join_lpr = 1;
+    while (join_lpr < 64 && join_lpr * 4 < a.dim) join_lpr *= 2;
+    const int64_t joins = (a.rows + kThreads / join_lpr - 1) / (kThreads / join_lpr);
+    k_run_join<TD><<<(unsigned)(joins < 65536 ? joins : 65536), kThreads, 0, st>>>(
+        a, w.runs, span, join_lpr, w.part);
     return hipGetLastError();
 }
 
@@ -685,7 +822,10 @@ hipError_t launch_lookup_grad(const LookupGradArgs& a, hipStream_t st) {
     if (a.n == 0)
         k_run_clear<<<(unsigned)((a.rows + kThreads - 1) / kThreads), kThreads, 0, st>>>(w.runs,
                                                                                       a.rows);
-    else if (!is_local(a.n, a.rows))
+    else if (is_short(a.n, a.rows)) {
+        k_sort_short<<<1, kShortThreads, 0, st>>>(a, key_bits(a.rows), w.pairs[0], w.runs);
+        pairs = w.pairs[0];
+    } else if (!is_local(a.n, a.rows))
         pairs = sort_items(a.n) == 4 ? sort_ids<4>(a, w, st) : sort_ids<16>(a, w, st);
     if (a.dout_dtype == 0)
         return a.dtable_dtype == 0 ? grad_typed<float, float>(a, w, pairs, st)
