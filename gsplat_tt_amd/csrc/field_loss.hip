@@ -106,49 +106,38 @@ __global__ __launch_bounds__(kThreads) void k_loss_rows(LossArgs a, int64_t padd
         weight[i] = l < 0 ? 0.0f : a.scale * (a.row_weight != nullptr ? a.row_weight[i] : 1.0f);
 }
 
-// Parts of (rows, dim) as (padded, kd), zeros in the padding and masked rows.
+// A row's 8 values from column c, cut into parts; zeros past the row.
+template <typename T, int NP>
+__device__ __forceinline__ void load_parts(const T* row, int dim, int c, bool on, quad* out) {
+    float v[8];
+    if (on && c + 8 <= dim) {
+        load_any<8>(row + c, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = plain_input<NP>(v[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            v[e] = on && c + e < dim ? plain_input<NP>(to_float(row[c + e])) : 0.0f;
+    }
+    split8<NP>(v, out);
+}
+
+// Parts of (rows, dim) as (padded, ld), zeros in the padding and in masked rows.
 template <typename T, int NP>
 __global__ __launch_bounds__(kThreads) void k_parts(const T* src, int64_t rows, int64_t stride,
                                                     int dim, const int32_t* label, int64_t padded,
-                                                    int kd, bf16* out) {
-    const int64_t total = padded * kd;
+                                                    int ld, quad* out) {
+    const int units = ld / 8;
+    const int64_t total = padded * units;
     for (int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x; e < total;
          e += (int64_t)gridDim.x * kThreads) {
-        const int64_t r = e / kd;
-        const int c = (int)(e - r * kd);
-        float v = 0.0f;
-        if (r < rows && c < dim && (label == nullptr || label[r] >= 0))
-            v = plain_input<NP>(to_float(src[r * stride + c]));
-        bf16 part[NP];
-        split<NP>(v, part);
+        const int64_t r = e / units;
+        const int c = (int)(e - r * units) * 8;
+        quad part[NP];
+        load_parts<T, NP>(src + r * stride, dim, c,
+                          r < rows && (label == nullptr || label[r] >= 0), part);
 #pragma unroll
         for (int p = 0; p < NP; ++p) out[p * total + e] = part[p];
-    }
-}
-
-// The same transposed: (dq, padded), dq >= dim a multiple of the tile.
-template <typename T, int NP>
-__global__ __launch_bounds__(kThreads) void k_parts_t(const T* src, int64_t rows, int64_t stride,
-                                                      int dim, const int32_t* label, int64_t padded,
-                                                      int dq, bf16* out) {
-    __shared__ float tile[32][33];
-    const int64_t r0 = (int64_t)blockIdx.x * 32;
-    const int c0 = blockIdx.y * 32, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    for (int k = ty; k < 32; k += 8) {
-        const int64_t r = r0 + k;
-        const int c = c0 + tx;
-        float v = 0.0f;
-        if (r < rows && c < dim && (label == nullptr || label[r] >= 0))
-            v = plain_input<NP>(to_float(src[r * stride + c]));
-        tile[k][tx] = v;
-    }
-    __syncthreads();
-    for (int k = ty; k < 32; k += 8) {
-        bf16 part[NP];
-        split<NP>(tile[tx][k], part);
-#pragma unroll
-        for (int p = 0; p < NP; ++p)
-            out[(size_t)p * dq * padded + (size_t)(c0 + k) * padded + r0 + tx] = part[p];
     }
 }
 
@@ -158,129 +147,250 @@ struct Mat {
     int64_t ld, plane;  // elements between rows and between parts
 };
 
-// acc += A[m0.., k0..k1) B[n0.., k0..k1)^T for a 128 x 128 tile, 4 waves of
-// 64 x 64. Rows of 64 bf16 (128 bytes) in LDS; a row's 16-byte pieces are
-// placed by (piece ^ row % 8), so that 8 lanes reading one column of pieces
-// touch all banks once.
-template <int NP>
-__device__ __forceinline__ void tile_product(const Mat& A, const Mat& B, int64_t m0, int64_t n0,
-                                             int64_t k0, int64_t k1, quad (*lds)[2][kTile * 8],
-                                             f32x4 acc[4][4]) {
-    const int t = threadIdx.x, lane = t & 63, w = t >> 6;
-    const int wm = (w >> 1) * 64, wn = (w & 1) * 64;
-    const int steps_k = (int)((k1 - k0) / kStep);
-    const int steps = steps_k * Products<NP>::kCount;
-    quad ra[4], rb[4];
-    auto fetch = [&](int s) {
-        const int q = s / steps_k;
-        const int64_t k = k0 + (int64_t)(s - q * steps_k) * kStep;
-        const bf16* pa = A.p + Products<NP>::a(q) * A.plane + m0 * A.ld + k;
-        const bf16* pb = B.p + Products<NP>::b(q) * B.plane + n0 * B.ld + k;
+// One operand's 128 x 64 tile in LDS (1024 quads). K: rows of the matrix hold the
+// summed index, and the tile's 128 rows of 64 are placed by (piece ^ row % 8), so
+// that 8 lanes reading one column of pieces touch all banks once. Not K: the
+// matrix's rows are the summed index; 64 rows of 128, 32-byte pieces placed by
+// (piece ^ row % 8), read through the transposing LDS load: in a group of 16
+// lanes, lane s reads 4 values of row s / 4 at column 4 (s % 4), and lane g gets
+// column g of the 4 rows.
+template <bool K>
+struct Side {
+    quad r[4];
+    __device__ __forceinline__ void fetch(const Mat& m, int part, int64_t row0, int64_t k) {
+        const bf16* p = m.p + part * m.plane + (K ? row0 * m.ld + k : k * m.ld + row0);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int e = t + j * kThreads, r = e >> 3, c = e & 7;
-            ra[j] = *reinterpret_cast<const quad*>(pa + r * A.ld + c * 8);
-            rb[j] = *reinterpret_cast<const quad*>(pb + r * B.ld + c * 8);
+            const int e = threadIdx.x + j * kThreads;
+            const int row = K ? e >> 3 : e >> 4, c = K ? e & 7 : e & 15;
+            r[j] = *reinterpret_cast<const quad*>(p + row * m.ld + c * 8);
         }
-    };
-    auto keep = [&](int buf) {
+    }
+    __device__ __forceinline__ void keep(quad* lds) const {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int e = t + j * kThreads, r = e >> 3, c = e & 7;
-            lds[buf][0][r * 8 + (c ^ (r & 7))] = ra[j];
-            lds[buf][1][r * 8 + (c ^ (r & 7))] = rb[j];
+            const int e = threadIdx.x + j * kThreads;
+            const int row = K ? e >> 3 : e >> 4, c = K ? e & 7 : e & 15;
+            lds[K ? row * 8 + (c ^ (row & 7)) : row * 16 + ((c ^ ((row & 7) << 1)))] = r[j];
+        }
+    }
+    // the operand of rows b .. b + 15, summed index 32 h .. 32 h + 31
+    __device__ __forceinline__ static bf16x8 operand(const quad* lds, int b, int h) {
+        const int lane = threadIdx.x & 63, g = lane >> 4;
+        if (K) {
+            const int row = b + (lane & 15), c = h * 4 + g;
+            return __builtin_bit_cast(bf16x8, lds[row * 8 + (c ^ (row & 7))]);
+        }
+        typedef __attribute__((ext_vector_type(4))) short s16x4;
+        typedef __attribute__((address_space(3))) s16x4* lds4;
+        const int s = lane & 15, row = h * 32 + g * 8 + (s >> 2);
+        const char* at = reinterpret_cast<const char*>(lds) + (s & 3) * 8;
+        s16x4 half[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int r = row + 4 * u;
+            half[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds4)(at + r * 256 + (((b >> 4) ^ (r & 7)) * 32)));
+        }
+        return __builtin_bit_cast(
+            bf16x8, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+};
+
+// Tiles of A B^T one after the other for one workgroup: 4 waves of 64 x 64, 64 of
+// the summed index a step, the next step's operands on their way from memory
+// while this one's are multiplied, also across tiles. `rows(tile)` gives the
+// tile's first rows of A and B; `done(tile, acc)` takes its 128 x 128 sums.
+#define GS_TILE_LDS __shared__ quad lds[2][2][kTile * 8]
+template <int NP, bool AK, bool BK, class Rows, class Done>
+__device__ __forceinline__ void tile_products(const Mat& A, const Mat& B, int64_t k0, int64_t k1,
+                                              int tiles, quad (*lds)[2][kTile * 8], Rows rows,
+                                              Done done) {
+    const int w = threadIdx.x >> 6, wm = (w >> 1) * 64, wn = (w & 1) * 64;
+    const int steps_k = (int)((k1 - k0) / kStep), per_tile = steps_k * Products<NP>::kCount;
+    Side<AK> a;
+    Side<BK> b;
+    int tile_f = 0, q_f = 0, k_f = 0;  // the next step to fetch
+    auto fetch = [&] {
+        const auto at = rows(tile_f);
+        const int64_t k = k0 + (int64_t)k_f * kStep;
+        a.fetch(A, Products<NP>::a(q_f), at.m, k);
+        b.fetch(B, Products<NP>::b(q_f), at.n, k);
+        if (++k_f == steps_k) {
+            k_f = 0;
+            if (++q_f == Products<NP>::kCount) {
+                q_f = 0;
+                ++tile_f;
+            }
         }
     };
-    if (steps == 0) return;
-    fetch(0);
-    keep(0);
+    f32x4 acc[4][4];
+    auto clear = [&] {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    };
+    clear();
+    const int steps = per_tile * tiles;
+    if (steps > 0) {
+        fetch();
+        a.keep(lds[0][0]);
+        b.keep(lds[0][1]);
+    }
     __syncthreads();
+    int left = per_tile, tile = 0;
     for (int s = 0; s < steps; ++s) {
         const int buf = s & 1;
-        if (s + 1 < steps) fetch(s + 1);
+        if (s + 1 < steps) fetch();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            quad fa[4], fb[4];
+            bf16x8 fa[4], fb[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int c = h * 4 + (lane >> 4);
-                const int r = wm + i * 16 + (lane & 15), n = wn + i * 16 + (lane & 15);
-                fa[i] = lds[buf][0][r * 8 + (c ^ (r & 7))];
-                fb[i] = lds[buf][1][n * 8 + (c ^ (n & 7))];
+                fa[i] = Side<AK>::operand(lds[buf][0], wm + i * 16, h);
+                fb[i] = Side<BK>::operand(lds[buf][1], wn + i * 16, h);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                        __builtin_bit_cast(bf16x8, fa[i]), __builtin_bit_cast(bf16x8, fb[j]),
-                        acc[i][j], 0, 0, 0);
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], fb[j], acc[i][j], 0,
+                                                                        0, 0);
         }
-        if (s + 1 < steps) keep(buf ^ 1);
+        if (s + 1 < steps) {
+            a.keep(lds[buf ^ 1][0]);
+            b.keep(lds[buf ^ 1][1]);
+        }
+        if (--left == 0) {
+            done(tile++, acc);
+            clear();
+            left = per_tile;
+        }
         __syncthreads();
+    }
+    if (steps == 0) done(0, acc);
+}
+
+struct TileRows {
+    int64_t m, n;
+};
+
+// Scores of one tile of samples (columns) against a share of the table's tiles: a
+// lane keeps the largest and the sum of exp2(score - largest) of its 4 samples,
+// scores in log2 units, and joins the other lanes' at the end. A largest that is
+// infinite is taken as 0, so that infinite scores give infinite sums.
+template <int NP>
+__global__ __launch_bounds__(kThreads, 2) void k_loss_scores(Mat F, Mat T, int kd, int64_t rows,
+                                                          float scale2, const int32_t* label,
+                                                          int64_t padded, int tiles, int share,
+                                                          float2* part, float* label_score) {
+    GS_TILE_LDS;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int wm = (w >> 1) * 64, wn = (w & 1) * 64;
+    const int64_t n0 = (int64_t)blockIdx.x * kTile;
+    const int t0 = blockIdx.y * share, t1 = min(tiles, t0 + share);
+    float m[4], sum[4];
+    int32_t y[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        m[n] = -1e30f;
+        sum[n] = 0.0f;
+        y[n] = label[n0 + wn + n * 16 + (lane & 15)];
+    }
+    tile_products<NP, true, true>(
+        T, F, 0, kd, t1 - t0, lds,
+        [&](int t) { return TileRows{(int64_t)(t0 + t) * kTile, n0}; },
+        [&](int t, f32x4(&acc)[4][4]) {
+            const int64_t v0 = (int64_t)(t0 + t) * kTile + wm + (lane >> 4) * 4;
+            const int64_t v_wave = (int64_t)(t0 + t) * kTile + wm;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[i][n] *= scale2;
+                if (v_wave + 64 > rows) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (v0 + i * 16 + j >= rows) acc[i][n][j] = -INFINITY;
+                }
+                if (__any(y[n] >= v_wave && y[n] < v_wave + 64)) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (v0 + i * 16 + j == y[n])
+                                label_score[n0 + wn + n * 16 + (lane & 15)] = acc[i][n][j];
+                }
+                float mt = m[n];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) mt = fmaxf(mt, acc[i][n][j]);
+                const float base = mt < INFINITY ? mt : 0.0f;
+                const float was = m[n] < INFINITY ? m[n] : 0.0f;
+                float add = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        add += __builtin_amdgcn_exp2f(acc[i][n][j] - base);
+                sum[n] = sum[n] * __builtin_amdgcn_exp2f(was - base) + add;
+                m[n] = mt;
+            }
+        });
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+#pragma unroll
+        for (int o = 16; o < 64; o <<= 1) {
+            const float m2 = __shfl_xor(m[n], o, 64), s2 = __shfl_xor(sum[n], o, 64);
+            const float mm = fmaxf(m[n], m2), base = mm < INFINITY ? mm : 0.0f;
+            sum[n] = sum[n] * __builtin_amdgcn_exp2f((m[n] < INFINITY ? m[n] : 0.0f) - base) +
+                     s2 * __builtin_amdgcn_exp2f((m2 < INFINITY ? m2 : 0.0f) - base);
+            m[n] = mm;
+        }
+        if (lane < 16)
+            part[((int64_t)blockIdx.y * 2 + (w >> 1)) * padded + n0 + wn + n * 16 + lane] =
+                make_float2(m[n], sum[n]);
     }
 }
 
-#define GS_TILE_LDS __shared__ quad lds[2][2][kTile * 8]
-#define GS_TILE_ACC                    \
-    f32x4 acc[4][4];                   \
-    for (int i = 0; i < 4; ++i)        \
-        for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}
-
-// Per (64 columns, row): largest score and sum of exp2(score - largest), scores
-// in log2 units; and the label's own score. A largest that is not finite is
-// taken as 0, so that infinite scores give infinite sums.
-template <int NP>
-__global__ __launch_bounds__(kThreads) void k_loss_scores(Mat F, Mat T, int kd, int64_t rows,
-                                                          float scale2, const int32_t* label,
-                                                          int64_t padded, float2* part,
-                                                          float* label_score) {
-    GS_TILE_LDS;
-    GS_TILE_ACC;
-    const int64_t m0 = (int64_t)blockIdx.x * kTile, n0 = (int64_t)blockIdx.y * kTile;
-    tile_product<NP>(F, T, m0, n0, 0, kd, lds, acc);
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int wm = (w >> 1) * 64, wn = (w & 1) * 64;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t r = m0 + wm + i * 16 + (lane >> 4) * 4 + j;
-            const int32_t y = label[r];
-            float s[4], m = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int64_t v = n0 + wn + k * 16 + (lane & 15);
-                s[k] = v < rows ? acc[i][k][j] * scale2 : -INFINITY;
-                if (v == y) label_score[r] = s[k];
-                m = fmaxf(m, s[k]);
-            }
-            for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-            const float base = fabsf(m) < INFINITY ? m : 0.0f;
-            float sum = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) sum += exp2f(s[k] - base);
-            for (int o = 1; o < 16; o <<= 1) sum += __shfl_xor(sum, o, 64);
-            if ((lane & 15) == 0)
-                part[((int64_t)blockIdx.y * 2 + (w & 1)) * padded + r] = make_float2(m, sum);
-        }
-}
-
-// Joins a row's partials; lse2 is kept in log2 units for the gradients.
+// Joins the partials of a row's scores: 8 lanes a row. lse2 is kept in log2 units
+// for the gradients.
 __global__ __launch_bounds__(kThreads) void k_loss_join(LossArgs a, const float2* part, int parts,
                                                         int64_t padded, const int32_t* label,
                                                         const float* label_score, float* lse2) {
-    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (i >= padded) return;
-    float m = -INFINITY;
-    for (int k = 0; k < parts; ++k) m = fmaxf(m, part[k * padded + i].x);
-    const float base = fabsf(m) < INFINITY ? m : 0.0f;
-    float sum = 0.0f;
-    for (int k = 0; k < parts; ++k) {
-        const float2 p = part[k * padded + i];
-        sum += p.y * exp2f((fabsf(p.x) < INFINITY ? p.x : 0.0f) - base);
+    const int sub = threadIdx.x >> 5;  // of the workgroup's 32 rows
+    const int64_t i = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
+    __shared__ float2 lds[8][32];
+    float m = -1e30f, sum = 0.0f;
+    if (i < padded)
+        for (int k0 = sub; k0 < parts; k0 += 8 * 4) {
+            float2 p[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                p[u] = k0 + u * 8 < parts ? part[(int64_t)(k0 + u * 8) * padded + i]
+                                          : make_float2(-1e30f, 0.0f);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const float mm = fmaxf(m, p[u].x), base = mm < INFINITY ? mm : 0.0f;
+                sum = sum * __builtin_amdgcn_exp2f((m < INFINITY ? m : 0.0f) - base) +
+                      p[u].y * __builtin_amdgcn_exp2f((p[u].x < INFINITY ? p[u].x : 0.0f) - base);
+                m = mm;
+            }
+        }
+    lds[sub][threadIdx.x & 31] = make_float2(m, sum);
+    __syncthreads();
+    if (sub != 0 || i >= padded) return;
+    for (int k = 1; k < 8; ++k) {
+        const float2 p = lds[k][threadIdx.x & 31];
+        const float mm = fmaxf(m, p.x), base = mm < INFINITY ? mm : 0.0f;
+        sum = sum * __builtin_amdgcn_exp2f((m < INFINITY ? m : 0.0f) - base) +
+              p.y * __builtin_amdgcn_exp2f((p.x < INFINITY ? p.x : 0.0f) - base);
+        m = mm;
     }
-    const float l = base + log2f(sum);
+    const float l = (m < INFINITY ? m : 0.0f) + log2f(sum);
     const bool on = label[i] >= 0;
     if (lse2 != nullptr) lse2[i] = on ? l : 0.0f;
     if (i < a.n) {
@@ -289,93 +399,172 @@ __global__ __launch_bounds__(kThreads) void k_loss_join(LossArgs a, const float2
     }
 }
 
-// G of one piece (rows r0.., table rows v0..) and its transpose, in parts.
+// exp2 of a gradient's exponent. The bare instruction gives 0 below 2^-126, which
+// fp32 gradients, times weight * scale, would show; for bf16 ones it is left so.
 template <int NP>
-__global__ __launch_bounds__(kThreads) void k_loss_g(Mat F, Mat T, int kd, int64_t rows,
+__device__ __forceinline__ float grad_exp2(float x) {
+    return NP == 1 ? __builtin_amdgcn_exp2f(x) : exp2f(x);
+}
+
+// G of one piece (samples r0.., table rows v0..) in parts, (rc, vc) each.
+template <int NP>
+__global__ __launch_bounds__(kThreads, 2) void k_loss_g(Mat F, Mat T, int kd, int64_t rows,
                                                      float scale2, const int32_t* label,
                                                      const float* weight, const float* lse2,
                                                      int64_t r0, int64_t v0, int64_t rc, int64_t vc,
-                                                     bf16* G, bf16* GT) {
+                                                     int share, bf16* G) {
     GS_TILE_LDS;
-    GS_TILE_ACC;
-    const int64_t m0 = (int64_t)blockIdx.x * kTile, n0 = (int64_t)blockIdx.y * kTile;
-    tile_product<NP>(F, T, r0 + m0, v0 + n0, 0, kd, lds, acc);
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int wm = (w >> 1) * 64, wn = (w & 1) * 64;
+    const int64_t n0 = (int64_t)blockIdx.x * kTile;
+    const int t0 = blockIdx.y * share, t1 = min((int)(vc / kTile), t0 + share);
+    int32_t y[4];
+    float wt[4], l2[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t rl = m0 + wm + i * 16 + (lane >> 4) * 4;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int64_t vl = n0 + wn + k * 16 + (lane & 15);
-            bf16 g[4][NP];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int64_t r = r0 + rl + j;
-                const int32_t y = label[r];
-                float v = 0.0f;
-                if (y >= 0 && v0 + vl < rows)
-                    v = weight[r] * (exp2f(acc[i][k][j] * scale2 - lse2[r]) -
-                                     (v0 + vl == y ? 1.0f : 0.0f));
-                split<NP>(v, g[j]);
-            }
-#pragma unroll
-            for (int p = 0; p < NP; ++p) {
-                VecOf<bf16, 4> u;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    u.v[j] = g[j][p];
-                    G[p * rc * vc + (rl + j) * vc + vl] = g[j][p];
-                }
-                *reinterpret_cast<VecOf<bf16, 4>*>(GT + p * rc * vc + vl * rc + rl) = u;
-            }
-        }
+    for (int n = 0; n < 4; ++n) {
+        const int64_t i = r0 + n0 + wn + n * 16 + (lane & 15);
+        y[n] = label[i];
+        wt[n] = weight[i];
+        l2[n] = lse2[i];
     }
+    tile_products<NP, true, true>(
+        T, F, 0, kd, t1 - t0, lds,
+        [&](int t) { return TileRows{v0 + (int64_t)(t0 + t) * kTile, r0 + n0}; },
+        [&](int t, f32x4(&acc)[4][4]) {
+            const int64_t tile = (int64_t)(t0 + t) * kTile + wm;  // within the piece
+            const int64_t at = tile + (lane >> 4) * 4;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const bool any = __any(y[n] >= v0 + tile && y[n] < v0 + tile + 64);
+                bf16* row = G + (n0 + wn + n * 16 + (lane & 15)) * vc + at;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float v[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        v[j] = grad_exp2<NP>(fmaf(acc[i][n][j], scale2, -l2[n]));
+                    if (any) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (v0 + at + i * 16 + j == y[n]) v[j] -= 1.0f;
+                    }
+                    const bool in = v0 + tile + 64 <= rows;  // else some rows are padding
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        v[j] = y[n] >= 0 && (in || v0 + at + i * 16 + j < rows) ? v[j] * wt[n] : 0.0f;
+                    uint32_t p0[NP], p1[NP];
+                    split2<NP>(v[0], v[1], p0);
+                    split2<NP>(v[2], v[3], p1);
+#pragma unroll
+                    for (int p = 0; p < NP; ++p)
+                        *reinterpret_cast<uint2*>(row + p * rc * vc + i * 16) =
+                            make_uint2(p0[p], p1[p]);
+                }
+            }
+        });
 }
 
-// slices[z] (m, dq) = A B^T over the z-th share of the summed index.
-template <int NP>
-__global__ __launch_bounds__(kThreads) void k_loss_sum(Mat A, Mat B, int64_t k, int64_t share,
-                                                       int64_t m, int dq, float* slices) {
+// Where a product's sums go: with one share of the summed index onto the earlier
+// pieces' (`sum`), and with the last piece, rounded, into the caller's rows, masked
+// rows as zeros; with several shares each into its slice, for k_loss_fold.
+template <typename T>
+struct SumOut {
+    float* slices;
+    float* sum;
+    int first, last;
+    int64_t m;
+    int dq;
+    T* out;
+    int64_t rows, stride;
+    int dim;
+    const int32_t* label;
+    __device__ __forceinline__ void put(int64_t r, int c, float v) const {
+        if (!first) v += sum[r * dq + c];
+        if (!last)
+            sum[r * dq + c] = v;
+        else if (r < rows && c < dim)
+            out[r * stride + c] = from_float<T>(label != nullptr && label[r] < 0 ? 0.0f : v);
+    }
+};
+
+// A share (blockIdx.z) of A B over the summed index, for 128 x 128 sums. A: G, by
+// samples (AK) or transposed; B's rows are the summed index.
+template <typename T, int NP, bool AK>
+__global__ __launch_bounds__(kThreads, 2) void k_loss_sum(Mat A, Mat B, int64_t k, int64_t share,
+                                                       SumOut<T> o) {
     GS_TILE_LDS;
-    GS_TILE_ACC;
     const int64_t m0 = (int64_t)blockIdx.x * kTile, n0 = (int64_t)blockIdx.y * kTile;
     const int64_t k0 = min(k, share * blockIdx.z), k1 = min(k, k0 + share);
-    tile_product<NP>(A, B, m0, n0, k0, k1, lds, acc);
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int wm = (w >> 1) * 64, wn = (w & 1) * 64;
-    float* out = slices + (size_t)blockIdx.z * m * dq;
+    tile_products<NP, AK, false>(
+        A, B, k0, k1, 1, lds, [&](int) { return TileRows{m0, n0}; },
+        [&](int, f32x4(&acc)[4][4]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+                for (int n = 0; n < 4; ++n)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                out[(m0 + wm + i * 16 + (lane >> 4) * 4 + j) * dq + n0 + wn + n * 16 + (lane & 15)] =
-                    acc[i][n][j];
+                    for (int j = 0; j < 4; ++j) {
+                        const int64_t r = m0 + wm + i * 16 + (lane >> 4) * 4 + j;
+                        const int c = (int)n0 + wn + n * 16 + (lane & 15);
+                        if (gridDim.z > 1)
+                            o.slices[((int64_t)blockIdx.z * o.m + r) * o.dq + c] = acc[i][n][j];
+                        else
+                            o.put(r, c, acc[i][n][j]);
+                    }
+        });
 }
 
-// Adds the slices in order (and the earlier pieces' sum), and rounds the last
-// sum into the caller's rows; masked rows get zeros.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void k_loss_fold(const float* slices, int nz, int64_t m,
-                                                        int dq, float* sum, int first, int last,
-                                                        T* out, int64_t rows, int64_t stride,
-                                                        int dim, const int32_t* label) {
-    const int64_t total = m * dq;
-    for (int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x; e < total;
-         e += (int64_t)gridDim.x * kThreads) {
-        float s = first ? 0.0f : sum[e];
-        for (int z = 0; z < nz; ++z) s += slices[(size_t)z * total + e];
-        if (!last) {
-            sum[e] = s;
-            continue;
+// Adds nz slices (m, dq) in order: 4 columns a thread, the slices over Z threads.
+template <typename T, int Z>
+__global__ __launch_bounds__(kThreads) void k_loss_fold(SumOut<T> o, int nz) {
+    __shared__ f32x4 lds[Z > 1 ? kThreads : 1];
+    constexpr int kItems = kThreads / Z;
+    const int64_t total = o.m * (o.dq / 4);
+    const int z0 = threadIdx.x / kItems;
+    for (int64_t e0 = (int64_t)blockIdx.x * kItems; e0 < total; e0 += (int64_t)gridDim.x * kItems) {
+        const int64_t e = e0 + threadIdx.x % kItems;
+        f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (e < total)
+            for (int z = z0; z < nz; z += Z * 4) {
+                f32x4 v[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    v[u] = z + u * Z < nz ? reinterpret_cast<const f32x4*>(
+                                                o.slices)[(int64_t)(z + u * Z) * total + e]
+                                          : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int u = 0; u < 4; ++u) s += v[u];
+            }
+        if (Z > 1) {
+            __syncthreads();
+            lds[threadIdx.x] = s;
+            __syncthreads();
+            if (z0 != 0) continue;
+            for (int z = 1; z < Z; ++z) s += lds[z * kItems + threadIdx.x];
         }
-        const int64_t r = e / dq;
-        const int c = (int)(e - r * dq);
-        if (r < rows && c < dim)
-            out[r * stride + c] = from_float<T>(label != nullptr && label[r] < 0 ? 0.0f : s);
+        if (e >= total) continue;
+        const int64_t r = e / (o.dq / 4);
+        const int c = (int)(e - r * (o.dq / 4)) * 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o.put(r, c + j, s[j]);
     }
+}
+
+unsigned blocks_for(int64_t items) {
+    const int64_t b = (items + kThreads - 1) / kThreads;
+    return (unsigned)(b < 65536 ? b : 65536);
+}
+
+template <typename T>
+hipError_t fold(const SumOut<T>& o, int nz, hipStream_t st) {
+    const int64_t items = o.m * (o.dq / 4);
+    if (nz <= 8)
+        k_loss_fold<T, 1><<<blocks_for(items), kThreads, 0, st>>>(o, nz);
+    else
+        k_loss_fold<T, 16><<<blocks_for(items * 16), kThreads, 0, st>>>(o, nz);
+    return hipGetLastError();
 }
 
 // ---------------------------------------------------------------- streaming
@@ -424,25 +613,8 @@ struct StreamArgs {
     int64_t padded;
 };
 
-// exp2 of a gradient's exponent. The bare instruction gives 0 below 2^-126, which
-// fp32 gradients, times weight * scale, would show; for bf16 ones it is left so.
-template <int NP>
-__device__ __forceinline__ float grad_exp2(float x) {
-    return NP == 1 ? __builtin_amdgcn_exp2f(x) : exp2f(x);
-}
-
 // Key of register r of a lane in half h.
 __device__ __forceinline__ constexpr int key_of(int r) { return (r & 3) + 8 * (r >> 2); }
-
-// A row's 8 values from column c, cut into parts; zeros past the row.
-template <typename T, int NP>
-__device__ __forceinline__ void load_parts(const T* row, int dim, int c, bool on, quad* out) {
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-        v[e] = on && c + e < dim ? plain_input<NP>(to_float(row[c + e])) : 0.0f;
-    split8<NP>(v, out);
-}
 
 // (rows, dim) as tiles of operands, one workgroup a tile; of samples (label) the
 // masked ones are zeros, and label and weight are written for the gradients.
@@ -766,21 +938,22 @@ __global__ __launch_bounds__(kThreads, (NP * KD >= (ROLE == kScores ? 256 : 128)
 // ---------------------------------------------------------------- pieces
 int64_t pad_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
-// Pieces of G: up to 8192 table rows by as many rows as make 2^26 values
-// (128 MB and as much for the transpose), which the cache behind the L2s holds.
+// Pieces of G: up to 8192 table rows by as many samples as make 2^27 values (256 MB
+// of bf16, what the cache behind the L2s holds), a third of that in three parts.
 struct LossPlan {
     int np, kd, dq;
     int64_t np_rows, vp, rc, vc;
-    int zf, zt;  // shares of the summed index: for dfeat and for dtable
+    int shares, share;    // of the table's tiles, for the scores
+    int zf, zt;           // of the summed index: for dfeat and for dtable
     int64_t share_f, share_t;
-    bf16 *F, *T, *FT, *TT, *G, *GT;
+    bf16 *F, *T, *G;
     float2* part;
     float *score, *lse2, *weight, *slices, *sum_f, *sum_t;
     int32_t* label;
     size_t bytes;
 
-    static void shares(int64_t tiles, int64_t k, int* z, int64_t* share) {
-        int64_t want = tiles >= 512 ? 1 : (512 + tiles - 1) / tiles;
+    static void split_k(int64_t tiles, int64_t k, int* z, int64_t* share) {
+        int64_t want = tiles >= 384 ? 1 : (512 + tiles - 1) / tiles;
         want = std::min<int64_t>(want, std::max<int64_t>(1, k / 512));
         *share = pad_to((k + want - 1) / want, kStep);
         *z = (int)((k + *share - 1) / *share);
@@ -792,35 +965,87 @@ struct LossPlan {
         np_rows = pad_to(n, kTile);
         vp = pad_to(rows, kTile);
         vc = std::min<int64_t>(vp, 8192);
-        rc = std::min<int64_t>(np_rows, std::max<int64_t>(kTile, ((1 << 26) / np / vc) / kTile * kTile));
-        shares(rc / kTile * (dq / kTile), vc, &zf, &share_f);
-        shares(vc / kTile * (dq / kTile), rc, &zt, &share_t);
+        rc = std::min<int64_t>(np_rows, std::max<int64_t>(kTile, ((1 << 27) / np / vc) / kTile * kTile));
+        split_k(rc / kTile * (dq / kTile), vc, &zf, &share_f);
+        split_k(vc / kTile * (dq / kTile), rc, &zt, &share_t);
+        // scores: about 4096 workgroups, where that leaves 8 tiles each
+        const int64_t tiles = vp / kTile, groups = np_rows / kTile;
+        const int64_t want = std::max<int64_t>(
+            1, std::min(tiles / (groups < 64 ? 1 : 8), (4096 + groups - 1) / std::max<int64_t>(groups, 1)));
+        share = (int)((tiles + want - 1) / want);
+        shares = (int)((tiles + share - 1) / share);
         Carve c(base);
-        F = c.take<bf16>((size_t)np * np_rows * kd);
-        T = c.take<bf16>((size_t)np * vp * kd);
-        part = c.take<float2>((size_t)(vp / 64) * np_rows);
+        F = c.take<bf16>((size_t)np * np_rows * dq);
+        T = c.take<bf16>((size_t)np * vp * dq);
+        part = c.take<float2>((size_t)shares * 2 * np_rows);
         score = c.take<float>((size_t)np_rows);
         label = c.take<int32_t>((size_t)np_rows);
-        FT = TT = G = GT = nullptr;
+        G = nullptr;
         lse2 = weight = slices = sum_f = sum_t = nullptr;
         if (grad) {
-            FT = c.take<bf16>((size_t)np * np_rows * dq);
-            TT = c.take<bf16>((size_t)np * vp * dq);
             lse2 = c.take<float>((size_t)np_rows);
             weight = c.take<float>((size_t)np_rows);
             G = c.take<bf16>((size_t)np * rc * vc);
-            GT = c.take<bf16>((size_t)np * rc * vc);
-            slices = c.take<float>(std::max((size_t)zf * rc * dq, (size_t)zt * vc * dq));
-            sum_f = c.take<float>((size_t)rc * dq);
-            sum_t = c.take<float>((size_t)vp * dq);
+            slices = c.take<float>(std::max((size_t)(zf > 1 ? zf : 0) * rc * dq,
+                                            (size_t)(zt > 1 ? zt : 0) * vc * dq));
+            sum_f = c.take<float>(vp > vc ? (size_t)rc * dq : 0);
+            sum_t = c.take<float>(np_rows > rc ? (size_t)vp * dq : 0);
         }
         bytes = c.bytes();
     }
 };
 
-unsigned blocks_for(int64_t items) {
-    const int64_t b = (items + kThreads - 1) / kThreads;
-    return (unsigned)(b < 65536 ? b : 65536);
+template <typename T, int NP>
+hipError_t loss_run(const LossArgs& a, bool grad, hipStream_t st) {
+    const LossPlan w(a.ws, a.n, a.rows, a.dim, a.dtype, grad);
+    const int64_t nr = w.np_rows;
+    const T* feat = static_cast<const T*>(a.feat);
+    const T* table = static_cast<const T*>(a.table);
+    const float scale2 = a.scale * kLog2e;
+    k_loss_rows<<<(unsigned)((nr + kThreads - 1) / kThreads), kThreads, 0, st>>>(a, nr, w.label,
+                                                                                 w.weight);
+    k_parts<T, NP><<<blocks_for(nr * w.dq / 8), kThreads, 0, st>>>(
+        feat, a.n, a.feat_stride, a.dim, w.label, nr, w.dq, reinterpret_cast<quad*>(w.F));
+    k_parts<T, NP><<<blocks_for(w.vp * w.dq / 8), kThreads, 0, st>>>(
+        table, a.rows, a.table_stride, a.dim, nullptr, w.vp, w.dq, reinterpret_cast<quad*>(w.T));
+    const Mat F{w.F, w.dq, nr * w.dq}, Tm{w.T, w.dq, w.vp * w.dq};
+    k_loss_scores<NP><<<dim3((unsigned)(nr / kTile), (unsigned)w.shares), kThreads, 0, st>>>(
+        F, Tm, w.kd, a.rows, scale2, w.label, nr, (int)(w.vp / kTile), w.share, w.part, w.score);
+    k_loss_join<<<(unsigned)((nr + 31) / 32), kThreads, 0, st>>>(a, w.part, w.shares * 2, nr,
+                                                                 w.label, w.score, w.lse2);
+    hipError_t e = hipGetLastError();
+    if (!grad || e != hipSuccess) return e;
+    for (int64_t r0 = 0; r0 < nr; r0 += w.rc) {
+        const int64_t rc = std::min(w.rc, nr - r0);
+        for (int64_t v0 = 0; v0 < w.vp; v0 += w.vc) {
+            const int64_t vc = std::min(w.vc, w.vp - v0);
+            // 8 tiles a workgroup where that leaves two workgroups a compute unit
+            const int share = (int)std::max<int64_t>(
+                1, std::min<int64_t>(8, rc / kTile * (vc / kTile) / 512));
+            k_loss_g<NP><<<dim3((unsigned)(rc / kTile), (unsigned)((vc / kTile + share - 1) / share)),
+                           kThreads, 0, st>>>(F, Tm, w.kd, a.rows, scale2, w.label, w.weight, w.lse2,
+                                              r0, v0, rc, vc, share, w.G);
+            const Mat G{w.G, vc, rc * vc};
+            const int zf = (int)((vc + w.share_f - 1) / w.share_f);
+            const SumOut<T> of{w.slices, w.sum_f, v0 == 0, v0 + vc >= w.vp, rc, w.dq,
+                               static_cast<T*>(a.dfeat) + r0 * a.dfeat_stride, a.n - r0,
+                               a.dfeat_stride, a.dim, w.label + r0};
+            k_loss_sum<T, NP, true>
+                <<<dim3((unsigned)(rc / kTile), (unsigned)(w.dq / kTile), zf), kThreads, 0, st>>>(
+                    G, {w.T + v0 * w.dq, w.dq, w.vp * w.dq}, vc, w.share_f, of);
+            if (zf > 1 && (e = fold(of, zf, st)) != hipSuccess) return e;
+            const int zt = (int)((rc + w.share_t - 1) / w.share_t);
+            const SumOut<T> ot{w.slices, w.sum_t + (w.sum_t != nullptr ? v0 * w.dq : 0), r0 == 0,
+                               r0 + rc >= nr, vc, w.dq,
+                               static_cast<T*>(a.dtable) + v0 * a.dtable_stride, a.rows - v0,
+                               a.dtable_stride, a.dim, nullptr};
+            k_loss_sum<T, NP, false>
+                <<<dim3((unsigned)(vc / kTile), (unsigned)(w.dq / kTile), zt), kThreads, 0, st>>>(
+                    G, {w.F + r0 * w.dq, w.dq, nr * w.dq}, rc, w.share_t, ot);
+            if (zt > 1 && (e = fold(ot, zt, st)) != hipSuccess) return e;
+        }
+    }
+    return hipGetLastError();
 }
 
 // Joins the shares' partials of a row's scores.
@@ -959,10 +1184,12 @@ hipError_t stream_run(const LossArgs& a, bool grad, hipStream_t st) {
     s.sums = w.sums;
     e = launch_stream<T, NP, KD, kGradFeat>(s, w.by_feat, st);
     if (e != hipSuccess) return e;
-    if (w.by_feat.count > 1)
-        k_loss_fold<T><<<blocks_for(a.n * KD), kThreads, 0, st>>>(
-            w.sums, w.by_feat.count, a.n, KD, nullptr, 1, 1, static_cast<T*>(a.dfeat), a.n,
-            a.dfeat_stride, a.dim, w.label);
+    if (w.by_feat.count > 1) {
+        e = fold(SumOut<T>{w.sums, nullptr, 1, 1, a.n, KD, static_cast<T*>(a.dfeat), a.n,
+                       a.dfeat_stride, a.dim, w.label},
+             w.by_feat.count, st);
+        if (e != hipSuccess) return e;
+    }
     s.q = table;
     s.nq = a.rows;
     s.q_stride = a.table_stride;
@@ -976,9 +1203,9 @@ hipError_t stream_run(const LossArgs& a, bool grad, hipStream_t st) {
     e = launch_stream<T, NP, KD, kGradTable>(s, w.by_table, st);
     if (e != hipSuccess) return e;
     if (w.by_table.count > 1)
-        k_loss_fold<T><<<blocks_for(a.rows * KD), kThreads, 0, st>>>(
-            w.sums, w.by_table.count, a.rows, KD, nullptr, 1, 1, static_cast<T*>(a.dtable), a.rows,
-            a.dtable_stride, a.dim, nullptr);
+        return fold(SumOut<T>{w.sums, nullptr, 1, 1, a.rows, KD, static_cast<T*>(a.dtable), a.rows,
+                       a.dtable_stride, a.dim, nullptr},
+             w.by_table.count, st);
     return hipGetLastError();
 }
 
@@ -988,57 +1215,6 @@ int stream_kd(int dim, int dtype) {
     for (int kd : {32, 64, 128, 256})
         if (dim <= kd) return dtype == 0 && kd > 128 ? 0 : kd;
     return 0;
-}
-
-template <typename T, int NP>
-hipError_t loss_run(const LossArgs& a, bool grad, hipStream_t st) {
-    const LossPlan w(a.ws, a.n, a.rows, a.dim, a.dtype, grad);
-    const int64_t nr = w.np_rows;
-    const T* feat = static_cast<const T*>(a.feat);
-    const T* table = static_cast<const T*>(a.table);
-    const float scale2 = a.scale * kLog2e;
-    k_loss_rows<<<(unsigned)((nr + kThreads - 1) / kThreads), kThreads, 0, st>>>(a, nr, w.label,
-                                                                                 w.weight);
-    k_parts<T, NP><<<blocks_for(nr * w.kd), kThreads, 0, st>>>(feat, a.n, a.feat_stride, a.dim,
-                                                               w.label, nr, w.kd, w.F);
-    k_parts<T, NP><<<blocks_for(w.vp * w.kd), kThreads, 0, st>>>(
-        table, a.rows, a.table_stride, a.dim, nullptr, w.vp, w.kd, w.T);
-    const Mat F{w.F, w.kd, nr * w.kd}, Tm{w.T, w.kd, w.vp * w.kd};
-    const dim3 grid((unsigned)(nr / kTile), (unsigned)(w.vp / kTile));
-    k_loss_scores<NP><<<grid, kThreads, 0, st>>>(F, Tm, w.kd, a.rows, scale2, w.label, nr, w.part,
-                                                 w.score);
-    k_loss_join<<<(unsigned)((nr + kThreads - 1) / kThreads), kThreads, 0, st>>>(
-        a, w.part, (int)(w.vp / 64), nr, w.label, w.score, w.lse2);
-    if (!grad) return hipGetLastError();
-    k_parts_t<T, NP><<<dim3((unsigned)(nr / 32), (unsigned)(w.dq / 32)), kThreads, 0, st>>>(
-        feat, a.n, a.feat_stride, a.dim, w.label, nr, w.dq, w.FT);
-    k_parts_t<T, NP><<<dim3((unsigned)(w.vp / 32), (unsigned)(w.dq / 32)), kThreads, 0, st>>>(
-        table, a.rows, a.table_stride, a.dim, nullptr, w.vp, w.dq, w.TT);
-    for (int64_t r0 = 0; r0 < nr; r0 += w.rc) {
-        const int64_t rc = std::min(w.rc, nr - r0);
-        for (int64_t v0 = 0; v0 < w.vp; v0 += w.vc) {
-            const int64_t vc = std::min(w.vc, w.vp - v0);
-            k_loss_g<NP><<<dim3((unsigned)(rc / kTile), (unsigned)(vc / kTile)), kThreads, 0, st>>>(
-                F, Tm, w.kd, a.rows, scale2, w.label, w.weight, w.lse2, r0, v0, rc, vc, w.G, w.GT);
-            const int zf = (int)((vc + w.share_f - 1) / w.share_f);
-            k_loss_sum<NP><<<dim3((unsigned)(rc / kTile), (unsigned)(w.dq / kTile), zf), kThreads,
-                             0, st>>>({w.G, vc, rc * vc}, {w.TT + v0, w.vp, w.dq * w.vp}, vc,
-                                      w.share_f, rc, w.dq, w.slices);
-            k_loss_fold<T><<<blocks_for(rc * w.dq), kThreads, 0, st>>>(
-                w.slices, zf, rc, w.dq, w.sum_f, v0 == 0, v0 + vc >= w.vp,
-                static_cast<T*>(a.dfeat) + r0 * a.dfeat_stride, a.n - r0, a.dfeat_stride, a.dim,
-                w.label + r0);
-            const int zt = (int)((rc + w.share_t - 1) / w.share_t);
-            k_loss_sum<NP><<<dim3((unsigned)(vc / kTile), (unsigned)(w.dq / kTile), zt), kThreads,
-                             0, st>>>({w.GT, rc, rc * vc}, {w.FT + r0, nr, w.dq * nr}, rc,
-                                      w.share_t, vc, w.dq, w.slices);
-            k_loss_fold<T><<<blocks_for(vc * w.dq), kThreads, 0, st>>>(
-                w.slices, zt, vc, w.dq, w.sum_t + v0 * w.dq, r0 == 0, r0 + rc >= nr,
-                static_cast<T*>(a.dtable) + v0 * a.dtable_stride, a.rows - v0, a.dtable_stride,
-                a.dim, nullptr);
-        }
-    }
-    return hipGetLastError();
 }
 
 }  // namespace
@@ -1052,16 +1228,13 @@ size_t label_loss_ws(int64_t n, int64_t rows, int dim, int dtype, bool grad) {
 hipError_t launch_label_loss(const LossArgs& a, bool grad, hipStream_t st) {
     if (a.n == 0) {  // no rows: the table's gradient is 0
         if (!grad) return hipSuccess;
-        const unsigned b = blocks_for(a.rows * a.dim);
+        const int dq = (int)pad_to(a.dim, 4);
         if (a.dtype == 0)
-            k_loss_fold<float><<<b, kThreads, 0, st>>>(nullptr, 0, a.rows, a.dim, nullptr, 1, 1,
-                                                       static_cast<float*>(a.dtable), a.rows,
-                                                       a.dtable_stride, a.dim, nullptr);
-        else
-            k_loss_fold<bf16><<<b, kThreads, 0, st>>>(nullptr, 0, a.rows, a.dim, nullptr, 1, 1,
-                                                      static_cast<bf16*>(a.dtable), a.rows,
-                                                      a.dtable_stride, a.dim, nullptr);
-        return hipGetLastError();
+            return fold(SumOut<float>{nullptr, nullptr, 1, 1, a.rows, dq,
+                                      static_cast<float*>(a.dtable), a.rows, a.dtable_stride, a.dim,
+                                      nullptr}, 0, st);
+        return fold(SumOut<bf16>{nullptr, nullptr, 1, 1, a.rows, dq, static_cast<bf16*>(a.dtable),
+                                 a.rows, a.dtable_stride, a.dim, nullptr}, 0, st);
     }
     const bool f = a.dtype == 0;
     switch (stream_kd(a.dim, a.dtype)) {
