@@ -276,6 +276,15 @@ struct TileRows {
     int64_t m, n;
 };
 
+// Largest score and sum of exp2(score - largest) of two sets of scores, into the
+// first. A largest that is infinite counts as 0 there, so that the sum is infinite.
+__device__ __forceinline__ void join_sums(float& m, float& sum, float m2, float s2) {
+    const float mm = fmaxf(m, m2), base = mm < INFINITY ? mm : 0.0f;
+    sum = sum * __builtin_amdgcn_exp2f((m < INFINITY ? m : 0.0f) - base) +
+          s2 * __builtin_amdgcn_exp2f((m2 < INFINITY ? m2 : 0.0f) - base);
+    m = mm;
+}
+
 // Scores of one tile of samples (columns) against a share of the table's tiles: a
 // lane keeps the largest and the sum of exp2(score - largest) of its 4 samples,
 // scores in log2 units, and joins the other lanes' at the end. A largest that is
@@ -345,10 +354,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_loss_scores(Mat F, Mat T, int k
 #pragma unroll
         for (int o = 16; o < 64; o <<= 1) {
             const float m2 = __shfl_xor(m[n], o, 64), s2 = __shfl_xor(sum[n], o, 64);
-            const float mm = fmaxf(m[n], m2), base = mm < INFINITY ? mm : 0.0f;
-            sum[n] = sum[n] * __builtin_amdgcn_exp2f((m[n] < INFINITY ? m[n] : 0.0f) - base) +
-                     s2 * __builtin_amdgcn_exp2f((m2 < INFINITY ? m2 : 0.0f) - base);
-            m[n] = mm;
+            join_sums(m[n], sum[n], m2, s2);
         }
         if (lane < 16)
             part[((int64_t)blockIdx.y * 2 + (w >> 1)) * padded + n0 + wn + n * 16 + lane] =
@@ -356,42 +362,34 @@ __global__ __launch_bounds__(kThreads, 2) void k_loss_scores(Mat F, Mat T, int k
     }
 }
 
-// Joins the partials of a row's scores: 8 lanes a row. lse2 is kept in log2 units
-// for the gradients.
+// Joins the partials (parts, padded) of a row's scores: 8 threads a row. lse2, for
+// the gradients, is in log2 units.
 __global__ __launch_bounds__(kThreads) void k_loss_join(LossArgs a, const float2* part, int parts,
-                                                        int64_t padded, const int32_t* label,
-                                                        const float* label_score, float* lse2) {
+                                                        int64_t padded, const float* label_score,
+                                                        float* lse2) {
     const int sub = threadIdx.x >> 5;  // of the workgroup's 32 rows
     const int64_t i = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
     __shared__ float2 lds[8][32];
     float m = -1e30f, sum = 0.0f;
     if (i < padded)
-        for (int k0 = sub; k0 < parts; k0 += 8 * 4) {
-            float2 p[4];
+        for (int k0 = sub; k0 < parts; k0 += 8 * 8) {
+            float2 p[8];
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < 8; ++u)
                 p[u] = k0 + u * 8 < parts ? part[(int64_t)(k0 + u * 8) * padded + i]
                                           : make_float2(-1e30f, 0.0f);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const float mm = fmaxf(m, p[u].x), base = mm < INFINITY ? mm : 0.0f;
-                sum = sum * __builtin_amdgcn_exp2f((m < INFINITY ? m : 0.0f) - base) +
-                      p[u].y * __builtin_amdgcn_exp2f((p[u].x < INFINITY ? p[u].x : 0.0f) - base);
-                m = mm;
-            }
+            for (int u = 0; u < 8; ++u) join_sums(m, sum, p[u].x, p[u].y);
         }
     lds[sub][threadIdx.x & 31] = make_float2(m, sum);
     __syncthreads();
     if (sub != 0 || i >= padded) return;
     for (int k = 1; k < 8; ++k) {
         const float2 p = lds[k][threadIdx.x & 31];
-        const float mm = fmaxf(m, p.x), base = mm < INFINITY ? mm : 0.0f;
-        sum = sum * __builtin_amdgcn_exp2f((m < INFINITY ? m : 0.0f) - base) +
-              p.y * __builtin_amdgcn_exp2f((p.x < INFINITY ? p.x : 0.0f) - base);
-        m = mm;
+        join_sums(m, sum, p.x, p.y);
     }
     const float l = (m < INFINITY ? m : 0.0f) + log2f(sum);
-    const bool on = label[i] >= 0;
+    const bool on = i < a.n && load_id(a.labels, a.labels64, i, a.rows, nullptr) >= 0;
     if (lse2 != nullptr) lse2[i] = on ? l : 0.0f;
     if (i < a.n) {
         if (a.loss != nullptr) a.loss[i] = on ? (l - label_score[i]) * kLn2 : 0.0f;
@@ -889,23 +887,20 @@ __global__ __launch_bounds__(kThreads, (NP * KD >= (ROLE == kScores ? 256 : 128)
         for (int b = 0; b < 2; ++b) {
             const int64_t i = q0 + b * 32 + col;
             const float m2 = __shfl_xor(m[b], 32, 64), s2 = __shfl_xor(sum[b], 32, 64);
-            const float mm = fmaxf(m[b], m2), base = mm < INFINITY ? mm : 0.0f;
-            const float total =
-                sum[b] * __builtin_amdgcn_exp2f((m[b] < INFINITY ? m[b] : 0.0f) - base) +
-                s2 * __builtin_amdgcn_exp2f((m2 < INFINITY ? m2 : 0.0f) - base);
+            join_sums(m[b], sum[b], m2, s2);
             // the half that holds the label's score gives it to the other
             const bool here = y[b] >= 0 && ((y[b] >> 2) & 1) == h;
             const float o2 = __shfl_xor(own[b], 32, 64);
             const float mine = here ? own[b] : o2;
             if (h != 0 || i >= a.nq) continue;
             if (gridDim.y == 1) {
-                const float l = base + log2f(total);
+                const float l = (m[b] < INFINITY ? m[b] : 0.0f) + log2f(sum[b]);
                 const bool on = y[b] >= 0;
                 if (a.loss != nullptr) a.loss[i] = on ? (l - mine) * kLn2 : 0.0f;
                 if (a.lse != nullptr) a.lse[i] = on ? l * kLn2 : 0.0f;
                 if (a.lse2_out != nullptr) a.lse2_out[i] = on ? l : 0.0f;
             } else {
-                a.part[blockIdx.y * a.padded + i] = make_float2(mm, total);
+                a.part[blockIdx.y * a.padded + i] = make_float2(m[b], sum[b]);
                 if (y[b] >= (int64_t)t0 * 32 && y[b] < (int64_t)t1 * 32) a.label_score[i] = mine;
             }
         }
@@ -1012,7 +1007,7 @@ hipError_t loss_run(const LossArgs& a, bool grad, hipStream_t st) {
     k_loss_scores<NP><<<dim3((unsigned)(nr / kTile), (unsigned)w.shares), kThreads, 0, st>>>(
         F, Tm, w.kd, a.rows, scale2, w.label, nr, (int)(w.vp / kTile), w.share, w.part, w.score);
     k_loss_join<<<(unsigned)((nr + 31) / 32), kThreads, 0, st>>>(a, w.part, w.shares * 2, nr,
-                                                                 w.label, w.score, w.lse2);
+                                                                 w.score, w.lse2);
     hipError_t e = hipGetLastError();
     if (!grad || e != hipSuccess) return e;
     for (int64_t r0 = 0; r0 < nr; r0 += w.rc) {
@@ -1046,25 +1041,6 @@ hipError_t loss_run(const LossArgs& a, bool grad, hipStream_t st) {
         }
     }
     return hipGetLastError();
-}
-
-// Joins the shares' partials of a row's scores.
-__global__ __launch_bounds__(kThreads) void k_stream_join(StreamArgs a, int shares) {
-    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (i >= a.nq) return;
-    const bool on = load_id(a.labels, a.labels64, i, a.table_rows, nullptr) >= 0;
-    float m = -INFINITY;
-    for (int k = 0; k < shares; ++k) m = fmaxf(m, a.part[k * a.padded + i].x);
-    const float base = m < INFINITY ? m : 0.0f;
-    float sum = 0.0f;
-    for (int k = 0; k < shares; ++k) {
-        const float2 p = a.part[k * a.padded + i];
-        sum += p.y * __builtin_amdgcn_exp2f((p.x < INFINITY ? p.x : 0.0f) - base);
-    }
-    const float l = base + log2f(sum);
-    if (a.loss != nullptr) a.loss[i] = on ? (l - a.label_score[i]) * kLn2 : 0.0f;
-    if (a.lse != nullptr) a.lse[i] = on ? l * kLn2 : 0.0f;
-    if (a.lse2_out != nullptr) a.lse2_out[i] = on ? l : 0.0f;
 }
 
 // Shares of the streamed side: enough workgroups for the chip (two a compute
@@ -1173,8 +1149,8 @@ hipError_t stream_run(const LossArgs& a, bool grad, hipStream_t st) {
     e = launch_stream<T, NP, KD, kScores>(s, w.scores, st);
     if (e != hipSuccess) return e;
     if (w.scores.count > 1)
-        k_stream_join<<<(unsigned)((a.n + kThreads - 1) / kThreads), kThreads, 0, st>>>(
-            s, w.scores.count);
+        k_loss_join<<<(unsigned)((a.n + 31) / 32), kThreads, 0, st>>>(a, w.part, w.scores.count, a.n,
+                                                                      w.score, w.lse2);
     if (!grad) return hipGetLastError();
     k_operands<T, NP, KD, true><<<(unsigned)w.tf, kThreads, 0, st>>>(
         feat, a.n, a.feat_stride, a.dim, a, w.label, w.weight, w.lse2, w.F);
@@ -1209,18 +1185,136 @@ hipError_t stream_run(const LossArgs& a, bool grad, hipStream_t st) {
     return hipGetLastError();
 }
 
-// Padded row length that the streaming kernels take, 0: none. Past it a wave's
-// own rows and sums no longer fit its registers.
-int stream_kd(int dim, int dtype) {
-    for (int kd : {32, 64, 128, 256})
-        if (dim <= kd) return dtype == 0 && kd > 128 ? 0 : kd;
+// Padded row length that the streaming kernels take, 0: none. Past 128 a wave's own
+// rows and sums leave it alone on its unit: 20000 x 8000 of 256 bf16 with gradients
+// took 1073 us so, in pieces 803; of 128 456 against 536 (fp32 854 against 1438).
+int stream_kd(int dim) {
+    for (int kd : {32, 64, 128})
+        if (dim <= kd) return kd;
     return 0;
+}
+
+// ---------------------------------------------------------------- few samples
+// Losses of up to kFew samples, a picked pixel or a handful: the table is read once
+// and nothing is laid out. `lpr` lanes a table row take its dot products with all
+// samples, held in LDS in fp32; a workgroup's slots keep each sample's largest
+// score and sum, and k_loss_join adds the workgroups up. Bound by the table's bytes
+// (or, below about 1 MB, by the two launches).
+constexpr int kFew = 8;
+constexpr int kFewValues = 12288;  // samples * dim in LDS: 48 KB
+
+template <typename T, int VEC>
+__global__ __launch_bounds__(kThreads) void k_loss_few(LossArgs a, int lpr, float scale2,
+                                                       float2* part, float* label_score) {
+    __shared__ float f[kFewValues];
+    __shared__ float2 lds[kThreads / 64][kFew];
+    const int n = (int)a.n, dim = a.dim;
+    const T* feat = static_cast<const T*>(a.feat);
+    const T* table = static_cast<const T*>(a.table);
+    for (int e = threadIdx.x; e < n * dim; e += kThreads)
+        f[e] = to_float(feat[(int64_t)(e / dim) * a.feat_stride + e % dim]);
+    int32_t y[kFew];
+#pragma unroll
+    for (int q = 0; q < kFew; ++q)
+        y[q] = q < n ? load_id(a.labels, a.labels64, q, a.rows,
+                               blockIdx.x == 0 && threadIdx.x == 0 ? a.flags : nullptr)
+                     : -1;
+    __syncthreads();
+    const int slots = kThreads / lpr, slot = threadIdx.x / lpr, lane = threadIdx.x % lpr;
+    float m[kFew], sum[kFew];
+#pragma unroll
+    for (int q = 0; q < kFew; ++q) {
+        m[q] = -1e30f;
+        sum[q] = 0.0f;
+    }
+    for (int64_t v = (int64_t)blockIdx.x * slots + slot; v < a.rows;
+         v += (int64_t)gridDim.x * slots) {
+        const T* row = table + v * a.table_stride;
+        float dot[kFew];
+#pragma unroll
+        for (int q = 0; q < kFew; ++q) dot[q] = 0.0f;
+        for (int c = lane * VEC; c < dim; c += lpr * VEC) {
+            float t[VEC];
+            const int w = min(VEC, dim - c);
+            if (w == VEC) {
+                load_any<VEC>(row + c, t);
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) t[j] = j < w ? to_float(row[c + j]) : 0.0f;
+            }
+#pragma unroll
+            for (int q = 0; q < kFew; ++q)
+                if (q < n)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j)
+                        if (j < w) dot[q] = fmaf(t[j], f[q * dim + c + j], dot[q]);
+        }
+#pragma unroll
+        for (int q = 0; q < kFew; ++q) {
+            if (q >= n) continue;
+            for (int o = 1; o < lpr; o <<= 1) dot[q] += __shfl_xor(dot[q], o, 64);
+            const float s = dot[q] * scale2;
+            if (v == y[q] && lane == 0) label_score[q] = s;
+            const float mm = fmaxf(m[q], s), base = mm < INFINITY ? mm : 0.0f;
+            sum[q] = sum[q] * __builtin_amdgcn_exp2f((m[q] < INFINITY ? m[q] : 0.0f) - base) +
+                     __builtin_amdgcn_exp2f(s - base);
+            m[q] = mm;
+        }
+    }
+    // over the slots: within the wave, then the waves (the lanes of a slot agree)
+#pragma unroll
+    for (int q = 0; q < kFew; ++q) {
+        if (q >= n) continue;
+        for (int o = lpr; o < 64; o <<= 1) {
+            const float m2 = __shfl_xor(m[q], o, 64), s2 = __shfl_xor(sum[q], o, 64);
+            join_sums(m[q], sum[q], m2, s2);
+        }
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6][q] = make_float2(m[q], sum[q]);
+    }
+    __syncthreads();
+    if (threadIdx.x < n) {
+        float2 r = lds[0][threadIdx.x];
+#pragma unroll
+        for (int k = 1; k < kThreads / 64; ++k)
+            join_sums(r.x, r.y, lds[k][threadIdx.x].x, lds[k][threadIdx.x].y);
+        part[(int64_t)blockIdx.x * n + threadIdx.x] = r;
+    }
+}
+
+bool is_few(int64_t n, int dim, bool grad) { return !grad && n <= kFew && n * dim <= kFewValues; }
+
+struct FewPlan {
+    int lpr, blocks;
+    float2* part;
+    float* score;
+    size_t bytes;
+    FewPlan(void* base, int64_t n, int64_t rows, int dim, int dtype) {
+        const int vec = dtype == 0 ? 4 : 8;
+        lpr = 1;
+        while (lpr < 64 && lpr * vec < dim) lpr *= 2;
+        const int64_t slots = kThreads / lpr;
+        blocks = (int)std::min<int64_t>(512, (rows + slots - 1) / slots);
+        Carve c(base);
+        part = c.take<float2>((size_t)blocks * n);
+        score = c.take<float>((size_t)n);
+        bytes = c.bytes();
+    }
+};
+
+template <typename T>
+hipError_t few_run(const LossArgs& a, hipStream_t st) {
+    const FewPlan w(a.ws, a.n, a.rows, a.dim, a.dtype);
+    k_loss_few<T, 16 / sizeof(T)><<<w.blocks, kThreads, 0, st>>>(a, w.lpr, a.scale * kLog2e, w.part,
+                                                                 w.score);
+    k_loss_join<<<1, kThreads, 0, st>>>(a, w.part, w.blocks, a.n, w.score, nullptr);
+    return hipGetLastError();
 }
 
 }  // namespace
 
 size_t label_loss_ws(int64_t n, int64_t rows, int dim, int dtype, bool grad) {
-    const int kd = stream_kd(dim, dtype);
+    if (is_few(n, dim, grad)) return FewPlan(nullptr, n, rows, dim, dtype).bytes;
+    const int kd = stream_kd(dim);
     if (kd != 0) return StreamPlan(nullptr, n, rows, dtype == 0 ? 3 : 1, kd, grad).bytes;
     return LossPlan(nullptr, n, rows, dim, dtype, grad).bytes;
 }
@@ -1237,12 +1331,12 @@ hipError_t launch_label_loss(const LossArgs& a, bool grad, hipStream_t st) {
                                  a.rows, a.dtable_stride, a.dim, nullptr}, 0, st);
     }
     const bool f = a.dtype == 0;
-    switch (stream_kd(a.dim, a.dtype)) {
+    if (is_few(a.n, a.dim, grad)) return f ? few_run<float>(a, st) : few_run<bf16>(a, st);
+    switch (stream_kd(a.dim)) {
         case 32: return f ? stream_run<float, 3, 32>(a, grad, st) : stream_run<bf16, 1, 32>(a, grad, st);
         case 64: return f ? stream_run<float, 3, 64>(a, grad, st) : stream_run<bf16, 1, 64>(a, grad, st);
         case 128:
             return f ? stream_run<float, 3, 128>(a, grad, st) : stream_run<bf16, 1, 128>(a, grad, st);
-        case 256: return stream_run<bf16, 1, 256>(a, grad, st);
         default: return f ? loss_run<float, 3>(a, grad, st) : loss_run<bf16, 1>(a, grad, st);
     }
 }

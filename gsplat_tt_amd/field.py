@@ -32,11 +32,14 @@ def _rows(t, name, dim=None):
     """Pointer, rows, row stride of a (rows, dim) tensor with contiguous rows."""
     if t.dim() != 2:
         raise ValueError(f"{name} must have 2 dimensions, not {t.dim()}")
-    if dim is not None and t.shape[1] != dim:
-        raise ValueError(f"{name} must have {dim} columns, not {t.shape[1]}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    rows, cols = t.shape
+    if dim is not None and cols != dim:
+        raise ValueError(f"{name} must have {dim} columns, not {cols}")
+    if t.is_contiguous():
+        return t.data_ptr(), rows, cols
+    if cols > 1 and t.stride(1) != 1:
         raise ValueError(f"{name}: the values of a row must be contiguous")
-    return t.data_ptr(), t.shape[0], t.stride(0)
+    return t.data_ptr(), rows, t.stride(0)
 
 
 class FieldOps:
@@ -50,7 +53,10 @@ class FieldOps:
         self.ctx = ctx if ctx is not None else L.Context(device)
         self._L = self.ctx._L
         self.device = torch.device("cuda", self.ctx.device_index)
+        self._index = self.ctx.device_index
+        self._handle = self.ctx.handle
         self._flags = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._flags_ptr = self._flags.data_ptr()
         torch.cuda.current_stream(self.device).synchronize()
         self._sizes = {}
 
@@ -69,9 +75,7 @@ class FieldOps:
         if t.dim() != 1 or (n is not None and t.shape[0] != n):
             raise ValueError(f"{name} must be one-dimensional" +
                              (f" with {n} values" if n is not None else ""))
-        if t.shape[0] > 1 and t.stride(0) != 1:
-            t = t.contiguous()
-        return t
+        return t.contiguous()
 
     def _param(self, t, name, n):
         if t is None:
@@ -79,7 +83,7 @@ class FieldOps:
         self._own(t, name, (torch.float32,))
         if t.dim() != 1 or t.shape[0] != n:
             raise ValueError(f"{name} must be one-dimensional with {n} values")
-        return t if n <= 1 or t.stride(0) == 1 else t.contiguous()
+        return t.contiguous()
 
     def _out(self, out, shape, dtype, name):
         if out is None:
@@ -102,7 +106,7 @@ class FieldOps:
         return torch.empty(size, dtype=torch.uint8, device=self.device), size
 
     def _stream(self):
-        return torch.cuda.current_stream(self.device).cuda_stream
+        return torch.cuda.current_stream(self._index).cuda_stream
 
     def check(self):
         """Waits for the current stream and raises ValueError when a call since the
@@ -124,9 +128,9 @@ class FieldOps:
         out = self._out(out, (n, dim), dtype or table.dtype, "out")
         po, _, so = _rows(out, "out")
         L._check(self._L.gs_lookup_dev(
-            self.ctx.handle, p, rows, stride, _DTYPES[table.dtype], ids.data_ptr(),
+            self._handle, p, rows, stride, _DTYPES[table.dtype], ids.data_ptr(),
             int(ids.dtype == torch.int64), n, dim, float(scale), po, so, _DTYPES[out.dtype],
-            self._flags.data_ptr(), self._stream()))
+            self._flags_ptr, self._stream()))
         return out
 
     def lookup_grad(self, dout, ids, rows, scale=1.0, out=None, accumulate=False, dtype=None):
@@ -143,9 +147,9 @@ class FieldOps:
         po, _, so = _rows(out, "out")
         ws, size = self._workspace("gs_lookup_grad_workspace", n, int(rows), dim)
         L._check(self._L.gs_lookup_grad_dev(
-            self.ctx.handle, p, stride, _DTYPES[dout.dtype], ids.data_ptr(),
+            self._handle, p, stride, _DTYPES[dout.dtype], ids.data_ptr(),
             int(ids.dtype == torch.int64), n, dim, float(scale), int(bool(accumulate)), po,
-            int(rows), so, _DTYPES[out.dtype], ws.data_ptr(), size, self._flags.data_ptr(),
+            int(rows), so, _DTYPES[out.dtype], ws.data_ptr(), size, self._flags_ptr,
             self._stream()))
         return out
 
@@ -159,6 +163,8 @@ class FieldOps:
                              (f" = {tuple(shape)}" if shape is not None else ""))
         if dtype is not None and t.dtype != dtype:
             raise TypeError(f"{name} must have the type {dtype}")
+        if t.is_contiguous():
+            return t.data_ptr(), t.stride(0), t.shape[-1]
         if t.shape[-1] > 1 and t.stride(-1) != 1:
             raise ValueError(f"{name}: the channels of a pixel must be contiguous")
         pixel, step = None, None
@@ -194,14 +200,13 @@ class FieldOps:
         px, bx, sx = self._image(x, "x")
         d, keep = self._norm(x, groups, weight, bias, act, eps)
         if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=self.device)
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
         py, by, sy = self._image(out, "out", x.shape, x.dtype)
         stats = torch.zeros if d.pixels == 0 else torch.empty
-        mean = stats((x.shape[0], int(groups)), dtype=torch.float32, device=self.device)
-        rstd = stats((x.shape[0], int(groups)), dtype=torch.float32, device=self.device)
+        mean, rstd = stats((2, d.batch, d.groups), dtype=torch.float32, device=self.device)
         ws, size = self._workspace("gs_group_norm_workspace", d.batch, d.pixels, d.channels)
         L._check(self._L.gs_group_norm_dev(
-            self.ctx.handle, ctypes.byref(d), px, bx, sx, py, by, sy, mean.data_ptr(),
+            self._handle, ctypes.byref(d), px, bx, sx, py, by, sy, mean.data_ptr(),
             rstd.data_ptr(), ws.data_ptr(), size, self._stream()))
         del keep
         return out, mean, rstd
@@ -214,20 +219,20 @@ class FieldOps:
         pd, bd, sd = self._image(dy, "dy", x.shape, x.dtype)
         d, keep = self._norm(x, groups, weight, bias, act, eps)
         if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=self.device)
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
         po, bo, so = self._image(out, "out", x.shape, x.dtype)
         for t, name in ((mean, "mean"), (rstd, "rstd")):
             self._own(t, name, (torch.float32,))
             if tuple(t.shape) != (d.batch, d.groups) or not t.is_contiguous():
                 raise ValueError(f"{name} must be group_norm()'s: contiguous {d.batch, d.groups}")
-        dparam = torch.empty((2, d.channels), dtype=torch.float32, device=self.device)
+        dweight, dbias = torch.empty((2, d.channels), dtype=torch.float32, device=self.device)
         ws, size = self._workspace("gs_group_norm_workspace", d.batch, d.pixels, d.channels)
         L._check(self._L.gs_group_norm_grad_dev(
-            self.ctx.handle, ctypes.byref(d), pd, bd, sd, px, bx, sx, mean.data_ptr(),
-            rstd.data_ptr(), po, bo, so, dparam[0].data_ptr(), dparam[1].data_ptr(),
+            self._handle, ctypes.byref(d), pd, bd, sd, px, bx, sx, mean.data_ptr(),
+            rstd.data_ptr(), po, bo, so, dweight.data_ptr(), dbias.data_ptr(),
             ws.data_ptr(), size, self._stream()))
         del keep
-        return out, dparam[0], dparam[1]
+        return out, dweight, dbias
 
     # ---- label loss
     def _loss(self, feat, table, labels, scale):
@@ -246,12 +251,11 @@ class FieldOps:
         """(loss, lse), fp32 (n): cross entropy of the scores scale * feat @ table.T
         against `labels`, and the scores' log sum exp; 0 and 0 for masked labels."""
         d, keep = self._loss(feat, table, labels, scale)
-        loss = torch.empty(d.n, dtype=torch.float32, device=self.device)
-        lse = torch.empty(d.n, dtype=torch.float32, device=self.device)
+        loss, lse = torch.empty((2, d.n), dtype=torch.float32, device=self.device)
         ws, size = self._workspace("gs_label_loss_workspace", d.n, d.rows, d.dim, d.dtype, 0)
         L._check(self._L.gs_label_loss_dev(
-            self.ctx.handle, ctypes.byref(d), loss.data_ptr(), lse.data_ptr(), ws.data_ptr(),
-            size, self._flags.data_ptr(), self._stream()))
+            self._handle, ctypes.byref(d), loss.data_ptr(), lse.data_ptr(), ws.data_ptr(),
+            size, self._flags_ptr, self._stream()))
         del keep
         return loss, lse
 
@@ -261,8 +265,7 @@ class FieldOps:
         sum(row_weight * loss) in the inputs' type; row_weight (n) fp32, None: ones."""
         d, keep = self._loss(feat, table, labels, scale)
         row_weight = self._param(row_weight, "row_weight", d.n)
-        loss = torch.empty(d.n, dtype=torch.float32, device=self.device)
-        lse = torch.empty(d.n, dtype=torch.float32, device=self.device)
+        loss, lse = torch.empty((2, d.n), dtype=torch.float32, device=self.device)
         dfeat = self._out(dfeat, feat.shape, feat.dtype, "dfeat")
         dtable = self._out(dtable, table.shape, table.dtype, "dtable")
         if dfeat.dtype != feat.dtype or dtable.dtype != feat.dtype:
@@ -271,9 +274,9 @@ class FieldOps:
         pt, _, stt = _rows(dtable, "dtable")
         ws, size = self._workspace("gs_label_loss_workspace", d.n, d.rows, d.dim, d.dtype, 1)
         L._check(self._L.gs_label_loss_grad_dev(
-            self.ctx.handle, ctypes.byref(d),
+            self._handle, ctypes.byref(d),
             None if row_weight is None else row_weight.data_ptr(), loss.data_ptr(),
-            lse.data_ptr(), pf, sf, pt, stt, ws.data_ptr(), size, self._flags.data_ptr(),
+            lse.data_ptr(), pf, sf, pt, stt, ws.data_ptr(), size, self._flags_ptr,
             self._stream()))
         del keep
         return loss, lse, dfeat, dtable
