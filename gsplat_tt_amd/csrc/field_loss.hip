@@ -566,8 +566,8 @@ hipError_t fold(const SumOut<T>& o, int nz, hipStream_t st) {
 }
 
 // ---------------------------------------------------------------- streaming
-// For rows short enough that a wave keeps its own in registers: a workgroup
-// holds 4 x 64 "queries", the other side's rows ("keys") stream through LDS, 32
+// For rows short enough that a wave keeps its own in registers: each of a
+// workgroup's 4 waves holds 32 QB "queries", the other side's rows ("keys") stream through LDS, 32
 // a tile, and neither scores nor G ever leave the registers.
 //
 // The scores of a tile are made transposed, keys by queries: a lane then holds
@@ -604,7 +604,7 @@ struct StreamArgs {
     float *label_score, *loss, *lse, *lse2_out;
     uint32_t* flags;
     int64_t table_rows;
-    // gradients: into out where there is one share, else into (share, padded, KD) sums
+    // gradients: into out where there is one share, else into (share, padded, row) sums
     void* out;
     int64_t out_stride;
     float* sums;
@@ -614,13 +614,22 @@ struct StreamArgs {
 // Key of register r of a lane in half h.
 __device__ __forceinline__ constexpr int key_of(int r) { return (r & 3) + 8 * (r >> 2); }
 
+// Row length of the second product, whose operands are 32 columns wide.
+constexpr int padded_dim(int ks) { return (ks + 31) / 32 * 32; }
+// Blocks of 32 queries a wave. A key's operand read from LDS serves QB products of
+// each part: with one part two blocks are needed to feed the matrix cores, with
+// three one does, and two waves a unit fit.
+template <int NP>
+constexpr int kBlocks = NP == 1 ? 2 : 1;
+
 // (rows, dim) as tiles of operands, one workgroup a tile; of samples (label) the
 // masked ones are zeros, and label and weight are written for the gradients.
-template <typename T, int NP, int KD, bool SECOND>
+template <typename T, int NP, int KS, bool SECOND>
 __global__ __launch_bounds__(kThreads) void k_operands(const T* src, int64_t rows, int64_t stride,
                                                        int dim, LossArgs a, int32_t* label,
                                                        float* weight, float* lse2, quad* out) {
-    __shared__ float tile[32][KD + 1];
+    constexpr int DD = padded_dim(KS);
+    __shared__ float tile[32][DD + 1];
     __shared__ int32_t lab[32];
     const int64_t r0 = (int64_t)blockIdx.x * 32;
     if (threadIdx.x < 32) {
@@ -635,14 +644,14 @@ __global__ __launch_bounds__(kThreads) void k_operands(const T* src, int64_t row
         lab[threadIdx.x] = l;
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < 32 * KD; e += kThreads) {
-        const int r = e / KD, c = e % KD;
+    for (int e = threadIdx.x; e < 32 * DD; e += kThreads) {
+        const int r = e / DD, c = e % DD;
         float v = 0.0f;
         if (r0 + r < rows && c < dim && lab[r] >= 0) v = plain_input<NP>(to_float(src[(r0 + r) * stride + c]));
         tile[r][c] = v;
     }
     __syncthreads();
-    constexpr int kFirst = KD / 16 * 64, kSecond = SECOND ? KD / 32 * 2 * 64 : 0;
+    constexpr int kFirst = KS / 16 * 64, kSecond = SECOND ? DD / 32 * 2 * 64 : 0;
     quad* to = out + (size_t)blockIdx.x * NP * (kFirst + kSecond);
     for (int e = threadIdx.x; e < kFirst + kSecond; e += kThreads) {
         const int lane = e & 63, h = lane >> 5;
@@ -666,32 +675,37 @@ __global__ __launch_bounds__(kThreads) void k_operands(const T* src, int64_t row
     }
 }
 
-template <typename T, int NP, int KD, int ROLE>
+// Whether a kernel's registers leave it one wave a unit (two with spills were
+// slower: 20000 x 5000 of 128 fp32 with gradients 1137 against 811 us).
+constexpr bool one_a_unit(int ks, int role) { return role != kScores && ks >= 128; }
+
+template <typename T, int NP, int KS, int ROLE>
 struct StreamShape {
-    static constexpr int kPieces = NP * KD / 16 * 64 * (ROLE == kScores ? 1 : 2);  // quad a tile
+    static constexpr int kPieces =  // quads of a tile
+        NP * 64 * (KS / 16 + (ROLE == kScores ? 0 : padded_dim(KS) / 16));
     // tiles per step: about 16 KB
     static constexpr int kTiles = kPieces * 16 >= 16384 ? 1 : (kPieces * 16 >= 8192 ? 2 : 4);
     static constexpr int kStage = kPieces * kTiles;
     static constexpr size_t kLds = 2 * kStage * 16 + (ROLE == kGradTable ? 2 * kTiles * 32 * 12 : 0);
 };
 
-template <typename T, int NP, int KD, int ROLE>
-__global__ __launch_bounds__(kThreads, (NP * KD >= (ROLE == kScores ? 256 : 128) ? 1 : 2)) void k_stream(StreamArgs a) {
-    using Shape = StreamShape<T, NP, KD, ROLE>;
-    constexpr int KJ = KD / 16, DB = KD / 32, TS = Shape::kTiles, STAGE = Shape::kStage;
-    constexpr int PER = STAGE / kThreads;
-    static_assert(STAGE % kThreads == 0, "a stage is whole rounds of loads");
+template <typename T, int NP, int KS, int ROLE>
+__global__ __launch_bounds__(kThreads, one_a_unit(KS, ROLE) ? 1 : 2) void k_stream(StreamArgs a) {
+    using Shape = StreamShape<T, NP, KS, ROLE>;
+    constexpr int QB = kBlocks<NP>, KJ = KS / 16, DD = padded_dim(KS), DB = DD / 32;
+    constexpr int TS = Shape::kTiles, STAGE = Shape::kStage;
+    constexpr int PER = (STAGE + kThreads - 1) / kThreads;
     extern __shared__ quad lds[];
     float* info = reinterpret_cast<float*>(lds + 2 * STAGE);  // kGradTable: lse2, weight, label
     const int t = threadIdx.x, lane = t & 63, h = lane >> 5, col = lane & 31;
-    const int64_t q0 = ((int64_t)blockIdx.x * 4 + (t >> 6)) * 64;
+    const int64_t q0 = ((int64_t)blockIdx.x * 4 + (t >> 6)) * (32 * QB);
 
     // the wave's own queries, as right operands of the scores
-    quad q[2][KJ][NP];
-    int32_t y[2];
-    float lse2[2];
+    quad q[QB][KJ][NP];
+    int32_t y[QB];
+    float lse2[QB];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < QB; ++b) {
         const int64_t i = q0 + b * 32 + col;
         bool on = i < a.nq;
         y[b] = -1;
@@ -714,14 +728,17 @@ __global__ __launch_bounds__(kThreads, (NP * KD >= (ROLE == kScores ? 256 : 128)
         for (int j = 0; j < KJ; ++j) load_parts<T, NP>(row, a.dim, 16 * j + 8 * h, on, q[b][j]);
     }
 
-    f32x16 acc[2][ROLE == kScores ? 1 : DB];
-    float m[2], sum[2], own[2];
+    f32x16 acc[QB][ROLE == kScores ? 1 : DB];
+    float m[QB], sum[QB], own[QB];
     if (ROLE == kScores) {
-        m[0] = m[1] = -1e30f;
-        sum[0] = sum[1] = own[0] = own[1] = 0.0f;
+#pragma unroll
+        for (int b = 0; b < QB; ++b) {
+            m[b] = -1e30f;
+            sum[b] = own[b] = 0.0f;
+        }
     } else {
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < QB; ++b)
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -737,13 +754,15 @@ __global__ __launch_bounds__(kThreads, (NP * KD >= (ROLE == kScores ? 256 : 128)
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
             const int e = k * kThreads + t;
-            pre[k] = from[(size_t)(e / Shape::kPieces) * a.tile_stride + e % Shape::kPieces];
+            if (STAGE % kThreads == 0 || e < STAGE)
+                pre[k] = from[(size_t)(e / Shape::kPieces) * a.tile_stride + e % Shape::kPieces];
         }
     };
     auto keep = [&](int s) {
         quad* to = lds + (s & 1) * STAGE + t;
 #pragma unroll
-        for (int k = 0; k < PER; ++k) to[k * kThreads] = pre[k];
+        for (int k = 0; k < PER; ++k)
+            if (STAGE % kThreads == 0 || k * kThreads + t < STAGE) to[k * kThreads] = pre[k];
         if (ROLE == kGradTable) {
             float* f = info + (s & 1) * TS * 96;
             for (int k = t; k < TS * 32; k += kThreads) {
@@ -765,9 +784,9 @@ __global__ __launch_bounds__(kThreads, (NP * KD >= (ROLE == kScores ? 256 : 128)
             const int tile = t0 + s * TS + u;
             if (tile >= t1) break;
             const quad* kf = stage + u * Shape::kPieces + lane;
-            f32x16 sc[2];
+            f32x16 sc[QB];
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+            for (int b = 0; b < QB; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) sc[b][r] = 0.0f;
 #pragma unroll
@@ -779,7 +798,7 @@ __global__ __launch_bounds__(kThreads, (NP * KD >= (ROLE == kScores ? 256 : 128)
 #pragma unroll
                 for (int i = 0; i < Products<NP>::kCount; ++i)
 #pragma unroll
-                    for (int b = 0; b < 2; ++b)
+                    for (int b = 0; b < QB; ++b)
                         sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
                             k[Products<NP>::a(i)],
                             __builtin_bit_cast(bf16x8, q[b][j][Products<NP>::b(i)]), sc[b], 0, 0, 0);
@@ -787,7 +806,7 @@ __global__ __launch_bounds__(kThreads, (NP * KD >= (ROLE == kScores ? 256 : 128)
             const int64_t k0 = (int64_t)tile * 32;
             if (ROLE == kScores) {
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
+                for (int b = 0; b < QB; ++b) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) sc[b][r] *= a.scale2;
                     if (k0 + 32 > a.nk) {
@@ -816,10 +835,10 @@ __global__ __launch_bounds__(kThreads, (NP * KD >= (ROLE == kScores ? 256 : 128)
                 }
                 continue;
             }
-            quad g[2][2][NP];
+            quad g[QB][2][NP];
             const float* f = info + (s & 1) * TS * 96 + u * 32;
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
+            for (int b = 0; b < QB; ++b) {
                 float v[16];
                 if (ROLE == kGradFeat) {
 #pragma unroll
@@ -872,7 +891,7 @@ __global__ __launch_bounds__(kThreads, (NP * KD >= (ROLE == kScores ? 256 : 128)
 #pragma unroll
                     for (int i = 0; i < Products<NP>::kCount; ++i)
 #pragma unroll
-                        for (int b = 0; b < 2; ++b)
+                        for (int b = 0; b < QB; ++b)
                             acc[b][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
                                 __builtin_bit_cast(bf16x8, g[b][f2][Products<NP>::a(i)]),
                                 k[Products<NP>::b(i)], acc[b][d], 0, 0, 0);
@@ -884,7 +903,7 @@ __global__ __launch_bounds__(kThreads, (NP * KD >= (ROLE == kScores ? 256 : 128)
 
     if (ROLE == kScores) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < QB; ++b) {
             const int64_t i = q0 + b * 32 + col;
             const float m2 = __shfl_xor(m[b], 32, 64), s2 = __shfl_xor(sum[b], 32, 64);
             join_sums(m[b], sum[b], m2, s2);
@@ -907,7 +926,7 @@ __global__ __launch_bounds__(kThreads, (NP * KD >= (ROLE == kScores ? 256 : 128)
         return;
     }
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < QB; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int64_t i = q0 + b * 32 + key_of(r) + 4 * h;
@@ -923,7 +942,7 @@ __global__ __launch_bounds__(kThreads, (NP * KD >= (ROLE == kScores ? 256 : 128)
                 const int c = d * 32 + col;
                 const float v = on ? acc[b][d][r] * w : 0.0f;
                 if (gridDim.y > 1)
-                    a.sums[((size_t)blockIdx.y * a.padded + i) * KD + c] = v;
+                    a.sums[((size_t)blockIdx.y * a.padded + i) * DD + c] = v;
                 else if (c < a.dim)
                     static_cast<T*>(a.out)[i * a.out_stride + c] = from_float<T>(v);
             }
@@ -1043,16 +1062,28 @@ hipError_t loss_run(const LossArgs& a, bool grad, hipStream_t st) {
     return hipGetLastError();
 }
 
-// Shares of the streamed side: enough workgroups for the chip (two a compute
-// unit), at least `least` tiles each, at most `most` of them.
+// Shares of the streamed side: whole rounds of workgroups on the chip, `at_once` of
+// which it holds, with at least `least` tiles a share and at most `most` shares.
 struct Shares {
     int count, tiles;
-    Shares(int64_t queries, int64_t tiles_all, int least, int64_t most) {
-        const int64_t groups = (queries + 255) / 256;
-        int64_t want = groups >= 512 ? 1 : (512 + groups - 1) / std::max<int64_t>(groups, 1);
-        want = std::min(want, std::max<int64_t>(1, tiles_all / least));
-        want = std::max<int64_t>(1, std::min(want, most));
-        tiles = (int)((tiles_all + want - 1) / want);
+    Shares(int64_t queries, int per, int64_t tiles_all, int at_once, int least, int64_t most) {
+        const int64_t groups = std::max<int64_t>(1, (queries + per - 1) / per);
+        const int64_t cap =
+            std::max<int64_t>(1, std::min(most, std::max<int64_t>(1, tiles_all / least)));
+        // the fewest shares that leave at most a tenth of the last round empty, of those
+        // that make no more than four rounds
+        int64_t best = 1;
+        double best_full = 0.0;
+        for (int64_t want = 1; want <= cap && (want == 1 || groups * want <= 4 * at_once); ++want) {
+            const int64_t all = groups * want;
+            const double full = (double)all / (double)((all + at_once - 1) / at_once * at_once);
+            if (full > best_full + 1e-9) {
+                best = want;
+                best_full = full;
+            }
+            if (full >= 0.9) break;
+        }
+        tiles = (int)((tiles_all + best - 1) / best);
         count = (int)((tiles_all + tiles - 1) / tiles);
     }
 };
@@ -1066,15 +1097,23 @@ struct StreamPlan {
     float *weight, *lse2, *score, *sums;
     float2* part;
     size_t bytes;
+    // workgroups that the chip holds
+    static int at_once(int ks, int role) { return one_a_unit(ks, role) ? 256 : 512; }
     // partial sums of the gradients: at most 64 MB a side
     static int64_t most(int64_t rows, int kd) {
         return std::max<int64_t>(1, ((int64_t)1 << 24) / std::max<int64_t>(1, rows * kd));
     }
-    StreamPlan(void* base, int64_t n, int64_t rows, int np, int kd, bool grad)
-        : tf((n + 31) / 32), tt((rows + 31) / 32), scores(n, tt, 4, 512),
-          by_feat(n, tt, 8, most(n, kd)), by_table(rows, tf, 8, most(rows, kd)) {
+    StreamPlan(void* base, int64_t n, int64_t rows, int np, int ks, bool grad)
+        : tf((n + 31) / 32), tt((rows + 31) / 32),
+          scores(n, np == 1 ? 256 : 128, tt, at_once(ks, kScores), 4, 512),
+          by_feat(n, np == 1 ? 256 : 128, tt, at_once(ks, kGradFeat), 4,
+                  most(n, padded_dim(ks))),
+          by_table(rows, np == 1 ? 256 : 128, tf, at_once(ks, kGradTable), 4,
+                   most(rows, padded_dim(ks))) {
         Carve c(base);
-        const size_t first = (size_t)np * kd / 16 * 64, tile = grad ? 2 * first : first;
+        const int kd = padded_dim(ks);
+        const size_t first = (size_t)np * ks / 16 * 64;
+        const size_t tile = first + (grad ? (size_t)np * kd / 16 * 64 : 0);
         T = c.take<quad>((tt + 4) * tile);
         part = c.take<float2>(scores.count > 1 ? (size_t)scores.count * n : 0);
         score = c.take<float>(scores.count > 1 ? (size_t)n : 0);
@@ -1094,30 +1133,31 @@ struct StreamPlan {
     }
 };
 
-template <typename T, int NP, int KD, int ROLE>
+template <typename T, int NP, int KS, int ROLE>
 hipError_t launch_stream(const StreamArgs& a, const Shares& sh, hipStream_t st) {
-    constexpr size_t lds = StreamShape<T, NP, KD, ROLE>::kLds;
+    constexpr size_t lds = StreamShape<T, NP, KS, ROLE>::kLds;
     if (lds > 65536) {  // above the default limit of a launch
         const hipError_t e =
-            hipFuncSetAttribute(reinterpret_cast<const void*>(&k_stream<T, NP, KD, ROLE>),
+            hipFuncSetAttribute(reinterpret_cast<const void*>(&k_stream<T, NP, KS, ROLE>),
                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
     }
-    k_stream<T, NP, KD, ROLE>
-        <<<dim3((unsigned)((a.nq + 255) / 256), (unsigned)sh.count), kThreads, lds, st>>>(a);
+    constexpr int kQueries = 128 * kBlocks<NP>;
+    k_stream<T, NP, KS, ROLE><<<dim3((unsigned)((a.nq + kQueries - 1) / kQueries),
+                                     (unsigned)sh.count), kThreads, lds, st>>>(a);
     return hipGetLastError();
 }
 
-template <typename T, int NP, int KD>
+template <typename T, int NP, int KS>
 hipError_t stream_run(const LossArgs& a, bool grad, hipStream_t st) {
-    const StreamPlan w(a.ws, a.n, a.rows, NP, KD, grad);
+    const StreamPlan w(a.ws, a.n, a.rows, NP, KS, grad);
     const T* feat = static_cast<const T*>(a.feat);
     const T* table = static_cast<const T*>(a.table);
     if (grad)
-        k_operands<T, NP, KD, true><<<(unsigned)w.tt, kThreads, 0, st>>>(
+        k_operands<T, NP, KS, true><<<(unsigned)w.tt, kThreads, 0, st>>>(
             table, a.rows, a.table_stride, a.dim, a, nullptr, nullptr, nullptr, w.T);
     else
-        k_operands<T, NP, KD, false><<<(unsigned)w.tt, kThreads, 0, st>>>(
+        k_operands<T, NP, KS, false><<<(unsigned)w.tt, kThreads, 0, st>>>(
             table, a.rows, a.table_stride, a.dim, a, nullptr, nullptr, nullptr, w.T);
     StreamArgs s{};
     s.q = feat;
@@ -1144,24 +1184,24 @@ hipError_t stream_run(const LossArgs& a, bool grad, hipStream_t st) {
     s.padded = a.n;
     hipError_t e;
     // the gradients' tiles hold both products' operands, the scores take the first
-    constexpr int kFirst = NP * KD / 16 * 64;
-    s.tile_stride = grad ? 2 * kFirst : kFirst;
-    e = launch_stream<T, NP, KD, kScores>(s, w.scores, st);
+    constexpr int DD = padded_dim(KS), kFirst = NP * KS / 16 * 64;
+    s.tile_stride = kFirst + (grad ? NP * DD / 16 * 64 : 0);
+    e = launch_stream<T, NP, KS, kScores>(s, w.scores, st);
     if (e != hipSuccess) return e;
     if (w.scores.count > 1)
         k_loss_join<<<(unsigned)((a.n + 31) / 32), kThreads, 0, st>>>(a, w.part, w.scores.count, a.n,
                                                                       w.score, w.lse2);
     if (!grad) return hipGetLastError();
-    k_operands<T, NP, KD, true><<<(unsigned)w.tf, kThreads, 0, st>>>(
+    k_operands<T, NP, KS, true><<<(unsigned)w.tf, kThreads, 0, st>>>(
         feat, a.n, a.feat_stride, a.dim, a, w.label, w.weight, w.lse2, w.F);
     s.share = w.by_feat.tiles;
     s.out = a.dfeat;
     s.out_stride = a.dfeat_stride;
     s.sums = w.sums;
-    e = launch_stream<T, NP, KD, kGradFeat>(s, w.by_feat, st);
+    e = launch_stream<T, NP, KS, kGradFeat>(s, w.by_feat, st);
     if (e != hipSuccess) return e;
     if (w.by_feat.count > 1) {
-        e = fold(SumOut<T>{w.sums, nullptr, 1, 1, a.n, KD, static_cast<T*>(a.dfeat), a.n,
+        e = fold(SumOut<T>{w.sums, nullptr, 1, 1, a.n, DD, static_cast<T*>(a.dfeat), a.n,
                        a.dfeat_stride, a.dim, w.label},
              w.by_feat.count, st);
         if (e != hipSuccess) return e;
@@ -1176,10 +1216,10 @@ hipError_t stream_run(const LossArgs& a, bool grad, hipStream_t st) {
     s.out = a.dtable;
     s.out_stride = a.dtable_stride;
     s.padded = a.rows;
-    e = launch_stream<T, NP, KD, kGradTable>(s, w.by_table, st);
+    e = launch_stream<T, NP, KS, kGradTable>(s, w.by_table, st);
     if (e != hipSuccess) return e;
     if (w.by_table.count > 1)
-        return fold(SumOut<T>{w.sums, nullptr, 1, 1, a.rows, KD, static_cast<T*>(a.dtable), a.rows,
+        return fold(SumOut<T>{w.sums, nullptr, 1, 1, a.rows, DD, static_cast<T*>(a.dtable), a.rows,
                        a.dtable_stride, a.dim, nullptr},
              w.by_table.count, st);
     return hipGetLastError();
@@ -1188,9 +1228,9 @@ hipError_t stream_run(const LossArgs& a, bool grad, hipStream_t st) {
 // Padded row length that the streaming kernels take, 0: none. Past 128 a wave's own
 // rows and sums leave it alone on its unit: 20000 x 8000 of 256 bf16 with gradients
 // took 1073 us so, in pieces 803; of 128 456 against 536 (fp32 854 against 1438).
-int stream_kd(int dim) {
-    for (int kd : {32, 64, 128})
-        if (dim <= kd) return kd;
+int stream_ks(int dim) {
+    for (int ks : {16, 32, 48, 64, 128})
+        if (dim <= ks) return ks;
     return 0;
 }
 
@@ -1314,8 +1354,8 @@ hipError_t few_run(const LossArgs& a, hipStream_t st) {
 
 size_t label_loss_ws(int64_t n, int64_t rows, int dim, int dtype, bool grad) {
     if (is_few(n, dim, grad)) return FewPlan(nullptr, n, rows, dim, dtype).bytes;
-    const int kd = stream_kd(dim);
-    if (kd != 0) return StreamPlan(nullptr, n, rows, dtype == 0 ? 3 : 1, kd, grad).bytes;
+    const int ks = stream_ks(dim);
+    if (ks != 0) return StreamPlan(nullptr, n, rows, dtype == 0 ? 3 : 1, ks, grad).bytes;
     return LossPlan(nullptr, n, rows, dim, dtype, grad).bytes;
 }
 
@@ -1332,8 +1372,10 @@ hipError_t launch_label_loss(const LossArgs& a, bool grad, hipStream_t st) {
     }
     const bool f = a.dtype == 0;
     if (is_few(a.n, a.dim, grad)) return f ? few_run<float>(a, st) : few_run<bf16>(a, st);
-    switch (stream_kd(a.dim)) {
+    switch (stream_ks(a.dim)) {
+        case 16: return f ? stream_run<float, 3, 16>(a, grad, st) : stream_run<bf16, 1, 16>(a, grad, st);
         case 32: return f ? stream_run<float, 3, 32>(a, grad, st) : stream_run<bf16, 1, 32>(a, grad, st);
+        case 48: return f ? stream_run<float, 3, 48>(a, grad, st) : stream_run<bf16, 1, 48>(a, grad, st);
         case 64: return f ? stream_run<float, 3, 64>(a, grad, st) : stream_run<bf16, 1, 64>(a, grad, st);
         case 128:
             return f ? stream_run<float, 3, 128>(a, grad, st) : stream_run<bf16, 1, 128>(a, grad, st);
