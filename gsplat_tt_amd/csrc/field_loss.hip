@@ -147,51 +147,67 @@ struct Mat {
     int64_t ld, plane;  // elements between rows and between parts
 };
 
+// The wave's number, known to be the same in all its lanes.
+__device__ __forceinline__ int wave_id() {
+    return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+}
+
 // One operand's 128 x 64 tile in LDS (1024 quads). K: rows of the matrix hold the
 // summed index, and the tile's 128 rows of 64 are placed by (piece ^ row % 8), so
 // that 8 lanes reading one column of pieces touch all banks once. Not K: the
 // matrix's rows are the summed index; 64 rows of 128, 32-byte pieces placed by
 // (piece ^ row % 8), read through the transposing LDS load: in a group of 16
 // lanes, lane s reads 4 values of row s / 4 at column 4 (s % 4), and lane g gets
-// column g of the 4 rows.
-template <bool K>
+// column g of the 4 rows. Addresses are a base common to the wave and one lane
+// offset: with one 64-bit address a load, the registers do not last.
+//
+// PAIRS (with K): block i of 16 rows takes rows 32 (i / 2) + 8 (s / 4) + 4 (i % 2) +
+// s % 4 instead of 16 i + s, so that a lane's sums of two blocks are 8 rows in a row.
+template <bool K, bool PAIRS = false>
 struct Side {
+    __device__ __forceinline__ static uint32_t place(uint32_t row) {
+        return PAIRS ? (row & 3) | ((row >> 1) & 4) : row & 7;
+    }
     quad r[4];
+    uint32_t from, to;  // the lane's byte offset in memory, its first quad in LDS
+    int64_t ld;
+    __device__ __forceinline__ explicit Side(const Mat& m) : ld(m.ld) {
+        const uint32_t t = threadIdx.x, row = K ? t >> 3 : t >> 4, c = K ? t & 7 : t & 15;
+        from = (row * (uint32_t)m.ld + c * 8) * 2;
+        to = K ? row * 8 + (c ^ place(row)) : row * 16 + (c ^ ((row & 7) << 1));
+    }
     __device__ __forceinline__ void fetch(const Mat& m, int part, int64_t row0, int64_t k) {
-        const bf16* p = m.p + part * m.plane + (K ? row0 * m.ld + k : k * m.ld + row0);
+        const char* p = reinterpret_cast<const char*>(m.p + part * m.plane +
+                                                      (K ? row0 * ld + k : k * ld + row0));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int e = threadIdx.x + j * kThreads;
-            const int row = K ? e >> 3 : e >> 4, c = K ? e & 7 : e & 15;
-            r[j] = *reinterpret_cast<const quad*>(p + row * m.ld + c * 8);
-        }
+        for (int j = 0; j < 4; ++j)
+            r[j] = *reinterpret_cast<const quad*>(p + (int64_t)j * (K ? 64 : 32) * ld + from);
     }
     __device__ __forceinline__ void keep(quad* lds) const {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int e = threadIdx.x + j * kThreads;
-            const int row = K ? e >> 3 : e >> 4, c = K ? e & 7 : e & 15;
-            lds[K ? row * 8 + (c ^ (row & 7)) : row * 16 + ((c ^ ((row & 7) << 1)))] = r[j];
-        }
+        for (int j = 0; j < 4; ++j) lds[to + j * 256] = r[j];
     }
-    // the operand of rows b .. b + 15, summed index 32 h .. 32 h + 31
-    __device__ __forceinline__ static bf16x8 operand(const quad* lds, int b, int h) {
-        const int lane = threadIdx.x & 63, g = lane >> 4;
+    // the operand of rows b + 16 i .. + 15 (b 0 or 64, the same in the wave), summed
+    // index 32 h .. 32 h + 31
+    __device__ __forceinline__ static bf16x8 operand(const quad* lds, int b, int i, int h) {
+        const int lane = threadIdx.x & 63, g = lane >> 4, s = lane & 15;
         if (K) {
-            const int row = b + (lane & 15), c = h * 4 + g;
-            return __builtin_bit_cast(bf16x8, lds[row * 8 + (c ^ (row & 7))]);
+            const uint32_t row = PAIRS ? (s >> 2) * 8 + (s & 3) : s;
+            const quad* at = lds + row * 8 + ((g ^ place(row)) ^ (h * 4));
+            return __builtin_bit_cast(
+                bf16x8, at[(b + (PAIRS ? (i >> 1) * 32 + (i & 1) * 4 : i * 16)) * 8]);
         }
         typedef __attribute__((ext_vector_type(4))) short s16x4;
         typedef __attribute__((address_space(3))) s16x4* lds4;
-        const int s = lane & 15, row = h * 32 + g * 8 + (s >> 2);
-        const char* at = reinterpret_cast<const char*>(lds) + (s & 3) * 8;
+        // row r = 32 h + 8 g + 4 u + s / 4: its piece b / 16 + i lies at
+        // 4 (b / 64 ^ u) + (i ^ s / 4)
+        const char* at = reinterpret_cast<const char*>(lds) + (g * 8 + (s >> 2)) * 256 +
+                         (s & 3) * 8 + (i ^ (s >> 2)) * 32;
         s16x4 half[2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int r = row + 4 * u;
+        for (int u = 0; u < 2; ++u)
             half[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (lds4)(at + r * 256 + (((b >> 4) ^ (r & 7)) * 32)));
-        }
+                (lds4)(at + h * 8192 + u * 1024 + ((b >> 6) ^ u) * 128));
         return __builtin_bit_cast(
             bf16x8, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
     }
@@ -200,16 +216,18 @@ struct Side {
 // Tiles of A B^T one after the other for one workgroup: 4 waves of 64 x 64, 64 of
 // the summed index a step, the next step's operands on their way from memory
 // while this one's are multiplied, also across tiles. `rows(tile)` gives the
-// tile's first rows of A and B; `done(tile, acc)` takes its 128 x 128 sums.
-#define GS_TILE_LDS __shared__ quad lds[2][2][kTile * 8]
-template <int NP, bool AK, bool BK, class Rows, class Done>
+// tile's first rows of A and B; `done(tile, acc)` takes its 128 x 128 sums. LDS
+// holds one step: the other workgroup of the compute unit fills the waits.
+#define GS_TILE_LDS __shared__ quad lds[2][kTile * 8]
+template <int NP, bool AK, bool BK, bool PAIRS = false, class Rows, class Done>
 __device__ __forceinline__ void tile_products(const Mat& A, const Mat& B, int64_t k0, int64_t k1,
-                                              int tiles, quad (*lds)[2][kTile * 8], Rows rows,
+                                              int tiles, quad (*lds)[kTile * 8], Rows rows,
                                               Done done) {
-    const int w = threadIdx.x >> 6, wm = (w >> 1) * 64, wn = (w & 1) * 64;
+    const int w = wave_id(), wm = (w >> 1) * 64, wn = (w & 1) * 64;
     const int steps_k = (int)((k1 - k0) / kStep), per_tile = steps_k * Products<NP>::kCount;
-    Side<AK> a;
-    Side<BK> b;
+    using SideA = Side<AK, PAIRS>;
+    SideA a(A);
+    Side<BK> b(B);
     int tile_f = 0, q_f = 0, k_f = 0;  // the next step to fetch
     auto fetch = [&] {
         const auto at = rows(tile_f);
@@ -233,23 +251,27 @@ __device__ __forceinline__ void tile_products(const Mat& A, const Mat& B, int64_
     };
     clear();
     const int steps = per_tile * tiles;
-    if (steps > 0) {
-        fetch();
-        a.keep(lds[0][0]);
-        b.keep(lds[0][1]);
-    }
-    __syncthreads();
+    if (steps > 0) fetch();
     int left = per_tile, tile = 0;
     for (int s = 0; s < steps; ++s) {
-        const int buf = s & 1;
+        __syncthreads();
+        a.keep(lds[0]);
+        b.keep(lds[1]);
+        __syncthreads();
         if (s + 1 < steps) fetch();
+        if (left == 0) {  // here the tile's stores have a step's time until loads wait for them
+            done(tile++, acc);
+            clear();
+            left = per_tile;
+        }
+        --left;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             bf16x8 fa[4], fb[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                fa[i] = Side<AK>::operand(lds[buf][0], wm + i * 16, h);
-                fb[i] = Side<BK>::operand(lds[buf][1], wn + i * 16, h);
+                fa[i] = SideA::operand(lds[0], wm, i, h);
+                fb[i] = Side<BK>::operand(lds[1], wn, i, h);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -258,18 +280,8 @@ __device__ __forceinline__ void tile_products(const Mat& A, const Mat& B, int64_
                     acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], fb[j], acc[i][j], 0,
                                                                         0, 0);
         }
-        if (s + 1 < steps) {
-            a.keep(lds[buf ^ 1][0]);
-            b.keep(lds[buf ^ 1][1]);
-        }
-        if (--left == 0) {
-            done(tile++, acc);
-            clear();
-            left = per_tile;
-        }
-        __syncthreads();
     }
-    if (steps == 0) done(0, acc);
+    done(tile, acc);
 }
 
 struct TileRows {
@@ -295,7 +307,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_loss_scores(Mat F, Mat T, int k
                                                           int64_t padded, int tiles, int share,
                                                           float2* part, float* label_score) {
     GS_TILE_LDS;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, w = wave_id();
     const int wm = (w >> 1) * 64, wn = (w & 1) * 64;
     const int64_t n0 = (int64_t)blockIdx.x * kTile;
     const int t0 = blockIdx.y * share, t1 = min(tiles, t0 + share);
@@ -412,7 +424,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_loss_g(Mat F, Mat T, int kd, in
                                                      int64_t r0, int64_t v0, int64_t rc, int64_t vc,
                                                      int share, bf16* G) {
     GS_TILE_LDS;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, w = wave_id();
     const int wm = (w >> 1) * 64, wn = (w & 1) * 64;
     const int64_t n0 = (int64_t)blockIdx.x * kTile;
     const int t0 = blockIdx.y * share, t1 = min((int)(vc / kTile), t0 + share);
@@ -425,38 +437,36 @@ __global__ __launch_bounds__(kThreads, 2) void k_loss_g(Mat F, Mat T, int kd, in
         wt[n] = weight[i];
         l2[n] = lse2[i];
     }
-    tile_products<NP, true, true>(
+    tile_products<NP, true, true, true>(
         T, F, 0, kd, t1 - t0, lds,
         [&](int t) { return TileRows{v0 + (int64_t)(t0 + t) * kTile, r0 + n0}; },
         [&](int t, f32x4(&acc)[4][4]) {
             const int64_t tile = (int64_t)(t0 + t) * kTile + wm;  // within the piece
-            const int64_t at = tile + (lane >> 4) * 4;
+            const int64_t at = tile + (lane >> 4) * 8;
+            const bool in = v0 + tile + 64 <= rows;  // else some rows are padding
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
                 const bool any = __any(y[n] >= v0 + tile && y[n] < v0 + tile + 64);
                 bf16* row = G + (n0 + wn + n * 16 + (lane & 15)) * vc + at;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float v[4];
+                for (int i = 0; i < 2; ++i) {  // 8 values of blocks 2 i and 2 i + 1
+                    float v[8];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        v[j] = grad_exp2<NP>(fmaf(acc[i][n][j], scale2, -l2[n]));
+                    for (int j = 0; j < 8; ++j)
+                        v[j] = grad_exp2<NP>(fmaf(acc[2 * i + (j >> 2)][n][j & 3], scale2, -l2[n]));
                     if (any) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            if (v0 + at + i * 16 + j == y[n]) v[j] -= 1.0f;
+                        for (int j = 0; j < 8; ++j)
+                            if (v0 + at + i * 32 + j == y[n]) v[j] -= 1.0f;
                     }
-                    const bool in = v0 + tile + 64 <= rows;  // else some rows are padding
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        v[j] = y[n] >= 0 && (in || v0 + at + i * 16 + j < rows) ? v[j] * wt[n] : 0.0f;
-                    uint32_t p0[NP], p1[NP];
-                    split2<NP>(v[0], v[1], p0);
-                    split2<NP>(v[2], v[3], p1);
+                    for (int j = 0; j < 8; ++j)
+                        v[j] = y[n] >= 0 && (in || v0 + at + i * 32 + j < rows) ? v[j] * wt[n] : 0.0f;
+                    quad part[NP];
+                    split8<NP>(v, part);
 #pragma unroll
                     for (int p = 0; p < NP; ++p)
-                        *reinterpret_cast<uint2*>(row + p * rc * vc + i * 16) =
-                            make_uint2(p0[p], p1[p]);
+                        *reinterpret_cast<quad*>(row + p * rc * vc + i * 32) = part[p];
                 }
             }
         });
@@ -476,41 +486,74 @@ struct SumOut {
     int64_t rows, stride;
     int dim;
     const int32_t* label;
-    __device__ __forceinline__ void put(int64_t r, int c, float v) const {
-        if (!first) v += sum[r * dq + c];
-        if (!last)
-            sum[r * dq + c] = v;
-        else if (r < rows && c < dim)
-            out[r * stride + c] = from_float<T>(label != nullptr && label[r] < 0 ? 0.0f : v);
+    // 4 values from column c of row r
+    __device__ __forceinline__ void put(int64_t r, int c, f32x4 v) const {
+        f32x4* to = reinterpret_cast<f32x4*>(sum + r * dq + c);
+        if (!first) v += *to;
+        if (!last) {
+            *to = v;
+            return;
+        }
+        if (r >= rows || c >= dim) return;
+        if (label != nullptr && label[r] < 0) v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        const float x[4] = {v[0], v[1], v[2], v[3]};
+        T* row = out + r * stride + c;
+        if (c + 4 <= dim) {
+            store_any<4>(row, x);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (c + j < dim) row[j] = from_float<T>(x[j]);
+        }
     }
 };
 
 // A share (blockIdx.z) of A B over the summed index, for 128 x 128 sums. A: G, by
-// samples (AK) or transposed; B's rows are the summed index.
+// samples (AK) or transposed; B's rows are the summed index. The sums leave through
+// LDS, half of the columns at a time, as rows of whole vectors: straight from the
+// registers the 64 addresses of a lane spilled.
 template <typename T, int NP, bool AK>
 __global__ __launch_bounds__(kThreads, 2) void k_loss_sum(Mat A, Mat B, int64_t k, int64_t share,
-                                                       SumOut<T> o) {
-    GS_TILE_LDS;
+                                                          SumOut<T> o) {
+    constexpr int kRow = 68;  // floats of a row of 64, so that rows 4 apart use other banks
+    __shared__ quad buf[kTile * kRow / 4];
+    static_assert(kTile * kRow / 4 >= 2 * kTile * 8, "the operands' tiles fit");
     const int64_t m0 = (int64_t)blockIdx.x * kTile, n0 = (int64_t)blockIdx.y * kTile;
     const int64_t k0 = min(k, share * blockIdx.z), k1 = min(k, k0 + share);
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, w = wave_id();
     const int wm = (w >> 1) * 64, wn = (w & 1) * 64;
     tile_products<NP, AK, false>(
-        A, B, k0, k1, 1, lds, [&](int) { return TileRows{m0, n0}; },
+        A, B, k0, k1, 1, reinterpret_cast<quad(*)[kTile * 8]>(buf),
+        [&](int) { return TileRows{m0, n0}; },
         [&](int, f32x4(&acc)[4][4]) {
+            float* f = reinterpret_cast<float*>(buf);
+#pragma unroll 1
+            for (int half = 0; half < 2; ++half) {
+                __syncthreads();
+                if (wn == half * 64) {
+                    float* at = f + (wm + (lane >> 4) * 4) * kRow + (lane & 15);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+                    for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int n = 0; n < 4; ++n)
+                        for (int n = 0; n < 4; ++n)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int64_t r = m0 + wm + i * 16 + (lane >> 4) * 4 + j;
-                        const int c = (int)n0 + wn + n * 16 + (lane & 15);
-                        if (gridDim.z > 1)
-                            o.slices[((int64_t)blockIdx.z * o.m + r) * o.dq + c] = acc[i][n][j];
-                        else
-                            o.put(r, c, acc[i][n][j]);
-                    }
+                            for (int j = 0; j < 4; ++j)
+                                at[(i * 16 + j) * kRow + n * 16] = acc[i][n][j];
+                }
+                __syncthreads();
+#pragma unroll 2
+                for (int e = threadIdx.x; e < kTile * 16; e += kThreads) {
+                    const int r = e >> 4, c = (e & 15) * 4;
+                    const f32x4 v = *reinterpret_cast<const f32x4*>(f + r * kRow + c);
+                    const int64_t row = m0 + r;
+                    const int column = (int)n0 + half * 64 + c;
+                    if (gridDim.z > 1)
+                        *reinterpret_cast<f32x4*>(
+                            o.slices + ((int64_t)blockIdx.z * o.m + row) * o.dq + column) = v;
+                    else
+                        o.put(row, column, v);
+                }
+            }
         });
 }
 
@@ -545,8 +588,7 @@ __global__ __launch_bounds__(kThreads) void k_loss_fold(SumOut<T> o, int nz) {
         if (e >= total) continue;
         const int64_t r = e / (o.dq / 4);
         const int c = (int)(e - r * (o.dq / 4)) * 4;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o.put(r, c + j, s[j]);
+        o.put(r, c, s);
     }
 }
 
@@ -953,7 +995,8 @@ __global__ __launch_bounds__(kThreads, one_a_unit(KS, ROLE) ? 1 : 2) void k_stre
 int64_t pad_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 // Pieces of G: up to 8192 table rows by as many samples as make 2^27 values (256 MB
-// of bf16, what the cache behind the L2s holds), a third of that in three parts.
+// of bf16, what the cache behind the L2s holds), a third of that in three parts;
+// more table rows where there are few samples.
 struct LossPlan {
     int np, kd, dq;
     int64_t np_rows, vp, rc, vc;
@@ -979,7 +1022,9 @@ struct LossPlan {
         np_rows = pad_to(n, kTile);
         vp = pad_to(rows, kTile);
         vc = std::min<int64_t>(vp, 8192);
-        rc = std::min<int64_t>(np_rows, std::max<int64_t>(kTile, ((1 << 27) / np / vc) / kTile * kTile));
+        const int64_t area = (1 << 27) / np;
+        rc = std::min<int64_t>(np_rows, std::max<int64_t>(kTile, area / vc / kTile * kTile));
+        vc = std::min<int64_t>(vp, std::max<int64_t>(vc, area / std::max<int64_t>(rc, 1) / kTile * kTile));
         split_k(rc / kTile * (dq / kTile), vc, &zf, &share_f);
         split_k(vc / kTile * (dq / kTile), rc, &zt, &share_t);
         // scores: about 4096 workgroups, where that leaves 8 tiles each
