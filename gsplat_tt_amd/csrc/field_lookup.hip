@@ -327,15 +327,18 @@ __global__ __launch_bounds__(kShortThreads) void k_sort_short(LookupGradArgs a, 
 // at once; runs over several stretches are joined by a segmented scan over the
 // slots, in a fixed order.
 //
-// Two uses. Where ids have to be sorted over the whole list (LOCAL false), spans
+// Three uses. Where ids have to be sorted over the whole list (kSorted), spans
 // follow that order: a run inside a span is a row's whole sum, and a span's first
 // and last run, where they go on in its neighbours, are added up by k_run_join
-// from `part` (span, 2, dim). With few rows (LOCAL) no such sort is needed: a span
+// from `part` (span, 2, dim). With few rows (kLocal) no such sort is needed: a span
 // is some consecutive ids that the workgroup sorts itself, and each row's sum
 // over it goes to `part` (span, rows, dim). That reads dout almost in order, in 2
-// launches instead of 5.
+// launches instead of 5. With few ids (kOwn) each workgroup takes kLocalRows rows
+// of the table, looks through all ids for them and writes those rows whole: one
+// launch.
+enum { kSorted = 0, kLocal = 1, kOwn = 2 };
 constexpr int kSpan = 4096;      // most entries of a span
-constexpr int kLocalRows = 128;  // most rows for LOCAL: a quarter of the least span
+constexpr int kLocalRows = 128;  // most rows for kLocal: a quarter of the least span
 
 // scale * acc into (or onto) values lo .. hi - 1 of VEC ones of a row, at once where
 // that is all of them.
@@ -364,7 +367,7 @@ __device__ __forceinline__ void put_row(TD* out, const float* acc, float scale, 
         }
 }
 
-template <typename TI, typename TD, int VEC, bool LOCAL>
+template <typename TI, typename TD, int VEC, int MODE>
 __global__ __launch_bounds__(kThreads) void k_run_sums(LookupGradArgs a, const uint2* pairs,
                                                        int span, int lpr, int bits, float* part,
                                                        uint2* runs) {
@@ -384,11 +387,15 @@ __global__ __launch_bounds__(kThreads) void k_run_sums(LookupGradArgs a, const u
     const bool col_on = c0 + lane * VEC < a.dim, whole = a.dim >= VEC;
     const int c = whole ? min(c0 + lane * VEC, a.dim - VEC) : 0;
     const int c_lo = c0 + lane * VEC - c, c_hi = whole ? VEC : a.dim;
-    const uint32_t rows = (uint32_t)a.rows;
-    const int64_t base = (int64_t)blockIdx.x * span;
-    const int m = (int)min((int64_t)span, a.n - base);
+    // kOwn: the workgroup's rows of the table, and keys counted from their first
+    const int64_t row0 = MODE == kOwn ? (int64_t)blockIdx.x * kLocalRows : 0;
+    const uint32_t rows = (uint32_t)(MODE == kOwn ? min((int64_t)kLocalRows, a.rows - row0) : a.rows);
+    const int64_t base = MODE == kOwn ? 0 : (int64_t)blockIdx.x * span;
+    int m = (int)min((int64_t)span, a.n - base);
     uint32_t before = kNone, after = kNone;  // the neighbours' keys
-    if (LOCAL) {
+    if (MODE != kSorted) {
+        uint32_t* const flags = blockIdx.y == 0 && (MODE == kLocal || blockIdx.x == 0) ? a.flags
+                                                                                     : nullptr;
         __shared__ uint32_t cnt[kWaves][kLocalRows + 1];
         __shared__ uint32_t scan[kWaves];
         for (int k = t; k < kWaves * (kLocalRows + 1); k += kThreads) (&cnt[0][0])[k] = 0u;
@@ -399,8 +406,11 @@ __global__ __launch_bounds__(kThreads) void k_run_sums(LookupGradArgs a, const u
         for (int k = 0; k < kSpan / kThreads; ++k) {
             const int i = w * (span / kWaves) + k * 64 + l;
             if (k < span / kThreads) {
-                key[k] = i < m ? sort_key(a, nullptr, base + i, blockIdx.y == 0 ? a.flags : nullptr)
-                               : 0u;
+                key[k] = i < m ? sort_key(a, nullptr, base + i, flags) : 0u;
+                if (MODE == kOwn) {
+                    const int64_t own = (int64_t)key[k] - row0;
+                    key[k] = own >= 0 && own < rows ? (uint32_t)own : rows;
+                }
                 rank[k] = wave_rank(key[k], i < m, bits, cnt[w]);
             }
         }
@@ -426,14 +436,20 @@ __global__ __launch_bounds__(kThreads) void k_run_sums(LookupGradArgs a, const u
             }
         }
         __syncthreads();
+        if (MODE == kOwn) m = (int)cnt[0][rows];  // those of other rows came last
         // rows that no id of the span names
-        float* row0 = part + (size_t)blockIdx.x * rows * a.dim;
-        for (uint32_t v = slot; v < rows; v += slots) {
-            const uint32_t lo = cnt[0][v];
-            if (lo < (uint32_t)m && skey[lo] == v) continue;
-            const float zero[VEC] = {};
-            if (col_on) put_row<float, VEC>(row0 + (size_t)v * a.dim + c, zero, 1.0f, 0, c_lo, c_hi);
-        }
+        if (MODE == kLocal || !a.accumulate)
+            for (uint32_t v = slot; v < rows; v += slots) {
+                const uint32_t lo = cnt[0][v];
+                if ((lo < (uint32_t)m && skey[lo] == v) || !col_on) continue;
+                const float zero[VEC] = {};
+                if (MODE == kLocal)
+                    put_row<float, VEC>(part + ((size_t)blockIdx.x * rows + v) * a.dim + c, zero,
+                                        1.0f, 0, c_lo, c_hi);
+                else
+                    put_row<TD, VEC>(dtable + (row0 + v) * a.dtable_stride + c, zero, 1.0f, 0, c_lo,
+                                     c_hi);
+            }
     } else {
         for (int i = t; i < m; i += kThreads) {
             const uint2 p = pairs[base + i];
@@ -455,17 +471,17 @@ __global__ __launch_bounds__(kThreads) void k_run_sums(LookupGradArgs a, const u
     // its last, 2 neither
     auto finish = [&](uint32_t key, const float* acc, int which) {
         if (key >= rows) return;
-        if (LOCAL || which < 2) {
-            const size_t row = LOCAL ? (size_t)blockIdx.x * rows + key
-                                     : (size_t)blockIdx.x * 2 + which;
+        if (MODE == kLocal || (MODE == kSorted && which < 2)) {
+            const size_t row = MODE == kLocal ? (size_t)blockIdx.x * rows + key
+                                              : (size_t)blockIdx.x * 2 + which;
             put_row<float, VEC>(part + row * a.dim + c, acc, 1.0f, 0, c_lo, c_hi);
         } else {
-            put_row<TD, VEC>(dtable + (int64_t)key * a.dtable_stride + c, acc, a.scale,
+            put_row<TD, VEC>(dtable + (row0 + key) * a.dtable_stride + c, acc, a.scale,
                              a.accumulate, c_lo, c_hi);
         }
     };
 
-    const int per = (span + slots - 1) / slots, lo = min(m, slot * per), hi = min(m, lo + per);
+    const int per = ((MODE == kOwn ? m : span) + slots - 1) / slots, lo = min(m, slot * per), hi = min(m, lo + per);
     float acc[VEC], head[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) acc[j] = head[j] = 0.0f;
@@ -665,7 +681,7 @@ __global__ __launch_bounds__(kThreads) void k_run_join(LookupGradArgs a, const u
     }
 }
 
-// LOCAL's join: a workgroup per row and 16 columns, 16 slots over the spans.
+// kLocal's join: a workgroup per row and 16 columns, 16 slots over the spans.
 template <typename TD>
 __global__ __launch_bounds__(kThreads) void k_local_join(LookupGradArgs a, int spans,
                                                          const float* part) {
@@ -700,11 +716,20 @@ int key_bits(int64_t rows) {  // keys 0 .. rows
     return b;
 }
 
-// Consecutive ids of a LOCAL span: as many as leave two workgroups a compute unit.
+// Consecutive ids of a kLocal span: as many as leave two workgroups a compute unit.
 int local_span(int64_t n) {
     int s = 512;
     while (s < kSpan && n / (2 * s) >= 512) s *= 2;
     return s;
+}
+
+// Few enough ids that every workgroup may look through them all, and that one
+// workgroup may sum them all, should they be one row's (with more than a few where
+// the table gives kLocal no work to share: 4096 x 32 into one row took 41 us so, 13
+// by kLocal; 1000 x 32 into 5000 rows 11, and 20 sorted).
+bool is_own(int64_t n, int64_t rows, int dim) {
+    return n > 0 && n <= (rows > kLocalRows ? kSpan : 1024) && n * dim <= (1 << 17) &&
+           rows <= (1 << 20);
 }
 
 bool is_local(int64_t n, int64_t rows) { return rows <= kLocalRows && n > 0; }
@@ -732,7 +757,8 @@ struct GradWs {
     size_t bytes;
     GradWs(void* base, int64_t n, int64_t rows, int dim) {
         Carve c(base);
-        if (is_local(n, rows)) {
+        if (is_own(n, rows, dim)) {
+        } else if (is_local(n, rows)) {
             const int span = local_span(n);
             part = c.take<float>((size_t)((n + span - 1) / span) * rows * dim);
         } else {
@@ -756,9 +782,16 @@ hipError_t grad_typed(const LookupGradArgs& a, const GradWs& w, const uint2* pai
     int lpr = 1;
     while (lpr < 64 && lpr < units) lpr *= 2;
     const unsigned cols = (unsigned)((units + lpr - 1) / lpr);
+    if (is_own(a.n, a.rows, a.dim)) {
+        const int span = (int)((a.n + kThreads - 1) / kThreads) * kThreads;
+        k_run_sums<TI, TD, VEC, kOwn>
+            <<<dim3((unsigned)((a.rows + kLocalRows - 1) / kLocalRows), cols), kThreads, span * 8, st>>>(
+                a, nullptr, span, lpr, key_bits(kLocalRows), nullptr, nullptr);
+        return hipGetLastError();
+    }
     if (is_local(a.n, a.rows)) {
         const int span = local_span(a.n), spans = (int)((a.n + span - 1) / span);
-        k_run_sums<TI, TD, VEC, true><<<dim3((unsigned)spans, cols), kThreads, span * 8, st>>>(
+        k_run_sums<TI, TD, VEC, kLocal><<<dim3((unsigned)spans, cols), kThreads, span * 8, st>>>(
             a, nullptr, span, lpr, key_bits(a.rows), w.part, nullptr);
         k_local_join<TD><<<dim3((unsigned)a.rows, (unsigned)((a.dim + 15) / 16)), kThreads, 0, st>>>(
             a, spans, w.part);
@@ -767,7 +800,7 @@ hipError_t grad_typed(const LookupGradArgs& a, const GradWs& w, const uint2* pai
     // a slot's stretch holds the 8 rows that it loads at a time
     const int span = std::max(span_of(a.n), std::min(kSpan, kThreads / lpr * 8));
     if (a.n > 0)
-        k_run_sums<TI, TD, VEC, false>
+        k_run_sums<TI, TD, VEC, kSorted>
             <<<dim3((unsigned)((a.n + span - 1) / span), cols), kThreads, span * 8, st>>>(
                 a, pairs, span, lpr, 0, w.part, w.runs);
     int join_lpr = 1;
@@ -822,7 +855,9 @@ hipError_t launch_lookup_grad(const LookupGradArgs& a, hipStream_t st) {
     if (a.n == 0)
         k_run_clear<<<(unsigned)((a.rows + kThreads - 1) / kThreads), kThreads, 0, st>>>(w.runs,
                                                                                       a.rows);
-    else if (is_short(a.n, a.rows)) {
+    else if (is_own(a.n, a.rows, a.dim)) {
+        // the one launch of grad_typed
+    } else if (is_short(a.n, a.rows)) {
         k_sort_short<<<1, kShortThreads, 0, st>>>(a, key_bits(a.rows), w.pairs[0], w.runs);
         pairs = w.pairs[0];
     } else if (!is_local(a.n, a.rows))

@@ -399,8 +399,8 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_finish(NormArgs a, int c
     }
 }
 
-__global__ __launch_bounds__(kThreads) void k_norm_grad_params(NormArgs a, const float2* sums) {
-    const int c = blockIdx.x * kThreads + threadIdx.x;
+// dweight and dbias of channel c: its sums over the images.
+__device__ __forceinline__ void grad_params(const NormArgs& a, const float2* sums, int c) {
     if (c >= a.channels) return;
     float db = 0.0f, dw = 0.0f;
     for (int64_t b = 0; b < a.batch; ++b) {
@@ -410,6 +410,9 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_params(NormArgs a, const
     }
     if (a.dbias != nullptr) a.dbias[c] = db;
     if (a.dweight != nullptr) a.dweight[c] = dw;
+}
+__global__ __launch_bounds__(kThreads) void k_norm_grad_params(NormArgs a, const float2* sums) {
+    grad_params(a, sums, blockIdx.x * kThreads + threadIdx.x);
 }
 
 // dx = rstd w dz - rstd m1 - xh rstd m2
@@ -426,8 +429,13 @@ __device__ __forceinline__ void grad_of(const Channels<VEC>& ch, const float* rw
 
 template <typename T, int VEC, int ACT>
 __global__ __launch_bounds__(kThreads) void k_norm_grad_apply(NormArgs a, int chunks,
-                                                              const float2* means) {
+                                                              const float2* means,
+                                                              const float2* sums) {
     constexpr int AHEAD = kAhead / 2;
+    // with few images the parameters' gradients need no launch of their own
+    if (sums != nullptr && blockIdx.y == 0)
+        for (int c = blockIdx.x * kThreads + threadIdx.x; c < a.channels; c += gridDim.x * kThreads)
+            grad_params(a, sums, c);
     const Place p = place_of<VEC>(a.pixels, a.channels, chunks);
     if (!p.on) return;
     const Channels<VEC> ch(a, p.b, p.c);
@@ -618,6 +626,9 @@ int chunks_of(int64_t batch, int64_t pixels) {
     return k < 1 ? 1 : (int)k;
 }
 
+// Images whose sums one thread adds in passing.
+constexpr int64_t kFewImages = 16;
+
 struct NormWs {
     float2 *part, *sums, *means;
     size_t bytes;
@@ -665,9 +676,11 @@ hipError_t norm_run(const NormArgs& a, bool grad, hipStream_t st) {
     } else {
         k_norm_grad_sums<T, VEC, ACT><<<grid, kThreads, 0, st>>>(a, chunks, w.part);
         k_norm_grad_finish<<<groups, kThreads, 0, st>>>(a, chunks, w.part, w.sums, w.means);
-        k_norm_grad_params<<<(unsigned)((a.channels + kThreads - 1) / kThreads), kThreads, 0, st>>>(
-            a, w.sums);
-        k_norm_grad_apply<T, VEC, ACT><<<grid, kThreads, 0, st>>>(a, chunks, w.means);
+        if (a.batch > kFewImages)
+            k_norm_grad_params<<<(unsigned)((a.channels + kThreads - 1) / kThreads), kThreads, 0,
+                                 st>>>(a, w.sums);
+        k_norm_grad_apply<T, VEC, ACT><<<grid, kThreads, 0, st>>>(
+            a, chunks, w.means, a.batch > kFewImages ? nullptr : w.sums);
     }
     return hipGetLastError();
 }
@@ -691,7 +704,9 @@ hipError_t norm_typed(const NormArgs& a, bool grad, hipStream_t st) {
     const bool vec = a.channels % VEC == 0 && rows_ok(a.x, a.x_batch, a.x_pixel) &&
                      rows_ok(a.y, a.y_batch, a.y_pixel) && rows_ok(a.dy, a.dy_batch, a.dy_pixel) &&
                      rows_ok(a.dx, a.dx_batch, a.dx_pixel);
-    return vec ? norm_act<T, VEC>(a, grad, st) : norm_act<T, 1>(a, grad, st);
+    // groups that make no vectors, but are small enough, still go in one launch
+    if (vec && (small_group<VEC>(a) || !small_group<1>(a))) return norm_act<T, VEC>(a, grad, st);
+    return norm_act<T, 1>(a, grad, st);
 }
 
 }  // namespace
