@@ -758,6 +758,7 @@ struct GradWs {
     GradWs(void* base, int64_t n, int64_t rows, int dim) {
         Carve c(base);
         if (is_own(n, rows, dim)) {
+            totals = c.take<uint32_t>(1);  // not used: every size asks for a workspace
         } else if (is_local(n, rows)) {
             const int span = local_span(n);
             part = c.take<float>((size_t)((n + span - 1) / span) * rows * dim);

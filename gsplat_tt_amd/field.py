@@ -18,12 +18,15 @@ the call by the caller, as for any torch operation. There is no CPU fallback.
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
 from . import _lib as L
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+_ID_TYPES = (torch.int32, torch.int64)
+_PARAM_TYPES = (torch.float32,)
 _ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 FLAG_ID_RANGE = 1
 
@@ -62,16 +65,16 @@ class FieldOps:
 
     # ---- checks
     def _own(self, t, name, dtypes=_DTYPES):
+        if isinstance(t, torch.Tensor) and t.get_device() == self._index and t.dtype in dtypes:
+            return t
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a torch tensor")
         if t.device != self.device:
             raise ValueError(f"{name} is on {t.device}, not on {self.device}")
-        if t.dtype not in dtypes:
-            raise TypeError(f"{name} has the type {t.dtype}")
-        return t
+        raise TypeError(f"{name} has the type {t.dtype}")
 
     def _ids(self, t, name, n=None):
-        self._own(t, name, (torch.int32, torch.int64))
+        self._own(t, name, _ID_TYPES)
         if t.dim() != 1 or (n is not None and t.shape[0] != n):
             raise ValueError(f"{name} must be one-dimensional" +
                              (f" with {n} values" if n is not None else ""))
@@ -80,7 +83,7 @@ class FieldOps:
     def _param(self, t, name, n):
         if t is None:
             return None
-        self._own(t, name, (torch.float32,))
+        self._own(t, name, _PARAM_TYPES)
         if t.dim() != 1 or t.shape[0] != n:
             raise ValueError(f"{name} must be one-dimensional with {n} values")
         return t.contiguous()
@@ -89,7 +92,7 @@ class FieldOps:
         if out is None:
             return torch.empty(shape, dtype=dtype, device=self.device)
         self._own(out, name)
-        if tuple(out.shape) != tuple(shape):
+        if out.shape != torch.Size(shape):
             raise ValueError(f"{name} must be {tuple(shape)}, not {tuple(out.shape)}")
         return out
 
@@ -158,10 +161,10 @@ class FieldOps:
         """Pointer, image stride, pixel stride of a (batch, ..., channels) tensor whose
         pixels lie at one distance."""
         self._own(t, name)
-        if t.dim() < 2 or (shape is not None and tuple(t.shape) != tuple(shape)):
+        if t.dim() < 2 or (shape is not None and t.shape != shape):
             raise ValueError(f"{name} must be (batch, pixels..., channels)" +
                              (f" = {tuple(shape)}" if shape is not None else ""))
-        if dtype is not None and t.dtype != dtype:
+        if dtype is not None and t.dtype is not dtype:
             raise TypeError(f"{name} must have the type {dtype}")
         if t.is_contiguous():
             return t.data_ptr(), t.stride(0), t.shape[-1]
@@ -183,12 +186,10 @@ class FieldOps:
     def _norm(self, x, groups, weight, bias, act, eps):
         if act not in _ACTS:
             raise ValueError(f"act must be one of {sorted(_ACTS)}")
-        c = x.shape[-1]
+        shape = x.shape
+        c = shape[-1]
         weight, bias = self._param(weight, "weight", c), self._param(bias, "bias", c)
-        pixels = 1
-        for k in x.shape[1:-1]:
-            pixels *= k
-        d = L.GsGroupNorm(x.shape[0], pixels, c, int(groups), _ACTS[act], _DTYPES[x.dtype],
+        d = L.GsGroupNorm(shape[0], math.prod(shape[1:-1]), c, int(groups), _ACTS[act], _DTYPES[x.dtype],
                           float(eps), 0, None if weight is None else weight.data_ptr(),
                           None if bias is None else bias.data_ptr())
         return d, (weight, bias)
@@ -221,10 +222,11 @@ class FieldOps:
         if out is None:
             out = torch.empty_like(x, memory_format=torch.contiguous_format)
         po, bo, so = self._image(out, "out", x.shape, x.dtype)
+        stats = (d.batch, d.groups)
         for t, name in ((mean, "mean"), (rstd, "rstd")):
-            self._own(t, name, (torch.float32,))
-            if tuple(t.shape) != (d.batch, d.groups) or not t.is_contiguous():
-                raise ValueError(f"{name} must be group_norm()'s: contiguous {d.batch, d.groups}")
+            self._own(t, name, _PARAM_TYPES)
+            if t.shape != stats or not t.is_contiguous():
+                raise ValueError(f"{name} must be group_norm()'s: contiguous {stats}")
         dweight, dbias = torch.empty((2, d.channels), dtype=torch.float32, device=self.device)
         ws, size = self._workspace("gs_group_norm_workspace", d.batch, d.pixels, d.channels)
         L._check(self._L.gs_group_norm_grad_dev(
