@@ -625,6 +625,15 @@ hipError_t fold(const SumOut<T>& o, int nz, hipStream_t st) {
 // [part][dim / 32][f].
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 
+//
+// kScores: losses alone. kGradFeat: losses and dfeat in one pass over the table: the
+// sums of e_v table_v, e_v = exp2(score_v - m), go along with the sum of e_v, both
+// scaled down when a query's largest score has grown past m by more than kSlack
+// (at a query's first tile, then hardly ever). The label's row stays out of the
+// rounded products: dfeat = weight (sums / sum + (e_label / sum - 1) table_label),
+// its factor in fp32, so that a label with almost all of its row's probability
+// costs no digits. kGradTable: the table's gradient, with the losses known.
+constexpr float kSlack = 8.0f;
 enum { kScores = 0, kGradFeat = 1, kGradTable = 2 };
 
 struct StreamArgs {
@@ -639,19 +648,31 @@ struct StreamArgs {
     // of the samples, whichever side they are: label, weight * scale, lse in log2 units
     const int32_t* label;
     const float *weight, *lse2;
-    // kScores
+    // kScores, kGradFeat
     const void* labels;
     int labels64;
     float2* part;
     float *label_score, *loss, *lse, *lse2_out;
     uint32_t* flags;
     int64_t table_rows;
+    // kGradFeat
+    const void* table;
+    int64_t table_stride;
+    const float* row_weight;
+    float scale;
     // gradients: into out where there is one share, else into (share, padded, row) sums
     void* out;
     int64_t out_stride;
     float* sums;
     int64_t padded;
 };
+
+// The larger of lane l's and lane l ^ 32's value.
+__device__ __forceinline__ float max_of_halves(float v) {
+    const uint32_t u = __float_as_uint(v);
+    const auto both = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
 
 // Key of register r of a lane in half h.
 __device__ __forceinline__ constexpr int key_of(int r) { return (r & 3) + 8 * (r >> 2); }
@@ -725,8 +746,8 @@ template <typename T, int NP, int KS, int ROLE>
 struct StreamShape {
     static constexpr int kPieces =  // quads of a tile
         NP * 64 * (KS / 16 + (ROLE == kScores ? 0 : padded_dim(KS) / 16));
-    // tiles per step: about 16 KB
-    static constexpr int kTiles = kPieces * 16 >= 16384 ? 1 : (kPieces * 16 >= 8192 ? 2 : 4);
+    // tiles per step: 8 to 24 KB (more takes registers on the way to LDS)
+    static constexpr int kTiles = kPieces * 16 >= 16384 ? 1 : (kPieces * 16 >= 6144 ? 2 : 4);
     static constexpr int kStage = kPieces * kTiles;
     static constexpr size_t kLds = 2 * kStage * 16 + (ROLE == kGradTable ? 2 * kTiles * 32 * 12 : 0);
 };
@@ -745,23 +766,14 @@ __global__ __launch_bounds__(kThreads, one_a_unit(KS, ROLE) ? 1 : 2) void k_stre
     // the wave's own queries, as right operands of the scores
     quad q[QB][KJ][NP];
     int32_t y[QB];
-    float lse2[QB];
 #pragma unroll
     for (int b = 0; b < QB; ++b) {
         const int64_t i = q0 + b * 32 + col;
         bool on = i < a.nq;
         y[b] = -1;
-        lse2[b] = 0.0f;
-        if (ROLE == kScores) {
+        if (ROLE != kGradTable) {
             if (on) y[b] = load_id(a.labels, a.labels64, i, a.table_rows,
                                    blockIdx.y == 0 && h == 0 ? a.flags : nullptr);
-            on = y[b] >= 0;
-        }
-        if (ROLE == kGradFeat) {
-            if (on) {
-                y[b] = a.label[i];
-                lse2[b] = a.lse2[i];
-            }
             on = y[b] >= 0;
         }
         if (ROLE == kGradTable) y[b] = (int32_t)min(i, (int64_t)0x7FFFFFFF);
@@ -772,13 +784,12 @@ __global__ __launch_bounds__(kThreads, one_a_unit(KS, ROLE) ? 1 : 2) void k_stre
 
     f32x16 acc[QB][ROLE == kScores ? 1 : DB];
     float m[QB], sum[QB], own[QB];
-    if (ROLE == kScores) {
 #pragma unroll
-        for (int b = 0; b < QB; ++b) {
-            m[b] = -1e30f;
-            sum[b] = own[b] = 0.0f;
-        }
-    } else {
+    for (int b = 0; b < QB; ++b) {
+        m[b] = -1e30f;
+        sum[b] = own[b] = 0.0f;
+    }
+    if (ROLE != kScores) {
 #pragma unroll
         for (int b = 0; b < QB; ++b)
 #pragma unroll
@@ -846,7 +857,7 @@ __global__ __launch_bounds__(kThreads, one_a_unit(KS, ROLE) ? 1 : 2) void k_stre
                             __builtin_bit_cast(bf16x8, q[b][j][Products<NP>::b(i)]), sc[b], 0, 0, 0);
             }
             const int64_t k0 = (int64_t)tile * 32;
-            if (ROLE == kScores) {
+            if (ROLE != kGradTable) {
 #pragma unroll
                 for (int b = 0; b < QB; ++b) {
 #pragma unroll
@@ -865,6 +876,24 @@ __global__ __launch_bounds__(kThreads, one_a_unit(KS, ROLE) ? 1 : 2) void k_stre
                     float mt = m[b];
 #pragma unroll
                     for (int r = 0; r < 16; ++r) mt = fmaxf(mt, sc[b][r]);
+                    if (ROLE == kGradFeat) {
+                        // both halves' keys enter the same sums
+                        mt = max_of_halves(mt);
+                        if (__any(mt > m[b] + kSlack)) {
+                            mt = mt > m[b] + kSlack ? mt : m[b];
+                            const float down = __builtin_amdgcn_exp2f(
+                                (m[b] < INFINITY ? m[b] : 0.0f) - (mt < INFINITY ? mt : 0.0f));
+                            sum[b] *= down;
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) {
+                                const float f = __shfl(down, key_of(r) + 4 * h, 64);
+#pragma unroll
+                                for (int d = 0; d < DB; ++d) acc[b][d][r] *= f;
+                            }
+                            m[b] = mt;
+                        }
+                        continue;  // the exponentials follow with the second product
+                    }
                     // an infinite largest counts as 0: the sum is infinite too then
                     const float base = mt < INFINITY ? mt : 0.0f;
                     const float was = m[b] < INFINITY ? m[b] : 0.0f;
@@ -875,7 +904,7 @@ __global__ __launch_bounds__(kThreads, one_a_unit(KS, ROLE) ? 1 : 2) void k_stre
                     sum[b] = sum[b] * __builtin_amdgcn_exp2f(was - base) + add;
                     m[b] = mt;
                 }
-                continue;
+                if (ROLE == kScores) continue;
             }
             quad g[QB][2][NP];
             const float* f = info + (s & 1) * TS * 96 + u * 32;
@@ -883,14 +912,17 @@ __global__ __launch_bounds__(kThreads, one_a_unit(KS, ROLE) ? 1 : 2) void k_stre
             for (int b = 0; b < QB; ++b) {
                 float v[16];
                 if (ROLE == kGradFeat) {
+                    const float base = m[b] < INFINITY ? m[b] : 0.0f;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        v[r] = grad_exp2<NP>(fmaf(sc[b][r], a.scale2, -lse2[b]));
+                    for (int r = 0; r < 16; ++r) {
+                        v[r] = __builtin_amdgcn_exp2f(sc[b][r] - base);
+                        sum[b] += v[r];
+                    }
                     const int64_t yl = y[b] - k0;
                     if (__any(yl >= 0 && yl < 32)) {
 #pragma unroll
                         for (int r = 0; r < 16; ++r)
-                            if (yl == key_of(r) + 4 * h) v[r] -= 1.0f;
+                            if (yl == key_of(r) + 4 * h) v[r] = 0.0f;
                     }
                 } else {
                     const int yk = __float_as_int(f[2 * TS * 32 + col]);
@@ -943,7 +975,8 @@ __global__ __launch_bounds__(kThreads, one_a_unit(KS, ROLE) ? 1 : 2) void k_stre
         __syncthreads();
     }
 
-    if (ROLE == kScores) {
+    float w[QB], label_f[QB];  // kGradFeat: weight * scale, and the label row's factor
+    if (ROLE != kGradTable) {
 #pragma unroll
         for (int b = 0; b < QB; ++b) {
             const int64_t i = q0 + b * 32 + col;
@@ -953,7 +986,13 @@ __global__ __launch_bounds__(kThreads, one_a_unit(KS, ROLE) ? 1 : 2) void k_stre
             const bool here = y[b] >= 0 && ((y[b] >> 2) & 1) == h;
             const float o2 = __shfl_xor(own[b], 32, 64);
             const float mine = here ? own[b] : o2;
-            if (h != 0 || i >= a.nq) continue;
+            w[b] = 0.0f;
+            label_f[b] =
+                __builtin_amdgcn_exp2f(mine - (m[b] < INFINITY ? m[b] : 0.0f)) / sum[b] - 1.0f;
+            if (i >= a.nq) continue;
+            if (ROLE == kGradFeat && y[b] >= 0)
+                w[b] = a.scale * (a.row_weight != nullptr ? a.row_weight[i] : 1.0f);
+            if (h != 0) continue;
             if (gridDim.y == 1) {
                 const float l = (m[b] < INFINITY ? m[b] : 0.0f) + log2f(sum[b]);
                 const bool on = y[b] >= 0;
@@ -965,30 +1004,110 @@ __global__ __launch_bounds__(kThreads, one_a_unit(KS, ROLE) ? 1 : 2) void k_stre
                 if (y[b] >= (int64_t)t0 * 32 && y[b] < (int64_t)t1 * 32) a.label_score[i] = mine;
             }
         }
-        return;
+        if (ROLE == kScores) return;
     }
 #pragma unroll
     for (int b = 0; b < QB; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const int64_t i = q0 + b * 32 + key_of(r) + 4 * h;
-            if (i >= a.nq) continue;
-            float w = 1.0f;
-            bool on = true;
-            if (ROLE == kGradFeat) {
-                on = a.label[i] >= 0;
-                w = a.weight[i];
+            const int row = key_of(r) + 4 * h;  // whose lane holds what belongs to it
+            const int64_t i = q0 + b * 32 + row;
+            int32_t label = 0;
+            float over = 1.0f, weight = 1.0f, factor = 0.0f;
+            if (ROLE == kGradFeat && gridDim.y == 1) {
+                label = __shfl(y[b], row, 64);
+                over = 1.0f / __shfl(sum[b], row, 64);
+                weight = __shfl(w[b], row, 64);
+                factor = __shfl(label_f[b], row, 64);
             }
+            if (i >= a.nq) continue;
+            const T* own_row = static_cast<const T*>(a.table) + (int64_t)max(label, 0) * a.table_stride;
 #pragma unroll
             for (int d = 0; d < (ROLE == kScores ? 1 : DB); ++d) {
                 const int c = d * 32 + col;
-                const float v = on ? acc[b][d][r] * w : 0.0f;
-                if (gridDim.y > 1)
+                float v = acc[b][d][r];
+                if (gridDim.y > 1) {
                     a.sums[((size_t)blockIdx.y * a.padded + i) * DD + c] = v;
-                else if (c < a.dim)
+                } else if (c < a.dim) {
+                    if (ROLE == kGradFeat)
+                        v = label >= 0 ? weight * fmaf(v, over, factor * to_float(own_row[c])) : 0.0f;
                     static_cast<T*>(a.out)[i * a.out_stride + c] = from_float<T>(v);
+                }
             }
         }
+}
+
+// Losses and dfeat from the shares of kGradFeat: DD / 4 threads a row and 4 columns
+// each, Z times as many with every Z-th share each.
+template <typename T, int DD, int Z>
+__global__ __launch_bounds__(kThreads) void k_feat_join(StreamArgs a, int shares) {
+    constexpr int kLanes = DD / 4, kRows = kThreads / (kLanes * Z);
+    __shared__ f32x4 sums[Z > 1 ? kThreads : 1];
+    __shared__ float2 stats[Z > 1 ? kThreads : 1];
+    const int at = threadIdx.x / kLanes, row = at % kRows, z = at / kRows;
+    const int64_t i = (int64_t)blockIdx.x * kRows + row;
+    const int c = threadIdx.x % kLanes * 4;
+    float m = -1e30f, sum = 0.0f;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto add = [&](float m2, float s2, f32x4 v2) {
+        const float mm = fmaxf(m, m2), base = mm < INFINITY ? mm : 0.0f;
+        const float f = __builtin_amdgcn_exp2f((m < INFINITY ? m : 0.0f) - base);
+        const float f2 = __builtin_amdgcn_exp2f((m2 < INFINITY ? m2 : 0.0f) - base);
+        sum = sum * f + s2 * f2;
+        v = v * f + v2 * f2;
+        m = mm;
+    };
+    if (i < a.nq)
+        for (int s0 = z; s0 < shares; s0 += 4 * Z) {
+            float2 p[4];
+            f32x4 x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (s0 + u * Z < shares) {
+                    const int64_t from = (int64_t)(s0 + u * Z) * a.padded + i;
+                    p[u] = a.part[from];
+                    x[u] = *reinterpret_cast<const f32x4*>(a.sums + from * DD + c);
+                }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (s0 + u * Z < shares) add(p[u].x, p[u].y, x[u]);
+        }
+    if (Z > 1) {
+        sums[threadIdx.x] = v;
+        stats[threadIdx.x] = make_float2(m, sum);
+        __syncthreads();
+        if (z != 0) return;
+        for (int k = 1; k < Z; ++k) {
+            const int from = threadIdx.x + k * kRows * kLanes;
+            add(stats[from].x, stats[from].y, sums[from]);
+        }
+    }
+    if (i >= a.nq) return;
+    const int32_t y = load_id(a.labels, a.labels64, i, a.table_rows, nullptr);
+    if (c == 0) {
+        const float l = (m < INFINITY ? m : 0.0f) + log2f(sum);
+        if (a.loss != nullptr) a.loss[i] = y >= 0 ? (l - a.label_score[i]) * kLn2 : 0.0f;
+        if (a.lse != nullptr) a.lse[i] = y >= 0 ? l * kLn2 : 0.0f;
+        a.lse2_out[i] = y >= 0 ? l : 0.0f;
+    }
+    const T* own_row = static_cast<const T*>(a.table) + (int64_t)max(y, 0) * a.table_stride;
+    const float over = 1.0f / sum;
+    const float factor =
+        y >= 0 ? __builtin_amdgcn_exp2f(a.label_score[i] - (m < INFINITY ? m : 0.0f)) * over - 1.0f
+               : 0.0f;
+    const float w = a.scale * (a.row_weight != nullptr ? a.row_weight[i] : 1.0f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (c + j < a.dim)
+            static_cast<T*>(a.out)[i * a.out_stride + c + j] = from_float<T>(
+                y >= 0 ? w * fmaf(v[j], over, factor * to_float(own_row[c + j])) : 0.0f);
+}
+
+template <typename T, int DD, int Z>
+hipError_t feat_join(const StreamArgs& a, int shares, hipStream_t st) {
+    constexpr int kRows = kThreads / (DD / 4 * Z);
+    k_feat_join<T, DD, Z><<<(unsigned)((a.nq + kRows - 1) / kRows), kThreads, 0, st>>>(a, shares);
+    return hipGetLastError();
 }
 
 // ---------------------------------------------------------------- pieces
@@ -1160,8 +1279,9 @@ struct StreamPlan {
         const size_t first = (size_t)np * ks / 16 * 64;
         const size_t tile = first + (grad ? (size_t)np * kd / 16 * 64 : 0);
         T = c.take<quad>((tt + 4) * tile);
-        part = c.take<float2>(scores.count > 1 ? (size_t)scores.count * n : 0);
-        score = c.take<float>(scores.count > 1 ? (size_t)n : 0);
+        const int shares = grad ? by_feat.count : scores.count;
+        part = c.take<float2>(shares > 1 ? (size_t)shares * n : 0);
+        score = c.take<float>(shares > 1 ? (size_t)n : 0);
         F = nullptr;
         label = nullptr;
         weight = lse2 = sums = nullptr;
@@ -1220,7 +1340,6 @@ hipError_t stream_run(const LossArgs& a, bool grad, hipStream_t st) {
     s.label = w.label;
     s.weight = w.weight;
     s.lse2 = w.lse2;
-    s.share = w.scores.tiles;
     s.part = w.part;
     s.label_score = w.score;
     s.loss = a.loss;
@@ -1228,29 +1347,35 @@ hipError_t stream_run(const LossArgs& a, bool grad, hipStream_t st) {
     s.lse2_out = w.lse2;
     s.padded = a.n;
     hipError_t e;
-    // the gradients' tiles hold both products' operands, the scores take the first
     constexpr int DD = padded_dim(KS), kFirst = NP * KS / 16 * 64;
-    s.tile_stride = kFirst + (grad ? NP * DD / 16 * 64 : 0);
-    e = launch_stream<T, NP, KS, kScores>(s, w.scores, st);
-    if (e != hipSuccess) return e;
-    if (w.scores.count > 1)
-        k_loss_join<<<(unsigned)((a.n + 31) / 32), kThreads, 0, st>>>(a, w.part, w.scores.count, a.n,
-                                                                      w.score, w.lse2);
-    if (!grad) return hipGetLastError();
-    k_operands<T, NP, KS, true><<<(unsigned)w.tf, kThreads, 0, st>>>(
-        feat, a.n, a.feat_stride, a.dim, a, w.label, w.weight, w.lse2, w.F);
+    if (!grad) {
+        s.tile_stride = kFirst;
+        s.share = w.scores.tiles;
+        e = launch_stream<T, NP, KS, kScores>(s, w.scores, st);
+        if (e == hipSuccess && w.scores.count > 1) {
+            k_loss_join<<<(unsigned)((a.n + 31) / 32), kThreads, 0, st>>>(
+                a, w.part, w.scores.count, a.n, w.score, nullptr);
+            e = hipGetLastError();
+        }
+        return e;
+    }
+    s.tile_stride = kFirst + NP * DD / 16 * 64;
+    s.table = table;
+    s.table_stride = a.table_stride;
+    s.row_weight = a.row_weight;
+    s.scale = a.scale;
     s.share = w.by_feat.tiles;
     s.out = a.dfeat;
     s.out_stride = a.dfeat_stride;
     s.sums = w.sums;
     e = launch_stream<T, NP, KS, kGradFeat>(s, w.by_feat, st);
     if (e != hipSuccess) return e;
-    if (w.by_feat.count > 1) {
-        e = fold(SumOut<T>{w.sums, nullptr, 1, 1, a.n, DD, static_cast<T*>(a.dfeat), a.n,
-                       a.dfeat_stride, a.dim, w.label},
-             w.by_feat.count, st);
-        if (e != hipSuccess) return e;
-    }
+    if (w.by_feat.count > 1)
+        e = w.by_feat.count > 16 ? feat_join<T, DD, 8>(s, w.by_feat.count, st)
+                                 : feat_join<T, DD, 1>(s, w.by_feat.count, st);
+    if (e != hipSuccess) return e;
+    k_operands<T, NP, KS, true><<<(unsigned)w.tf, kThreads, 0, st>>>(
+        feat, a.n, a.feat_stride, a.dim, a, w.label, w.weight, w.lse2, w.F);
     s.q = table;
     s.nq = a.rows;
     s.q_stride = a.table_stride;
