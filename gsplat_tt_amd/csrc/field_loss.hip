@@ -9,11 +9,17 @@
 // All products run on the matrix cores with bf16 operands and fp32 sums. fp32
 // inputs are cut into three bf16 parts of 8 bits each (exact: 24 bits) and the
 // six products whose weight is above 2^-24 are added up, which keeps fp32's
-// precision at 6/16 of the cost of the fp32 matrix instructions.
+// precision at 6/16 of the cost of the fp32 matrix instructions. Bf16 inputs are
+// the operands as they are; their G is rounded to bf16, as their gradients are in
+// the end.
 //
-// Operands are first laid out with the summed index contiguous and padded to
-// the tiles, rows that a mask leaves out zeroed. The gradients go in pieces of
-// rows and of the table, G of one piece at a time in the workspace.
+// Three ways, by size:
+//   few        up to 8 samples, losses alone: one read of the table, no layout.
+//   streaming  rows of at most 128: scores and G stay in registers, the other
+//              side streams through LDS (k_stream), 3 products in 2 passes.
+//   pieces     longer rows: 128 x 128 tiles, G of one piece at a time in the
+//              workspace, 4 products (the scores are made twice, once for lse).
+// All sums are made in an order that depends on the sizes alone.
 #include <algorithm>
 
 #include "field.h"
@@ -32,6 +38,8 @@ constexpr int kThreads = 256;
 constexpr int kTile = 128;  // rows and columns of a workgroup's tile
 constexpr int kStep = 64;   // summed index per step
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// Where a running maximum begins: finite, so that differences of two are numbers.
+constexpr float kLowest = -3.402823466e38f;
 
 // Part p of a value: the leading 8 significant bits, the next 8, the rest.
 // Cutting off (not rounding) leaves exact remainders.
@@ -70,13 +78,6 @@ __device__ __forceinline__ void split8(const float* v, quad* out) {
 #pragma unroll
     for (int p = 0; p < NP; ++p) out[p] = quad{w[0][p], w[1][p], w[2][p], w[3][p]};
 }
-template <int NP>
-__device__ __forceinline__ void split(float v, bf16* out) {
-    uint32_t w[NP];
-    split2<NP>(v, 0.0f, w);
-#pragma unroll
-    for (int p = 0; p < NP; ++p) out[p] = __builtin_bit_cast(bf16x2, w[p])[0];
-}
 // The products of parts: (0,0) for one part; for three, all with p + q <= 2.
 template <int NP>
 struct Products;
@@ -109,6 +110,14 @@ __global__ __launch_bounds__(kThreads) void k_loss_rows(LossArgs a, int64_t padd
 // A row's 8 values from column c, cut into parts; zeros past the row.
 template <typename T, int NP>
 __device__ __forceinline__ void load_parts(const T* row, int dim, int c, bool on, quad* out) {
+    if constexpr (NP == 1 && sizeof(T) == 2) {
+        if (c + 8 <= dim) {  // as they are
+            quad u = {0u, 0u, 0u, 0u};
+            if (on) __builtin_memcpy(&u, row + c, sizeof(u));
+            out[0] = u;
+            return;
+        }
+    }
     float v[8];
     if (on && c + 8 <= dim) {
         load_any<8>(row + c, v);
@@ -315,7 +324,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_loss_scores(Mat F, Mat T, int k
     int32_t y[4];
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
-        m[n] = -1e30f;
+        m[n] = kLowest;
         sum[n] = 0.0f;
         y[n] = label[n0 + wn + n * 16 + (lane & 15)];
     }
@@ -382,14 +391,14 @@ __global__ __launch_bounds__(kThreads) void k_loss_join(LossArgs a, const float2
     const int sub = threadIdx.x >> 5;  // of the workgroup's 32 rows
     const int64_t i = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
     __shared__ float2 lds[8][32];
-    float m = -1e30f, sum = 0.0f;
+    float m = kLowest, sum = 0.0f;
     if (i < padded)
         for (int k0 = sub; k0 < parts; k0 += 8 * 8) {
             float2 p[8];
 #pragma unroll
             for (int u = 0; u < 8; ++u)
                 p[u] = k0 + u * 8 < parts ? part[(int64_t)(k0 + u * 8) * padded + i]
-                                          : make_float2(-1e30f, 0.0f);
+                                          : make_float2(kLowest, 0.0f);
 #pragma unroll
             for (int u = 0; u < 8; ++u) join_sums(m, sum, p[u].x, p[u].y);
         }
@@ -609,8 +618,8 @@ hipError_t fold(const SumOut<T>& o, int nz, hipStream_t st) {
 
 // ---------------------------------------------------------------- streaming
 // For rows short enough that a wave keeps its own in registers: each of a
-// workgroup's 4 waves holds 32 QB "queries", the other side's rows ("keys") stream through LDS, 32
-// a tile, and neither scores nor G ever leave the registers.
+// workgroup's 4 waves holds 32 QB "queries", the other side's rows ("keys") stream
+// through LDS, 32 a tile, and neither scores nor G ever leave the registers.
 //
 // The scores of a tile are made transposed, keys by queries: a lane then holds
 // 16 keys' scores of one query, the sums over keys need no other lane until the
@@ -623,8 +632,6 @@ hipError_t fold(const SumOut<T>& o, int nz, hipStream_t st) {
 // bytes a lane), so that LDS is filled and read in order: per tile the operands
 // of the scores, [part][dim / 16], then those of the second product,
 // [part][dim / 32][f].
-typedef __attribute__((ext_vector_type(16))) float f32x16;
-
 //
 // kScores: losses alone. kGradFeat: losses and dfeat in one pass over the table: the
 // sums of e_v table_v, e_v = exp2(score_v - m), go along with the sum of e_v, both
@@ -633,6 +640,10 @@ typedef __attribute__((ext_vector_type(16))) float f32x16;
 // rounded products: dfeat = weight (sums / sum + (e_label / sum - 1) table_label),
 // its factor in fp32, so that a label with almost all of its row's probability
 // costs no digits. kGradTable: the table's gradient, with the losses known.
+//
+// MEASURED
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+
 constexpr float kSlack = 8.0f;
 enum { kScores = 0, kGradFeat = 1, kGradTable = 2 };
 
@@ -710,7 +721,8 @@ __global__ __launch_bounds__(kThreads) void k_operands(const T* src, int64_t row
     for (int e = threadIdx.x; e < 32 * DD; e += kThreads) {
         const int r = e / DD, c = e % DD;
         float v = 0.0f;
-        if (r0 + r < rows && c < dim && lab[r] >= 0) v = plain_input<NP>(to_float(src[(r0 + r) * stride + c]));
+        if (r0 + r < rows && c < dim && lab[r] >= 0)
+            v = plain_input<NP>(to_float(src[(r0 + r) * stride + c]));
         tile[r][c] = v;
     }
     __syncthreads();
@@ -786,7 +798,7 @@ __global__ __launch_bounds__(kThreads, one_a_unit(KS, ROLE) ? 1 : 2) void k_stre
     float m[QB], sum[QB], own[QB];
 #pragma unroll
     for (int b = 0; b < QB; ++b) {
-        m[b] = -1e30f;
+        m[b] = kLowest;
         sum[b] = own[b] = 0.0f;
     }
     if (ROLE != kScores) {
@@ -1047,7 +1059,7 @@ __global__ __launch_bounds__(kThreads) void k_feat_join(StreamArgs a, int shares
     const int at = threadIdx.x / kLanes, row = at % kRows, z = at / kRows;
     const int64_t i = (int64_t)blockIdx.x * kRows + row;
     const int c = threadIdx.x % kLanes * 4;
-    float m = -1e30f, sum = 0.0f;
+    float m = kLowest, sum = 0.0f;
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
     auto add = [&](float m2, float s2, f32x4 v2) {
         const float mm = fmaxf(m, m2), base = mm < INFINITY ? mm : 0.0f;
@@ -1434,7 +1446,7 @@ __global__ __launch_bounds__(kThreads) void k_loss_few(LossArgs a, int lpr, floa
     float m[kFew], sum[kFew];
 #pragma unroll
     for (int q = 0; q < kFew; ++q) {
-        m[q] = -1e30f;
+        m[q] = kLowest;
         sum[q] = 0.0f;
     }
     for (int64_t v = (int64_t)blockIdx.x * slots + slot; v < a.rows;

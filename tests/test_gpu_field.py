@@ -466,6 +466,103 @@ def test_label_loss_in_several_pieces(ops):
         assert ((got.cuda() - ref).abs() <= 1.05 * BF * (size + ref.abs()) + 1e-30).all()
 
 
+# ------------------------------------------------------------------ larger sizes
+@pytest.mark.parametrize("n,rows,dim,hot", [
+    (4000, 3000, 64, 0), (4000, 3000, 64, 0.9), (2_200_003, 5000, 3, 0.3), (700_001, 100, 8, 0.5),
+    (200_003, 40_000, 20, 0.7), (1025, 129, 130, 0)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_lookup_grad_of_long_lists(ops, n, rows, dim, hot, dtype):
+    test_lookup_grad(ops, n, rows, dim, hot, dtype)
+
+
+@pytest.mark.parametrize("bt,pixels,c,groups", [(20, (9, 11), 64, 8), (17, (70, 61), 48, 6),
+                                                (2, (131, 257), 12, 4), (33, (5,), 7, 7)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_group_norm_of_batches(ops, bt, pixels, c, groups, dtype):
+    test_group_norm(ops, bt, pixels, c, groups, dtype, "silu")
+
+
+@pytest.mark.parametrize("n,rows,dim", [
+    (5000, 3000, 16), (20_000, 600, 45), (600, 20_000, 128), (4099, 2500, 48), (3001, 4097, 64),
+    (2000, 2500, 129), (1500, 1601, 260), (9, 30_000, 8), (30_000, 3, 60)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_label_loss_of_many(ops, n, rows, dim, dtype):
+    test_label_loss(ops, n, rows, dim, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_label_loss_of_long_rows_in_several_pieces(ops, dtype):
+    """More samples and more table rows than one piece of score gradients holds."""
+    dim, scale = 130, 8.0
+    host = _loss_case(9000, 17_000, dim, dtype, 13)
+    feat, table, labels, weight = (t.cuda() for t in host)
+    got = ops.label_loss_grad(feat, table, labels, weight, scale=scale)
+    loss, _, dfeat, dtable = (t.to(D64) for t in got)
+    f, t, on = feat.to(D64), table.to(D64), labels >= 0
+    at = labels.clamp(min=0)[:, None]
+    s = scale * f @ t.T
+    lse = torch.logsumexp(s, 1)
+    e = ((dim + 8) * EPS * scale * (f.abs() @ t.abs().T) + 4 * EPS * s.abs()).amax(1)
+    e = 2 * (e + 16 * EPS * (1 + lse.abs() + s.abs().amax(1)))
+    want = torch.where(on, lse - s.gather(1, at)[:, 0], torch.zeros_like(lse))
+    assert ((loss - want).abs() <= e).all()
+    p = torch.exp(s - lse[:, None])
+    del s
+    w = torch.where(on, weight.to(D64) * scale, torch.zeros_like(lse))[:, None]
+    g = p.scatter_add(1, at, torch.full_like(lse, -1.0)[:, None]) * w
+    eg = p.scatter_add(1, at, torch.ones_like(lse)[:, None])  # p + one
+    eg = w * (2 * p * e[:, None] + 4 * EPS * eg) + (BF if dtype == BF16 else 2.0 ** -22) * g.abs()
+    del p
+    out = BF if dtype == BF16 else 0.0
+    for got, a, b, ea in ((dfeat, g, t, eg), (dtable, g.T, f, eg.T)):
+        ref = a @ b
+        tol = (ea + (a.shape[1] + 8) * EPS * a.abs()) @ b.abs() + out * ref.abs() + 1e-38
+        assert ((got - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("n,dim", [(3, 16), (100, 16), (100, 200)])
+def test_label_loss_of_lowest_scores(ops, n, dim):
+    """All scores near the lowest values that fp32 holds: finite, and the table's
+    rows equal."""
+    feat, table = torch.full((n, dim), -1e18).cuda(), torch.full((50, dim), 1e18).cuda()
+    labels = torch.arange(n).cuda() % 50
+    loss, lse = ops.label_loss(feat, table, labels)
+    want = -float(np.float32(1e18)) ** 2 * dim
+    assert ((lse.double() - want).abs() <= (dim + 24) * EPS * abs(want)).all()
+    assert (loss.abs() <= (dim + 24) * 2 * EPS * abs(want)).all()
+
+
+def test_offsets_past_32_bits(ops):
+    """Rows 2^20 elements apart, and a table of more than 2^32 elements."""
+    far = 1 << 20
+    room = torch.empty(3000 * far, dtype=BF16, device="cuda")
+    view = room.as_strided((3000, 32), (far, 1))
+    feat, table, labels, weight = _loss_case(3000, 40, 32, BF16, 14)
+    view.copy_(feat)
+    a = (table.cuda(), labels.cuda(), weight.cuda())
+    near = ops.label_loss_grad(feat.cuda(), *a, scale=3.0)
+    assert all(torch.equal(p, q) for p, q in zip(near, ops.label_loss_grad(view, *a, scale=3.0)))
+    ids = _ids(_gen(15), 2000, 3000).cuda()
+    assert torch.equal(ops.lookup(view, ids), ops.lookup(feat.cuda(), ids))
+    assert torch.equal(ops.lookup_grad(view, a[1], 40), ops.lookup_grad(feat.cuda(), a[1], 40))
+    x = room.as_strided((1, 3000, 32), (3000 * far, far, 1))
+    one, two = ops.group_norm(x, 4, act="silu"), ops.group_norm(feat.cuda()[None], 4, act="silu")
+    assert all(torch.equal(p, q) for p, q in zip(one, two))
+    del room, view, x
+    rows = (1 << 26) + 3  # of 64
+    big = torch.empty(rows, 64, dtype=BF16, device="cuda")
+    big[-3000:] = 1.0
+    big[-3000:, :32] = feat.cuda()
+    at = torch.where(ids < 0, ids, ids + rows - 3000)
+    assert torch.equal(ops.lookup(big, at)[:, :32], ops.lookup(feat.cuda(), ids))
+    del big
+    d = _randn(_gen(16), 2000, 64).cuda()
+    out = ops.lookup_grad(d, at, rows)
+    want, tol = _grad_ref(d.cpu(), ids.cpu(), 3000, 1.0)
+    _close(out[-3000:], want, tol, "dtable")
+    assert not out[:-3000].any()
+
+
 @pytest.mark.parametrize("which", ["feat", "table"])
 def test_label_loss_grad_matches_differences(ops, which):
     feat, table, labels, weight = _loss_case(40, 30, 8, F32, 13)
