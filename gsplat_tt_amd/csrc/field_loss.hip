@@ -177,24 +177,25 @@ struct Side {
     __device__ __forceinline__ static uint32_t place(uint32_t row) {
         return PAIRS ? (row & 3) | ((row >> 1) & 4) : row & 7;
     }
-    quad r[4];
-    uint32_t from, to;  // the lane's byte offset in memory, its first quad in LDS
+    uint32_t from;  // the lane's byte offset in memory
     int64_t ld;
     __device__ __forceinline__ explicit Side(const Mat& m) : ld(m.ld) {
-        const uint32_t t = threadIdx.x, row = K ? t >> 3 : t >> 4, c = K ? t & 7 : t & 15;
+        const uint32_t t = threadIdx.x, row = K ? t >> 3 : t >> 4;
+        const uint32_t c = K ? (t & 7) ^ place(row) : (t & 15) ^ ((row & 7) << 1);
         from = (row * (uint32_t)m.ld + c * 8) * 2;
-        to = K ? row * 8 + (c ^ place(row)) : row * 16 + (c ^ ((row & 7) << 1));
     }
-    __device__ __forceinline__ void fetch(const Mat& m, int part, int64_t row0, int64_t k) {
+    // Straight into LDS: a wave's 64 quads lie there in lane order.
+    __device__ __forceinline__ void fetch(const Mat& m, int part, int64_t row0, int64_t k,
+                                          quad* lds) const {
+        typedef const __attribute__((address_space(1))) void* from_t;
+        typedef __attribute__((address_space(3))) void* to_t;
         const char* p = reinterpret_cast<const char*>(m.p + part * m.plane +
                                                       (K ? row0 * ld + k : k * ld + row0));
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            r[j] = *reinterpret_cast<const quad*>(p + (int64_t)j * (K ? 64 : 32) * ld + from);
-    }
-    __device__ __forceinline__ void keep(quad* lds) const {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) lds[to + j * 256] = r[j];
+            __builtin_amdgcn_global_load_lds(
+                (from_t)(p + (int64_t)j * (K ? 64 : 32) * ld + from),
+                (to_t)(lds + j * 256 + wave_id() * 64), 16, 0, 0);
     }
     // the operand of rows b + 16 i .. + 15 (b 0 or 64, the same in the wave), summed
     // index 32 h .. 32 h + 31
@@ -224,13 +225,21 @@ struct Side {
 
 // Tiles of A B^T one after the other for one workgroup: 4 waves of 64 x 64, 64 of
 // the summed index a step, the next step's operands on their way from memory
-// while this one's are multiplied, also across tiles. `rows(tile)` gives the
-// tile's first rows of A and B; `done(tile, acc)` takes its 128 x 128 sums. LDS
-// holds one step: the other workgroup of the compute unit fills the waits.
-#define GS_TILE_LDS __shared__ quad lds[2][kTile * 8]
+// straight into the other half of LDS while this one's are multiplied, also across
+// tiles. `rows(tile)` gives the tile's first rows of A and B; `done(tile, acc)`
+// takes its 128 x 128 sums. All of a step's operands are read from LDS before the
+// next loads are started: the compiler cannot tell the halves apart, and would have
+// a read after them wait for all of them.
+//
+// Bound by LDS: 64 KB read and 32 written a step at 128 bytes a cycle are 768 cycles,
+// the 128 products of a unit's 4 matrix cores 512; two workgroups share a compute
+// unit. Through registers a step took 5 to 10 % longer. Tiles of 256 x 128 in steps
+// of 32 move a quarter less, but G's epilogue spilled: 30011 x 32003 of 512 bf16 5.45
+// against 5.20 ms, though sums alone gained a seventh.
+#define GS_TILE_LDS __shared__ quad lds[4 * kTile * 8]
 template <int NP, bool AK, bool BK, bool PAIRS = false, class Rows, class Done>
 __device__ __forceinline__ void tile_products(const Mat& A, const Mat& B, int64_t k0, int64_t k1,
-                                              int tiles, quad (*lds)[kTile * 8], Rows rows,
+                                              int tiles, quad* lds, Rows rows,
                                               Done done) {
     const int w = wave_id(), wm = (w >> 1) * 64, wn = (w & 1) * 64;
     const int steps_k = (int)((k1 - k0) / kStep), per_tile = steps_k * Products<NP>::kCount;
@@ -238,11 +247,11 @@ __device__ __forceinline__ void tile_products(const Mat& A, const Mat& B, int64_
     SideA a(A);
     Side<BK> b(B);
     int tile_f = 0, q_f = 0, k_f = 0;  // the next step to fetch
-    auto fetch = [&] {
+    auto fetch = [&](quad* to) {
         const auto at = rows(tile_f);
         const int64_t k = k0 + (int64_t)k_f * kStep;
-        a.fetch(A, Products<NP>::a(q_f), at.m, k);
-        b.fetch(B, Products<NP>::b(q_f), at.n, k);
+        a.fetch(A, Products<NP>::a(q_f), at.m, k, to);
+        b.fetch(B, Products<NP>::b(q_f), at.n, k, to + kTile * 8);
         if (++k_f == steps_k) {
             k_f = 0;
             if (++q_f == Products<NP>::kCount) {
@@ -260,14 +269,22 @@ __device__ __forceinline__ void tile_products(const Mat& A, const Mat& B, int64_
     };
     clear();
     const int steps = per_tile * tiles;
-    if (steps > 0) fetch();
+    if (steps > 0) fetch(lds);
     int left = per_tile, tile = 0;
     for (int s = 0; s < steps; ++s) {
+        const quad* la = lds + (s & 1) * (2 * kTile * 8);
+        const quad* lb = la + kTile * 8;
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's part has arrived
         __syncthreads();
-        a.keep(lds[0]);
-        b.keep(lds[1]);
-        __syncthreads();
-        if (s + 1 < steps) fetch();
+        bf16x8 fa[2][4], fb[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                fa[h][i] = SideA::operand(la, wm, i, h);
+                fb[h][i] = Side<BK>::operand(lb, wn, i, h);
+            }
+        if (s + 1 < steps) fetch(lds + ((s + 1) & 1) * (2 * kTile * 8));
         if (left == 0) {  // here the tile's stores have a step's time until loads wait for them
             done(tile++, acc);
             clear();
@@ -275,26 +292,43 @@ __device__ __forceinline__ void tile_products(const Mat& A, const Mat& B, int64_
         }
         --left;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            bf16x8 fa[4], fb[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                fa[i] = SideA::operand(lds[0], wm, i, h);
-                fb[i] = Side<BK>::operand(lds[1], wn, i, h);
-            }
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], fb[j], acc[i][j], 0,
-                                                                        0, 0);
-        }
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[h][i], fb[h][j],
+                                                                        acc[i][j], 0, 0, 0);
     }
     done(tile, acc);
 }
 
 struct TileRows {
     int64_t m, n;
+};
+
+// Work (x, y) of a workgroup, x < nx and, if it has any, y < ny: every eighth
+// workgroup runs on the same XCD, and there `gy` values of y follow each other with
+// one x, so that its L2 serves what belongs to x to all of them, and the y's parts
+// to the x's that run beside. With x first in plain order, samples came from beyond
+// the L2 for every tile of scores and G once per 128 columns of the sums: 30011 x
+// 32003 of 512 bf16 took 5.23 ms, so 4.87.
+struct Spot {
+    int x, y;
+};
+__device__ __forceinline__ Spot spot(int nx, int gy) {
+    const int k = blockIdx.x >> 3, e = k / gy * 8 + (blockIdx.x & 7);
+    return {e % nx, e / nx * gy + k % gy};
+}
+constexpr int kSpot = 8;  // y's of the scores and of G: 4 took 5.00 ms of the above
+struct SpotGrid {
+    int gy;
+    unsigned blocks;
+    SpotGrid(int64_t nx, int64_t ny, int64_t most) {
+        const int64_t groups = (ny + most - 1) / most;
+        gy = (int)((ny + groups - 1) / groups);
+        blocks = (unsigned)((nx * groups + 7) / 8 * 8 * gy);
+    }
 };
 
 // Largest score and sum of exp2(score - largest) of two sets of scores, into the
@@ -314,12 +348,15 @@ template <int NP>
 __global__ __launch_bounds__(kThreads, 2) void k_loss_scores(Mat F, Mat T, int kd, int64_t rows,
                                                           float scale2, const int32_t* label,
                                                           int64_t padded, int tiles, int share,
-                                                          float2* part, float* label_score) {
+                                                          int gy, float2* part,
+                                                          float* label_score) {
     GS_TILE_LDS;
     const int lane = threadIdx.x & 63, w = wave_id();
     const int wm = (w >> 1) * 64, wn = (w & 1) * 64;
-    const int64_t n0 = (int64_t)blockIdx.x * kTile;
-    const int t0 = blockIdx.y * share, t1 = min(tiles, t0 + share);
+    const Spot at = spot((int)(padded / kTile), gy);
+    const int64_t n0 = (int64_t)at.x * kTile;
+    const int t0 = at.y * share, t1 = min(tiles, t0 + share);
+    if (t0 >= tiles) return;
     float m[4], sum[4];
     int32_t y[4];
 #pragma unroll
@@ -378,7 +415,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_loss_scores(Mat F, Mat T, int k
             join_sums(m[n], sum[n], m2, s2);
         }
         if (lane < 16)
-            part[((int64_t)blockIdx.y * 2 + (w >> 1)) * padded + n0 + wn + n * 16 + lane] =
+            part[((int64_t)at.y * 2 + (w >> 1)) * padded + n0 + wn + n * 16 + lane] =
                 make_float2(m[n], sum[n]);
     }
 }
@@ -431,12 +468,14 @@ __global__ __launch_bounds__(kThreads, 2) void k_loss_g(Mat F, Mat T, int kd, in
                                                      float scale2, const int32_t* label,
                                                      const float* weight, const float* lse2,
                                                      int64_t r0, int64_t v0, int64_t rc, int64_t vc,
-                                                     int share, bf16* G) {
+                                                     int share, int gy, bf16* G) {
     GS_TILE_LDS;
     const int lane = threadIdx.x & 63, w = wave_id();
     const int wm = (w >> 1) * 64, wn = (w & 1) * 64;
-    const int64_t n0 = (int64_t)blockIdx.x * kTile;
-    const int t0 = blockIdx.y * share, t1 = min((int)(vc / kTile), t0 + share);
+    const Spot place = spot((int)(rc / kTile), gy);
+    const int64_t n0 = (int64_t)place.x * kTile;
+    const int t0 = place.y * share, t1 = min((int)(vc / kTile), t0 + share);
+    if (t0 >= t1) return;
     int32_t y[4];
     float wt[4], l2[4];
 #pragma unroll
@@ -523,16 +562,20 @@ struct SumOut {
 // registers the 64 addresses of a lane spilled.
 template <typename T, int NP, bool AK>
 __global__ __launch_bounds__(kThreads, 2) void k_loss_sum(Mat A, Mat B, int64_t k, int64_t share,
-                                                          SumOut<T> o) {
+                                                          int nz, SumOut<T> o) {
     constexpr int kRow = 68;  // floats of a row of 64, so that rows 4 apart use other banks
-    __shared__ quad buf[kTile * kRow / 4];
-    static_assert(kTile * kRow / 4 >= 2 * kTile * 8, "the operands' tiles fit");
-    const int64_t m0 = (int64_t)blockIdx.x * kTile, n0 = (int64_t)blockIdx.y * kTile;
-    const int64_t k0 = min(k, share * blockIdx.z), k1 = min(k, k0 + share);
+    __shared__ quad buf[4 * kTile * 8];
+    static_assert(kTile * kRow / 4 <= 4 * kTile * 8, "half of the sums fits");
+    const int nm = (int)(o.m / kTile);
+    const Spot at = spot(nm * nz, o.dq / kTile);
+    const int z = at.x / nm;
+    if (at.y >= o.dq / kTile) return;
+    const int64_t m0 = (int64_t)(at.x % nm) * kTile, n0 = (int64_t)at.y * kTile;
+    const int64_t k0 = min(k, share * z), k1 = min(k, k0 + share);
     const int lane = threadIdx.x & 63, w = wave_id();
     const int wm = (w >> 1) * 64, wn = (w & 1) * 64;
     tile_products<NP, AK, false>(
-        A, B, k0, k1, 1, reinterpret_cast<quad(*)[kTile * 8]>(buf),
+        A, B, k0, k1, 1, buf,
         [&](int) { return TileRows{m0, n0}; },
         [&](int, f32x4(&acc)[4][4]) {
             float* f = reinterpret_cast<float*>(buf);
@@ -556,9 +599,9 @@ __global__ __launch_bounds__(kThreads, 2) void k_loss_sum(Mat A, Mat B, int64_t 
                     const f32x4 v = *reinterpret_cast<const f32x4*>(f + r * kRow + c);
                     const int64_t row = m0 + r;
                     const int column = (int)n0 + half * 64 + c;
-                    if (gridDim.z > 1)
+                    if (nz > 1)
                         *reinterpret_cast<f32x4*>(
-                            o.slices + ((int64_t)blockIdx.z * o.m + row) * o.dq + column) = v;
+                            o.slices + ((int64_t)z * o.m + row) * o.dq + column) = v;
                     else
                         o.put(row, column, v);
                 }
@@ -1125,9 +1168,13 @@ hipError_t feat_join(const StreamArgs& a, int shares, hipStream_t st) {
 // ---------------------------------------------------------------- pieces
 int64_t pad_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
-// Pieces of G: up to 8192 table rows by as many samples as make 2^27 values (256 MB
-// of bf16, what the cache behind the L2s holds), a third of that in three parts;
-// more table rows where there are few samples.
+// Pieces of G: up to 16384 table rows by as many samples as make 1 GB of bf16 parts,
+// more table rows where there are few samples; all pieces of one size, so that
+// none leaves the chip half empty. Of 256 MB, which the cache behind the L2s holds,
+// the pieces were too many: 30011 x 32003 of 512 bf16 4.81 against 4.64 ms, 20000 x
+// 50257 of 384 4.43 against 4.02 (512 MB: 4.75, 4.06).
+constexpr int64_t kPieceValues = (int64_t)1 << 29;
+constexpr int kAtOnce = 512;  // workgroups that the chip holds
 struct LossPlan {
     int np, kd, dq;
     int64_t np_rows, vp, rc, vc;
@@ -1140,11 +1187,28 @@ struct LossPlan {
     int32_t* label;
     size_t bytes;
 
+    // Shares of the summed index for `tiles` tiles of sums: the fewest that leave at
+    // most a tenth of the chip's rounds of workgroups empty, or come nearest. 576
+    // tiles in one share took 1020 us, 448 of the same length 554.
     static void split_k(int64_t tiles, int64_t k, int* z, int64_t* share) {
-        int64_t want = tiles >= 384 ? 1 : (512 + tiles - 1) / tiles;
-        want = std::min<int64_t>(want, std::max<int64_t>(1, k / 512));
-        *share = pad_to((k + want - 1) / want, kStep);
-        *z = (int)((k + *share - 1) / *share);
+        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(16, k / 512));
+        int64_t best = 1;
+        double best_full = 0.0;
+        for (int64_t want = 1; want <= most && best_full < 0.9; ++want) {
+            const int64_t all = tiles * want;
+            const double full = (double)all / (double)((all + kAtOnce - 1) / kAtOnce * kAtOnce);
+            if (full > best_full + 1e-9) {
+                best = want;
+                best_full = full;
+            }
+        }
+        *share = pad_to((k + best - 1) / best, kStep);
+        *z = *share == 0 ? 1 : (int)((k + *share - 1) / *share);
+    }
+    // `all` in equal pieces of at most `most`
+    static int64_t piece(int64_t all, int64_t most) {
+        const int64_t pieces = std::max<int64_t>(1, (all + most - 1) / most);
+        return pad_to((all + pieces - 1) / pieces, kTile);
     }
     LossPlan(void* base, int64_t n, int64_t rows, int dim, int dtype, bool grad) {
         np = dtype == 0 ? 3 : 1;
@@ -1152,10 +1216,10 @@ struct LossPlan {
         dq = (int)pad_to(dim, kTile);
         np_rows = pad_to(n, kTile);
         vp = pad_to(rows, kTile);
-        vc = std::min<int64_t>(vp, 8192);
-        const int64_t area = (1 << 27) / np;
-        rc = std::min<int64_t>(np_rows, std::max<int64_t>(kTile, area / vc / kTile * kTile));
-        vc = std::min<int64_t>(vp, std::max<int64_t>(vc, area / std::max<int64_t>(rc, 1) / kTile * kTile));
+        const int64_t area = kPieceValues / np;
+        vc = piece(vp, 16384);
+        rc = piece(np_rows, std::max<int64_t>(kTile, area / std::max(vc, (int64_t)kTile)));
+        vc = piece(vp, std::max(vc, area / std::max(rc, (int64_t)kTile)));
         split_k(rc / kTile * (dq / kTile), vc, &zf, &share_f);
         split_k(vc / kTile * (dq / kTile), rc, &zt, &share_t);
         // scores: about 4096 workgroups, where that leaves 8 tiles each
@@ -1199,8 +1263,10 @@ hipError_t loss_run(const LossArgs& a, bool grad, hipStream_t st) {
     k_parts<T, NP><<<blocks_for(w.vp * w.dq / 8), kThreads, 0, st>>>(
         table, a.rows, a.table_stride, a.dim, nullptr, w.vp, w.dq, reinterpret_cast<quad*>(w.T));
     const Mat F{w.F, w.dq, nr * w.dq}, Tm{w.T, w.dq, w.vp * w.dq};
-    k_loss_scores<NP><<<dim3((unsigned)(nr / kTile), (unsigned)w.shares), kThreads, 0, st>>>(
-        F, Tm, w.kd, a.rows, scale2, w.label, nr, (int)(w.vp / kTile), w.share, w.part, w.score);
+    const SpotGrid gs(nr / kTile, w.shares, kSpot);
+    k_loss_scores<NP><<<gs.blocks, kThreads, 0, st>>>(F, Tm, w.kd, a.rows, scale2, w.label, nr,
+                                                      (int)(w.vp / kTile), w.share, gs.gy, w.part,
+                                                      w.score);
     k_loss_join<<<(unsigned)((nr + 31) / 32), kThreads, 0, st>>>(a, w.part, w.shares * 2, nr,
                                                                  w.score, w.lse2);
     hipError_t e = hipGetLastError();
@@ -1212,17 +1278,18 @@ hipError_t loss_run(const LossArgs& a, bool grad, hipStream_t st) {
             // 8 tiles a workgroup where that leaves two workgroups a compute unit
             const int share = (int)std::max<int64_t>(
                 1, std::min<int64_t>(8, rc / kTile * (vc / kTile) / 512));
-            k_loss_g<NP><<<dim3((unsigned)(rc / kTile), (unsigned)((vc / kTile + share - 1) / share)),
-                           kThreads, 0, st>>>(F, Tm, w.kd, a.rows, scale2, w.label, w.weight, w.lse2,
-                                              r0, v0, rc, vc, share, w.G);
+            const SpotGrid gg(rc / kTile, (vc / kTile + share - 1) / share, kSpot);
+            k_loss_g<NP><<<gg.blocks, kThreads, 0, st>>>(F, Tm, w.kd, a.rows, scale2, w.label,
+                                                         w.weight, w.lse2, r0, v0, rc, vc, share,
+                                                         gg.gy, w.G);
             const Mat G{w.G, vc, rc * vc};
             const int zf = (int)((vc + w.share_f - 1) / w.share_f);
             const SumOut<T> of{w.slices, w.sum_f, v0 == 0, v0 + vc >= w.vp, rc, w.dq,
                                static_cast<T*>(a.dfeat) + r0 * a.dfeat_stride, a.n - r0,
                                a.dfeat_stride, a.dim, w.label + r0};
             k_loss_sum<T, NP, true>
-                <<<dim3((unsigned)(rc / kTile), (unsigned)(w.dq / kTile), zf), kThreads, 0, st>>>(
-                    G, {w.T + v0 * w.dq, w.dq, w.vp * w.dq}, vc, w.share_f, of);
+                <<<SpotGrid(rc / kTile * zf, w.dq / kTile, w.dq).blocks, kThreads, 0, st>>>(
+                    G, {w.T + v0 * w.dq, w.dq, w.vp * w.dq}, vc, w.share_f, zf, of);
             if (zf > 1 && (e = fold(of, zf, st)) != hipSuccess) return e;
             const int zt = (int)((rc + w.share_t - 1) / w.share_t);
             const SumOut<T> ot{w.slices, w.sum_t + (w.sum_t != nullptr ? v0 * w.dq : 0), r0 == 0,
@@ -1230,8 +1297,8 @@ hipError_t loss_run(const LossArgs& a, bool grad, hipStream_t st) {
                                static_cast<T*>(a.dtable) + v0 * a.dtable_stride, a.rows - v0,
                                a.dtable_stride, a.dim, nullptr};
             k_loss_sum<T, NP, false>
-                <<<dim3((unsigned)(vc / kTile), (unsigned)(w.dq / kTile), zt), kThreads, 0, st>>>(
-                    G, {w.F + r0 * w.dq, w.dq, nr * w.dq}, rc, w.share_t, ot);
+                <<<SpotGrid(vc / kTile * zt, w.dq / kTile, w.dq).blocks, kThreads, 0, st>>>(
+                    G, {w.F + r0 * w.dq, w.dq, nr * w.dq}, rc, w.share_t, zt, ot);
             if (zt > 1 && (e = fold(ot, zt, st)) != hipSuccess) return e;
         }
     }

@@ -490,34 +490,36 @@ def test_label_loss_of_many(ops, n, rows, dim, dtype):
     test_label_loss(ops, n, rows, dim, dtype)
 
 
-@pytest.mark.parametrize("dtype", [F32, BF16])
-def test_label_loss_of_long_rows_in_several_pieces(ops, dtype):
+@pytest.mark.parametrize("n,dtype", [(9000, F32), (9000, BF16), (25_000, F32), (70_000, BF16)])
+def test_label_loss_of_long_rows_in_several_pieces(ops, n, dtype):
     """More samples and more table rows than one piece of score gradients holds."""
-    dim, scale = 130, 8.0
-    host = _loss_case(9000, 17_000, dim, dtype, 13)
+    dim, scale, rows = 130, 8.0, 17_000
+    host = _loss_case(n, rows, dim, dtype, 13)
     feat, table, labels, weight = (t.cuda() for t in host)
     got = ops.label_loss_grad(feat, table, labels, weight, scale=scale)
     loss, _, dfeat, dtable = (t.to(D64) for t in got)
-    f, t, on = feat.to(D64), table.to(D64), labels >= 0
-    at = labels.clamp(min=0)[:, None]
-    s = scale * f @ t.T
-    lse = torch.logsumexp(s, 1)
-    e = ((dim + 8) * EPS * scale * (f.abs() @ t.abs().T) + 4 * EPS * s.abs()).amax(1)
-    e = 2 * (e + 16 * EPS * (1 + lse.abs() + s.abs().amax(1)))
-    want = torch.where(on, lse - s.gather(1, at)[:, 0], torch.zeros_like(lse))
-    assert ((loss - want).abs() <= e).all()
-    p = torch.exp(s - lse[:, None])
-    del s
-    w = torch.where(on, weight.to(D64) * scale, torch.zeros_like(lse))[:, None]
-    g = p.scatter_add(1, at, torch.full_like(lse, -1.0)[:, None]) * w
-    eg = p.scatter_add(1, at, torch.ones_like(lse)[:, None])  # p + one
-    eg = w * (2 * p * e[:, None] + 4 * EPS * eg) + (BF if dtype == BF16 else 2.0 ** -22) * g.abs()
-    del p
-    out = BF if dtype == BF16 else 0.0
-    for got, a, b, ea in ((dfeat, g, t, eg), (dtable, g.T, f, eg.T)):
-        ref = a @ b
-        tol = (ea + (a.shape[1] + 8) * EPS * a.abs()) @ b.abs() + out * ref.abs() + 1e-38
-        assert ((got - ref).abs() <= tol).all()
+    t, out, part = table.to(D64), BF if dtype == BF16 else 0.0, BF if dtype == BF16 else 2.0 ** -22
+    want_t, tol_t = torch.zeros_like(t), torch.zeros_like(t)
+    for i in range(0, n, 5000):
+        at = slice(i, i + 5000)
+        f, on, y = feat[at].to(D64), labels[at] >= 0, labels[at].clamp(min=0)[:, None]
+        s = scale * f @ t.T
+        lse = torch.logsumexp(s, 1)
+        e = ((dim + 8) * EPS * scale * (f.abs() @ t.abs().T) + 4 * EPS * s.abs()).amax(1)
+        e = 2 * (e + 16 * EPS * (1 + lse.abs() + s.abs().amax(1)))
+        want = torch.where(on, lse - s.gather(1, y)[:, 0], torch.zeros_like(lse))
+        assert ((loss[at] - want).abs() <= e).all()
+        p = torch.exp(s - lse[:, None])
+        w = torch.where(on, weight[at].to(D64) * scale, torch.zeros_like(lse))[:, None]
+        g = p.scatter_add(1, y, torch.full_like(lse, -1.0)[:, None]) * w
+        eg = p.scatter_add(1, y, torch.ones_like(lse)[:, None])  # p + one
+        eg = w * (2 * p * e[:, None] + 4 * EPS * eg) + part * g.abs()
+        ref = g @ t
+        tol = (eg + (rows + 8) * EPS * g.abs()) @ t.abs() + out * ref.abs() + 1e-38
+        assert ((dfeat[at] - ref).abs() <= tol).all()
+        want_t += g.T @ f
+        tol_t += (eg + (n + 8) * EPS * g.abs()).T @ f.abs()
+    assert ((dtable - want_t).abs() <= tol_t + out * want_t.abs() + 1e-38).all()
 
 
 @pytest.mark.parametrize("n,dim", [(3, 16), (100, 16), (100, 200)])
