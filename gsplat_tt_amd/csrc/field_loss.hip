@@ -96,17 +96,6 @@ struct Products<3> {
 };
 
 // ---------------------------------------------------------------- layout
-// Labels as 32-bit (-1: masked) with their weights; rows past n are masked.
-__global__ __launch_bounds__(kThreads) void k_loss_rows(LossArgs a, int64_t padded, int32_t* label,
-                                                        float* weight) {
-    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (i >= padded) return;
-    const int32_t l = i < a.n ? load_id(a.labels, a.labels64, i, a.rows, a.flags) : -1;
-    label[i] = l;
-    if (weight != nullptr)
-        weight[i] = l < 0 ? 0.0f : a.scale * (a.row_weight != nullptr ? a.row_weight[i] : 1.0f);
-}
-
 // A row's 8 values from column c, cut into parts; zeros past the row.
 template <typename T, int NP>
 __device__ __forceinline__ void load_parts(const T* row, int dim, int c, bool on, quad* out) {
@@ -131,22 +120,42 @@ __device__ __forceinline__ void load_parts(const T* row, int dim, int c, bool on
     split8<NP>(v, out);
 }
 
-// Parts of (rows, dim) as (padded, ld), zeros in the padding and in masked rows.
+// Parts of the samples as (nr, ld) and of the table as (vp, ld), zeros in the padding
+// and in masked samples; labels as 32-bit (-1: masked), with their weights where the
+// gradients need them.
 template <typename T, int NP>
-__global__ __launch_bounds__(kThreads) void k_parts(const T* src, int64_t rows, int64_t stride,
-                                                    int dim, const int32_t* label, int64_t padded,
-                                                    int ld, quad* out) {
+__global__ __launch_bounds__(kThreads) void k_parts(LossArgs a, int64_t nr, int64_t vp, int ld,
+                                                    int32_t* label, float* weight, quad* F,
+                                                    quad* table) {
     const int units = ld / 8;
-    const int64_t total = padded * units;
+    const int64_t samples = nr * units, total = samples + vp * units;
     for (int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x; e < total;
          e += (int64_t)gridDim.x * kThreads) {
-        const int64_t r = e / units;
-        const int c = (int)(e - r * units) * 8;
+        const bool of_table = e >= samples;
+        const int64_t u = of_table ? e - samples : e, r = u / units;
+        const int c = (int)(u - r * units) * 8;
         quad part[NP];
-        load_parts<T, NP>(src + r * stride, dim, c,
-                          r < rows && (label == nullptr || label[r] >= 0), part);
+        if (of_table) {
+            load_parts<T, NP>(static_cast<const T*>(a.table) + r * a.table_stride, a.dim, c,
+                              r < a.rows, part);
+        } else {
+            const int32_t l = r < a.n ? load_id(a.labels, a.labels64, r, a.rows,
+                                                c == 0 ? a.flags : nullptr)
+                                      : -1;
+            if (c == 0) {
+                label[r] = l;
+                if (weight != nullptr)
+                    weight[r] =
+                        l < 0 ? 0.0f
+                              : a.scale * (a.row_weight != nullptr ? a.row_weight[r] : 1.0f);
+            }
+            load_parts<T, NP>(static_cast<const T*>(a.feat) + r * a.feat_stride, a.dim, c, l >= 0,
+                              part);
+        }
+        quad* out = of_table ? table : F;
+        const int64_t plane = of_table ? total - samples : samples;
 #pragma unroll
-        for (int p = 0; p < NP; ++p) out[p * total + e] = part[p];
+        for (int p = 0; p < NP; ++p) out[p * plane + u] = part[p];
     }
 }
 
@@ -1220,10 +1229,13 @@ struct LossPlan {
     size_t bytes;
 
     // Shares of the summed index for `tiles` tiles of sums: the fewest that leave at
-    // most a tenth of the chip's rounds of workgroups empty, or come nearest. 576
-    // tiles in one share took 1020 us, 448 of the same length 554.
-    static void split_k(int64_t tiles, int64_t k, int* z, int64_t* share) {
-        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(16, k / 512));
+    // most a tenth of the chip's rounds of workgroups empty, or come nearest (576
+    // tiles in one share took 1020 us, 448 of the same length 554), and are worth the
+    // slices: 4 steps, in three parts 12. With shares of 512 at least, and 16 at
+    // most, 45 samples by 12078 rows of 512 fp32 took 180 us, so 137; with 128 in one
+    // part 1000 x 1200 of 512 bf16 69 us, so 60.
+    void split_k(int64_t tiles, int64_t k, int* z, int64_t* share) const {
+        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(64, k / (np == 1 ? 256 : 128)));
         int64_t best = 1;
         double best_full = 0.0;
         for (int64_t want = 1; want <= most && best_full < 0.9; ++want) {
@@ -1285,15 +1297,10 @@ template <typename T, int NP>
 hipError_t loss_run(const LossArgs& a, bool grad, hipStream_t st) {
     const LossPlan w(a.ws, a.n, a.rows, a.dim, a.dtype, grad);
     const int64_t nr = w.np_rows;
-    const T* feat = static_cast<const T*>(a.feat);
-    const T* table = static_cast<const T*>(a.table);
     const float scale2 = a.scale * kLog2e;
-    k_loss_rows<<<(unsigned)((nr + kThreads - 1) / kThreads), kThreads, 0, st>>>(a, nr, w.label,
-                                                                                 w.weight);
-    k_parts<T, NP><<<blocks_for(nr * w.dq / 8), kThreads, 0, st>>>(
-        feat, a.n, a.feat_stride, a.dim, w.label, nr, w.dq, reinterpret_cast<quad*>(w.F));
-    k_parts<T, NP><<<blocks_for(w.vp * w.dq / 8), kThreads, 0, st>>>(
-        table, a.rows, a.table_stride, a.dim, nullptr, w.vp, w.dq, reinterpret_cast<quad*>(w.T));
+    k_parts<T, NP><<<blocks_for((nr + w.vp) * w.dq / 8), kThreads, 0, st>>>(
+        a, nr, w.vp, w.dq, w.label, w.weight, reinterpret_cast<quad*>(w.F),
+        reinterpret_cast<quad*>(w.T));
     const Mat F{w.F, w.dq, nr * w.dq}, Tm{w.T, w.dq, w.vp * w.dq};
     const SpotGrid gs(nr / kTile, w.shares, kSpot);
     k_loss_scores<NP><<<gs.blocks, kThreads, 0, st>>>(F, Tm, w.kd, a.rows, scale2, w.label, nr,
