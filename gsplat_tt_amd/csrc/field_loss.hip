@@ -720,7 +720,11 @@ hipError_t fold(const SumOut<T>& o, int nz, hipStream_t st) {
 // its factor in fp32, so that a label with almost all of its row's probability
 // costs no digits. kGradTable: the table's gradient, with the losses known.
 //
-// MEASURED
+// Bound by the matrix cores and, in fp32, as much by cutting the exponentials into
+// parts (88 of about 440 vector instructions a tile beside 42 products of 16 cycles).
+// 10007 x 8192 of 48 fp32: losses and dfeat 134 us, dtable 122, at 6 + 6 products of
+// each pair 0.78 PFLOP/s of bf16. 307200 x 150 of 32 bf16, losses alone: 18 us, where
+// the 46 million exponentials take 8 at the transcendental rate and the bytes 5.
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 
 constexpr float kSlack = 8.0f;
@@ -1515,7 +1519,8 @@ hipError_t stream_run(const LossArgs& a, bool grad, hipStream_t st) {
 
 // Padded row length that the streaming kernels take, 0: none. Past 128 a wave's own
 // rows and sums leave it alone on its unit: 20000 x 8000 of 256 bf16 with gradients
-// took 1073 us so, in pieces 803; of 128 456 against 536 (fp32 854 against 1438).
+// took 1073 us so, in pieces 511. Of 128 with gradients 361 against 344, fp32 (20000
+// x 5000) 665 against 1019; losses alone (50000 x 20000) 319 against 390.
 int stream_ks(int dim) {
     for (int ks : {16, 32, 48, 64, 128})
         if (dim <= ks) return ks;
@@ -1524,75 +1529,101 @@ int stream_ks(int dim) {
 
 // ---------------------------------------------------------------- few samples
 // Losses of up to kFew samples, a picked pixel or a handful: the table is read once
-// and nothing is laid out. `lpr` lanes a table row take its dot products with all
-// samples, held in LDS in fp32; a workgroup's slots keep each sample's largest
-// score and sum, and k_loss_join adds the workgroups up. Bound by the table's bytes
-// (or, below about 1 MB, by the two launches).
+// and nothing is laid out. `lpr` lanes take kFewRows table rows at a time, whose dot
+// products with all samples, held in LDS in fp32, share one read of them; a
+// workgroup's slots keep each sample's largest score and sum, and k_loss_join adds
+// the workgroups up. Bound by the table's bytes (or, below about 1 MB, by the two
+// launches, 15 us with the call): 1 by 100000 of 512 fp32 50 us, 4.1 TB/s; a row at a
+// time 114. 8 by 100000 of 64 fp32 30 us, by streaming 34; one 19 and 37.
 constexpr int kFew = 8;
 constexpr int kFewValues = 12288;  // samples * dim in LDS: 48 KB
+constexpr int kFewRows = 4;
 
-template <typename T, int VEC>
+template <typename T, int VEC, int NQ>
 __global__ __launch_bounds__(kThreads) void k_loss_few(LossArgs a, int lpr, float scale2,
                                                        float2* part, float* label_score) {
     __shared__ float f[kFewValues];
-    __shared__ float2 lds[kThreads / 64][kFew];
+    __shared__ float2 lds[kThreads / 64][NQ];
     const int n = (int)a.n, dim = a.dim;
     const T* feat = static_cast<const T*>(a.feat);
     const T* table = static_cast<const T*>(a.table);
     for (int e = threadIdx.x; e < n * dim; e += kThreads)
         f[e] = to_float(feat[(int64_t)(e / dim) * a.feat_stride + e % dim]);
-    int32_t y[kFew];
+    int32_t y[NQ];
 #pragma unroll
-    for (int q = 0; q < kFew; ++q)
+    for (int q = 0; q < NQ; ++q)
         y[q] = q < n ? load_id(a.labels, a.labels64, q, a.rows,
                                blockIdx.x == 0 && threadIdx.x == 0 ? a.flags : nullptr)
                      : -1;
     __syncthreads();
     const int slots = kThreads / lpr, slot = threadIdx.x / lpr, lane = threadIdx.x % lpr;
-    float m[kFew], sum[kFew];
+    const int64_t step = (int64_t)gridDim.x * slots;
+    float m[NQ], sum[NQ];
 #pragma unroll
-    for (int q = 0; q < kFew; ++q) {
+    for (int q = 0; q < NQ; ++q) {
         m[q] = kLowest;
         sum[q] = 0.0f;
     }
-    for (int64_t v = (int64_t)blockIdx.x * slots + slot; v < a.rows;
-         v += (int64_t)gridDim.x * slots) {
-        const T* row = table + v * a.table_stride;
-        float dot[kFew];
+    for (int64_t v0 = (int64_t)blockIdx.x * slots + slot; v0 < a.rows; v0 += kFewRows * step) {
+        float dot[kFewRows][NQ];
 #pragma unroll
-        for (int q = 0; q < kFew; ++q) dot[q] = 0.0f;
+        for (int u = 0; u < kFewRows; ++u)
+#pragma unroll
+            for (int q = 0; q < NQ; ++q) dot[u][q] = 0.0f;
         for (int c = lane * VEC; c < dim; c += lpr * VEC) {
-            float t[VEC];
+            float t[kFewRows][VEC];
             const int w = min(VEC, dim - c);
-            if (w == VEC) {
-                load_any<VEC>(row + c, t);
-            } else {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) t[j] = j < w ? to_float(row[c + j]) : 0.0f;
+            for (int u = 0; u < kFewRows; ++u) {
+                // past the table: the first of the rows again, the products unused
+                const int64_t v = v0 + u * step < a.rows ? v0 + u * step : v0;
+                const T* row = table + v * a.table_stride + c;
+                if (w == VEC) {
+                    load_any<VEC>(row, t[u]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) t[u][j] = j < w ? to_float(row[j]) : 0.0f;
+                }
             }
 #pragma unroll
-            for (int q = 0; q < kFew; ++q)
-                if (q < n)
+            for (int q = 0; q < NQ; ++q) {
+                if (q >= n) break;
+                float x[VEC];
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j)
-                        if (j < w) dot[q] = fmaf(t[j], f[q * dim + c + j], dot[q]);
+                for (int j = 0; j < VEC; ++j) x[j] = j < w ? f[q * dim + c + j] : 0.0f;
+#pragma unroll
+                for (int u = 0; u < kFewRows; ++u)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) dot[u][q] = fmaf(t[u][j], x[j], dot[u][q]);
+            }
         }
+        for (int o = 1; o < lpr; o <<= 1)
 #pragma unroll
-        for (int q = 0; q < kFew; ++q) {
-            if (q >= n) continue;
-            for (int o = 1; o < lpr; o <<= 1) dot[q] += __shfl_xor(dot[q], o, 64);
-            const float s = dot[q] * scale2;
-            if (v == y[q] && lane == 0) label_score[q] = s;
-            const float mm = fmaxf(m[q], s), base = mm < INFINITY ? mm : 0.0f;
-            sum[q] = sum[q] * __builtin_amdgcn_exp2f((m[q] < INFINITY ? m[q] : 0.0f) - base) +
-                     __builtin_amdgcn_exp2f(s - base);
+            for (int u = 0; u < kFewRows; ++u)
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) dot[u][q] += __shfl_xor(dot[u][q], o, 64);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
+            if (q >= n) break;
+            float mm = m[q];
+#pragma unroll
+            for (int u = 0; u < kFewRows; ++u) {
+                const int64_t v = v0 + u * step;
+                dot[u][q] = v < a.rows ? dot[u][q] * scale2 : -INFINITY;
+                if (v == y[q] && lane == 0) label_score[q] = dot[u][q];
+                mm = fmaxf(mm, dot[u][q]);
+            }
+            const float base = mm < INFINITY ? mm : 0.0f;
+            sum[q] *= __builtin_amdgcn_exp2f((m[q] < INFINITY ? m[q] : 0.0f) - base);
+#pragma unroll
+            for (int u = 0; u < kFewRows; ++u) sum[q] += __builtin_amdgcn_exp2f(dot[u][q] - base);
             m[q] = mm;
         }
     }
     // over the slots: within the wave, then the waves (the lanes of a slot agree)
 #pragma unroll
-    for (int q = 0; q < kFew; ++q) {
-        if (q >= n) continue;
+    for (int q = 0; q < NQ; ++q) {
+        if (q >= n) break;
         for (int o = lpr; o < 64; o <<= 1) {
             const float m2 = __shfl_xor(m[q], o, 64), s2 = __shfl_xor(sum[q], o, 64);
             join_sums(m[q], sum[q], m2, s2);
@@ -1609,7 +1640,12 @@ __global__ __launch_bounds__(kThreads) void k_loss_few(LossArgs a, int lpr, floa
     }
 }
 
-bool is_few(int64_t n, int dim, bool grad) { return !grad && n <= kFew && n * dim <= kFewValues; }
+// Of several samples the dot products' sums over lanes weigh with long bf16 rows, and
+// their scores are left to the pieces: 2 by 100000 of 512 95 us so, 78 in pieces (8:
+// 135 and 78), one 54 and 78. In fp32 8 took 111 and 232.
+bool is_few(int64_t n, int dim, int dtype, bool grad) {
+    return !grad && n <= kFew && n * dim <= kFewValues && (n == 1 || dtype == 0 || dim <= 128);
+}
 
 struct FewPlan {
     int lpr, blocks;
@@ -1632,8 +1668,12 @@ struct FewPlan {
 template <typename T>
 hipError_t few_run(const LossArgs& a, hipStream_t st) {
     const FewPlan w(a.ws, a.n, a.rows, a.dim, a.dtype);
-    k_loss_few<T, 16 / sizeof(T)><<<w.blocks, kThreads, 0, st>>>(a, w.lpr, a.scale * kLog2e, w.part,
-                                                                 w.score);
+    constexpr int VEC = 16 / sizeof(T);
+    const float scale2 = a.scale * kLog2e;
+    if (a.n == 1)
+        k_loss_few<T, VEC, 1><<<w.blocks, kThreads, 0, st>>>(a, w.lpr, scale2, w.part, w.score);
+    else
+        k_loss_few<T, VEC, kFew><<<w.blocks, kThreads, 0, st>>>(a, w.lpr, scale2, w.part, w.score);
     k_loss_join<<<1, kThreads, 0, st>>>(a, w.part, w.blocks, a.n, w.score, nullptr);
     return hipGetLastError();
 }
@@ -1641,7 +1681,7 @@ hipError_t few_run(const LossArgs& a, hipStream_t st) {
 }  // namespace
 
 size_t label_loss_ws(int64_t n, int64_t rows, int dim, int dtype, bool grad) {
-    if (is_few(n, dim, grad)) return FewPlan(nullptr, n, rows, dim, dtype).bytes;
+    if (is_few(n, dim, dtype, grad)) return FewPlan(nullptr, n, rows, dim, dtype).bytes;
     const int ks = stream_ks(dim);
     if (ks != 0) return StreamPlan(nullptr, n, rows, dtype == 0 ? 3 : 1, ks, grad).bytes;
     return LossPlan(nullptr, n, rows, dim, dtype, grad).bytes;
@@ -1659,7 +1699,7 @@ hipError_t launch_label_loss(const LossArgs& a, bool grad, hipStream_t st) {
                                  a.rows, a.dtable_stride, a.dim, nullptr}, 0, st);
     }
     const bool f = a.dtype == 0;
-    if (is_few(a.n, a.dim, grad)) return f ? few_run<float>(a, st) : few_run<bf16>(a, st);
+    if (is_few(a.n, a.dim, a.dtype, grad)) return f ? few_run<float>(a, st) : few_run<bf16>(a, st);
     switch (stream_ks(a.dim)) {
         case 16: return f ? stream_run<float, 3, 16>(a, grad, st) : stream_run<bf16, 1, 16>(a, grad, st);
         case 32: return f ? stream_run<float, 3, 32>(a, grad, st) : stream_run<bf16, 1, 32>(a, grad, st);

@@ -425,8 +425,9 @@ int gs_train_loss(gs_ctx* ctx, const float* image, const float* target, int heig
  *   result is rounded once, to nearest even.
  * - strides are in elements, between rows (or images, pixels); the values of a
  *   row are contiguous. Inputs may overlap each other and themselves (a stride
- *   of 0 repeats a row); an output overlaps nothing, except that gs_group_norm_dev's y may be x and
- *   gs_group_norm_grad_dev's dx may be x or dy, with the same strides.
+ *   of 0 repeats a row); an output overlaps nothing, except that
+ *   gs_group_norm_dev's y may be x and gs_group_norm_grad_dev's dx may be x or
+ *   dy, with the same strides.
  * - ids and labels: int32 (ids64 0) or int64 (1). One below 0 is masked. One at
  *   or past `rows` is treated as masked too, and bit GS_FLAG_ID_RANGE is set in
  *   *flags (a device word that the caller clears and reads; NULL: not wanted).
@@ -513,8 +514,10 @@ int gs_label_loss_dev(gs_ctx* ctx, const gs_label_loss* in, float* loss, float* 
                       void* workspace, int64_t workspace_bytes, uint32_t* flags, void* stream);
 /* The losses and the gradients of sum_i row_weight[i] loss_i (row_weight (n) fp32,
  * NULL: 1): dfeat (n, dim) and dtable (rows, dim) of the inputs' dtype; masked
- * rows of dfeat are zeros. For bf16 inputs the scores' gradients are rounded to
- * bf16 before they are multiplied, as operands of the matrix cores. */
+ * rows of dfeat are zeros. For bf16 inputs the scores' gradients (or, for dfeat
+ * of rows up to 128, the exponentials) are rounded to bf16 before they are
+ * multiplied, as operands of the matrix cores. The workspace is at most about 1
+ * GB beside copies of the inputs. */
 int gs_label_loss_grad_dev(gs_ctx* ctx, const gs_label_loss* in, const float* row_weight,
                            float* loss, float* lse, void* dfeat, int64_t dfeat_stride,
                            void* dtable, int64_t dtable_stride, void* workspace,

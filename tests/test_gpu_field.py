@@ -482,6 +482,17 @@ def test_group_norm_of_batches(ops, bt, pixels, c, groups, dtype):
     test_group_norm(ops, bt, pixels, c, groups, dtype, "silu")
 
 
+@pytest.mark.parametrize("n,rows,dim", [(1, 1003, 700), (2, 40_001, 33), (8, 2500, 300),
+                                        (8, 70_000, 7), (3, 17, 520), (7, 900, 128)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_label_loss_of_few(ops, n, rows, dim, dtype):
+    feat, table, labels, weight = _loss_case(n, rows, dim, dtype, n + dim)
+    r = _loss_ref(feat, table, labels, weight, 10.0)
+    loss, lse = ops.label_loss(feat.cuda(), table.cuda(), labels.cuda(), scale=10.0)
+    _close(loss, r["loss"], r["e"], "loss")
+    _close(lse, r["lse"], r["e"], "lse")
+
+
 @pytest.mark.parametrize("n,rows,dim", [
     (5000, 3000, 16), (20_000, 600, 45), (600, 20_000, 128), (4099, 2500, 48), (3001, 4097, 64),
     (2000, 2500, 129), (1500, 1601, 260), (9, 30_000, 8), (30_000, 3, 60)])
