@@ -240,7 +240,8 @@ struct Side {
 // next loads are started: the compiler cannot tell the halves apart, and would have
 // a read after them wait for all of them.
 //
-// Bound by LDS: 64 KB read and 32 written a step at 128 bytes a cycle are 768 cycles,
+// Bound by LDS (30011 x 32003 of 512 bf16: scores 1008 TFLOP/s, G 780, dfeat 803,
+// dtable 910; G and the sums by their bytes as well): 64 KB read and 32 written a step at 128 bytes a cycle are 768 cycles,
 // the 128 products of a unit's 4 matrix cores 512; two workgroups share a compute
 // unit. Through registers a step took 5 to 10 % longer. Tiles of 256 x 128 in steps
 // of 32 move a quarter less, but G's epilogue spilled: 30011 x 32003 of 512 bf16 5.45
@@ -722,8 +723,8 @@ hipError_t fold(const SumOut<T>& o, int nz, hipStream_t st) {
 //
 // Bound by the matrix cores and, in fp32, as much by cutting the exponentials into
 // parts (88 of about 440 vector instructions a tile beside 42 products of 16 cycles).
-// 10007 x 8192 of 48 fp32: losses and dfeat 134 us, dtable 122, at 6 + 6 products of
-// each pair 0.78 PFLOP/s of bf16. 307200 x 150 of 32 bf16, losses alone: 18 us, where
+// 10007 x 8192 of 48 fp32: losses and dfeat 134 us, dtable 122, at six bf16 products
+// for each one 0.70 and 0.77 PFLOP/s. 307200 x 150 of 32 bf16, losses alone: 18 us, where
 // the 46 million exponentials take 8 at the transcendental rate and the bytes 5.
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 

@@ -469,7 +469,7 @@ def test_label_loss_in_several_pieces(ops):
 # ------------------------------------------------------------------ larger sizes
 @pytest.mark.parametrize("n,rows,dim,hot", [
     (4000, 3000, 64, 0), (4000, 3000, 64, 0.9), (2_200_003, 5000, 3, 0.3), (700_001, 100, 8, 0.5),
-    (200_003, 40_000, 20, 0.7), (1025, 129, 130, 0)])
+    (200_003, 40_000, 20, 0.7), (1025, 129, 130, 0), (4_300_001, 70_000, 2, 0.2)])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_lookup_grad_of_long_lists(ops, n, rows, dim, hot, dtype):
     test_lookup_grad(ops, n, rows, dim, hot, dtype)
