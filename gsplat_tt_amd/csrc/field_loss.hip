@@ -174,9 +174,9 @@ __device__ __forceinline__ int wave_id() {
 // summed index, and the tile's 128 rows of 64 are placed by (piece ^ row % 8), so
 // that 8 lanes reading one column of pieces touch all banks once. Not K: the
 // matrix's rows are the summed index; 64 rows of 128, 32-byte pieces placed by
-// (piece ^ row % 8), read through the transposing LDS load: in a group of 16
-// lanes, lane s reads 4 values of row s / 4 at column 4 (s % 4), and lane g gets
-// column g of the 4 rows. Addresses are a base common to the wave and one lane
+// (piece ^ the row's bits 0, 1 and 2 ^ 3), read through the transposing LDS load: in a
+// group of 16 lanes, lane s reads 4 values of row s / 4 at column 4 (s % 4), and lane
+// g gets column g of the 4 rows; two groups touch all banks once. Addresses are a base common to the wave and one lane
 // offset: with one 64-bit address a load, the registers do not last.
 //
 // PAIRS (with K): block i of 16 rows takes rows 32 (i / 2) + 8 (s / 4) + 4 (i % 2) +
@@ -184,13 +184,14 @@ __device__ __forceinline__ int wave_id() {
 template <bool K, bool PAIRS = false>
 struct Side {
     __device__ __forceinline__ static uint32_t place(uint32_t row) {
+        if (!K) return (row & 3) | ((row ^ (row >> 1)) & 4);
         return PAIRS ? (row & 3) | ((row >> 1) & 4) : row & 7;
     }
     uint32_t from;  // the lane's byte offset in memory
     int64_t ld;
     __device__ __forceinline__ explicit Side(const Mat& m) : ld(m.ld) {
         const uint32_t t = threadIdx.x, row = K ? t >> 3 : t >> 4;
-        const uint32_t c = K ? (t & 7) ^ place(row) : (t & 15) ^ ((row & 7) << 1);
+        const uint32_t c = K ? (t & 7) ^ place(row) : (t & 15) ^ (place(row) << 1);
         from = (row * (uint32_t)m.ld + c * 8) * 2;
     }
     // Straight into LDS: a wave's 64 quads lie there in lane order.
@@ -219,14 +220,14 @@ struct Side {
         typedef __attribute__((ext_vector_type(4))) short s16x4;
         typedef __attribute__((address_space(3))) s16x4* lds4;
         // row r = 32 h + 8 g + 4 u + s / 4: its piece b / 16 + i lies at
-        // 4 (b / 64 ^ u) + (i ^ s / 4)
+        // 4 (b / 64 ^ u ^ g % 2) + (i ^ s / 4)
         const char* at = reinterpret_cast<const char*>(lds) + (g * 8 + (s >> 2)) * 256 +
                          (s & 3) * 8 + (i ^ (s >> 2)) * 32;
         s16x4 half[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
             half[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (lds4)(at + h * 8192 + u * 1024 + ((b >> 6) ^ u) * 128));
+                (lds4)(at + h * 8192 + u * 1024 + ((b >> 6) ^ u ^ (g & 1)) * 128));
         return __builtin_bit_cast(
             bf16x8, __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
     }
@@ -240,12 +241,13 @@ struct Side {
 // next loads are started: the compiler cannot tell the halves apart, and would have
 // a read after them wait for all of them.
 //
-// Bound by LDS (30011 x 32003 of 512 bf16: scores 1008 TFLOP/s, G 780, dfeat 803,
-// dtable 910; G and the sums by their bytes as well): 64 KB read and 32 written a step at 128 bytes a cycle are 768 cycles,
-// the 128 products of a unit's 4 matrix cores 512; two workgroups share a compute
-// unit. Through registers a step took 5 to 10 % longer. Tiles of 256 x 128 in steps
-// of 32 move a quarter less, but G's epilogue spilled: 30011 x 32003 of 512 bf16 5.45
-// against 5.20 ms, though sums alone gained a seventh.
+// 30011 x 32003 of 512 bf16: scores 1008 TFLOP/s, G 780, dfeat 803, dtable 910. The
+// matrix cores are busy half of the time, LDS a quarter to a half: bound by the wait
+// for the next step's loads, a step's products ahead of their use, and G and its sums
+// by their bytes. Two steps ahead would need LDS reads that the compiler does not hold
+// up for loads in flight. Through registers a step took 5 to 10 % longer. Tiles of 256
+// x 128 in steps of 32 move a quarter less, but G's epilogue spilled: 5.45 against 5.20
+// ms, though sums alone gained a seventh.
 #define GS_TILE_LDS __shared__ quad lds[4 * kTile * 8]
 template <int NP, bool AK, bool BK, bool PAIRS = false, class Rows, class Done>
 __device__ __forceinline__ void tile_products(const Mat& A, const Mat& B, int64_t k0, int64_t k1,
