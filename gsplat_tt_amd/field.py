@@ -57,7 +57,6 @@ class FieldOps:
         self._L = self.ctx._L
         self.device = torch.device("cuda", self.ctx.device_index)
         self._index = self.ctx.device_index
-        self._handle = self.ctx.handle
         self._flags = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._flags_ptr = self._flags.data_ptr()
         torch.cuda.current_stream(self.device).synchronize()
@@ -131,7 +130,7 @@ class FieldOps:
         out = self._out(out, (n, dim), dtype or table.dtype, "out")
         po, _, so = _rows(out, "out")
         L._check(self._L.gs_lookup_dev(
-            self._handle, p, rows, stride, _DTYPES[table.dtype], ids.data_ptr(),
+            self.ctx.handle, p, rows, stride, _DTYPES[table.dtype], ids.data_ptr(),
             int(ids.dtype == torch.int64), n, dim, float(scale), po, so, _DTYPES[out.dtype],
             self._flags_ptr, self._stream()))
         return out
@@ -150,7 +149,7 @@ class FieldOps:
         po, _, so = _rows(out, "out")
         ws, size = self._workspace("gs_lookup_grad_workspace", n, int(rows), dim)
         L._check(self._L.gs_lookup_grad_dev(
-            self._handle, p, stride, _DTYPES[dout.dtype], ids.data_ptr(),
+            self.ctx.handle, p, stride, _DTYPES[dout.dtype], ids.data_ptr(),
             int(ids.dtype == torch.int64), n, dim, float(scale), int(bool(accumulate)), po,
             int(rows), so, _DTYPES[out.dtype], ws.data_ptr(), size, self._flags_ptr,
             self._stream()))
@@ -207,7 +206,7 @@ class FieldOps:
         mean, rstd = stats((2, d.batch, d.groups), dtype=torch.float32, device=self.device)
         ws, size = self._workspace("gs_group_norm_workspace", d.batch, d.pixels, d.channels)
         L._check(self._L.gs_group_norm_dev(
-            self._handle, ctypes.byref(d), px, bx, sx, py, by, sy, mean.data_ptr(),
+            self.ctx.handle, ctypes.byref(d), px, bx, sx, py, by, sy, mean.data_ptr(),
             rstd.data_ptr(), ws.data_ptr(), size, self._stream()))
         del keep
         return out, mean, rstd
@@ -230,7 +229,7 @@ class FieldOps:
         dweight, dbias = torch.empty((2, d.channels), dtype=torch.float32, device=self.device)
         ws, size = self._workspace("gs_group_norm_workspace", d.batch, d.pixels, d.channels)
         L._check(self._L.gs_group_norm_grad_dev(
-            self._handle, ctypes.byref(d), pd, bd, sd, px, bx, sx, mean.data_ptr(),
+            self.ctx.handle, ctypes.byref(d), pd, bd, sd, px, bx, sx, mean.data_ptr(),
             rstd.data_ptr(), po, bo, so, dweight.data_ptr(), dbias.data_ptr(),
             ws.data_ptr(), size, self._stream()))
         del keep
@@ -256,7 +255,7 @@ class FieldOps:
         loss, lse = torch.empty((2, d.n), dtype=torch.float32, device=self.device)
         ws, size = self._workspace("gs_label_loss_workspace", d.n, d.rows, d.dim, d.dtype, 0)
         L._check(self._L.gs_label_loss_dev(
-            self._handle, ctypes.byref(d), loss.data_ptr(), lse.data_ptr(), ws.data_ptr(),
+            self.ctx.handle, ctypes.byref(d), loss.data_ptr(), lse.data_ptr(), ws.data_ptr(),
             size, self._flags_ptr, self._stream()))
         del keep
         return loss, lse
@@ -276,7 +275,7 @@ class FieldOps:
         pt, _, stt = _rows(dtable, "dtable")
         ws, size = self._workspace("gs_label_loss_workspace", d.n, d.rows, d.dim, d.dtype, 1)
         L._check(self._L.gs_label_loss_grad_dev(
-            self._handle, ctypes.byref(d),
+            self.ctx.handle, ctypes.byref(d),
             None if row_weight is None else row_weight.data_ptr(), loss.data_ptr(),
             lse.data_ptr(), pf, sf, pt, stt, ws.data_ptr(), size, self._flags_ptr,
             self._stream()))
