@@ -16,6 +16,8 @@ using gs::GsError;
 constexpr int64_t kMaxRows = (int64_t)1 << 30;
 constexpr int64_t kMaxIds = ((int64_t)1 << 31) - 2;
 constexpr int kMaxDim = 65536;
+// a launch takes fewer than 2^32 threads: 2 a sample when the samples are streamed
+constexpr int64_t kMaxSamples = ((int64_t)1 << 31) - 256;
 constexpr int64_t kMaxLabels = (int64_t)1 << 22;
 constexpr int64_t kMaxImages = (int64_t)1 << 20;
 constexpr int64_t kMaxPixels = (int64_t)1 << 40;
@@ -115,7 +117,7 @@ gs::LossArgs loss_args(const gs_label_loss* d, float* loss, float* lse, void* ws
     REQUIRE(d != nullptr, "label_loss: null description");
     REQUIRE(d->n >= 0, "label_loss: n must not be negative");
     REQUIRE(d->rows >= 1, "label_loss: the table needs a row");
-    LIMIT(d->n <= kMaxIds, "label_loss: n past 2^31 - 2");
+    LIMIT(d->n <= kMaxSamples, "label_loss: n past 2^31 - 256");
     LIMIT(d->rows <= kMaxLabels, "label_loss: rows past 2^22");
     check_dim(d->dim, "label_loss");
     check_dtype(d->dtype, "label_loss");
@@ -303,7 +305,7 @@ int gs_group_norm_grad_dev(gs_ctx* ctx, const gs_group_norm* norm, const void* d
 }
 
 int64_t gs_label_loss_workspace(int64_t n, int64_t rows, int dim, int dtype, int grad) {
-    if (n < 0 || n > kMaxIds || rows < 1 || rows > kMaxLabels || dim < 1 || dim > kMaxDim ||
+    if (n < 0 || n > kMaxSamples || rows < 1 || rows > kMaxLabels || dim < 1 || dim > kMaxDim ||
         (dtype != GS_F32 && dtype != GS_BF16))
         return -1;
     return n == 0 ? 0 : (int64_t)gs::label_loss_ws(n, rows, dim, dtype, grad != 0);

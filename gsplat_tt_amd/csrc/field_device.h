@@ -109,6 +109,22 @@ __device__ __forceinline__ uint32_t block_excl_scan(uint32_t v, uint32_t* lds, u
     return before + s - v;
 }
 
+// Most blocks of a grid that its kernel walks over with: a launch takes fewer than 2^32
+// threads a dimension, 2^24 blocks of 256.
+constexpr int64_t kMostBlocks = (int64_t)1 << 22;
+inline unsigned blocks_of(int64_t items, int64_t per_block) {
+    const int64_t b = (items + per_block - 1) / per_block;
+    return (unsigned)(b < kMostBlocks ? b : kMostBlocks);
+}
+
+// Returns a launch's error: nothing runs on what it would have written. (A later launch
+// that succeeds would hide it.)
+#define GS_LAUNCHED()                               \
+    do {                                            \
+        const hipError_t e_ = hipGetLastError();    \
+        if (e_ != hipSuccess) return e_;            \
+    } while (0)
+
 // Consecutive 256-byte aligned arrays of a workspace; a null base only counts.
 struct Carve {
     uintptr_t base;

@@ -120,9 +120,7 @@ hipError_t lookup_run(const LookupArgs& a, hipStream_t st) {
     R = R < 8 ? 8 : (R > kLookupRows ? kLookupRows : R);
     // fewer where that leaves compute units idle
     while (R > 8 && a.n / R < 1024) R = R / 2 / 8 * 8 < 8 ? 8 : R / 2 / 8 * 8;
-    const int64_t blocks = (a.n + R - 1) / R;
-    const dim3 grid((unsigned)(blocks < (1 << 30) ? blocks : (1 << 30)));
-    k_lookup<TT, TO, VEC, FLAT><<<grid, kThreads, 0, st>>>(a, (int)R);
+    k_lookup<TT, TO, VEC, FLAT><<<blocks_of(a.n, R), kThreads, 0, st>>>(a, (int)R);
     return hipGetLastError();
 }
 
@@ -803,6 +801,7 @@ hipError_t grad_typed(const LookupGradArgs& a, const GradWs& w, const uint2* pai
         const int span = local_span(a.n), spans = (int)((a.n + span - 1) / span);
         k_run_sums<TI, TD, VEC, kLocal><<<dim3((unsigned)spans, cols), kThreads, span * 8, st>>>(
             a, nullptr, span, lpr, key_bits(a.rows), w.part, nullptr);
+        GS_LAUNCHED();
         k_local_join<TD><<<dim3((unsigned)a.rows, (unsigned)((a.dim + 15) / 16)), kThreads, 0, st>>>(
             a, spans, w.part);
         return hipGetLastError();
@@ -813,6 +812,7 @@ hipError_t grad_typed(const LookupGradArgs& a, const GradWs& w, const uint2* pai
         k_run_sums<TI, TD, VEC, kSorted>
             <<<dim3((unsigned)((a.n + span - 1) / span), cols), kThreads, span * 8, st>>>(
                 a, pairs, span, lpr, 0, w.part, w.runs);
+    GS_LAUNCHED();
     int join_lpr = 1;
     while (join_lpr < 64 && join_lpr * 4 < a.dim) join_lpr *= 2;
     const int64_t joins = (a.rows + kThreads / join_lpr - 1) / (kThreads / join_lpr);
@@ -822,7 +822,8 @@ hipError_t grad_typed(const LookupGradArgs& a, const GradWs& w, const uint2* pai
 }
 
 template <int ITEMS>
-const uint2* sort_ids(const LookupGradArgs& a, const GradWs& w, hipStream_t st) {
+hipError_t sort_ids(const LookupGradArgs& a, const GradWs& w, const uint2** sorted,
+                    hipStream_t st) {
     const int bits = key_bits(a.rows), passes = (bits + 7) / 8;
     const unsigned blocks = (unsigned)((a.n + kThreads * ITEMS - 1) / (kThreads * ITEMS));
     const uint2* pairs = nullptr;
@@ -830,13 +831,17 @@ const uint2* sort_ids(const LookupGradArgs& a, const GradWs& w, hipStream_t st) 
         const int b = (bits - done + passes - p - 1) / (passes - p);
         k_sort_count<ITEMS><<<blocks, kThreads, 0, st>>>(a, pairs, done, b, w.counts,
                                                          p == 0 ? w.runs : nullptr);
+        GS_LAUNCHED();
         k_sort_scan<<<1u << b, kThreads, 0, st>>>(w.counts, (int)blocks, w.totals);
+        GS_LAUNCHED();
         k_sort_scatter<ITEMS><<<blocks, kThreads, 0, st>>>(a, pairs, done, b, w.counts, w.totals,
                                                            w.pairs[p & 1]);
+        GS_LAUNCHED();
         pairs = w.pairs[p & 1];
         done += b;
     }
-    return pairs;
+    *sorted = pairs;
+    return hipSuccess;
 }
 
 __global__ __launch_bounds__(kThreads) void k_run_clear(uint2* runs, int64_t rows) {
@@ -862,6 +867,7 @@ hipError_t launch_lookup_grad(const LookupGradArgs& a, hipStream_t st) {
     if (a.rows == 0) return hipSuccess;
     const GradWs w(a.ws, a.n, a.rows, a.dim);
     const uint2* pairs = nullptr;
+    hipError_t e = hipSuccess;
     if (a.n == 0)
         k_run_clear<<<(unsigned)((a.rows + kThreads - 1) / kThreads), kThreads, 0, st>>>(w.runs,
                                                                                       a.rows);
@@ -871,7 +877,9 @@ hipError_t launch_lookup_grad(const LookupGradArgs& a, hipStream_t st) {
         k_sort_short<<<1, kShortThreads, 0, st>>>(a, key_bits(a.rows), w.pairs[0], w.runs);
         pairs = w.pairs[0];
     } else if (!is_local(a.n, a.rows))
-        pairs = sort_items(a.n) == 4 ? sort_ids<4>(a, w, st) : sort_ids<16>(a, w, st);
+        e = sort_items(a.n) == 4 ? sort_ids<4>(a, w, &pairs, st) : sort_ids<16>(a, w, &pairs, st);
+    if (e != hipSuccess) return e;
+    GS_LAUNCHED();
     if (a.dout_dtype == 0)
         return a.dtable_dtype == 0 ? grad_typed<float, float>(a, w, pairs, st)
                                    : grad_typed<float, bf16>(a, w, pairs, st);

@@ -452,32 +452,35 @@ __global__ __launch_bounds__(kThreads) void k_loss_join(LossArgs a, const float2
                                                         int64_t padded, const float* label_score,
                                                         float* lse2) {
     const int sub = threadIdx.x >> 5;  // of the workgroup's 32 rows
-    const int64_t i = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
     __shared__ float2 lds[8][32];
-    float m = kLowest, sum = 0.0f;
-    if (i < padded)
-        for (int k0 = sub; k0 < parts; k0 += 8 * 8) {
-            float2 p[8];
+    for (int64_t i0 = (int64_t)blockIdx.x * 32; i0 < padded; i0 += (int64_t)gridDim.x * 32) {
+        const int64_t i = i0 + (threadIdx.x & 31);
+        float m = kLowest, sum = 0.0f;
+        if (i < padded)
+            for (int k0 = sub; k0 < parts; k0 += 8 * 8) {
+                float2 p[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-                p[u] = k0 + u * 8 < parts ? part[(int64_t)(k0 + u * 8) * padded + i]
-                                          : make_float2(kLowest, 0.0f);
+                for (int u = 0; u < 8; ++u)
+                    p[u] = k0 + u * 8 < parts ? part[(int64_t)(k0 + u * 8) * padded + i]
+                                              : make_float2(kLowest, 0.0f);
 #pragma unroll
-            for (int u = 0; u < 8; ++u) join_sums(m, sum, p[u].x, p[u].y);
+                for (int u = 0; u < 8; ++u) join_sums(m, sum, p[u].x, p[u].y);
+            }
+        __syncthreads();
+        lds[sub][threadIdx.x & 31] = make_float2(m, sum);
+        __syncthreads();
+        if (sub != 0 || i >= padded) continue;
+        for (int k = 1; k < 8; ++k) {
+            const float2 p = lds[k][threadIdx.x & 31];
+            join_sums(m, sum, p.x, p.y);
         }
-    lds[sub][threadIdx.x & 31] = make_float2(m, sum);
-    __syncthreads();
-    if (sub != 0 || i >= padded) return;
-    for (int k = 1; k < 8; ++k) {
-        const float2 p = lds[k][threadIdx.x & 31];
-        join_sums(m, sum, p.x, p.y);
-    }
-    const float l = (m < INFINITY ? m : 0.0f) + log2f(sum);
-    const bool on = i < a.n && load_id(a.labels, a.labels64, i, a.rows, nullptr) >= 0;
-    if (lse2 != nullptr) lse2[i] = on ? l : 0.0f;
-    if (i < a.n) {
-        if (a.loss != nullptr) a.loss[i] = on ? (l - label_score[i]) * kLn2 : 0.0f;
-        if (a.lse != nullptr) a.lse[i] = on ? l * kLn2 : 0.0f;
+        const float l = (m < INFINITY ? m : 0.0f) + log2f(sum);
+        const bool on = i < a.n && load_id(a.labels, a.labels64, i, a.rows, nullptr) >= 0;
+        if (lse2 != nullptr) lse2[i] = on ? l : 0.0f;
+        if (i < a.n) {
+            if (a.loss != nullptr) a.loss[i] = on ? (l - label_score[i]) * kLn2 : 0.0f;
+            if (a.lse != nullptr) a.lse[i] = on ? l * kLn2 : 0.0f;
+        }
     }
 }
 
@@ -684,10 +687,7 @@ __global__ __launch_bounds__(kThreads) void k_loss_fold(SumOut<T> o, int nz) {
     }
 }
 
-unsigned blocks_for(int64_t items) {
-    const int64_t b = (items + kThreads - 1) / kThreads;
-    return (unsigned)(b < 65536 ? b : 65536);
-}
+unsigned blocks_for(int64_t items) { return std::min(65536u, blocks_of(items, kThreads)); }
 
 template <typename T>
 hipError_t fold(const SumOut<T>& o, int nz, hipStream_t st) {
@@ -783,7 +783,7 @@ constexpr int padded_dim(int ks) { return (ks + 31) / 32 * 32; }
 template <int NP>
 constexpr int kBlocks = NP == 1 ? 2 : 1;
 
-// (rows, dim) as tiles of operands, one workgroup a tile; of samples (label) the
+// (rows, dim) as tiles of operands, a workgroup a tile (or several); of samples (label) the
 // masked ones are zeros, and label and weight are written for the gradients. Bound by
 // latency: 10007 x 48 fp32 7 us.
 template <typename T, int NP, int KS, bool SECOND>
@@ -793,47 +793,52 @@ __global__ __launch_bounds__(kThreads) void k_operands(const T* src, int64_t row
     constexpr int DD = padded_dim(KS);
     __shared__ float tile[32][DD + 1];
     __shared__ int32_t lab[32];
-    const int64_t r0 = (int64_t)blockIdx.x * 32;
-    if (threadIdx.x < 32) {
-        int32_t l = 0;
-        if (label != nullptr) {
-            const int64_t i = r0 + threadIdx.x;
-            l = i < rows ? load_id(a.labels, a.labels64, i, a.rows, nullptr) : -1;
-            label[i] = l;
-            weight[i] = l < 0 ? 0.0f : a.scale * (a.row_weight != nullptr ? a.row_weight[i] : 1.0f);
-            if (i >= rows) lse2[i] = 0.0f;  // the others' come from the scores
-        }
-        lab[threadIdx.x] = l;
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < 32 * DD; e += kThreads) {
-        const int r = e / DD, c = e % DD;
-        float v = 0.0f;
-        if (r0 + r < rows && c < dim && lab[r] >= 0)
-            v = plain_input<NP>(to_float(src[(r0 + r) * stride + c]));
-        tile[r][c] = v;
-    }
-    __syncthreads();
     constexpr int kFirst = KS / 16 * 64, kSecond = SECOND ? DD / 32 * 2 * 64 : 0;
-    quad* to = out + (size_t)blockIdx.x * NP * (kFirst + kSecond);
-    for (int e = threadIdx.x; e < kFirst + kSecond; e += kThreads) {
-        const int lane = e & 63, h = lane >> 5;
-        float v[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            if (e < kFirst) {
-                v[k] = tile[lane & 31][(e >> 6) * 16 + 8 * h + k];
-            } else {
-                const int b = (e - kFirst) >> 6;  // dim / 32, f
-                v[k] = tile[16 * (b & 1) + 4 * h + k + (k < 4 ? 0 : 4)][(b >> 1) * 32 + (lane & 31)];
+    for (int64_t r0 = (int64_t)blockIdx.x * 32; r0 < rows; r0 += (int64_t)gridDim.x * 32) {
+        __syncthreads();
+        if (threadIdx.x < 32) {
+            int32_t l = 0;
+            if (label != nullptr) {
+                const int64_t i = r0 + threadIdx.x;
+                l = i < rows ? load_id(a.labels, a.labels64, i, a.rows, nullptr) : -1;
+                label[i] = l;
+                weight[i] =
+                    l < 0 ? 0.0f : a.scale * (a.row_weight != nullptr ? a.row_weight[i] : 1.0f);
+                if (i >= rows) lse2[i] = 0.0f;  // the others' come from the scores
             }
+            lab[threadIdx.x] = l;
         }
-        quad piece[NP];
-        split8<NP>(v, piece);
+        __syncthreads();
+        for (int e = threadIdx.x; e < 32 * DD; e += kThreads) {
+            const int r = e / DD, c = e % DD;
+            float v = 0.0f;
+            if (r0 + r < rows && c < dim && lab[r] >= 0)
+                v = plain_input<NP>(to_float(src[(r0 + r) * stride + c]));
+            tile[r][c] = v;
+        }
+        __syncthreads();
+        quad* to = out + (size_t)(r0 / 32) * NP * (kFirst + kSecond);
+        for (int e = threadIdx.x; e < kFirst + kSecond; e += kThreads) {
+            const int lane = e & 63, h = lane >> 5;
+            float v[8];
 #pragma unroll
-        for (int p = 0; p < NP; ++p) {
-            const size_t at = e < kFirst ? p * kFirst + e : NP * kFirst + p * kSecond + (e - kFirst);
-            to[at] = piece[p];
+            for (int k = 0; k < 8; ++k) {
+                if (e < kFirst) {
+                    v[k] = tile[lane & 31][(e >> 6) * 16 + 8 * h + k];
+                } else {
+                    const int b = (e - kFirst) >> 6;  // dim / 32, f
+                    v[k] =
+                        tile[16 * (b & 1) + 4 * h + k + (k < 4 ? 0 : 4)][(b >> 1) * 32 + (lane & 31)];
+                }
+            }
+            quad piece[NP];
+            split8<NP>(v, piece);
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+                const size_t at =
+                    e < kFirst ? p * kFirst + e : NP * kFirst + p * kSecond + (e - kFirst);
+                to[at] = piece[p];
+            }
         }
     }
 }
@@ -1311,13 +1316,15 @@ hipError_t loss_run(const LossArgs& a, bool grad, hipStream_t st) {
     k_parts<T, NP><<<blocks_for((nr + w.vp) * w.dq / 8), kThreads, 0, st>>>(
         a, nr, w.vp, w.dq, w.label, w.weight, reinterpret_cast<quad*>(w.F),
         reinterpret_cast<quad*>(w.T));
+    GS_LAUNCHED();
     const Mat F{w.F, w.dq, nr * w.dq}, Tm{w.T, w.dq, w.vp * w.dq};
     const SpotGrid gs(nr / kTile, w.shares, kSpot);
     k_loss_scores<NP><<<gs.blocks, kThreads, 0, st>>>(F, Tm, w.kd, a.rows, scale2, w.label, nr,
                                                       (int)(w.vp / kTile), w.share, gs.gy, w.part,
                                                       w.score);
-    k_loss_join<<<(unsigned)((nr + 31) / 32), kThreads, 0, st>>>(a, w.part, w.shares * 2, nr,
-                                                                 w.score, w.lse2);
+    GS_LAUNCHED();
+    k_loss_join<<<blocks_of(nr, 32), kThreads, 0, st>>>(a, w.part, w.shares * 2, nr, w.score,
+                                                        w.lse2);
     hipError_t e = hipGetLastError();
     if (!grad || e != hipSuccess) return e;
     for (int64_t r0 = 0; r0 < nr; r0 += w.rc) {
@@ -1331,6 +1338,7 @@ hipError_t loss_run(const LossArgs& a, bool grad, hipStream_t st) {
             k_loss_g<NP><<<gg.blocks, kThreads, 0, st>>>(F, Tm, w.kd, a.rows, scale2, w.label,
                                                          w.weight, w.lse2, r0, v0, rc, vc, share,
                                                          gg.gy, w.G);
+            GS_LAUNCHED();
             const Mat G{w.G, vc, rc * vc};
             const int zf = (int)((vc + w.share_f - 1) / w.share_f);
             const SumOut<T> of{w.slices, w.sum_f, v0 == 0, v0 + vc >= w.vp, rc, w.dq,
@@ -1339,6 +1347,7 @@ hipError_t loss_run(const LossArgs& a, bool grad, hipStream_t st) {
             k_loss_sum<T, NP, true>
                 <<<SpotGrid(rc / kTile * zf, w.dq / kTile, w.dq).blocks, kThreads, 0, st>>>(
                     G, {w.T + v0 * w.dq, w.dq, w.vp * w.dq}, vc, w.share_f, zf, of);
+            GS_LAUNCHED();
             if (zf > 1 && (e = fold(of, zf, st)) != hipSuccess) return e;
             const int zt = (int)((rc + w.share_t - 1) / w.share_t);
             const SumOut<T> ot{w.slices, w.sum_t + (w.sum_t != nullptr ? v0 * w.dq : 0), r0 == 0,
@@ -1348,6 +1357,7 @@ hipError_t loss_run(const LossArgs& a, bool grad, hipStream_t st) {
             k_loss_sum<T, NP, false>
                 <<<SpotGrid(vc / kTile * zt, w.dq / kTile, w.dq).blocks, kThreads, 0, st>>>(
                     G, {w.F + r0 * w.dq, w.dq, nr * w.dq}, rc, w.share_t, zt, ot);
+            GS_LAUNCHED();
             if (zt > 1 && (e = fold(ot, zt, st)) != hipSuccess) return e;
         }
     }
@@ -1447,11 +1457,12 @@ hipError_t stream_run(const LossArgs& a, bool grad, hipStream_t st) {
     const T* feat = static_cast<const T*>(a.feat);
     const T* table = static_cast<const T*>(a.table);
     if (grad)
-        k_operands<T, NP, KS, true><<<(unsigned)w.tt, kThreads, 0, st>>>(
+        k_operands<T, NP, KS, true><<<blocks_of(w.tt, 1), kThreads, 0, st>>>(
             table, a.rows, a.table_stride, a.dim, a, nullptr, nullptr, nullptr, w.T);
     else
-        k_operands<T, NP, KS, false><<<(unsigned)w.tt, kThreads, 0, st>>>(
+        k_operands<T, NP, KS, false><<<blocks_of(w.tt, 1), kThreads, 0, st>>>(
             table, a.rows, a.table_stride, a.dim, a, nullptr, nullptr, nullptr, w.T);
+    GS_LAUNCHED();
     StreamArgs s{};
     s.q = feat;
     s.nq = a.n;
@@ -1481,8 +1492,8 @@ hipError_t stream_run(const LossArgs& a, bool grad, hipStream_t st) {
         s.share = w.scores.tiles;
         e = launch_stream<T, NP, KS, kScores>(s, w.scores, st);
         if (e == hipSuccess && w.scores.count > 1) {
-            k_loss_join<<<(unsigned)((a.n + 31) / 32), kThreads, 0, st>>>(
-                a, w.part, w.scores.count, a.n, w.score, nullptr);
+            k_loss_join<<<blocks_of(a.n, 32), kThreads, 0, st>>>(a, w.part, w.scores.count, a.n,
+                                                                 w.score, nullptr);
             e = hipGetLastError();
         }
         return e;
@@ -1502,8 +1513,9 @@ hipError_t stream_run(const LossArgs& a, bool grad, hipStream_t st) {
         e = w.by_feat.count > 16 ? feat_join<T, DD, 8>(s, w.by_feat.count, st)
                                  : feat_join<T, DD, 1>(s, w.by_feat.count, st);
     if (e != hipSuccess) return e;
-    k_operands<T, NP, KS, true><<<(unsigned)w.tf, kThreads, 0, st>>>(
+    k_operands<T, NP, KS, true><<<blocks_of(w.tf, 1), kThreads, 0, st>>>(
         feat, a.n, a.feat_stride, a.dim, a, w.label, w.weight, w.lse2, w.F);
+    GS_LAUNCHED();
     s.q = table;
     s.nq = a.rows;
     s.q_stride = a.table_stride;
@@ -1680,6 +1692,7 @@ hipError_t few_run(const LossArgs& a, hipStream_t st) {
         k_loss_few<T, VEC, 1><<<w.blocks, kThreads, 0, st>>>(a, w.lpr, scale2, w.part, w.score);
     else
         k_loss_few<T, VEC, kFew><<<w.blocks, kThreads, 0, st>>>(a, w.lpr, scale2, w.part, w.score);
+    GS_LAUNCHED();
     k_loss_join<<<1, kThreads, 0, st>>>(a, w.part, w.blocks, a.n, w.score, nullptr);
     return hipGetLastError();
 }

@@ -204,43 +204,47 @@ __global__ __launch_bounds__(kThreads) void k_norm_stats(NormArgs a, int chunks,
                 make_float2(lds[j * kThreads + at].mean, lds[j * kThreads + at].m2);
 }
 
-// One workgroup per (image, group): joins its channels' chunks. Bound by latency, 5 to
-// 7 us.
+// A workgroup an (image, group), or several one after the other: joins its channels'
+// chunks. Bound by latency, 5 to 7 us.
 __global__ __launch_bounds__(kThreads) void k_norm_finish(NormArgs a, int chunks,
                                                           const float2* part) {
     __shared__ Moments lds[kThreads];
-    const int64_t b = blockIdx.x / a.groups;
-    const int g = blockIdx.x % a.groups, per_group = a.channels / a.groups;
+    const int per_group = a.channels / a.groups;
     const int64_t per = (a.pixels + chunks - 1) / chunks;
-    const float2* from = part + b * chunks * a.channels + (int64_t)g * per_group;
-    Moments m = {0.0f, 0.0f, 0.0f};
-    const int all = chunks * per_group;
-    for (int i0 = threadIdx.x; i0 < all; i0 += kThreads * 8) {
-        float2 v[8];
-        float n[8];
+    for (int64_t at = blockIdx.x; at < a.batch * a.groups; at += gridDim.x) {
+        const int64_t b = at / a.groups;
+        const float2* from = part + b * chunks * a.channels + (at - b * a.groups) * per_group;
+        Moments m = {0.0f, 0.0f, 0.0f};
+        const int all = chunks * per_group;
+        for (int i0 = threadIdx.x; i0 < all; i0 += kThreads * 8) {
+            float2 v[8];
+            float n[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const int i = min(i0 + u * kThreads, all - 1);
-            const int k = i / per_group, c = i - k * per_group;
-            const bool on = i0 + u * kThreads < all;
-            v[u] = from[(int64_t)k * a.channels + c];
-            if (!on) v[u] = make_float2(0.0f, 0.0f);
-            const int64_t p0 = min(a.pixels, per * k);
-            n[u] = on ? (float)(min(a.pixels, p0 + per) - p0) : 0.0f;
+            for (int u = 0; u < 8; ++u) {
+                const int i = min(i0 + u * kThreads, all - 1);
+                const int k = i / per_group, c = i - k * per_group;
+                const bool on = i0 + u * kThreads < all;
+                v[u] = from[(int64_t)k * a.channels + c];
+                if (!on) v[u] = make_float2(0.0f, 0.0f);
+                const int64_t p0 = min(a.pixels, per * k);
+                n[u] = on ? (float)(min(a.pixels, p0 + per) - p0) : 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) m = join(m, {n[u], v[u].x, v[u].y});
         }
-#pragma unroll
-        for (int u = 0; u < 8; ++u) m = join(m, {n[u], v[u].x, v[u].y});
-    }
-    lds[threadIdx.x] = m;
-    __syncthreads();
-    for (int o = kThreads / 2; o > 0; o >>= 1) {
-        if ((int)threadIdx.x < o) lds[threadIdx.x] = join(lds[threadIdx.x], lds[threadIdx.x + o]);
+        lds[threadIdx.x] = m;
         __syncthreads();
-    }
-    if (threadIdx.x == 0) {
-        const float count = (float)a.pixels * (float)per_group;
-        a.mean[blockIdx.x] = lds[0].mean;
-        a.rstd[blockIdx.x] = 1.0f / sqrtf(lds[0].m2 / count + a.eps);
+        for (int o = kThreads / 2; o > 0; o >>= 1) {
+            if ((int)threadIdx.x < o)
+                lds[threadIdx.x] = join(lds[threadIdx.x], lds[threadIdx.x + o]);
+            __syncthreads();
+        }
+        if (threadIdx.x == 0) {
+            const float count = (float)a.pixels * (float)per_group;
+            a.mean[at] = lds[0].mean;
+            a.rstd[at] = 1.0f / sqrtf(lds[0].m2 / count + a.eps);
+        }
+        __syncthreads();
     }
 }
 
@@ -355,54 +359,57 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_sums(NormArgs a, int chu
             part[p.part * a.channels + p.c + j] = make_float2(s1[j], s2[j]);
 }
 
-// One workgroup per (image, group): the group's channel sums over the chunks, and
-// m1, m2. Threads of one channel stand `per_group` apart (or walk over channels
-// when a group has more than the workgroup has threads).
+// A workgroup an (image, group), or several one after the other: the group's channel
+// sums over the chunks, and m1, m2. Threads of one channel stand `per_group` apart (or
+// walk over channels when a group has more than the workgroup has threads).
 __global__ __launch_bounds__(kThreads) void k_norm_grad_finish(NormArgs a, int chunks,
                                                                const float2* part, float2* sums,
                                                                float2* means) {
     __shared__ float2 lds[kThreads];
     __shared__ float red[kThreads / 64];
-    const int64_t b = blockIdx.x / a.groups;
-    const int g = blockIdx.x % a.groups, per_group = a.channels / a.groups;
-    float m1 = 0.0f, m2 = 0.0f;
+    const int per_group = a.channels / a.groups;
     const int cols = min(per_group, kThreads), rows = kThreads / cols;
     const int row = threadIdx.x / cols, col = threadIdx.x % cols;
-    for (int c0 = 0; c0 < per_group; c0 += cols) {
-        const bool on = row < rows && c0 + col < per_group;
-        const int c = g * per_group + c0 + col;
-        float s1[1] = {0.0f}, s2[1] = {0.0f};
-        if (on) {
-            const float2* from = part + b * chunks * a.channels + c;
-            for (int k0 = row; k0 < chunks; k0 += rows * 8) {
-                float2 v[8];
+    for (int64_t at = blockIdx.x; at < a.batch * a.groups; at += gridDim.x) {
+        const int64_t b = at / a.groups;
+        const int g = (int)(at - b * a.groups);
+        float m1 = 0.0f, m2 = 0.0f;
+        for (int c0 = 0; c0 < per_group; c0 += cols) {
+            const bool on = row < rows && c0 + col < per_group;
+            const int c = g * per_group + c0 + col;
+            float s1[1] = {0.0f}, s2[1] = {0.0f};
+            if (on) {
+                const float2* from = part + b * chunks * a.channels + c;
+                for (int k0 = row; k0 < chunks; k0 += rows * 8) {
+                    float2 v[8];
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const int k = k0 + u * rows;
-                    v[u] = from[(int64_t)min(k, chunks - 1) * a.channels];
-                    if (k >= chunks) v[u] = make_float2(0.0f, 0.0f);
-                }
+                    for (int u = 0; u < 8; ++u) {
+                        const int k = k0 + u * rows;
+                        v[u] = from[(int64_t)min(k, chunks - 1) * a.channels];
+                        if (k >= chunks) v[u] = make_float2(0.0f, 0.0f);
+                    }
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    s1[0] += v[u].x;
-                    s2[0] += v[u].y;
+                    for (int u = 0; u < 8; ++u) {
+                        s1[0] += v[u].x;
+                        s2[0] += v[u].y;
+                    }
                 }
             }
+            __syncthreads();
+            slots_sum<1, kThreads>(lds, threadIdx.x, row, rows, cols, s1, s2);
+            if (on && row == 0) {
+                const float w = a.weight != nullptr ? a.weight[c] : 1.0f;
+                sums[b * a.channels + c] = make_float2(s1[0], s2[0]);
+                m1 = fmaf(w, s1[0], m1);
+                m2 = fmaf(w, s2[0], m2);
+            }
         }
-        __syncthreads();
-        slots_sum<1, kThreads>(lds, threadIdx.x, row, rows, cols, s1, s2);
-        if (on && row == 0) {
-            const float w = a.weight != nullptr ? a.weight[c] : 1.0f;
-            sums[b * a.channels + c] = make_float2(s1[0], s2[0]);
-            m1 = fmaf(w, s1[0], m1);
-            m2 = fmaf(w, s2[0], m2);
+        m1 = block_sum<kThreads>(m1, red);
+        m2 = block_sum<kThreads>(m2, red);
+        if (threadIdx.x == 0) {
+            const float count = (float)a.pixels * (float)per_group;
+            means[at] = make_float2(m1 / count, m2 / count);
         }
-    }
-    m1 = block_sum<kThreads>(m1, red);
-    m2 = block_sum<kThreads>(m2, red);
-    if (threadIdx.x == 0) {
-        const float count = (float)a.pixels * (float)per_group;
-        means[blockIdx.x] = make_float2(m1 / count, m2 / count);
     }
 }
 
@@ -673,6 +680,7 @@ hipError_t norm_run(const NormArgs& a, bool grad, hipStream_t st) {
             k_norm_small<T, VEC, ACT><<<small, kSmallThreads, 0, st>>>(a);
         } else {
             k_norm_small_grad<T, VEC, ACT><<<small, kSmallThreads, 0, st>>>(a, w.sums);
+            GS_LAUNCHED();
             if (a.batch > 1)
                 k_norm_grad_params<<<(unsigned)((a.channels + kThreads - 1) / kThreads), kThreads,
                                      0, st>>>(a, w.sums);
@@ -680,17 +688,22 @@ hipError_t norm_run(const NormArgs& a, bool grad, hipStream_t st) {
         return hipGetLastError();
     }
     const dim3 grid((unsigned)(chunks * a.batch), (unsigned)((cols + kThreads - 1) / kThreads));
-    const unsigned groups = (unsigned)(a.batch * a.groups);
+    const unsigned groups = blocks_of(a.batch * a.groups, 1);
     if (!grad) {
         k_norm_stats<T, VEC><<<grid, kThreads, 0, st>>>(a, chunks, w.part);
+        GS_LAUNCHED();
         k_norm_finish<<<groups, kThreads, 0, st>>>(a, chunks, w.part);
+        GS_LAUNCHED();
         k_norm_apply<T, VEC, ACT><<<grid, kThreads, 0, st>>>(a, chunks);
     } else {
         k_norm_grad_sums<T, VEC, ACT><<<grid, kThreads, 0, st>>>(a, chunks, w.part);
+        GS_LAUNCHED();
         k_norm_grad_finish<<<groups, kThreads, 0, st>>>(a, chunks, w.part, w.sums, w.means);
+        GS_LAUNCHED();
         if (a.batch > kFewImages)
             k_norm_grad_params<<<(unsigned)((a.channels + kThreads - 1) / kThreads), kThreads, 0,
                                  st>>>(a, w.sums);
+        GS_LAUNCHED();
         k_norm_grad_apply<T, VEC, ACT><<<grid, kThreads, 0, st>>>(
             a, chunks, w.means, a.batch > kFewImages ? nullptr : w.sums);
     }

@@ -49,3 +49,9 @@ class _Stream:
 
     def synchronize(self):
         pass
+
+
+def test_label_loss_sizes_past_a_launch_are_refused():
+    lib = field.L.load_library()
+    assert lib.gs_label_loss_workspace(2 ** 31 - 256, 2, 1, 1, 0) > 0
+    assert lib.gs_label_loss_workspace(2 ** 31 - 255, 2, 1, 1, 0) == -1

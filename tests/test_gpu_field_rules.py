@@ -48,3 +48,69 @@ def test_a_closed_context_is_refused():
                  lambda: ops.label_loss_grad(table[:3], table, ids)):
         with pytest.raises(ValueError, match="null ctx"):
             call()
+
+
+# ------------------------------------------------------------------ sizes
+def test_group_norm_of_more_groups_than_a_grid_has_blocks(ops):
+    """2^24 groups of 4 values: with 256 threads each, 2^32 threads, past a launch."""
+    from tests.test_gpu_field import STEPS, _norm_ref
+    g = _gen(1)
+    x, dy = (_randn(g, 1 << 20, 1, 64, dtype=BF16) for _ in range(2))
+    w, b = 1 + 0.3 * _randn(g, 64), 0.3 * _randn(g, 64)
+    r = _norm_ref(x, 16, w, b, "silu", 1e-5, dy)
+    y, mean, rstd = ops.group_norm(x, 16, w, b, act="silu")
+    assert ((y.to(D64) - r["y"]).abs() <= STEPS * EPS * r["y_size"] + BF * r["y"].abs()).all()
+    dx, dw, db = ops.group_norm_grad(dy, x, mean, rstd, 16, w, b, act="silu")
+    assert ((dx.to(D64) - r["dx"]).abs() <= STEPS * EPS * r["dx_size"] + BF * r["dx"].abs()).all()
+    assert ((dw.to(D64) - r["dw"]).abs() <= STEPS * EPS * r["dw_size"]).all()
+    assert ((db.to(D64) - r["db"]).abs() <= STEPS * EPS * r["db_size"]).all()
+
+
+def test_lookup_of_more_rows_than_a_grid_has_blocks(ops):
+    """2^27 rows of odd length and stride, 8 a workgroup."""
+    n, dim = 1 << 27, 129
+    g = _gen(2)
+    table = _randn(g, 7, dim, dtype=BF16)
+    ids = torch.randint(-1, 7, (n,), generator=g, device="cuda", dtype=torch.int32)
+    room = torch.full((n, dim + 1), 5.0, dtype=BF16, device="cuda")
+    ops.lookup(table, ids, 1.0, out=room[:, :dim])
+    rows = torch.cat([table, torch.zeros(1, dim, dtype=BF16, device="cuda")])
+    for lo in range(0, n, 1 << 23):
+        at = slice(lo, lo + (1 << 23))
+        assert torch.equal(room[at, :dim], rows[ids[at].long()]), lo  # -1: the last, zeros
+        assert (room[at, dim] == 5).all()
+    del room, ids
+    torch.cuda.empty_cache()
+
+
+def test_label_loss_of_more_samples_than_a_grid_has_blocks(ops):
+    """2^29 samples and some, 32 a workgroup in their layout. A table row's sums run over
+    a share's products of 16 samples one after the other: 2^24 tiles of 32 in some hundred
+    shares make fewer than 2^18 of them."""
+    n, rows, scale = (1 << 29) + 37, 3, 2.0
+    g = _gen(3)
+    feat, table = _randn(g, n, 1, dtype=BF16), _randn(g, rows, 1, dtype=BF16)
+    labels = torch.randint(-1, rows, (n,), generator=g, device="cuda", dtype=torch.int32)
+    loss, lse, dfeat, dtable = ops.label_loss_grad(feat, table, labels, scale=scale)
+    t, want, size = table.to(D64), torch.zeros(rows, 1, dtype=D64, device="cuda"), 0.0
+    step = 1 << 24
+    for lo in range(0, n, step):
+        at = slice(lo, lo + step)
+        f, y = feat[at].to(D64), labels[at].long()
+        on, y = y >= 0, y.clamp(min=0)[:, None]
+        s = scale * f @ t.T
+        log = torch.logsumexp(s, 1)
+        one = torch.where(on, log - s.gather(1, y)[:, 0], 0.0)
+        assert ((loss[at].to(D64) - one).abs() <= 64 * EPS * (1 + s.abs().amax(1))).all(), lo
+        assert ((lse[at].to(D64) - torch.where(on, log, 0.0)).abs() <=
+                64 * EPS * (1 + s.abs().amax(1))).all(), lo
+        p = torch.exp(s - log[:, None])
+        d = p.scatter_add(1, y, torch.full_like(s[:, :1], -1.0)) * scale * on[:, None]
+        # the products' left operands and the result are rounded to bf16
+        near = 1.05 * BF * (d.abs() @ t.abs() + (d @ t).abs()) + 64 * EPS
+        assert ((dfeat[at].to(D64) - d @ t).abs() <= near).all(), lo
+        want += d.T @ f
+        size += (d.abs().T @ f.abs())
+    assert ((dtable.to(D64) - want).abs() <= (BF + 2.0 ** 18 * EPS) * size + BF * want.abs()).all()
+    del feat, labels, loss, lse, dfeat
+    torch.cuda.empty_cache()
