@@ -88,24 +88,24 @@ __device__ __forceinline__ float block_sum(float v, float* lds) {
     return s;
 }
 
-// What VEC channels from c of image b need, folded to one fused multiply-add a
-// step: xh = x r + o, z = xh w + bias. (The offset's rounding is that of a mean's
-// last place, which the mean itself has.)
+// What VEC channels from c of image b need: xh = (x - m) r, z = xh w + bias. The mean is
+// subtracted first: folded into one multiply-add, x r - m r, the product's rounding
+// stays as a share of m r, which a mean far from 0 makes larger than xh.
 template <int VEC>
 struct Channels {
-    float r[VEC], o[VEC], w[VEC], bias[VEC];
+    float m[VEC], r[VEC], w[VEC], bias[VEC];
     __device__ __forceinline__ Channels(const NormArgs& a, int64_t b, int c) {
         const int per_group = a.channels / a.groups;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
             const int64_t g = b * a.groups + (c + j) / per_group;
+            m[j] = a.mean[g];
             r[j] = a.rstd[g];
-            o[j] = -a.mean[g] * r[j];
             w[j] = a.weight != nullptr ? a.weight[c + j] : 1.0f;
             bias[j] = a.bias != nullptr ? a.bias[c + j] : 0.0f;
         }
     }
-    __device__ __forceinline__ float xh(float x, int j) const { return fmaf(x, r[j], o[j]); }
+    __device__ __forceinline__ float xh(float x, int j) const { return (x - m[j]) * r[j]; }
     __device__ __forceinline__ float z(float h, int j) const { return fmaf(h, w[j], bias[j]); }
 };
 
@@ -258,16 +258,12 @@ __global__ __launch_bounds__(kThreads) void k_norm_apply(NormArgs a, int chunks)
     if (!p.on) return;
     Channels<VEC> ch(a, p.b, p.c);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {  // xh is not needed: z = x k + c
-        ch.bias[j] = fmaf(ch.o[j], ch.w[j], ch.bias[j]);
-        ch.w[j] *= ch.r[j];
-    }
+    for (int j = 0; j < VEC; ++j) ch.w[j] *= ch.r[j];  // xh is not needed
     const T* x = static_cast<const T*>(a.x) + p.b * a.x_batch + p.c;
     T* y = static_cast<T*>(a.y) + p.b * a.y_batch + p.c;
     auto one = [&](float* v) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j)
-            v[j] = act<ACT>(ch.z(v[j], j));
+        for (int j = 0; j < VEC; ++j) v[j] = act<ACT>(ch.z(v[j] - ch.m[j], j));
     };
     int64_t q = p.p0 + p.slot;
     for (; q + (kAhead - 1) * p.slots < p.p1; q += kAhead * p.slots) {

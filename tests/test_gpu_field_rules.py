@@ -114,3 +114,39 @@ def test_label_loss_of_more_samples_than_a_grid_has_blocks(ops):
     assert ((dtable.to(D64) - want).abs() <= (BF + 2.0 ** 18 * EPS) * size + BF * want.abs()).all()
     del feat, labels, loss, lse, dfeat
     torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------ group norm's exactness
+@pytest.mark.parametrize("pixels,c,groups", [((9, 11), 16, 4), ((200, 111), 64, 2), ((70, 61), 6, 2)])
+@pytest.mark.parametrize("act", ["none", "relu"])
+def test_group_norm_far_means_cost_no_digits(ops, pixels, c, groups, act):
+    """From the statistics as they were returned, y, dx and the parameters' gradients
+    carry the roundings of the differences from the mean alone, however far it is: a
+    handful a value, and those of sums over a thread's pixels and a tree."""
+    g = _gen(c)
+    x = _randn(g, 2, *pixels, c) + 3e4 * (1 + torch.rand(c, generator=g, device="cuda") // 0.5)
+    per = c // groups
+    x = x.view(2, -1, groups, per)
+    x = (x - x.mean((1, 3), keepdim=True) + 3e4).view(2, *pixels, c)
+    w, b, dy = 1 + 0.3 * _randn(g, c), 0.3 * _randn(g, c), _randn(g, 2, *pixels, c)
+    y, mean, rstd = ops.group_norm(x, groups, w, b, act=act)
+    dx, dw, db = ops.group_norm_grad(dy, x, mean, rstd, groups, w, b, act=act)
+    v = x.to(D64).view(2, -1, groups, per)
+    m, r = (t.to(D64).view(2, 1, groups, 1) for t in (mean, rstd))
+    w64, b64 = w.to(D64).view(groups, per), b.to(D64).view(groups, per)
+    xh = (v - m) * r
+    z = xh * w64 + b64
+    near = 4 * EPS * ((xh * w64).abs() + z.abs())
+    want = z if act == "none" else z.clamp(min=0)
+    assert ((y.to(D64).view(v.shape) - want).abs() <= near).all()
+    dz = dy.to(D64).view(v.shape) * (1.0 if act == "none" else (z > 0))
+    assert act == "none" or not (z.abs() <= near).any()  # no slope is in doubt
+    steps = 96 * EPS
+    t = dz * w64
+    m1, m2 = t.mean((1, 3), keepdim=True), (t * xh).mean((1, 3), keepdim=True)
+    a1, a2 = t.abs().mean((1, 3), keepdim=True), (t * xh).abs().mean((1, 3), keepdim=True)
+    off = (dx.to(D64).view(v.shape) - r * (t - m1 - xh * m2)).abs()
+    assert (off <= steps * r * (t.abs() + a1 + xh.abs() * a2)).all()
+    for got, terms in ((dw, dz * xh), (db, dz)):
+        off = (got.to(D64).view(groups, per) - terms.sum((0, 1))).abs()
+        assert (off <= steps * terms.abs().sum((0, 1))).all()
