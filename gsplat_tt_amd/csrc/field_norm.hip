@@ -65,14 +65,16 @@ __device__ __forceinline__ float act_slope(float z) {
 }
 
 // Count, mean and sum of squared distances from the mean. Pieces are joined by
-// their means' difference, so that a mean far from 0 costs no digits.
+// their means' difference, so that a mean far from 0 costs no digits. An empty piece
+// (count and mean 0) joins as nothing: the other's mean stays as it is, and the square of
+// the difference, infinite for means past 1.8e19, is not formed before its factor 0.
 struct Moments {
     float n, mean, m2;
 };
 __device__ __forceinline__ Moments join(const Moments& a, const Moments& b) {
     const float n = a.n + b.n, d = b.mean - a.mean;
-    const float f = n > 0.0f ? b.n * __builtin_amdgcn_rcpf(n) : 0.0f;
-    return {n, fmaf(d, f, a.mean), a.m2 + fmaf(d * d, a.n * f, b.m2)};
+    const float f = a.n > 0.0f ? b.n * __builtin_amdgcn_rcpf(n) : 1.0f;
+    return {n, fmaf(d, f, a.mean), a.m2 + fmaf(d * (a.n * f), d, b.m2)};
 }
 
 // A wave's and then the workgroup's sum, the same order every time.
@@ -140,7 +142,8 @@ constexpr int kAhead = 4;
 // ---------------------------------------------------------------- statistics
 // Partials (batch, chunks, channels) of a chunk's mean and squared distances.
 // Four pixels at a time get a mean of their own, then their distances from it:
-// 3 operations a value, against 10 for a running mean. Bound by x's bytes: 921600 x 64
+// 3 operations a value, against 10 for a running mean; their sum in pairs, which for four
+// equal values is exact. Bound by x's bytes: 921600 x 64
 // bf16 (118 MB) 23 us, 5.2 TB/s.
 template <typename T, int VEC>
 __global__ __launch_bounds__(kThreads) void k_norm_stats(NormArgs a, int chunks, float2* part) {
@@ -160,15 +163,14 @@ __global__ __launch_bounds__(kThreads) void k_norm_stats(NormArgs a, int chunks,
             n = total;
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                float s = 0.0f, d2 = 0.0f;
-#pragma unroll
-                for (int k = 0; k < kAhead; ++k) s += v[k][j];
-                s *= 1.0f / kAhead;
+                static_assert(kAhead == 4, "two pairs");
+                const float s = ((v[0][j] + v[1][j]) + (v[2][j] + v[3][j])) * 0.25f;
+                float d2 = 0.0f;
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k) d2 = fmaf(v[k][j] - s, v[k][j] - s, d2);
                 const float d = s - mean[j];
                 mean[j] = fmaf(d, f, mean[j]);
-                m2[j] += fmaf(d * d, nf, d2);
+                m2[j] += fmaf(d * nf, d, d2);
             }
         }
         for (; q < p.p1; q += p.slots) {

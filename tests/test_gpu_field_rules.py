@@ -150,3 +150,16 @@ def test_group_norm_far_means_cost_no_digits(ops, pixels, c, groups, act):
     for got, terms in ((dw, dz * xh), (db, dz)):
         off = (got.to(D64).view(groups, per) - terms.sum((0, 1))).abs()
         assert (off <= steps * terms.abs().sum((0, 1))).all()
+
+
+@pytest.mark.parametrize("pixels,c,groups", [((9, 11), 16, 4), ((200, 111), 64, 2), ((70, 61), 6, 2)])
+@pytest.mark.parametrize("value", [1000.0, -77.7, 2e19])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_group_norm_of_constant_groups(ops, pixels, c, groups, value, dtype):
+    """A constant image has its value as the mean, variance 0, and the bias as output."""
+    x = torch.full((2, *pixels, c), value, dtype=dtype, device="cuda")
+    b = _randn(_gen(4), c)
+    y, mean, rstd = ops.group_norm(x, groups, None, b)
+    assert (mean == x.flatten()[0].float()).all()
+    assert ((rstd.to(D64) - 1e-5 ** -0.5).abs() <= 8 * EPS * 1e-5 ** -0.5).all()
+    assert torch.equal(y, b.to(dtype).expand(x.shape))
