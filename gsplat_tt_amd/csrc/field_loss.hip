@@ -886,6 +886,21 @@ __global__ __launch_bounds__(kThreads, one_a_unit(KS, ROLE) ? 1 : 2) void k_stre
 #pragma unroll
         for (int j = 0; j < KJ; ++j) load_parts<T, NP>(row, a.dim, 16 * j + 8 * h, on, q[b][j]);
     }
+    // kGradTable: whether a table row of the wave's holds infinities or NaN (its last part
+    // does then), whose products with masked samples, zeros, are NaN
+    bool odd = false;
+    if (ROLE == kGradTable) {
+#pragma unroll
+        for (int b = 0; b < QB; ++b)
+#pragma unroll
+            for (int j = 0; j < KJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t w = q[b][j][NP - 1][e];
+                    odd |= (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
+                }
+        odd = __any(odd);
+    }
 
     f32x16 acc[QB][ROLE == kScores ? 1 : DB];
     float m[QB], sum[QB], own[QB];
@@ -1058,6 +1073,14 @@ __global__ __launch_bounds__(kThreads, one_a_unit(KS, ROLE) ? 1 : 2) void k_stre
                         }
 #pragma unroll
                         for (int e = 0; e < 4; ++e) v[g4 * 4 + e] *= w[e];
+                        if (odd) {  // masked samples and padding have no gradient
+                            const int4 y4 = *reinterpret_cast<const int4*>(
+                                f + 2 * TS * 32 + g4 * 8 + 4 * h);
+                            const int yy[4] = {y4.x, y4.y, y4.z, y4.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                v[g4 * 4 + e] = yy[e] < 0 ? 0.0f : v[g4 * 4 + e];
+                        }
                     }
                 }
                 split8<NP>(v, g[b][0]);

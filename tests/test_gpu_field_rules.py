@@ -163,3 +163,16 @@ def test_group_norm_of_constant_groups(ops, pixels, c, groups, value, dtype):
     assert (mean == x.flatten()[0].float()).all()
     assert ((rstd.to(D64) - 1e-5 ** -0.5).abs() <= 8 * EPS * 1e-5 ** -0.5).all()
     assert torch.equal(y, b.to(dtype).expand(x.shape))
+
+
+# ------------------------------------------------------------------ values that are not finite
+@pytest.mark.parametrize("n,dim", [(37, 16), (64, 16), (200, 100), (37, 200)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_label_loss_of_masked_samples_against_any_table(ops, n, dim, dtype):
+    """With no label no table value reaches a result, beside padding too."""
+    g = _gen(n * dim)
+    feat, table = _randn(g, n, dim, dtype=dtype), _randn(g, 50, dim, dtype=dtype)
+    table[3, 0], table[9, 1], table[11] = math.nan, math.inf, -math.inf
+    none = torch.full((n,), -1, device="cuda")
+    for got in ops.label_loss_grad(feat, table, none, scale=2.0):
+        assert not got.any()
