@@ -7,8 +7,8 @@
 //   dfeat = G table;  dtable = G^T feat
 //
 // All products run on the matrix cores with bf16 operands and fp32 sums. fp32
-// inputs are cut into three bf16 parts of 8 bits each (exact: 24 bits) and the
-// six products whose weight is above 2^-24 are added up, which keeps fp32's
+// inputs are cut into three bf16 parts of 8 bits each (exact: 24 bits; for infinite
+// values see split8_input) and the six products whose weight is above 2^-24 are added up, which keeps fp32's
 // precision at 6/16 of the cost of the fp32 matrix instructions. Bf16 inputs are
 // the operands as they are; their G is rounded to bf16, as their gradients are in
 // the end.
@@ -46,7 +46,7 @@ constexpr float kLowest = -3.402823466e38f;
 __device__ __forceinline__ float cut_bf16(float v) {
     return __uint_as_float(__float_as_uint(v) & 0xFFFF0000u);
 }
-// An input is made canonical first: one that is not finite has parts that are not.
+// A NaN is made canonical first, so that its parts are NaN.
 template <int NP>
 __device__ __forceinline__ float plain_input(float v) {
     if (NP > 1 && v != v) return __uint_as_float(0x7FC00000u);
@@ -77,6 +77,30 @@ __device__ __forceinline__ void split8(const float* v, quad* out) {
     for (int k = 0; k < 4; ++k) split2<NP>(v[2 * k], v[2 * k + 1], w[k]);
 #pragma unroll
     for (int p = 0; p < NP; ++p) out[p] = quad{w[0][p], w[1][p], w[2][p], w[3][p]};
+}
+// The same of inputs. An infinite value has the parts (1, 0, inf) with its sign: its last
+// part meets the other value's first part alone, which is 0 only where that value is, so
+// the product is what arithmetic gives, also of two infinite values.
+template <int NP>
+__device__ __forceinline__ void split8_input(const float* v, quad* out) {
+    if constexpr (NP == 1) {
+        split8<NP>(v, out);
+    } else {
+        float u[8];
+        bool any = false;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const bool inf = fabsf(v[k]) == INFINITY;
+            u[k] = inf ? copysignf(1.0f, v[k]) : v[k];
+            any |= inf;
+        }
+        split8<NP>(u, out);
+        if (!any) return;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (fabsf(v[k]) == INFINITY)
+                out[NP - 1][k / 2] |= (__float_as_uint(v[k]) >> 16) << (k & 1) * 16;
+    }
 }
 // The products of parts: (0,0) for one part; for three, all with p + q <= 2.
 template <int NP>
@@ -117,7 +141,7 @@ __device__ __forceinline__ void load_parts(const T* row, int dim, int c, bool on
         for (int e = 0; e < 8; ++e)
             v[e] = on && c + e < dim ? plain_input<NP>(to_float(row[c + e])) : 0.0f;
     }
-    split8<NP>(v, out);
+    split8_input<NP>(v, out);
 }
 
 // Parts of the samples as (nr, ld) and of the table as (vp, ld), zeros in the padding
@@ -832,7 +856,7 @@ __global__ __launch_bounds__(kThreads) void k_operands(const T* src, int64_t row
                 }
             }
             quad piece[NP];
-            split8<NP>(v, piece);
+            split8_input<NP>(v, piece);
 #pragma unroll
             for (int p = 0; p < NP; ++p) {
                 const size_t at =

@@ -498,8 +498,9 @@ int gs_group_norm_grad_dev(gs_ctx* ctx, const gs_group_norm* norm, const void* d
  * l_iv = scale <feat_i, table_v>, lse_i = log sum_v exp(l_iv), loss_i = lse_i -
  * l_i,label(i); 0 and 0 for a masked label. feat (n, dim) and table (rows, dim)
  * of one dtype, dim at most 65536, rows 1 .. 2^22, n at most 2^31 - 256. The
- * scores are made in pieces and never kept. loss and lse (n) fp32, each may be
- * NULL. */
+ * scores are made in pieces and never kept; infinite values and NaN in rows that
+ * are not masked act as in plain arithmetic (a row of score -inf drops out). loss
+ * and lse (n) fp32, each may be NULL. */
 typedef struct gs_label_loss {
     const void* feat;
     const void* table;

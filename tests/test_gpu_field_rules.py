@@ -176,3 +176,90 @@ def test_label_loss_of_masked_samples_against_any_table(ops, n, dim, dtype):
     none = torch.full((n,), -1, device="cuda")
     for got in ops.label_loss_grad(feat, table, none, scale=2.0):
         assert not got.any()
+
+
+@pytest.mark.parametrize("n,dim", [(37, 16), (64, 16), (200, 100), (37, 200)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_label_loss_row_of_score_minus_infinity_has_no_gradient(ops, n, dim, dtype):
+    """One labelled sample among masked ones, whose score of one row is -inf."""
+    g = _gen(n * dim)
+    feat, none = _randn(g, n, dim, dtype=dtype), torch.full((n,), -1, device="cuda")
+    table = _randn(g, 50, dim, dtype=dtype)
+    table[11, 0] = -math.inf
+    feat[7] = feat[7].abs() + 0.5
+    none[7] = 4
+    dtable = ops.label_loss_grad(feat, table, none, scale=2.0)[3]
+    assert torch.isfinite(dtable).all() and not dtable[11].any() and dtable[4].any()
+
+
+def _same(got, want, tol):
+    """Equal where not finite, within tol elsewhere."""
+    got, fine = got.to(D64), torch.isfinite(want)
+    assert torch.equal(torch.isfinite(got), fine)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    there = ~fine & ~torch.isnan(want)
+    assert torch.equal(got[there], want[there])
+    assert ((got - want).abs() <= tol)[fine].all()
+
+
+def _loss64(feat, table, labels, scale):
+    f, t = feat.to(D64), table.to(D64)
+    on, y = labels >= 0, labels.clamp(min=0)[:, None]
+    f = torch.where(on[:, None], f, 0.0)  # masked samples hold anything
+    s = scale * (f @ t.T)
+    log = torch.logsumexp(s, 1)
+    loss = torch.where(on, log - s.gather(1, y)[:, 0], 0.0)
+    p = torch.exp(s - log[:, None])
+    d = torch.where(on[:, None], p.scatter_add(1, y, torch.full_like(s[:, :1], -1.0)) * scale, 0.0)
+    return loss, torch.where(on, log, 0.0), d, s
+
+
+@pytest.mark.parametrize("n,rows,dim", [(5, 40, 16), (101, 70, 16), (77, 300, 48), (300, 40, 100),
+                                        (45, 200, 130), (200, 140, 300)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_label_loss_of_infinite_values(ops, n, rows, dim, dtype):
+    """Infinite table values and features give the scores that arithmetic gives: a row
+    of score -inf drops out, +inf and NaN show."""
+    g = _gen(n + dim)
+    feat, table = _randn(g, n, dim).abs().to(dtype) + 0.25, _randn(g, rows, dim, dtype=dtype)
+    labels = torch.randint(-1, rows, (n,), generator=g, device="cuda")
+    labels[0] = -1  # masked
+    labels[1:3] = 0
+    labels = torch.where(labels == 5, 6, labels)
+    scale = 0.5
+    table[5, dim // 2] = -math.inf
+    table[5, 1] = -math.inf
+    loss, log, d, s = _loss64(feat, table, labels, scale)
+    assert torch.isfinite(loss).all() and (s[labels >= 0, 5] == -math.inf).all()
+    finite = torch.where(torch.isfinite(s), s, 0.0).abs()
+    size = scale * (feat.to(D64).abs() @ torch.where(torch.isinf(table), 0, table).to(D64).abs().T)
+    near = ((dim + 32) * EPS * size.amax(1) + 32 * EPS * (1 + finite.amax(1)))
+    a = ops.label_loss(feat, table, labels, scale=scale)
+    b = ops.label_loss_grad(feat, table, labels, scale=scale)
+    for got in (a, b):
+        _same(got[0], loss, 2 * near)
+        _same(got[1], log, 2 * near)
+    # gradients: the dropped row gets none; dfeat is not a number in the infinite columns
+    part = BF if dtype == BF16 else 2.0 ** -22
+    f = torch.where((labels >= 0)[:, None], feat, 0).to(D64)
+    t = torch.where(torch.isinf(table), 0, table).to(D64)
+    e = part + 2 * near[:, None] + (n + rows + 32) * EPS
+    tol = ((d.abs() * e + e * torch.exp(s - log[:, None]).nan_to_num(0.0) * scale))
+    _same(b[3], d.T @ f, tol.T @ f + BF * (d.T @ f).abs() * (dtype == BF16) + 1e-30)
+    want = d @ t
+    want[:, [1, dim // 2]] = math.nan
+    want[labels < 0] = 0.0
+    _same(b[2], want, tol @ t.abs() + BF * want.abs().nan_to_num(0.0) * (dtype == BF16) + 1e-30)
+    # features: +inf and -inf scores of one sample, and both infinite
+    feat[2, 3], feat[1, 1], feat[0, 0] = math.inf, math.inf, math.nan
+    table[:, 3] = table[:, 3].abs() + 0.25
+    table[[0, 5, 7], 3] = -1.0
+    loss, log, d, s = _loss64(feat, table, labels, scale)
+    assert torch.isinf(log[2]) and (s[2] == -math.inf).any() and torch.isinf(loss[2])
+    finite = torch.where(torch.isfinite(s), s, 0.0).abs()
+    size = scale * (torch.where(torch.isfinite(feat), feat, 0).to(D64).abs() @ t.abs().T)
+    near = ((dim + 32) * EPS * (size.amax(1) + 1) + 32 * EPS * (1 + finite.amax(1)))
+    for got in (ops.label_loss(feat, table, labels, scale=scale),
+                ops.label_loss_grad(feat, table, labels, scale=scale)):
+        _same(got[0], loss, 2 * near)
+        _same(got[1], log, 2 * near)
