@@ -263,3 +263,25 @@ def test_label_loss_of_infinite_values(ops, n, rows, dim, dtype):
                 ops.label_loss_grad(feat, table, labels, scale=scale)):
         _same(got[0], loss, 2 * near)
         _same(got[1], log, 2 * near)
+
+
+@pytest.mark.parametrize("pixels", [1, 3000])
+def test_gelu_keeps_its_digits(ops, pixels):
+    """gelu and its slope over the line, in one launch and in three. z comes from the
+    bias alone (x is constant). Phi(-|z|) = exp(-z^2 / 2) R: the exponent's rounding
+    moves the exponential by z^2 EPS, exponential, quotient, polynomial and products
+    take 16 EPS, and the polynomial's own error 4 EPS."""
+    c = 4096
+    z = torch.linspace(-9.0, 9.0, c, device="cuda")
+    x, dy = torch.zeros(1, pixels, c, device="cuda"), torch.zeros(1, pixels, c, device="cuda")
+    dy[:, 0] = 1.0
+    y, mean, rstd = ops.group_norm(x, 1, None, z, act="gelu")
+    _, _, db = ops.group_norm_grad(dy, x, mean, rstd, 1, None, z, act="gelu")
+    z = z.to(D64)
+    phi = 0.5 * torch.erfc(-z / math.sqrt(2))
+    tail = 0.5 * torch.erfc(z.abs() / math.sqrt(2))
+    off = (20 + z * z) * EPS * tail + 2 * EPS * phi  # of Phi
+    assert ((y.to(D64)[0, 0] - z * phi).abs() <= z.abs() * off + EPS * (z * phi).abs()).all()
+    bell = z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+    assert ((db.to(D64) - (phi + bell)).abs() <= off + (8 + z * z) * EPS * bell.abs() +
+            2 * EPS * (phi + bell).abs()).all()
