@@ -416,7 +416,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_grad_finish(NormArgs a, int c
     }
 }
 
-// dweight and dbias of channel c: its sums over the images.
+// dweight and dbias of channel c: its sums over a few images.
 __device__ __forceinline__ void grad_params(const NormArgs& a, const float2* sums, int c) {
     if (c >= a.channels) return;
     float db = 0.0f, dw = 0.0f;
@@ -428,8 +428,62 @@ __device__ __forceinline__ void grad_params(const NormArgs& a, const float2* sum
     if (a.dbias != nullptr) a.dbias[c] = db;
     if (a.dweight != nullptr) a.dweight[c] = dw;
 }
-__global__ __launch_bounds__(kThreads) void k_norm_grad_params(NormArgs a, const float2* sums) {
-    grad_params(a, sums, blockIdx.x * kThreads + threadIdx.x);
+// The same of many: a share of the images a workgroup, whose slots take 8 at a time; sums
+// in a tree, so that their error does not grow with the images. Into out (shares,
+// channels) for a second such launch, or (null) to the gradients.
+__global__ __launch_bounds__(kThreads) void k_norm_grad_params(NormArgs a, const float2* sums,
+                                                               int64_t images, int64_t share,
+                                                               float2* out) {
+    __shared__ float2 lds[kThreads];
+    constexpr int U = 8;
+    const int c0 = blockIdx.y * kThreads, cols = min(kThreads, a.channels - c0);
+    const int slots = kThreads / cols, slot = threadIdx.x / cols;
+    const int c = c0 + (int)threadIdx.x % cols;
+    const int64_t b0 = blockIdx.x * share, b1 = min(images, b0 + share);
+    float s1[1] = {0.0f}, s2[1] = {0.0f};
+    if (slot < slots)
+        for (int64_t b = b0 + slot; b < b1; b += U * slots) {
+            float2 v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                v[u] = b + u * slots < b1 ? sums[(b + u * slots) * a.channels + c]
+                                          : make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int o = U / 2; o > 0; o /= 2)
+#pragma unroll
+                for (int u = 0; u < o; ++u) {
+                    v[u].x += v[u + o].x;
+                    v[u].y += v[u + o].y;
+                }
+            s1[0] += v[0].x;
+            s2[0] += v[0].y;
+        }
+    slots_sum<1, kThreads>(lds, threadIdx.x, slot, slots, cols, s1, s2);
+    if (slot != 0) return;
+    if (out != nullptr) {
+        out[(int64_t)blockIdx.x * a.channels + c] = make_float2(s1[0], s2[0]);
+        return;
+    }
+    if (a.dbias != nullptr) a.dbias[c] = s1[0];
+    if (a.dweight != nullptr) a.dweight[c] = s2[0];
+}
+// One launch for some hundred images; two, with 32 images a share or 1024 shares, past
+// that. `part` holds (1024, channels). The gradient of 100000 images of one pixel and 512
+// channels takes 5.2 ms, 44.5 with one thread a channel.
+hipError_t launch_grad_params(const NormArgs& a, const float2* sums, int64_t images, float2* part,
+                              hipStream_t st) {
+    const unsigned cols = (unsigned)((a.channels + kThreads - 1) / kThreads);
+    if (images > 256) {
+        const int64_t share = (images + 1023) / 1024 > 32 ? (images + 1023) / 1024 : 32;
+        const int64_t shares = (images + share - 1) / share;
+        k_norm_grad_params<<<dim3((unsigned)shares, cols), kThreads, 0, st>>>(a, sums, images,
+                                                                              share, part);
+        GS_LAUNCHED();
+        sums = part;
+        images = shares;
+    }
+    k_norm_grad_params<<<dim3(1, cols), kThreads, 0, st>>>(a, sums, images, images, nullptr);
+    return hipGetLastError();
 }
 
 // dx = rstd w dz - rstd m1 - xh rstd m2. Bound as the sums are: 333666 x 48 fp32 relu
@@ -646,8 +700,8 @@ int chunks_of(int64_t batch, int64_t pixels) {
     return k < 1 ? 1 : (int)k;
 }
 
-// Images whose sums k_norm_grad_apply adds in passing; of more k_norm_grad_params does,
-// a launch of its own (2 images of 166833 x 48: 106 against 104 us for both passes, 8 of
+// Images whose sums k_norm_grad_apply adds in passing; of more launch_grad_params does,
+// with launches of its own (2 images of 166833 x 48: 106 against 104 us for both passes, 8 of
 // 76800 x 128 257 against 254).
 constexpr int64_t kFewImages = 16;
 
@@ -684,9 +738,7 @@ hipError_t norm_run(const NormArgs& a, bool grad, hipStream_t st) {
         } else {
             k_norm_small_grad<T, VEC, ACT><<<small, kSmallThreads, 0, st>>>(a, w.sums);
             GS_LAUNCHED();
-            if (a.batch > 1)
-                k_norm_grad_params<<<(unsigned)((a.channels + kThreads - 1) / kThreads), kThreads,
-                                     0, st>>>(a, w.sums);
+            if (a.batch > 1) return launch_grad_params(a, w.sums, a.batch, w.part, st);
         }
         return hipGetLastError();
     }
@@ -703,10 +755,10 @@ hipError_t norm_run(const NormArgs& a, bool grad, hipStream_t st) {
         GS_LAUNCHED();
         k_norm_grad_finish<<<groups, kThreads, 0, st>>>(a, chunks, w.part, w.sums, w.means);
         GS_LAUNCHED();
-        if (a.batch > kFewImages)
-            k_norm_grad_params<<<(unsigned)((a.channels + kThreads - 1) / kThreads), kThreads, 0,
-                                 st>>>(a, w.sums);
-        GS_LAUNCHED();
+        if (a.batch > kFewImages) {
+            const hipError_t e = launch_grad_params(a, w.sums, a.batch, w.part, st);
+            if (e != hipSuccess) return e;
+        }
         k_norm_grad_apply<T, VEC, ACT><<<grid, kThreads, 0, st>>>(
             a, chunks, w.means, a.batch > kFewImages ? nullptr : w.sums);
     }
@@ -750,11 +802,8 @@ hipError_t launch_group_norm(const NormArgs& a, hipStream_t st) {
 
 hipError_t launch_group_norm_grad(const NormArgs& a, hipStream_t st) {
     if (a.batch == 0 || a.pixels == 0) {
-        NormArgs e = a;  // no pixels: the parameters' gradients are 0
-        e.batch = 0;
-        k_norm_grad_params<<<(unsigned)((a.channels + kThreads - 1) / kThreads), kThreads, 0, st>>>(
-            e, nullptr);
-        return hipGetLastError();
+        // no pixels: the parameters' gradients are 0
+        return launch_grad_params(a, nullptr, 0, nullptr, st);
     }
     return a.dtype == 0 ? norm_typed<float>(a, true, st) : norm_typed<bf16>(a, true, st);
 }

@@ -285,3 +285,22 @@ def test_gelu_keeps_its_digits(ops, pixels):
     bell = z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
     assert ((db.to(D64) - (phi + bell)).abs() <= off + (8 + z * z) * EPS * bell.abs() +
             2 * EPS * (phi + bell).abs()).all()
+
+
+@pytest.mark.parametrize("batch,pixels,c", [(65_000, 4, 16), (1 << 18, 1, 64), (70_001, 3, 5),
+                                            (3000, 40, 300)])
+def test_group_norm_grad_of_long_batches(ops, batch, pixels, c):
+    """The parameters' gradients of many images: sums in a tree, whose error grows by a
+    rounding a level and not by one an image. A constant gradient rounds the same way at
+    every step of a long chain."""
+    g = _gen(batch)
+    x = _randn(g, batch, pixels, c)
+    dy = torch.full_like(x, 1.1)
+    y, mean, rstd = ops.group_norm(x, 1)
+    _, dw, db = ops.group_norm_grad(dy, x, mean, rstd, 1)
+    d = float(dy.flatten()[0])
+    steps = 64 * EPS  # 40 in a row and 24 joined at most
+    total = batch * pixels * d
+    assert ((db.to(D64) - total).abs() <= steps * total).all()
+    xh = (x.to(D64) - mean.to(D64)[:, :, None]) * rstd.to(D64)[:, :, None]
+    assert ((dw.to(D64) - (xh * d).sum((0, 1))).abs() <= steps * (xh.abs() * d).sum((0, 1))).all()
