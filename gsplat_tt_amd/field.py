@@ -13,7 +13,9 @@ label_loss / label_loss_grad  softmax cross entropy of features against a table
 The reference has no counterpart. Work is enqueued on torch's current stream of
 the context's device and nothing waits; outputs and workspaces come from torch's
 allocator on that stream. A tensor made on another stream must be ordered before
-the call by the caller, as for any torch operation. There is no CPU fallback.
+the call by the caller, as for any torch operation. The operators are not part of
+torch's graph: in grad mode a tensor that requires a gradient is refused, and the
+gradients are calls of their own. There is no CPU fallback.
 """
 from __future__ import annotations
 
@@ -45,6 +47,12 @@ def _rows(t, name, dim=None):
     return t.data_ptr(), rows, t.stride(0)
 
 
+def _written(out):
+    """Counts a given output as changed in place, for graphs that have saved it."""
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+
+
 class FieldOps:
     """The feature operators on one GPU: `ctx` (a Context) or a new one on `device`.
 
@@ -65,6 +73,9 @@ class FieldOps:
     # ---- checks
     def _own(self, t, name, dtypes=_DTYPES):
         if isinstance(t, torch.Tensor) and t.get_device() == self._index and t.dtype in dtypes:
+            if t.requires_grad and torch.is_grad_enabled():
+                raise ValueError(f"{name} requires a gradient, which these operators do not "
+                                 "record: detach() it or call under torch.no_grad()")
             return t
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a torch tensor")
@@ -93,6 +104,7 @@ class FieldOps:
         self._own(out, name)
         if out.shape != torch.Size(shape):
             raise ValueError(f"{name} must be {tuple(shape)}, not {tuple(out.shape)}")
+        _written(out)
         return out
 
     def _workspace(self, name, *sizes):
@@ -199,9 +211,12 @@ class FieldOps:
         are fp32."""
         px, bx, sx = self._image(x, "x")
         d, keep = self._norm(x, groups, weight, bias, act, eps)
+        given = out
         if out is None:
             out = torch.empty_like(x, memory_format=torch.contiguous_format)
         py, by, sy = self._image(out, "out", x.shape, x.dtype)
+        if given is not None:
+            _written(out)
         stats = torch.zeros if d.pixels == 0 else torch.empty
         mean, rstd = stats((2, d.batch, d.groups), dtype=torch.float32, device=self.device)
         ws, size = self._workspace("gs_group_norm_workspace", d.batch, d.pixels, d.channels)
@@ -218,9 +233,12 @@ class FieldOps:
         px, bx, sx = self._image(x, "x")
         pd, bd, sd = self._image(dy, "dy", x.shape, x.dtype)
         d, keep = self._norm(x, groups, weight, bias, act, eps)
+        given = out
         if out is None:
             out = torch.empty_like(x, memory_format=torch.contiguous_format)
         po, bo, so = self._image(out, "out", x.shape, x.dtype)
+        if given is not None:
+            _written(out)
         stats = (d.batch, d.groups)
         for t, name in ((mean, "mean"), (rstd, "rstd")):
             self._own(t, name, _PARAM_TYPES)

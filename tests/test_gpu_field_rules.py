@@ -304,3 +304,34 @@ def test_group_norm_grad_of_long_batches(ops, batch, pixels, c):
     assert ((db.to(D64) - total).abs() <= steps * total).all()
     xh = (x.to(D64) - mean.to(D64)[:, :, None]) * rstd.to(D64)[:, :, None]
     assert ((dw.to(D64) - (xh * d).sum((0, 1))).abs() <= steps * (xh.abs() * d).sum((0, 1))).all()
+
+
+def test_inputs_that_record_a_gradient_are_refused(ops):
+    """The operators are not part of torch's graph: in grad mode a tensor that requires a
+    gradient is an error, not a constant. Given outputs count as written in place."""
+    table = torch.randn(6, 4, device="cuda", requires_grad=True)
+    ids = torch.zeros(3, dtype=torch.int64, device="cuda")
+    x = torch.randn(1, 6, 4, device="cuda")
+    w = torch.ones(4, device="cuda", requires_grad=True)
+    y, mean, rstd = ops.group_norm(x, 2)
+    for call in (lambda: ops.lookup(table, ids),
+                 lambda: ops.lookup(table.detach(), ids, out=table[:3]),
+                 lambda: ops.lookup_grad(table[:3], ids, 4),
+                 lambda: ops.group_norm(x, 2, w),
+                 lambda: ops.group_norm(x, 2, None, w),
+                 lambda: ops.group_norm_grad(y, x, mean, rstd, 2, w),
+                 lambda: ops.label_loss(table[:3], table.detach(), ids),
+                 lambda: ops.label_loss_grad(table[:3].detach(), table, ids)):
+        with pytest.raises(ValueError, match="requires a gradient"):
+            call()
+    with torch.no_grad():
+        a = ops.lookup(table, ids)
+    assert torch.equal(a, ops.lookup(table.detach(), ids)) and torch.equal(a, table.detach()[ids])
+    out = torch.zeros(3, 4, device="cuda")
+    for call in (lambda: ops.lookup(table.detach(), ids, out=out),
+                 lambda: ops.lookup_grad(a, ids, 3, out=out),
+                 lambda: ops.group_norm(out.view(1, 3, 4), 2, out=out.view(1, 3, 4)),
+                 lambda: ops.label_loss_grad(a, table.detach(), ids, dfeat=out)):
+        before = out._version
+        call()
+        assert out._version > before
