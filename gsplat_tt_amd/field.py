@@ -123,11 +123,14 @@ class FieldOps:
         return torch.cuda.current_stream(self._index).cuda_stream
 
     def check(self):
-        """Waits for the current stream and raises ValueError when a call since the
-        last check was given an id or label at or past its table's rows."""
+        """Waits for the GPU, whatever streams the calls were made on, and raises
+        ValueError when one since the last check was given an id or label at or past
+        its table's rows."""
+        torch.cuda.synchronize(self.device)
         flags = int(self._flags.item())
         if flags:
             self._flags.zero_()
+            torch.cuda.current_stream(self.device).synchronize()
         if flags & FLAG_ID_RANGE:
             raise ValueError("an id or a label is at or past the table's rows")
 

@@ -335,3 +335,19 @@ def test_inputs_that_record_a_gradient_are_refused(ops):
         before = out._version
         call()
         assert out._version > before
+
+
+def test_check_waits_for_every_stream(ops):
+    """A report of a call that still waits on another stream is not missed."""
+    table = torch.ones(4, 5, device="cuda")
+    ids = torch.tensor([0, 9], device="cuda")
+    ops.lookup(table, ids[:1])
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)  # a tenth of a second or so
+        ops.lookup(table, ids)
+    with pytest.raises(ValueError, match="past"):
+        ops.check()
+    ops.check()
