@@ -844,6 +844,13 @@ hipError_t sort_ids(const LookupGradArgs& a, const GradWs& w, const uint2** sort
     return hipSuccess;
 }
 
+// Of a table without rows nothing is summed, but every id is past it.
+__global__ __launch_bounds__(kThreads) void k_report_ids(LookupGradArgs a) {
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < a.n;
+         i += (int64_t)gridDim.x * kThreads)
+        load_id(a.ids, a.ids64, i, a.rows, a.flags);
+}
+
 __global__ __launch_bounds__(kThreads) void k_run_clear(uint2* runs, int64_t rows) {
     const int64_t v = (int64_t)blockIdx.x * kThreads + threadIdx.x;
     if (v < rows) runs[v] = make_uint2(0u, 0u);
@@ -864,7 +871,11 @@ size_t lookup_grad_ws(int64_t n, int64_t rows, int dim) {
 }
 
 hipError_t launch_lookup_grad(const LookupGradArgs& a, hipStream_t st) {
-    if (a.rows == 0) return hipSuccess;
+    if (a.rows == 0) {
+        if (a.n == 0 || a.flags == nullptr) return hipSuccess;
+        k_report_ids<<<blocks_of(a.n, kThreads), kThreads, 0, st>>>(a);
+        return hipGetLastError();
+    }
     const GradWs w(a.ws, a.n, a.rows, a.dim);
     const uint2* pairs = nullptr;
     hipError_t e = hipSuccess;

@@ -351,3 +351,15 @@ def test_check_waits_for_every_stream(ops):
     with pytest.raises(ValueError, match="past"):
         ops.check()
     ops.check()
+
+
+def test_lookup_grad_without_rows_reports_ids(ops):
+    """Into a table without rows every id is past it; masked ones are not reported."""
+    dout = torch.ones(700, 5, device="cuda")
+    ids = torch.full((700,), -1, device="cuda")
+    assert ops.lookup_grad(dout, ids, 0).shape == (0, 5)
+    ops.check()
+    ids[-1] = 0
+    ops.lookup_grad(dout, ids.int(), 0)
+    with pytest.raises(ValueError, match="past"):
+        ops.check()
