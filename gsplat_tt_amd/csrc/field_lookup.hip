@@ -168,7 +168,7 @@ __device__ __forceinline__ uint32_t wave_rank(uint32_t digit, bool on, int bits,
     return n + before;
 }
 
-// Also clears the ids' runs, which k_run_sums fills in.
+// Also clears the ids' runs (unless null), which k_run_sums fills in.
 template <int ITEMS>
 __global__ __launch_bounds__(kThreads) void k_sort_count(LookupGradArgs a, const uint2* pairs,
                                                          int shift, int bits, uint32_t* counts,
@@ -821,16 +821,31 @@ hipError_t grad_typed(const LookupGradArgs& a, const GradWs& w, const uint2* pai
     return hipGetLastError();
 }
 
+__global__ __launch_bounds__(kThreads) void k_run_clear(uint2* runs, int64_t rows) {
+    const int64_t v = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (v < rows) runs[v] = make_uint2(0u, 0u);
+}
+
 template <int ITEMS>
 hipError_t sort_ids(const LookupGradArgs& a, const GradWs& w, const uint2** sorted,
                     hipStream_t st) {
     const int bits = key_bits(a.rows), passes = (bits + 7) / 8;
     const unsigned blocks = (unsigned)((a.n + kThreads * ITEMS - 1) / (kThreads * ITEMS));
     const uint2* pairs = nullptr;
+    // The runs are cleared in passing by the first count, whose blocks are the ids'; where
+    // that leaves a thread more than 256 rows, by the whole chip: 5000 ids into 2^27 rows
+    // took 3.31 ms, so 0.69 (into 100000 rows 62 us in passing, 71 with the launch).
+    uint2* in_passing = w.runs;
+    if (a.rows > (int64_t)blocks * kThreads * 256) {
+        k_run_clear<<<(unsigned)((a.rows + kThreads - 1) / kThreads), kThreads, 0, st>>>(w.runs,
+                                                                                      a.rows);
+        GS_LAUNCHED();
+        in_passing = nullptr;
+    }
     for (int p = 0, done = 0; p < passes; ++p) {
         const int b = (bits - done + passes - p - 1) / (passes - p);
         k_sort_count<ITEMS><<<blocks, kThreads, 0, st>>>(a, pairs, done, b, w.counts,
-                                                         p == 0 ? w.runs : nullptr);
+                                                         p == 0 ? in_passing : nullptr);
         GS_LAUNCHED();
         k_sort_scan<<<1u << b, kThreads, 0, st>>>(w.counts, (int)blocks, w.totals);
         GS_LAUNCHED();
@@ -849,11 +864,6 @@ __global__ __launch_bounds__(kThreads) void k_report_ids(LookupGradArgs a) {
     for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < a.n;
          i += (int64_t)gridDim.x * kThreads)
         load_id(a.ids, a.ids64, i, a.rows, a.flags);
-}
-
-__global__ __launch_bounds__(kThreads) void k_run_clear(uint2* runs, int64_t rows) {
-    const int64_t v = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (v < rows) runs[v] = make_uint2(0u, 0u);
 }
 
 }  // namespace

@@ -363,3 +363,31 @@ def test_lookup_grad_without_rows_reports_ids(ops):
     ops.lookup_grad(dout, ids.int(), 0)
     with pytest.raises(ValueError, match="past"):
         ops.check()
+
+
+def test_lookup_grad_of_few_ids_into_a_large_table(ops):
+    """Clearing what belongs to the table's rows is the whole chip's work: it costs about
+    as much as filling the table, not one workgroup's time."""
+    n, rows = 5000, (1 << 27) + 1
+    g = _gen(5)
+    ids = torch.randint(0, rows, (n,), generator=g, device="cuda")
+    dout, out = _randn(g, n, 2), torch.empty(rows, 2, device="cuda")
+
+    def best(call):
+        times = []
+        for _ in range(4):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            call()
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    took = best(lambda: ops.lookup_grad(dout, ids, rows, out=out))
+    assert took <= 10 * best(lambda: out.zero_()) + 1.0
+    ops.lookup_grad(dout, ids, rows, out=out)
+    want = torch.zeros(rows, 2, device="cuda").index_add_(0, ids, dout)
+    assert ((out - want).abs() <= 4 * EPS * want.abs() + 1e-6).all()
+    del out, want
+    torch.cuda.empty_cache()
