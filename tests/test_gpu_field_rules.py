@@ -391,3 +391,42 @@ def test_lookup_grad_of_few_ids_into_a_large_table(ops):
     assert ((out - want).abs() <= 4 * EPS * want.abs() + 1e-6).all()
     del out, want
     torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------ pieces that add up in place
+@pytest.mark.parametrize("n,rows,dim,dtype", [(19_501, 20_000, 768, F32),
+                                              (30_011, 32_003, 512, BF16)])
+def test_label_loss_pieces_add_up_without_slices(ops, n, rows, dim, dtype):
+    """Several pieces whose sums have one share: they go straight onto the earlier
+    pieces' sums, of the table and (fp32) of the samples too."""
+    scale, g = 8.0, _gen(6)
+    out, part = (BF, BF) if dtype == BF16 else (0.0, 2.0 ** -22)
+    table = _randn(g, rows, dim)
+    table /= table.norm(dim=1, keepdim=True)
+    labels = torch.randint(-1, rows, (n,), generator=g, device="cuda")
+    feat = (_randn(g, n, dim) / math.sqrt(dim) + 0.5 * table[labels.clamp(min=0)]).to(dtype)
+    table = table.to(dtype)
+    got = ops.label_loss_grad(feat, table, labels, scale=scale)
+    loss, _, dfeat, dtable = (t.to(D64) for t in got)
+    t = table.to(D64)
+    want_t, tol_t = torch.zeros_like(t), torch.zeros_like(t)
+    for i in range(0, n, 4000):
+        at = slice(i, i + 4000)
+        f, on, y = feat[at].to(D64), labels[at] >= 0, labels[at].clamp(min=0)[:, None]
+        s = scale * f @ t.T
+        log = torch.logsumexp(s, 1)
+        e = ((dim + 8) * EPS * scale * (f.abs() @ t.abs().T) + 4 * EPS * s.abs()).amax(1)
+        e = 2 * (e + 16 * EPS * (1 + log.abs() + s.abs().amax(1)))
+        want = torch.where(on, log - s.gather(1, y)[:, 0], 0.0)
+        assert ((loss[at] - want).abs() <= e).all()
+        p = torch.exp(s - log[:, None])
+        w = torch.where(on, scale, 0.0)[:, None].to(D64)
+        d = p.scatter_add(1, y, torch.full_like(log, -1.0)[:, None]) * w
+        ed = p.scatter_add(1, y, torch.ones_like(log)[:, None])
+        ed = w * (2 * p * e[:, None] + 4 * EPS * ed) + part * d.abs()
+        ref = d @ t
+        tol = (ed + (rows + 8) * EPS * d.abs()) @ t.abs() + out * ref.abs() + 1e-38
+        assert ((dfeat[at] - ref).abs() <= tol).all()
+        want_t += d.T @ f
+        tol_t += (ed + (n + 8) * EPS * d.abs()).T @ f.abs()
+    assert ((dtable - want_t).abs() <= tol_t + out * want_t.abs() + 1e-38).all()
