@@ -86,7 +86,6 @@ struct LossArgs {
     float scale;
     float *loss, *lse;  // (n)
     void* ws;
-    size_t ws_bytes;
     uint32_t* flags;
     // the gradients' own
     const float* row_weight;  // (n) or null (1)

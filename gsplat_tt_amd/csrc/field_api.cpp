@@ -149,7 +149,6 @@ gs::LossArgs loss_args(const gs_label_loss* d, float* loss, float* lse, void* ws
     a.loss = loss;
     a.lse = lse;
     a.ws = ws;
-    a.ws_bytes = (size_t)ws_bytes;
     a.flags = flags;
     return a;
 }
