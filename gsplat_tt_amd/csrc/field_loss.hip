@@ -11,14 +11,17 @@
 // values see split8_input) and the six products whose weight is above 2^-24 are added up, which keeps fp32's
 // precision at 6/16 of the cost of the fp32 matrix instructions. Bf16 inputs are
 // the operands as they are; their G is rounded to bf16, as their gradients are in
-// the end.
+// the end, since parts of G would double the products that it enters: 30011 x 32003 of
+// 512 the gradients are 0.0023 off (2-norm, relative), where rounding them alone gives
+// 0.0017.
 //
 // Three ways, by size:
 //   few        up to 8 samples, losses alone: one read of the table, no layout.
 //   streaming  rows of at most 128: scores and G stay in registers, the other
-//              side streams through LDS (k_stream), 3 products in 2 passes.
+//              side streams through LDS (k_stream), in 2 passes that each make the
+//              scores and one of the gradients.
 //   pieces     longer rows: 128 x 128 tiles, G of one piece at a time in the
-//              workspace, 4 products (the scores are made twice, once for lse).
+//              workspace; the scores are made twice here too, once for lse.
 // All sums are made in an order that depends on the sizes alone.
 #include <algorithm>
 
@@ -265,8 +268,8 @@ struct Side {
 // next loads are started: the compiler cannot tell the halves apart, and would have
 // a read after them wait for all of them.
 //
-// 30011 x 32003 of 512 bf16: scores 1008 TFLOP/s, G 780, dfeat 803, dtable 910. The
-// matrix cores are busy half of the time, LDS a quarter to a half: bound by the wait
+// 30011 x 32003 of 512 bf16: scores 1010 TFLOP/s, G 800, dfeat 810, dtable 930. The
+// matrix cores are busy 37 to 48 % of the time, LDS 18 to 24 %: bound by the wait
 // for the next step's loads, a step's products ahead of their use, and G and its sums
 // by their bytes. Two steps ahead would need LDS reads that the compiler does not hold
 // up for loads in flight. Through registers a step took 5 to 10 % longer. Tiles of 256
@@ -750,9 +753,10 @@ hipError_t fold(const SumOut<T>& o, int nz, hipStream_t st) {
 //
 // Bound by the matrix cores and, in fp32, as much by cutting the exponentials into
 // parts (88 of about 440 vector instructions a tile beside 42 products of 16 cycles).
-// 10007 x 8192 of 48 fp32: losses and dfeat 134 us, dtable 122, at six bf16 products
-// for each one 0.70 and 0.77 PFLOP/s. 307200 x 150 of 32 bf16, losses alone: 18 us, where
-// the 46 million exponentials take 8 at the transcendental rate and the bytes 5.
+// 10007 x 8192 of 48 fp32: losses and dfeat 111 us, dtable 104, at six bf16 products
+// for each one 0.85 and 0.91 PFLOP/s. 307200 x 150 of 32 bf16, losses alone: 17 us, where
+// the 46 million exponentials take 5 at the transcendental rate and the bytes 5; the
+// vector units are busy half of the time.
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 
 constexpr float kSlack = 8.0f;
@@ -1597,9 +1601,9 @@ int stream_ks(int dim) {
 // and nothing is laid out. `lpr` lanes take kFewRows table rows at a time, whose dot
 // products with all samples, held in LDS in fp32, share one read of them; a
 // workgroup's slots keep each sample's largest score and sum, and k_loss_join adds
-// the workgroups up. Bound by the table's bytes (or, below about 1 MB, by the two
-// launches, 15 us with the call): 1 by 100000 of 512 fp32 50 us, 4.1 TB/s; a row at a
-// time 114. 8 by 100000 of 64 fp32 30 us, by streaming 34; one 19 and 37.
+// the workgroups up. Bound by the table's bytes in fp32 (or, below about 1 MB, by the two
+// launches, 15 us with the call): 1 by 100000 of 512 fp32 45 us, 4.6 TB/s; a row at a
+// time 114. Of bf16, half the bytes, 45 too: bound by the sums over lanes. 8 by 100000 of 64 fp32 30 us, by streaming 34; one 19 and 37.
 constexpr int kFew = 8;
 constexpr int kFewValues = 12288;  // samples * dim in LDS: 48 KB
 constexpr int kFewRows = 4;

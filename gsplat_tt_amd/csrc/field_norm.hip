@@ -314,8 +314,9 @@ __device__ __forceinline__ void slots_sum(float2* lds, int at, int slot, int slo
 }
 
 // Partials (batch, chunks, channels) of sum dz and sum dz xh. Bound by the bytes of dy
-// and x, with gelu as much by its arithmetic: 333666 x 48 fp32 relu (128 MB) 23 us, 5.7
-// TB/s; 614400 x 128 bf16 gelu (315 MB) 88 us, 3.6 TB/s.
+// and x, with gelu as much by its arithmetic: 333666 x 48 fp32 relu (128 MB) 22 us, 5.8
+// TB/s; 614400 x 128 bf16 gelu (315 MB) 80 us, 3.9 TB/s, with the vector units busy 72 %
+// of the time.
 template <typename T, int VEC, int ACT>
 __global__ __launch_bounds__(kThreads) void k_norm_grad_sums(NormArgs a, int chunks, float2* part) {
     __shared__ float2 lds[kThreads * VEC];
@@ -487,7 +488,8 @@ hipError_t launch_grad_params(const NormArgs& a, const float2* sums, int64_t ima
 }
 
 // dx = rstd w dz - rstd m1 - xh rstd m2. Bound as the sums are: 333666 x 48 fp32 relu
-// 32 us, 6.1 TB/s read and written; 614400 x 128 bf16 gelu 88 us, 5.4 TB/s.
+// 31 us, 6.1 TB/s read and written; 614400 x 128 bf16 gelu 83 us, 5.7 TB/s, vector units
+// busy 74 %.
 template <int ACT, int VEC>
 __device__ __forceinline__ void grad_of(const Channels<VEC>& ch, const float* rw, const float* m1,
                                         const float* m2, float* v, const float* d) {
