@@ -110,15 +110,14 @@ __device__ __forceinline__ uint32_t block_excl_scan(uint32_t v, uint32_t* lds, u
 }
 
 // Most blocks of a grid that its kernel walks over with: a launch takes fewer than 2^32
-// threads a dimension, 2^24 blocks of 256.
+// threads a dimension, 2^24 blocks of 256 (2^24 were refused, two more ran as two).
 constexpr int64_t kMostBlocks = (int64_t)1 << 22;
 inline unsigned blocks_of(int64_t items, int64_t per_block) {
     const int64_t b = (items + per_block - 1) / per_block;
     return (unsigned)(b < kMostBlocks ? b : kMostBlocks);
 }
 
-// Returns a launch's error: nothing runs on what it would have written. (A later launch
-// that succeeds would hide it.)
+// Returns a launch's error, so that nothing runs on what it would have written.
 #define GS_LAUNCHED()                               \
     do {                                            \
         const hipError_t e_ = hipGetLastError();    \
