@@ -43,6 +43,8 @@ EXPORTED = (
     "gs_stream", "gs_lookup_dev", "gs_lookup_grad_workspace", "gs_lookup_grad_dev",
     "gs_group_norm_workspace", "gs_group_norm_dev", "gs_group_norm_grad_dev",
     "gs_label_loss_workspace", "gs_label_loss_dev", "gs_label_loss_grad_dev",
+    "gs_gated_linear_workspace", "gs_gated_linear_dev", "gs_gated_linear_grad_dev",
+    "gs_grad_norm_workspace", "gs_grad_norm_dev", "gs_grad_clip_dev",
 )
 TRAIN_PARAMS = ("means", "log_scales", "quats", "opacity_logits", "sh")
 
@@ -135,6 +137,20 @@ class GsLabelLoss(ctypes.Structure):
                 ("scale", ctypes.c_float)]
 
 
+class GsGatedLinear(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("w_gate", ctypes.c_void_p), ("w_up", ctypes.c_void_p),
+                ("b_gate", ctypes.c_void_p), ("b_up", ctypes.c_void_p), ("n", ctypes.c_int64),
+                ("hidden", ctypes.c_int64), ("x_stride", ctypes.c_int64),
+                ("gate_stride", ctypes.c_int64), ("up_stride", ctypes.c_int64),
+                ("dim", ctypes.c_int), ("dtype", ctypes.c_int), ("act", ctypes.c_int),
+                ("reserved", ctypes.c_int)]
+
+
+class GsTensor(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64),
+                ("stride", ctypes.c_int64), ("dtype", ctypes.c_int), ("reserved", ctypes.c_int)]
+
+
 def _field_argtypes(L):
     """Argument types of the feature operators (they are called often: typed
     arguments need no wrapping per call)."""
@@ -150,7 +166,16 @@ def _field_argtypes(L):
     L.gs_label_loss_workspace.argtypes = [q, q, i, i, i]
     L.gs_label_loss_dev.argtypes = [p, loss, p, p, p, q, p, p]
     L.gs_label_loss_grad_dev.argtypes = [p, loss, p, p, p, p, q, p, q, p, q, p, p]
-    for name in ("gs_lookup_grad_workspace", "gs_group_norm_workspace", "gs_label_loss_workspace"):
+    gated = ctypes.POINTER(GsGatedLinear)
+    L.gs_gated_linear_workspace.argtypes = [gated, i]
+    L.gs_gated_linear_dev.argtypes = [p, gated, p, q, p, q, p]
+    L.gs_gated_linear_grad_dev.argtypes = [p, gated, p, q, p, q, p, q, p, q, p, p, p, q, p]
+    # lists of GsTensor by their address
+    L.gs_grad_norm_workspace.argtypes = [p, q]
+    L.gs_grad_norm_dev.argtypes = [p, p, q, i, p, p, q, p]
+    L.gs_grad_clip_dev.argtypes = [p, p, p, q, p, ctypes.c_double, p]
+    for name in ("gs_lookup_grad_workspace", "gs_group_norm_workspace", "gs_label_loss_workspace",
+                 "gs_gated_linear_workspace", "gs_grad_norm_workspace"):
         getattr(L, name).restype = q
 
 

@@ -1,4 +1,5 @@
-// field.h - the feature operators (lookup, group norm, label loss): arguments
+// field.h - the feature operators (lookup, group norm, label loss, gated projections,
+// gradient norm and clipping): arguments
 // shared by the entry points (field_api.cpp) and the kernels, and the launchers.
 // Every launcher only enqueues kernels on the given stream: no allocation, no
 // copy, no memset and no wait, so all of them can be captured into a HIP graph.
@@ -96,6 +97,41 @@ struct LossArgs {
 };
 size_t label_loss_ws(int64_t n, int64_t rows, int dim, int dtype, bool grad);
 hipError_t launch_label_loss(const LossArgs& a, bool grad, hipStream_t st);
+
+struct GatedArgs {
+    const void* x;  // (n, dim)
+    int64_t n, x_stride;
+    const void *w_gate, *w_up;  // (hidden, dim)
+    int64_t hidden, gate_stride, up_stride;
+    const float *b_gate, *b_up;  // (hidden) or null
+    int dim, dtype, act;
+    void* h;  // (n, hidden)
+    int64_t h_stride;
+    void* ws;
+    // the gradients' own
+    const void* dh;
+    int64_t dh_stride;
+    void* dx;
+    int64_t dx_stride;
+    void *dw_gate, *dw_up;
+    int64_t dgate_stride, dup_stride;
+    float *db_gate, *db_up;  // (hidden) or null
+};
+size_t gated_linear_ws(const GatedArgs& a, bool grad);
+hipError_t launch_gated_linear(const GatedArgs& a, bool grad, hipStream_t st);
+
+// One tensor of a list: rows of cols values, stride apart.
+struct TensorRef {
+    void* data;
+    int64_t rows, cols, stride;
+    int dtype;
+};
+enum { kNormL2 = 0, kNormMax = 1 };  // GS_NORM_*
+size_t grad_norm_ws(const TensorRef* t, int64_t count);
+hipError_t launch_grad_norm(const TensorRef* t, int64_t count, int kind, float* norm, void* ws,
+                            hipStream_t st);
+hipError_t launch_grad_clip(const TensorRef* in, const TensorRef* out, int64_t count,
+                            const float* norm, double max_norm, hipStream_t st);
 
 // gs_api.cpp
 int ctx_device(const ::gs_ctx* ctx);

@@ -2,7 +2,9 @@
 // arguments, then the launchers of field.h on the caller's stream.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
+#include <vector>
 
 #include "../../include/gsplat_hip.h"
 #include "field.h"
@@ -21,6 +23,9 @@ constexpr int64_t kMaxSamples = ((int64_t)1 << 31) - 256;
 constexpr int64_t kMaxLabels = (int64_t)1 << 22;
 constexpr int64_t kMaxImages = (int64_t)1 << 20;
 constexpr int64_t kMaxPixels = (int64_t)1 << 40;
+constexpr int64_t kMaxHidden = (int64_t)1 << 20;
+constexpr int64_t kMaxTensors = (int64_t)1 << 20;
+constexpr int64_t kMaxValues = (int64_t)1 << 40;
 
 #define LIMIT(cond, msg)                                        \
     do {                                                        \
@@ -151,6 +156,110 @@ gs::LossArgs loss_args(const gs_label_loss* d, float* loss, float* lse, void* ws
     a.ws = ws;
     a.flags = flags;
     return a;
+}
+
+
+// The description alone, and its pointers if there is a row to compute.
+gs::GatedArgs gated_args(const gs_gated_linear* d, bool grad) {
+    REQUIRE(d != nullptr, "gated_linear: null description");
+    REQUIRE(d->n >= 0, "gated_linear: n must not be negative");
+    REQUIRE(d->hidden >= 1, "gated_linear: hidden must be at least 1");
+    LIMIT(d->n <= kMaxSamples, "gated_linear: n past 2^31 - 256");
+    LIMIT(d->hidden <= kMaxHidden, "gated_linear: hidden past 2^20");
+    check_dim(d->dim, "gated_linear");
+    check_dtype(d->dtype, "gated_linear");
+    REQUIRE(d->act >= GS_ACT_NONE && d->act <= GS_ACT_GELU, "gated_linear: unknown activation");
+    if (d->n > 0) {
+        check_ptr(d->x, d->dtype, "gated_linear: x");
+        check_rows(d->n, d->x_stride, d->dim, "gated_linear: x");
+        check_ptr(d->w_gate, d->dtype, "gated_linear: w_gate");
+        check_rows(d->hidden, d->gate_stride, d->dim, "gated_linear: w_gate");
+        check_ptr(d->w_up, d->dtype, "gated_linear: w_up");
+        check_rows(d->hidden, d->up_stride, d->dim, "gated_linear: w_up");
+    }
+    check_words(d->b_gate, "gated_linear: b_gate");
+    check_words(d->b_up, "gated_linear: b_up");
+    gs::GatedArgs a{};
+    a.x = d->x;
+    a.n = d->n;
+    a.x_stride = d->x_stride;
+    a.w_gate = d->w_gate;
+    a.w_up = d->w_up;
+    a.hidden = d->hidden;
+    a.gate_stride = d->gate_stride;
+    a.up_stride = d->up_stride;
+    a.b_gate = d->b_gate;
+    a.b_up = d->b_up;
+    a.dim = d->dim;
+    a.dtype = d->dtype;
+    a.act = d->act;
+    return a;
+}
+
+// A list of tensors, checked; those without values are left out of `to`.
+void tensor_list(const gs_tensor* t, int64_t count, const char* what, bool output,
+                 std::vector<gs::TensorRef>* to) {
+    REQUIRE(count >= 0, std::string(what) + ": negative count");
+    LIMIT(count <= kMaxTensors, std::string(what) + ": more than 2^20 tensors");
+    REQUIRE(count == 0 || t != nullptr, std::string(what) + ": null list");
+    to->reserve((size_t)count);
+    for (int64_t k = 0; k < count; ++k) {
+        const gs_tensor& one = t[k];
+        REQUIRE(one.rows >= 0 && one.cols >= 0, std::string(what) + ": negative size");
+        check_dtype(one.dtype, what);
+        if (one.rows == 0 || one.cols == 0) continue;
+        LIMIT(one.rows <= kMaxValues / one.cols, std::string(what) + ": more than 2^40 values");
+        check_ptr(one.data, one.dtype, what);
+        REQUIRE(one.rows == 1 || (one.stride >= 0 && one.stride < ((int64_t)1 << 40)),
+                std::string(what) + ": stride out of range");
+        REQUIRE(!output || one.rows == 1 || one.stride >= one.cols,
+                std::string(what) + ": rows overlap (stride below cols)");
+        gs::TensorRef r{one.data, one.rows, one.cols, one.stride, one.dtype};
+        if (r.rows == 1 || r.stride == r.cols)  // one run of values
+            r = {r.data, 1, r.rows * r.cols, r.rows * r.cols, r.dtype};
+        to->push_back(r);
+    }
+}
+
+// Bytes that a tensor reaches over.
+struct Span {
+    uintptr_t begin, end;
+    size_t row, stride;  // bytes of a row and between rows; stride 0: one row
+    bool written;
+};
+Span span_of(const gs::TensorRef& t, bool written) {
+    const size_t e = (size_t)gs::elem_bytes(t.dtype);
+    const uintptr_t p = reinterpret_cast<uintptr_t>(t.data);
+    return {p, p + ((size_t)(t.rows - 1) * (size_t)t.stride + (size_t)t.cols) * e,
+            (size_t)t.cols * e, t.rows > 1 ? (size_t)t.stride * e : 0, written};
+}
+// Whether two spans that overlap have no byte in common all the same: columns of one
+// matrix.
+bool apart(const Span& a, const Span& b) {
+    const size_t stride = a.stride != 0 ? a.stride : b.stride;
+    if (stride == 0 || (a.stride != 0 && b.stride != 0 && a.stride != b.stride)) return false;
+    if (a.row > stride || b.row > stride) return false;
+    // b's first byte as a column of a's rows
+    const size_t at = b.begin >= a.begin ? (b.begin - a.begin) % stride
+                                         : (stride - (a.begin - b.begin) % stride) % stride;
+    return at >= a.row && at + b.row <= stride;
+}
+void check_apart(std::vector<Span>& spans) {
+    std::sort(spans.begin(), spans.end(),
+              [](const Span& a, const Span& b) { return a.begin < b.begin; });
+    // `open`: earlier spans that reach past the present one's begin
+    std::vector<Span> open;
+    for (const Span& s : spans) {
+        size_t kept = 0;
+        for (const Span& o : open) {
+            if (o.end <= s.begin) continue;
+            REQUIRE(!(o.written || s.written) || apart(o, s),
+                    "grad_clip: an output shares memory with another tensor");
+            open[kept++] = o;
+        }
+        open.resize(kept);
+        open.push_back(s);
+    }
 }
 
 }  // namespace
@@ -341,6 +450,133 @@ int gs_label_loss_grad_dev(gs_ctx* ctx, const gs_label_loss* in, const float* ro
         a.dtable_stride = dtable_stride;
         const OnDevice on(ctx);
         HIPCHK(gs::launch_label_loss(a, true, static_cast<hipStream_t>(stream)));
+    });
+}
+
+int64_t gs_gated_linear_workspace(const gs_gated_linear* in, int grad) {
+    try {
+        return (int64_t)gs::gated_linear_ws(gated_args(in, grad != 0), grad != 0);
+    } catch (const std::exception& e) {
+        gs::g_err = e.what();
+        return -1;
+    }
+}
+
+int gs_gated_linear_dev(gs_ctx* ctx, const gs_gated_linear* in, void* h, int64_t h_stride,
+                        void* workspace, int64_t workspace_bytes, void* stream) {
+    return guard([&] {
+        gs::GatedArgs a = gated_args(in, false);
+        if (a.n > 0) {
+            check_ptr(h, a.dtype, "gated_linear: h");
+            check_rows(a.n, h_stride, (int)a.hidden, "gated_linear: h", true);
+            check_ws(workspace, workspace_bytes, gs::gated_linear_ws(a, false), "gated_linear");
+        }
+        a.h = h;
+        a.h_stride = h_stride;
+        a.ws = workspace;
+        REQUIRE(ctx, "null ctx");  // last: the other checks need no device
+        const OnDevice on(ctx);
+        HIPCHK(gs::launch_gated_linear(a, false, static_cast<hipStream_t>(stream)));
+    });
+}
+
+int gs_gated_linear_grad_dev(gs_ctx* ctx, const gs_gated_linear* in, const void* dh,
+                             int64_t dh_stride, void* dx, int64_t dx_stride, void* dw_gate,
+                             int64_t dw_gate_stride, void* dw_up, int64_t dw_up_stride,
+                             float* db_gate, float* db_up, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+    return guard([&] {
+        gs::GatedArgs a = gated_args(in, true);
+        if (a.n > 0) {
+            check_ptr(dh, a.dtype, "gated_linear_grad: dh");
+            check_rows(a.n, dh_stride, (int)a.hidden, "gated_linear_grad: dh");
+            check_ptr(dx, a.dtype, "gated_linear_grad: dx");
+            check_rows(a.n, dx_stride, a.dim, "gated_linear_grad: dx", true);
+            check_ws(workspace, workspace_bytes, gs::gated_linear_ws(a, true),
+                     "gated_linear_grad");
+        }
+        check_ptr(dw_gate, a.dtype, "gated_linear_grad: dw_gate");
+        check_rows(a.hidden, dw_gate_stride, a.dim, "gated_linear_grad: dw_gate", true);
+        check_ptr(dw_up, a.dtype, "gated_linear_grad: dw_up");
+        check_rows(a.hidden, dw_up_stride, a.dim, "gated_linear_grad: dw_up", true);
+        check_words(db_gate, "gated_linear_grad: db_gate");
+        check_words(db_up, "gated_linear_grad: db_up");
+        a.dh = dh;
+        a.dh_stride = dh_stride;
+        a.dx = dx;
+        a.dx_stride = dx_stride;
+        a.dw_gate = dw_gate;
+        a.dw_up = dw_up;
+        a.dgate_stride = dw_gate_stride;
+        a.dup_stride = dw_up_stride;
+        a.db_gate = db_gate;
+        a.db_up = db_up;
+        a.ws = workspace;
+        REQUIRE(ctx, "null ctx");  // last: the other checks need no device
+        const OnDevice on(ctx);
+        HIPCHK(gs::launch_gated_linear(a, true, static_cast<hipStream_t>(stream)));
+    });
+}
+
+int64_t gs_grad_norm_workspace(const gs_tensor* tensors, int64_t count) {
+    try {
+        std::vector<gs::TensorRef> t;
+        tensor_list(tensors, count, "grad_norm", false, &t);
+        return (int64_t)gs::grad_norm_ws(t.data(), (int64_t)t.size());
+    } catch (const std::exception& e) {
+        gs::g_err = e.what();
+        return -1;
+    }
+}
+
+int gs_grad_norm_dev(gs_ctx* ctx, const gs_tensor* tensors, int64_t count, int kind, float* norm,
+                     void* workspace, int64_t workspace_bytes, void* stream) {
+    return guard([&] {
+        REQUIRE(kind == GS_NORM_L2 || kind == GS_NORM_MAX, "grad_norm: unknown norm");
+        std::vector<gs::TensorRef> t;
+        tensor_list(tensors, count, "grad_norm", false, &t);
+        REQUIRE(norm != nullptr, "grad_norm: norm is null");
+        check_words(norm, "grad_norm: norm");
+        check_ws(workspace, workspace_bytes, gs::grad_norm_ws(t.data(), (int64_t)t.size()),
+                 "grad_norm");
+        REQUIRE(ctx, "null ctx");  // last: the other checks need no device
+        const OnDevice on(ctx);
+        HIPCHK(gs::launch_grad_norm(t.data(), (int64_t)t.size(), kind, norm, workspace,
+                                    static_cast<hipStream_t>(stream)));
+    });
+}
+
+int gs_grad_clip_dev(gs_ctx* ctx, const gs_tensor* in, const gs_tensor* out, int64_t count,
+                     const float* norm, double max_norm, void* stream) {
+    return guard([&] {
+        REQUIRE(max_norm >= 0.0, "grad_clip: max_norm must be a number, at least 0");
+        std::vector<gs::TensorRef> from, to;
+        tensor_list(in, count, "grad_clip: in", false, &from);
+        tensor_list(out, count, "grad_clip: out", true, &to);
+        bool alike = from.size() == to.size();
+        for (int64_t k = 0; k < count; ++k)
+            alike &= in[k].rows * in[k].cols == out[k].rows * out[k].cols;
+        for (size_t k = 0; alike && k < from.size(); ++k)
+            alike = from[k].rows == 1 || to[k].rows == 1 || from[k].rows == to[k].rows;
+        REQUIRE(alike, "grad_clip: an output's rows and cols are not its input's");
+        REQUIRE(norm != nullptr, "grad_clip: norm is null");
+        check_words(norm, "grad_clip: norm");
+        std::vector<Span> spans;
+        spans.reserve(2 * from.size());
+        for (size_t k = 0; k < from.size(); ++k) {
+            const gs::TensorRef &f = from[k], &t = to[k];
+            const bool same = f.data == t.data && f.rows == t.rows && f.cols == t.cols &&
+                              f.stride == t.stride && f.dtype == t.dtype;
+            if (!same) spans.push_back(span_of(f, false));
+            spans.push_back(span_of(t, true));
+        }
+        const uintptr_t at = reinterpret_cast<uintptr_t>(norm);
+        spans.push_back({at, at + 4, 4, 0, false});
+        check_apart(spans);
+        REQUIRE(ctx, "null ctx");  // last: the other checks need no device
+        const OnDevice on(ctx);
+        HIPCHK(gs::launch_grad_clip(from.data(), to.data(), (int64_t)from.size(), norm, max_norm,
+                                    static_cast<hipStream_t>(stream)));
     });
 }
 

@@ -1,4 +1,5 @@
-"""Learned features on splats: table lookups, group norm and the label loss.
+"""Learned features on splats: table lookups, group norm, gated projections, the label
+loss, and the norm and clipping of gradients.
 
 `FieldOps` runs the feature operators of the C ABI (include/gsplat_hip.h) on torch
 tensors on the GPU, forward and backward:
@@ -7,8 +8,11 @@ lookup / lookup_grad          rows of a feature table by id (codebooks of SH
                               coefficients, appearance rows per view), scaled
 group_norm / group_norm_grad  group norm with an activation over channels-last
                               feature images
+gated_linear / gated_linear_grad  the gated projections of a feed-forward block
 label_loss / label_loss_grad  softmax cross entropy of features against a table
                               of labels, without the scores in memory
+grad_norm / clip_grads        the global norm of many tensors, and their scaling
+                              down to a limit
 
 The reference has no counterpart. Work is enqueued on torch's current stream of
 the context's device and nothing waits; outputs and workspaces come from torch's
@@ -19,6 +23,7 @@ gradients are calls of their own. There is no CPU fallback.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import math
 
@@ -30,6 +35,7 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 _ID_TYPES = (torch.int32, torch.int64)
 _PARAM_TYPES = (torch.float32,)
 _ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+_NORMS = {"l2": 0, "max": 1}
 FLAG_ID_RANGE = 1
 
 
@@ -45,6 +51,28 @@ def _rows(t, name, dim=None):
     if cols > 1 and t.stride(1) != 1:
         raise ValueError(f"{name}: the values of a row must be contiguous")
     return t.data_ptr(), rows, t.stride(0)
+
+
+def _collapse(t):
+    """Rows, columns and row stride that visit a tensor's values in order, or None where
+    one stride between rows is not enough."""
+    rows, cols, stride, inner = 1, 1, 0, True
+    step = 1  # of the next dimension if it goes on with the run
+    for size, st in zip(reversed(t.shape), reversed(t.stride())):
+        if size == 1:
+            continue
+        if inner and st == step:
+            cols *= size
+            step *= size
+        elif inner:
+            inner, rows, stride = False, size, st
+            step = st * size
+        elif st == step:
+            rows *= size
+            step *= size
+        else:
+            return None
+    return rows, cols, stride if rows > 1 else cols
 
 
 def _written(out):
@@ -255,6 +283,152 @@ class FieldOps:
             ws.data_ptr(), size, self._stream()))
         del keep
         return out, dweight, dbias
+
+    # ---- gated projections
+    def _gated(self, x, w_gate, w_up, b_gate, b_up, act):
+        if act not in _ACTS:
+            raise ValueError(f"act must be one of {sorted(_ACTS)}")
+        self._own(x, "x")
+        px, n, sx = _rows(x, "x")
+        dim = x.shape[1]
+        weights = []
+        for w, name in ((w_gate, "w_gate"), (w_up, "w_up")):
+            self._own(w, name)
+            if w.dtype != x.dtype:
+                raise TypeError(f"x is {x.dtype}, {name} {w.dtype}")
+            weights.append(_rows(w, name, dim))
+        (pg, hidden, sg), (pu, rows, su) = weights
+        if rows != hidden:
+            raise ValueError(f"w_gate has {hidden} rows, w_up {rows}")
+        b_gate = self._param(b_gate, "b_gate", hidden)
+        b_up = self._param(b_up, "b_up", hidden)
+        return L.GsGatedLinear(px, pg, pu, None if b_gate is None else b_gate.data_ptr(),
+                               None if b_up is None else b_up.data_ptr(), n, hidden, sx, sg, su,
+                               dim, _DTYPES[x.dtype], _ACTS[act], 0), (b_gate, b_up)
+
+    def _gated_workspace(self, d, grad):
+        # -1 for what the call itself refuses
+        size = max(self._L.gs_gated_linear_workspace(ctypes.byref(d), grad), 0)
+        return torch.empty(size, dtype=torch.uint8, device=self.device), size
+
+    def gated_linear(self, x, w_gate, w_up, b_gate=None, b_up=None, act="silu", out=None):
+        """act(x @ w_gate.T + b_gate) * (x @ w_up.T + b_up): (n, hidden) of x's type, from
+        x (n, dim) and weights (hidden, dim) of one type; the biases (hidden) are fp32."""
+        d, keep = self._gated(x, w_gate, w_up, b_gate, b_up, act)
+        out = self._out(out, (d.n, d.hidden), x.dtype, "out")
+        if out.dtype != x.dtype:
+            raise TypeError(f"out must have the type {x.dtype}")
+        po, _, so = _rows(out, "out")
+        ws, size = self._gated_workspace(d, 0)
+        L._check(self._L.gs_gated_linear_dev(self.ctx.handle, ctypes.byref(d), po, so,
+                                             ws.data_ptr(), size, self._stream()))
+        del keep
+        return out
+
+    def gated_linear_grad(self, dh, x, w_gate, w_up, b_gate=None, b_up=None, act="silu",
+                          dx=None, dw_gate=None, dw_up=None):
+        """(dx, dw_gate, dw_up, db_gate, db_up) of gated_linear() from its output's
+        gradient and its inputs: in the inputs' type, the biases' in fp32 (None for a bias
+        that is None), the weights' and biases' summed over the rows."""
+        d, keep = self._gated(x, w_gate, w_up, b_gate, b_up, act)
+        self._own(dh, "dh")
+        if dh.dtype != x.dtype:
+            raise TypeError(f"x is {x.dtype}, dh {dh.dtype}")
+        ph, n, sh = _rows(dh, "dh", d.hidden)
+        if n != d.n:
+            raise ValueError(f"dh must have {d.n} rows, not {n}")
+        dx = self._out(dx, x.shape, x.dtype, "dx")
+        dw_gate = self._out(dw_gate, w_gate.shape, x.dtype, "dw_gate")
+        dw_up = self._out(dw_up, w_up.shape, x.dtype, "dw_up")
+        if not dx.dtype == dw_gate.dtype == dw_up.dtype == x.dtype:
+            raise TypeError(f"dx, dw_gate and dw_up must have the type {x.dtype}")
+        db_gate, db_up = (None if b is None else torch.empty(d.hidden, dtype=torch.float32,
+                                                             device=self.device)
+                          for b in (b_gate, b_up))
+        px, _, sx = _rows(dx, "dx")
+        pg, _, sg = _rows(dw_gate, "dw_gate")
+        pu, _, su = _rows(dw_up, "dw_up")
+        ws, size = self._gated_workspace(d, 1)
+        L._check(self._L.gs_gated_linear_grad_dev(
+            self.ctx.handle, ctypes.byref(d), ph, sh, px, sx, pg, sg, pu, su,
+            None if db_gate is None else db_gate.data_ptr(),
+            None if db_up is None else db_up.data_ptr(), ws.data_ptr(), size, self._stream()))
+        del keep
+        return dx, dw_gate, dw_up, db_gate, db_up
+
+    # ---- gradients of many tensors
+    def _tensors(self, tensors, name, like=None):
+        """The list as an array of gs_tensor, values in the order in which the tensors
+        (or their counterparts in `like`) lie in memory."""
+        flat = array.array("q")
+        for k, t in enumerate(tensors):
+            self._own(t, name)
+            lead = t if like is None else like[k]
+            if t.is_contiguous() and lead.is_contiguous():
+                cols = t.numel()
+                flat.extend((t.data_ptr(), 1, cols, cols, _DTYPES[t.dtype]))
+                continue
+            if _collapse(lead) is None:  # the order of memory, not that of the dimensions
+                t = t.permute(sorted(range(t.dim()), key=lead.stride, reverse=True))
+            rows = _collapse(t) if t.numel() else (1, 0, 0)
+            if rows is None:
+                raise ValueError(f"{name}[{k}]: the values must lie in rows at one distance" +
+                                 (" in grads' order" if like is not None else ""))
+            flat.extend((t.data_ptr(), *rows, _DTYPES[t.dtype]))
+        return flat
+
+    def _grad_norm(self, flat, count, kind):
+        if kind not in _NORMS:
+            raise ValueError(f"kind must be one of {sorted(_NORMS)}")
+        at = flat.buffer_info()[0]
+        size = max(self._L.gs_grad_norm_workspace(at, count), 0)  # -1: the call refuses it
+        ws = torch.empty(size, dtype=torch.uint8, device=self.device)
+        norm = torch.empty((), dtype=torch.float32, device=self.device)
+        L._check(self._L.gs_grad_norm_dev(self.ctx.handle, at, count, _NORMS[kind],
+                                          norm.data_ptr(), ws.data_ptr(), size, self._stream()))
+        return norm
+
+    def grad_norm(self, grads, kind="l2"):
+        """The global norm of a list of fp32 and bf16 tensors, an fp32 scalar on the GPU:
+        "l2", the root of the sum of all squares, or "max", the largest size of a value; 0
+        for no values, NaN if any value is."""
+        grads = list(grads)
+        return self._grad_norm(self._tensors(grads, "grads"), len(grads), kind)
+
+    def clip_grads(self, grads, max_norm, kind="l2", out=None, norm=None):
+        """Scales the tensors by min(1, max_norm / (norm + 1e-6)), in place or into the
+        tensors `out` (of the same shapes, fp32 or bf16; each tensor contiguous, or in the
+        same rows as its counterpart), and returns their global norm from before. `norm` (an fp32 scalar on the GPU) is taken instead of it if given,
+        as where it is summed over processes. In place nothing is written where the norm
+        is within the limit."""
+        grads = list(grads)
+        flat = self._tensors(grads, "grads")
+        to = flat
+        if out is None:
+            out = grads
+        else:
+            out = list(out)
+            if len(out) != len(grads):
+                raise ValueError(f"out has {len(out)} tensors, grads {len(grads)}")
+            for k, (o, g) in enumerate(zip(out, grads)):
+                if isinstance(o, torch.Tensor) and o.shape != g.shape:
+                    raise ValueError(f"out[{k}] must be {tuple(g.shape)}, not {tuple(o.shape)}")
+            to = self._tensors(out, "out", grads)
+        max_norm = float(max_norm)
+        if not max_norm >= 0.0:
+            raise ValueError("max_norm must be a number, at least 0")
+        if norm is None:
+            norm = self._grad_norm(flat, len(grads), kind)
+        else:
+            self._own(norm, "norm", _PARAM_TYPES)
+            if norm.numel() != 1:
+                raise ValueError("norm must be one value")
+        for t in out:
+            _written(t)
+        L._check(self._L.gs_grad_clip_dev(self.ctx.handle, flat.buffer_info()[0],
+                                          to.buffer_info()[0], len(grads), norm.data_ptr(),
+                                          max_norm, self._stream()))
+        return norm
 
     # ---- label loss
     def _loss(self, feat, table, labels, scale):

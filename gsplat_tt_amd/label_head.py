@@ -1,14 +1,16 @@
 """A label head on rendered features: the feature operators used together.
 
-    python -m gsplat_tt_amd.label_head [--gaussians N] [--steps K]
+    python -m gsplat_tt_amd.label_head [--gaussians N] [--steps K] [--hidden H] [--clip C]
 
 A synthetic scene's Gaussians carry codes into a codebook of feature rows
 (`lookup`), which the rasterizer renders three channels at a time into feature
 images. `LabelHead` adds a learned appearance row per view (`lookup` again), runs
-a group norm with silu, and scores every pixel against a table of label rows
+a group norm with silu, optionally a hidden layer of gated projections
+(`gated_linear`), and scores every pixel against a table of label rows
 (`label_loss`). A step is the whole forward and backward through
-`label_loss_grad`, `group_norm_grad` and `lookup_grad`, then Adam on the head's
-parameters. Pixels that show no Gaussian are masked.
+`label_loss_grad`, `gated_linear_grad`, `group_norm_grad` and `lookup_grad`, the
+gradients' clipping to a norm if one is given (`clip_grads`), then Adam on the
+head's parameters. Pixels that show no Gaussian are masked.
 """
 from __future__ import annotations
 
@@ -23,22 +25,30 @@ from .field import FieldOps
 
 
 class LabelHead:
-    """Appearance rows, norm and label table over (views, H, W, channels) features."""
+    """Appearance rows, norm, hidden layer (of `hidden` units, 0: none) and label table
+    over (views, H, W, channels) features."""
 
     GROUPS, SCALE = 4, 4.0
 
-    def __init__(self, ops: FieldOps, channels: int, labels: int, views: int, seed: int = 0):
+    def __init__(self, ops: FieldOps, channels: int, labels: int, views: int, seed: int = 0,
+                 hidden: int = 0):
         g = torch.Generator().manual_seed(seed)
 
         def param(t):
             return t.to(ops.device, torch.float32)
 
-        self.ops, self.labels, self.views = ops, labels, views
+        self.ops, self.labels, self.views, self.hidden = ops, labels, views, hidden
+        width = hidden or channels
         self.params = {"appearance": param(torch.zeros(views, channels)),
                        "weight": param(torch.ones(channels)),
                        "bias": param(torch.zeros(channels)),
-                       "table": param(torch.randn(labels, channels, generator=g) /
-                                      channels ** 0.5)}
+                       "table": param(torch.randn(labels, width, generator=g) / width ** 0.5)}
+        if hidden:
+            for k in ("w_gate", "w_up"):
+                self.params[k] = param(torch.randn(hidden, channels, generator=g) *
+                                       (2 / channels) ** 0.5)
+            self.params["b_gate"] = param(torch.zeros(hidden))
+            self.params["b_up"] = param(torch.zeros(hidden))
         self._moments = {k: (torch.zeros_like(v), torch.zeros_like(v))
                          for k, v in self.params.items()}
         self._steps = 0
@@ -49,7 +59,11 @@ class LabelHead:
         rows = self.ops.lookup(p["appearance"], view_ids)
         x = images + rows.view(images.shape)
         y, mean, rstd = self.ops.group_norm(x, self.GROUPS, p["weight"], p["bias"], act="silu")
-        return y.view(-1, y.shape[-1]), (x, mean, rstd)
+        feat = y.view(-1, y.shape[-1])
+        saved = (x, mean, rstd, feat)
+        if self.hidden:
+            feat = self.ops.gated_linear(feat, p["w_gate"], p["w_up"], p["b_gate"], p["b_up"])
+        return feat, saved
 
     def loss(self, images, view_ids, labels):
         """The cross entropy of every pixel, 0 for masked ones."""
@@ -60,21 +74,30 @@ class LabelHead:
         """(mean loss over the pixels with a label, gradients of the parameters); the
         mean stays on the GPU."""
         p = self.params
-        feat, (x, mean, rstd) = self._features(images, view_ids)
+        feat, (x, mean, rstd, normed) = self._features(images, view_ids)
         on = (labels >= 0).float()
         weight = on / on.sum().clamp(min=1)
         loss, _, dfeat, dtable = self.ops.label_loss_grad(feat, p["table"], labels, weight,
                                                           scale=self.SCALE)
+        grads = {"table": dtable}
+        if self.hidden:
+            dfeat, *rest = self.ops.gated_linear_grad(dfeat, normed, p["w_gate"], p["w_up"],
+                                                      p["b_gate"], p["b_up"])
+            grads.update(zip(("w_gate", "w_up", "b_gate", "b_up"), rest))
         dx, dweight, dbias = self.ops.group_norm_grad(dfeat.view(x.shape), x, mean, rstd,
                                                       self.GROUPS, p["weight"], p["bias"],
                                                       act="silu")
-        dapp = self.ops.lookup_grad(dx.view(feat.shape), view_ids, self.views)
-        return (loss * weight).sum(), {"appearance": dapp, "weight": dweight, "bias": dbias,
-                                       "table": dtable}
+        dapp = self.ops.lookup_grad(dx.view(normed.shape), view_ids, self.views)
+        grads.update(appearance=dapp, weight=dweight, bias=dbias)
+        return (loss * weight).sum(), grads
 
-    def step(self, images, view_ids, labels, lr=0.02, betas=(0.9, 0.99), eps=1e-8):
-        """One Adam step; returns the mean loss before it."""
+    def step(self, images, view_ids, labels, lr=0.02, betas=(0.9, 0.99), eps=1e-8,
+             max_norm=None):
+        """One Adam step, of the gradients scaled down to the global norm `max_norm` if
+        one is given; returns the mean loss before it."""
         loss, grads = self.gradients(images, view_ids, labels)
+        if max_norm is not None:
+            self.ops.clip_grads(grads.values(), max_norm)
         self._steps += 1
         for k, g in grads.items():
             m, v = self._moments[k]
@@ -130,12 +153,14 @@ def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     ap.add_argument("--gaussians", type=int, default=20_000)
     ap.add_argument("--steps", type=int, default=60)
+    ap.add_argument("--hidden", type=int, default=0, help="units of a hidden layer")
+    ap.add_argument("--clip", type=float, default=None, help="limit of the gradients' norm")
     args = ap.parse_args(argv)
     ops = FieldOps()
     images, view_ids, labels = synthetic(ops, gaussians=args.gaussians)
-    head = LabelHead(ops, images.shape[-1], 6, images.shape[0])
+    head = LabelHead(ops, images.shape[-1], 6, images.shape[0], hidden=args.hidden)
     for k in range(args.steps):
-        loss = head.step(images, view_ids, labels)
+        loss = head.step(images, view_ids, labels, max_norm=args.clip)
         if k % 10 == 0 or k == args.steps - 1:
             print(f"step {k}: loss {float(loss):.4f}", flush=True)
     ops.check()

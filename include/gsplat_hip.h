@@ -525,6 +525,62 @@ int gs_label_loss_grad_dev(gs_ctx* ctx, const gs_label_loss* in, const float* ro
                            void* dtable, int64_t dtable_stride, void* workspace,
                            int64_t workspace_bytes, uint32_t* flags, void* stream);
 
+/* Gated projections of n rows of features, the first half of a gated feed-forward
+ * block: h = act(gate) * up, gate = x Wg^T + bg, up = x Wu^T + bu. x (n, dim), w_gate and
+ * w_up (hidden, dim), h (n, hidden) of one dtype; b_gate and b_up (hidden) fp32 or NULL
+ * (0). dim at most 65536, hidden 1 .. 2^20, n at most 2^31 - 256. Infinite values and NaN
+ * act as in plain arithmetic. */
+typedef struct gs_gated_linear {
+    const void* x;
+    const void* w_gate;
+    const void* w_up;
+    const float* b_gate;
+    const float* b_up;
+    int64_t n, hidden;
+    int64_t x_stride, gate_stride, up_stride;
+    int dim, dtype;
+    int act; /* GS_ACT_* */
+    int reserved;
+} gs_gated_linear;
+/* Depends on the sizes, types, strides and the pointers' alignment in `in`. */
+int64_t gs_gated_linear_workspace(const gs_gated_linear* in, int grad);
+int gs_gated_linear_dev(gs_ctx* ctx, const gs_gated_linear* in, void* h, int64_t h_stride,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+/* Its gradients from dh (n, hidden); gate and up are made again. dx (n, dim), dw_gate and
+ * dw_up (hidden, dim) of in->dtype, db_gate and db_up (hidden) fp32 (each may be NULL),
+ * the weights' and biases' summed over the rows. For bf16 inputs the gradients of gate and
+ * up are rounded to bf16 before they are multiplied, as operands of the matrix cores. The
+ * workspace is at most about 1 GB beside copies of the weights. */
+int gs_gated_linear_grad_dev(gs_ctx* ctx, const gs_gated_linear* in, const void* dh,
+                             int64_t dh_stride, void* dx, int64_t dx_stride, void* dw_gate,
+                             int64_t dw_gate_stride, void* dw_up, int64_t dw_up_stride,
+                             float* db_gate, float* db_up, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+
+/* The global norm of a list of tensors (gradients): GS_NORM_L2 the root of the sum of all
+ * squares, summed in 64 bits; GS_NORM_MAX the largest size of a value. *norm (fp32, on the
+ * device) is 0 for no values, NaN if any value is. The list itself lies in host memory and
+ * is not used after the call; at most 2^20 tensors, 2^40 values in each. */
+#define GS_NORM_L2 0
+#define GS_NORM_MAX 1
+typedef struct gs_tensor {
+    void* data;           /* rows of cols values, consecutive, rows stride apart */
+    int64_t rows, cols;
+    int64_t stride;
+    int dtype;
+    int reserved;
+} gs_tensor;
+int64_t gs_grad_norm_workspace(const gs_tensor* tensors, int64_t count);
+int gs_grad_norm_dev(gs_ctx* ctx, const gs_tensor* tensors, int64_t count, int kind, float* norm,
+                     void* workspace, int64_t workspace_bytes, void* stream);
+/* out_k = in_k * min(1, max_norm / (*norm + 1e-6)) for every tensor of a list, the factor
+ * and the products in fp32; a NaN norm makes all values NaN. out_k has in_k's rows and
+ * cols, or one of the two has its values in one run (rows 1, or stride equal to cols); its
+ * dtype and stride are its own. It is in_k itself (all of its description; not written then
+ * where the factor is 1), or overlaps no tensor of the lists. max_norm >= 0. */
+int gs_grad_clip_dev(gs_ctx* ctx, const gs_tensor* in, const gs_tensor* out, int64_t count,
+                     const float* norm, double max_norm, void* stream);
+
 /* ---- device memory helpers (for callers without a GPU framework) ------ */
 int gs_dev_alloc(gs_ctx* ctx, int64_t bytes, void** ptr);
 int gs_dev_free(gs_ctx* ctx, void* ptr);
