@@ -283,6 +283,84 @@ __global__ __launch_bounds__(kThreads) void k_gated_db(GatedArgs a, const float*
     out[u.unit] = add ? out[u.unit] + v : v;
 }
 
+// ---------------------------------------------------------------- few rows
+// Up to 64 rows, without their gradients: every workgroup makes 16 hidden units of all
+// rows, its waves sharing the summed index; the operands come from memory as the matrix
+// cores take them, 8 values of a row a lane, so that nothing is laid out before.
+constexpr int kFewRows = 64;
+
+template <typename T, int NP, int ACT, int J>
+__global__ __launch_bounds__(kThreads) void k_gated_few(GatedArgs a) {
+    __shared__ f32x4 lds[kThreads / 64][2 * J][64];
+    const int lane = threadIdx.x & 63, w = wave_id(), g = lane >> 4, s = lane & 15;
+    const int64_t u0 = (int64_t)blockIdx.x * 16;
+    const bool on = u0 + s < a.hidden;
+    const int64_t unit = on ? u0 + s : 0;
+    const T* gate = static_cast<const T*>(a.w_gate) + unit * a.gate_stride;
+    const T* up = static_cast<const T*>(a.w_up) + unit * a.up_stride;
+    f32x4 acc[2][J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) acc[0][j] = acc[1][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k = w * 32; k < a.dim; k += kThreads / 64 * 32) {
+        quad wp[2][NP], xp[J][NP];
+        const int c = k + g * 8;
+        load_parts<T, NP>(gate, a.dim, c, on, wp[0]);
+        load_parts<T, NP>(up, a.dim, c, on, wp[1]);
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int64_t i = j * 16 + s;
+            load_parts<T, NP>(static_cast<const T*>(a.x) + (i < a.n ? i : 0) * a.x_stride, a.dim,
+                              c, i < a.n, xp[j]);
+        }
+#pragma unroll
+        for (int q = 0; q < Products<NP>::kCount; ++q)
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        __builtin_bit_cast(bf16x8, wp[t][Products<NP>::a(q)]),
+                        __builtin_bit_cast(bf16x8, xp[j][Products<NP>::b(q)]), acc[t][j], 0, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) lds[w][t * J + j][lane] = acc[t][j];
+    __syncthreads();
+    // wave w joins every fourth block of 16 rows: the lane's row is i, its units u0 + 4 g ..
+    for (int j = w; j < J; j += kThreads / 64) {
+        f32x4 z[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            z[t] = lds[0][t * J + j][lane];
+#pragma unroll
+            for (int v = 1; v < kThreads / 64; ++v) z[t] += lds[v][t * J + j][lane];
+        }
+        const int64_t i = j * 16 + s, u = u0 + g * 4;
+        if (i >= a.n) continue;
+        float h[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const bool in = u + k < a.hidden;
+            const float bg = in && a.b_gate != nullptr ? a.b_gate[u + k] : 0.0f;
+            const float bu = in && a.b_up != nullptr ? a.b_up[u + k] : 0.0f;
+            h[k] = act<ACT>(z[0][k] + bg) * (z[1][k] + bu);
+        }
+        store_cols<4>(static_cast<T*>(a.h) + i * a.h_stride, u, a.hidden, h);
+    }
+}
+
+bool is_few(const GatedArgs& a, bool grad) { return !grad && a.n <= kFewRows; }
+
+template <typename T, int NP, int ACT>
+hipError_t few_run(const GatedArgs& a, hipStream_t st) {
+    const unsigned blocks = (unsigned)((a.hidden + 15) / 16);
+    if (a.n <= 16) k_gated_few<T, NP, ACT, 1><<<blocks, kThreads, 0, st>>>(a);
+    else if (a.n <= 32) k_gated_few<T, NP, ACT, 2><<<blocks, kThreads, 0, st>>>(a);
+    else k_gated_few<T, NP, ACT, 4><<<blocks, kThreads, 0, st>>>(a);
+    return hipGetLastError();
+}
+
 // ---------------------------------------------------------------- plans
 // Bytes of x's parts and of [dgate, dup] in the workspace at most, about.
 constexpr int64_t kPieceBytes = (int64_t)1 << 30;
@@ -317,6 +395,7 @@ struct GatedPlan {
 
 template <typename T, int NP, int ACT>
 hipError_t gated_run(const GatedArgs& a, bool grad, hipStream_t st) {
+    if (is_few(a, grad)) return few_run<T, NP, ACT>(a, st);
     const GatedPlan w(a.ws, a.n, a.hidden, a.dim, NP, grad);
     const int kd = (int)pad_to(a.dim, kStep);
     const int64_t wu = w.wr * (w.ld / 8);
@@ -378,7 +457,8 @@ hipError_t gated_act(const GatedArgs& a, bool grad, hipStream_t st) {
 }  // namespace
 
 size_t gated_linear_ws(const GatedArgs& a, bool grad) {
-    return a.n == 0 ? 0 : GatedPlan(nullptr, a.n, a.hidden, a.dim, a.dtype == 0 ? 3 : 1, grad).bytes;
+    if (a.n == 0 || is_few(a, grad)) return 0;
+    return GatedPlan(nullptr, a.n, a.hidden, a.dim, a.dtype == 0 ? 3 : 1, grad).bytes;
 }
 
 hipError_t launch_gated_linear(const GatedArgs& a, bool grad, hipStream_t st) {

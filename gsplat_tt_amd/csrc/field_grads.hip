@@ -146,8 +146,13 @@ __device__ __forceinline__ void add_run(const T* p, int64_t n, Total<KIND>& t) {
 #pragma unroll
             for (int j = 0; j < V; ++j) t.add(v[k][j]);
     }
-    for (; i < n; i += step)
-        for (int j = 0; j < V && i + j < n; ++j) t.add(to_float(p[i + j]));
+    for (; i + V <= n; i += step) {
+        float v[V];
+        load_any<V>(p + i, v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) t.add(v[j]);
+    }
+    for (; i < n; ++i) t.add(to_float(p[i]));  // one thread's, fewer than V
 }
 template <typename T, int KIND>
 __device__ __forceinline__ void add_rows(const Entry& e, int64_t i0, int64_t n, Total<KIND>& t) {
@@ -202,8 +207,14 @@ __device__ __forceinline__ void scale_run(const TI* in, TO* out, int64_t n, floa
             store_any<V>(out + i + k * step, v[k]);
         }
     }
-    for (; i < n; i += step)
-        for (int j = 0; j < V && i + j < n; ++j) out[i + j] = from_float<TO>(to_float(in[i + j]) * f);
+    for (; i + V <= n; i += step) {
+        float v[V];
+        load_any<V>(in + i, v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] *= f;
+        store_any<V>(out + i, v);
+    }
+    for (; i < n; ++i) out[i] = from_float<TO>(to_float(in[i]) * f);  // one thread's
 }
 template <typename TI, typename TO>
 __device__ __forceinline__ void scale_part(const Entry& e, int64_t i0, int64_t n, float f) {

@@ -25,7 +25,9 @@ from __future__ import annotations
 
 import array
 import ctypes
+import itertools
 import math
+import operator
 
 import torch
 
@@ -37,6 +39,9 @@ _PARAM_TYPES = (torch.float32,)
 _ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 _NORMS = {"l2": 0, "max": 1}
 FLAG_ID_RANGE = 1
+_get_dtype = torch.Tensor.dtype.__get__
+_get_device = torch.Tensor.get_device
+_get_requires_grad = torch.Tensor.requires_grad.__get__
 
 
 def _rows(t, name, dim=None):
@@ -360,21 +365,33 @@ class FieldOps:
     def _tensors(self, tensors, name, like=None):
         """The list as an array of gs_tensor, values in the order in which the tensors
         (or their counterparts in `like`) lie in memory."""
-        flat = array.array("q")
-        for k, t in enumerate(tensors):
-            self._own(t, name)
-            lead = t if like is None else like[k]
-            if t.is_contiguous() and lead.is_contiguous():
-                cols = t.numel()
-                flat.extend((t.data_ptr(), 1, cols, cols, _DTYPES[t.dtype]))
-                continue
-            if _collapse(lead) is None:  # the order of memory, not that of the dimensions
-                t = t.permute(sorted(range(t.dim()), key=lead.stride, reverse=True))
-            rows = _collapse(t) if t.numel() else (1, 0, 0)
-            if rows is None:
-                raise ValueError(f"{name}[{k}]: the values must lie in rows at one distance" +
-                                 (" in grads' order" if like is not None else ""))
-            flat.extend((t.data_ptr(), *rows, _DTYPES[t.dtype]))
+        # a list at a time: attribute by attribute 100 tensors took 75 us, so 45
+        plain = set(map(type, tensors)) <= {torch.Tensor, torch.nn.Parameter}
+        if plain:
+            types = list(map(_DTYPES.get, map(_get_dtype, tensors)))
+            plain = None not in types and set(map(_get_device, tensors)) <= {self._index} and \
+                not (torch.is_grad_enabled() and any(map(_get_requires_grad, tensors)))
+        if not plain:
+            for t in tensors:
+                self._own(t, name)
+            types = [_DTYPES[t.dtype] for t in tensors]
+        sizes = list(map(torch.Tensor.numel, tensors))
+        flat = array.array("q", itertools.chain.from_iterable(
+            zip(map(torch.Tensor.data_ptr, tensors), itertools.repeat(1), sizes, sizes, types)))
+        if like is None:
+            like = tensors
+        if not (all(map(torch.Tensor.is_contiguous, tensors)) and
+                (like is tensors or all(map(torch.Tensor.is_contiguous, like)))):
+            for k, (t, lead) in enumerate(zip(tensors, like)):
+                if t.numel() == 0 or (t.is_contiguous() and lead.is_contiguous()):
+                    continue
+                if _collapse(lead) is None:  # the order of memory, not that of the dimensions
+                    t = t.permute(sorted(range(t.dim()), key=lead.stride, reverse=True))
+                rows = _collapse(t)
+                if rows is None:
+                    raise ValueError(f"{name}[{k}]: the values must lie in rows at one distance" +
+                                     (" in grads' order" if like is not tensors else ""))
+                flat[5 * k + 1:5 * k + 4] = array.array("q", rows)
         return flat
 
     def _grad_norm(self, flat, count, kind):
@@ -410,10 +427,15 @@ class FieldOps:
             out = list(out)
             if len(out) != len(grads):
                 raise ValueError(f"out has {len(out)} tensors, grads {len(grads)}")
-            for k, (o, g) in enumerate(zip(out, grads)):
-                if isinstance(o, torch.Tensor) and o.shape != g.shape:
-                    raise ValueError(f"out[{k}] must be {tuple(g.shape)}, not {tuple(o.shape)}")
-            to = self._tensors(out, "out", grads)
+            if any(map(operator.is_not, out, grads)):
+                for t in out:
+                    if not isinstance(t, torch.Tensor):
+                        raise TypeError("out must be torch tensors")
+                shapes = list(map(torch.Tensor.size, grads))
+                if list(map(torch.Tensor.size, out)) != shapes:
+                    k, o = next((k, o) for k, (o, s) in enumerate(zip(out, shapes)) if o.shape != s)
+                    raise ValueError(f"out[{k}] must be {tuple(shapes[k])}, not {tuple(o.shape)}")
+                to = self._tensors(out, "out", grads)
         max_norm = float(max_norm)
         if not max_norm >= 0.0:
             raise ValueError("max_norm must be a number, at least 0")
@@ -423,8 +445,11 @@ class FieldOps:
             self._own(norm, "norm", _PARAM_TYPES)
             if norm.numel() != 1:
                 raise ValueError("norm must be one value")
-        for t in out:
-            _written(t)
+        if any(map(torch.Tensor.is_inference, out)):
+            for t in out:
+                _written(t)
+        elif out:
+            torch.autograd.graph.increment_version(out)
         L._check(self._L.gs_grad_clip_dev(self.ctx.handle, flat.buffer_info()[0],
                                           to.buffer_info()[0], len(grads), norm.data_ptr(),
                                           max_norm, self._stream()))
