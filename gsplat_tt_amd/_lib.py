@@ -173,7 +173,7 @@ def _field_argtypes(L):
     # lists of GsTensor by their address
     L.gs_grad_norm_workspace.argtypes = [p, q]
     L.gs_grad_norm_dev.argtypes = [p, p, q, i, p, p, q, p]
-    L.gs_grad_clip_dev.argtypes = [p, p, p, q, p, ctypes.c_double, p]
+    L.gs_grad_clip_dev.argtypes = [p, p, p, q, i, p, ctypes.c_double, p, q, p]
     for name in ("gs_lookup_grad_workspace", "gs_group_norm_workspace", "gs_label_loss_workspace",
                  "gs_gated_linear_workspace", "gs_grad_norm_workspace"):
         getattr(L, name).restype = q

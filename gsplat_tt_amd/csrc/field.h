@@ -126,12 +126,12 @@ struct TensorRef {
     int64_t rows, cols, stride;
     int dtype;
 };
-enum { kNormL2 = 0, kNormMax = 1 };  // GS_NORM_*
+enum { kNormGiven = -1, kNormL2 = 0, kNormMax = 1 };  // GS_NORM_*
 size_t grad_norm_ws(const TensorRef* t, int64_t count);
 hipError_t launch_grad_norm(const TensorRef* t, int64_t count, int kind, float* norm, void* ws,
                             hipStream_t st);
-hipError_t launch_grad_clip(const TensorRef* in, const TensorRef* out, int64_t count,
-                            const float* norm, double max_norm, hipStream_t st);
+hipError_t launch_grad_clip(const TensorRef* in, const TensorRef* out, int64_t count, int kind,
+                            float* norm, double max_norm, void* ws, hipStream_t st);
 
 // gs_api.cpp
 int ctx_device(const ::gs_ctx* ctx);

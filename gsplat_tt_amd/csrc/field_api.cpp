@@ -547,8 +547,11 @@ int gs_grad_norm_dev(gs_ctx* ctx, const gs_tensor* tensors, int64_t count, int k
 }
 
 int gs_grad_clip_dev(gs_ctx* ctx, const gs_tensor* in, const gs_tensor* out, int64_t count,
-                     const float* norm, double max_norm, void* stream) {
+                     int kind, float* norm, double max_norm, void* workspace,
+                     int64_t workspace_bytes, void* stream) {
     return guard([&] {
+        REQUIRE(kind == GS_NORM_L2 || kind == GS_NORM_MAX || kind == GS_NORM_GIVEN,
+                "grad_clip: unknown norm");
         REQUIRE(max_norm >= 0.0, "grad_clip: max_norm must be a number, at least 0");
         std::vector<gs::TensorRef> from, to;
         tensor_list(in, count, "grad_clip: in", false, &from);
@@ -561,6 +564,9 @@ int gs_grad_clip_dev(gs_ctx* ctx, const gs_tensor* in, const gs_tensor* out, int
         REQUIRE(alike, "grad_clip: an output's rows and cols are not its input's");
         REQUIRE(norm != nullptr, "grad_clip: norm is null");
         check_words(norm, "grad_clip: norm");
+        if (kind != GS_NORM_GIVEN)
+            check_ws(workspace, workspace_bytes, gs::grad_norm_ws(from.data(), (int64_t)from.size()),
+                     "grad_clip");
         std::vector<Span> spans;
         spans.reserve(2 * from.size());
         for (size_t k = 0; k < from.size(); ++k) {
@@ -571,12 +577,12 @@ int gs_grad_clip_dev(gs_ctx* ctx, const gs_tensor* in, const gs_tensor* out, int
             spans.push_back(span_of(t, true));
         }
         const uintptr_t at = reinterpret_cast<uintptr_t>(norm);
-        spans.push_back({at, at + 4, 4, 0, false});
+        spans.push_back({at, at + 4, 4, 0, kind != GS_NORM_GIVEN});
         check_apart(spans);
         REQUIRE(ctx, "null ctx");  // last: the other checks need no device
         const OnDevice on(ctx);
-        HIPCHK(gs::launch_grad_clip(from.data(), to.data(), (int64_t)from.size(), norm, max_norm,
-                                    static_cast<hipStream_t>(stream)));
+        HIPCHK(gs::launch_grad_clip(from.data(), to.data(), (int64_t)from.size(), kind, norm,
+                                    max_norm, workspace, static_cast<hipStream_t>(stream)));
     });
 }
 

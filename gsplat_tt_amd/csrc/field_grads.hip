@@ -191,6 +191,12 @@ __global__ __launch_bounds__(1024) void k_norm_join(const Total<KIND>* part, int
     if (threadIdx.x == 0) *norm = t.norm();
 }
 
+// The factor of a norm; NaN stays NaN.
+__device__ __forceinline__ float factor_of(float norm, double max_norm) {
+    const double most = max_norm / ((double)norm + 1e-6);
+    return most >= 1.0 ? 1.0f : (float)most;
+}
+
 template <typename TI, typename TO>
 __device__ __forceinline__ void scale_run(const TI* in, TO* out, int64_t n, float f) {
     constexpr int V = 16 / sizeof(TI);
@@ -238,9 +244,7 @@ __global__ __launch_bounds__(kThreads) void k_clip(List<ROWS> list, const float*
                                                    double max_norm) {
     const uint32_t b = gridDim.x - 1 - blockIdx.x;
     const Entry e = list.entry(tensor_of(list, b));
-    // NaN stays NaN
-    const double most = max_norm / ((double)*norm + 1e-6);
-    const float f = most >= 1.0 ? 1.0f : (float)most;
+    const float f = factor_of(*norm, max_norm);
     if (f == 1.0f && e.in == e.out) return;
     const int64_t i0 = (int64_t)(b - e.first) * list.chunk;
     const int64_t n = min(list.chunk, e.n - i0);
@@ -251,6 +255,83 @@ __global__ __launch_bounds__(kThreads) void k_clip(List<ROWS> list, const float*
         if (e.out_type == 0) scale_part<bf16, float>(e, i0, n, f);
         else scale_part<bf16, bf16>(e, i0, n, f);
     }
+}
+
+// ---------------------------------------------------------------- small lists
+// Few values in all (a head's parameters): one workgroup, one launch, which keeps them in
+// registers until the factor is known. `first` counts units of 4 values here.
+constexpr int kSmallThreads = 1024, kSmallUnits = 8;  // of a thread
+
+template <int KIND, bool CLIP>
+__global__ __launch_bounds__(kSmallThreads) void k_grad_small(List<false> list, uint32_t units,
+                                                              float* norm, double max_norm) {
+    __shared__ uint32_t first[List<false>::kMost];
+    if ((int)threadIdx.x < list.count) first[threadIdx.x] = list.first(threadIdx.x);
+    __syncthreads();
+    float v[kSmallUnits][kVec];
+    Total<KIND> t = {};
+#pragma unroll
+    for (int k = 0; k < kSmallUnits; ++k) {
+        const uint32_t u = k * kSmallThreads + threadIdx.x;
+        if (u >= units) break;
+        int lo = 0, hi = list.count - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (first[mid] <= u) lo = mid; else hi = mid - 1;
+        }
+        const Entry e = list.entry(lo);
+        const int i = (int)(u - e.first) * kVec, n = min(kVec, (int)e.n - i);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+            v[k][j] = j >= n ? 0.0f
+                      : e.in_type == 0 ? static_cast<const float*>(e.in)[i + j]
+                                       : to_float(static_cast<const bf16*>(e.in)[i + j]);
+            t.add(v[k][j]);
+        }
+    }
+    t = block_total<KIND, kSmallThreads>(t);
+    const float total = t.norm();
+    if (threadIdx.x == 0) *norm = total;
+    if (!CLIP) return;
+    const float f = factor_of(total, max_norm);
+#pragma unroll
+    for (int k = 0; k < kSmallUnits; ++k) {
+        const uint32_t u = k * kSmallThreads + threadIdx.x;
+        if (u >= units) break;
+        int lo = 0, hi = list.count - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (first[mid] <= u) lo = mid; else hi = mid - 1;
+        }
+        const Entry e = list.entry(lo);
+        if (f == 1.0f && e.in == e.out) continue;
+        const int i = (int)(u - e.first) * kVec, n = min(kVec, (int)e.n - i);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j)
+            if (j < n) {
+                if (e.out_type == 0) static_cast<float*>(e.out)[i + j] = v[k][j] * f;
+                else static_cast<bf16*>(e.out)[i + j] = from_float<bf16>(v[k][j] * f);
+            }
+    }
+}
+
+// Whether one workgroup takes a list, and then the list.
+bool small_list(const TensorRef* in, const TensorRef* out, int64_t count, List<false>* list,
+                uint32_t* units) {
+    if (count > List<false>::kMost) return false;
+    *units = 0;
+    list->count = (int)count;
+    list->chunk = 0;
+    for (int64_t k = 0; k < count; ++k) {
+        const TensorRef &i = in[k], &o = out != nullptr ? out[k] : in[k];
+        const int64_t n = i.rows * i.cols;
+        if (i.rows > 1 || o.rows > 1 || n > kSmallThreads * kSmallUnits * kVec) return false;
+        list->set((int)k, Entry{i.data, o.data, n, *units, (uint16_t)i.dtype, (uint16_t)o.dtype,
+                                0, 0, 0});
+        *units += (uint32_t)((n + kVec - 1) / kVec);
+        if (*units > kSmallThreads * kSmallUnits) return false;
+    }
+    return true;
 }
 
 // ---------------------------------------------------------------- launches
@@ -321,12 +402,36 @@ size_t grad_norm_ws(const TensorRef* t, int64_t count) {
 
 hipError_t launch_grad_norm(const TensorRef* t, int64_t count, int kind, float* norm, void* ws,
                             hipStream_t st) {
+    List<false> small;
+    uint32_t units;
+    if (small_list(t, nullptr, count, &small, &units)) {
+        if (kind == kNormMax)
+            k_grad_small<kNormMax, false><<<1, kSmallThreads, 0, st>>>(small, units, norm, 0.0);
+        else
+            k_grad_small<kNormL2, false><<<1, kSmallThreads, 0, st>>>(small, units, norm, 0.0);
+        return hipGetLastError();
+    }
     return kind == kNormMax ? norm_run<kNormMax>(t, count, norm, ws, st)
                             : norm_run<kNormL2>(t, count, norm, ws, st);
 }
 
-hipError_t launch_grad_clip(const TensorRef* in, const TensorRef* out, int64_t count,
-                            const float* norm, double max_norm, hipStream_t st) {
+hipError_t launch_grad_clip(const TensorRef* in, const TensorRef* out, int64_t count, int kind,
+                            float* norm, double max_norm, void* ws, hipStream_t st) {
+    if (kind != kNormGiven) {
+        List<false> small;
+        uint32_t units;
+        if (small_list(in, out, count, &small, &units)) {
+            if (kind == kNormMax)
+                k_grad_small<kNormMax, true><<<1, kSmallThreads, 0, st>>>(small, units, norm,
+                                                                          max_norm);
+            else
+                k_grad_small<kNormL2, true><<<1, kSmallThreads, 0, st>>>(small, units, norm,
+                                                                         max_norm);
+            return hipGetLastError();
+        }
+        const hipError_t e = launch_grad_norm(in, count, kind, norm, ws, st);
+        if (e != hipSuccess) return e;
+    }
     const int64_t chunk = chunk_of(in, count);
     auto launch = [&](const auto& list, uint32_t blocks) {
         k_clip<<<blocks, kThreads, 0, st>>>(list, norm, max_norm);

@@ -37,7 +37,7 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 _ID_TYPES = (torch.int32, torch.int64)
 _PARAM_TYPES = (torch.float32,)
 _ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
-_NORMS = {"l2": 0, "max": 1}
+_NORMS, _NORM_GIVEN = {"l2": 0, "max": 1}, -1
 FLAG_ID_RANGE = 1
 _get_dtype = torch.Tensor.dtype.__get__
 _get_device = torch.Tensor.get_device
@@ -314,7 +314,10 @@ class FieldOps:
     def _gated_workspace(self, d, grad):
         # -1 for what the call itself refuses
         size = max(self._L.gs_gated_linear_workspace(ctypes.byref(d), grad), 0)
-        return torch.empty(size, dtype=torch.uint8, device=self.device), size
+        if size == 0:
+            return None, None, 0
+        ws = torch.empty(size, dtype=torch.uint8, device=self.device)
+        return ws, ws.data_ptr(), size
 
     def gated_linear(self, x, w_gate, w_up, b_gate=None, b_up=None, act="silu", out=None):
         """act(x @ w_gate.T + b_gate) * (x @ w_up.T + b_up): (n, hidden) of x's type, from
@@ -324,10 +327,10 @@ class FieldOps:
         if out.dtype != x.dtype:
             raise TypeError(f"out must have the type {x.dtype}")
         po, _, so = _rows(out, "out")
-        ws, size = self._gated_workspace(d, 0)
-        L._check(self._L.gs_gated_linear_dev(self.ctx.handle, ctypes.byref(d), po, so,
-                                             ws.data_ptr(), size, self._stream()))
-        del keep
+        ws, at, size = self._gated_workspace(d, 0)
+        L._check(self._L.gs_gated_linear_dev(self.ctx.handle, ctypes.byref(d), po, so, at,
+                                             size, self._stream()))
+        del keep, ws
         return out
 
     def gated_linear_grad(self, dh, x, w_gate, w_up, b_gate=None, b_up=None, act="silu",
@@ -353,12 +356,12 @@ class FieldOps:
         px, _, sx = _rows(dx, "dx")
         pg, _, sg = _rows(dw_gate, "dw_gate")
         pu, _, su = _rows(dw_up, "dw_up")
-        ws, size = self._gated_workspace(d, 1)
+        ws, at, size = self._gated_workspace(d, 1)
         L._check(self._L.gs_gated_linear_grad_dev(
             self.ctx.handle, ctypes.byref(d), ph, sh, px, sx, pg, sg, pu, su,
             None if db_gate is None else db_gate.data_ptr(),
-            None if db_up is None else db_up.data_ptr(), ws.data_ptr(), size, self._stream()))
-        del keep
+            None if db_up is None else db_up.data_ptr(), at, size, self._stream()))
+        del keep, ws
         return dx, dw_gate, dw_up, db_gate, db_up
 
     # ---- gradients of many tensors
@@ -394,23 +397,26 @@ class FieldOps:
                 flat[5 * k + 1:5 * k + 4] = array.array("q", rows)
         return flat
 
-    def _grad_norm(self, flat, count, kind):
+    def _norm_room(self, flat, count, kind):
+        """The norm's number, the norm, the workspace and its size."""
         if kind not in _NORMS:
             raise ValueError(f"kind must be one of {sorted(_NORMS)}")
-        at = flat.buffer_info()[0]
-        size = max(self._L.gs_grad_norm_workspace(at, count), 0)  # -1: the call refuses it
-        ws = torch.empty(size, dtype=torch.uint8, device=self.device)
-        norm = torch.empty((), dtype=torch.float32, device=self.device)
-        L._check(self._L.gs_grad_norm_dev(self.ctx.handle, at, count, _NORMS[kind],
-                                          norm.data_ptr(), ws.data_ptr(), size, self._stream()))
-        return norm
+        # -1 for what the call itself refuses
+        size = max(self._L.gs_grad_norm_workspace(flat.buffer_info()[0], count), 0)
+        return (_NORMS[kind], torch.empty((), dtype=torch.float32, device=self.device),
+                torch.empty(size, dtype=torch.uint8, device=self.device), size)
 
     def grad_norm(self, grads, kind="l2"):
         """The global norm of a list of fp32 and bf16 tensors, an fp32 scalar on the GPU:
         "l2", the root of the sum of all squares, or "max", the largest size of a value; 0
         for no values, NaN if any value is."""
         grads = list(grads)
-        return self._grad_norm(self._tensors(grads, "grads"), len(grads), kind)
+        flat = self._tensors(grads, "grads")
+        number, norm, ws, size = self._norm_room(flat, len(grads), kind)
+        L._check(self._L.gs_grad_norm_dev(self.ctx.handle, flat.buffer_info()[0], len(grads),
+                                          number, norm.data_ptr(), ws.data_ptr(), size,
+                                          self._stream()))
+        return norm
 
     def clip_grads(self, grads, max_norm, kind="l2", out=None, norm=None):
         """Scales the tensors by min(1, max_norm / (norm + 1e-6)), in place or into the
@@ -440,8 +446,10 @@ class FieldOps:
         if not max_norm >= 0.0:
             raise ValueError("max_norm must be a number, at least 0")
         if norm is None:
-            norm = self._grad_norm(flat, len(grads), kind)
+            number, norm, ws, size = self._norm_room(flat, len(grads), kind)
+            ws = ws.data_ptr()
         else:
+            number, ws, size = _NORM_GIVEN, None, 0
             self._own(norm, "norm", _PARAM_TYPES)
             if norm.numel() != 1:
                 raise ValueError("norm must be one value")
@@ -451,8 +459,8 @@ class FieldOps:
         elif out:
             torch.autograd.graph.increment_version(out)
         L._check(self._L.gs_grad_clip_dev(self.ctx.handle, flat.buffer_info()[0],
-                                          to.buffer_info()[0], len(grads), norm.data_ptr(),
-                                          max_norm, self._stream()))
+                                          to.buffer_info()[0], len(grads), number,
+                                          norm.data_ptr(), max_norm, ws, size, self._stream()))
         return norm
 
     # ---- label loss

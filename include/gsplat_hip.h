@@ -563,6 +563,7 @@ int gs_gated_linear_grad_dev(gs_ctx* ctx, const gs_gated_linear* in, const void*
  * is not used after the call; at most 2^20 tensors, 2^40 values in each. */
 #define GS_NORM_L2 0
 #define GS_NORM_MAX 1
+#define GS_NORM_GIVEN -1 /* gs_grad_clip_dev alone */
 typedef struct gs_tensor {
     void* data;           /* rows of cols values, consecutive, rows stride apart */
     int64_t rows, cols;
@@ -573,13 +574,17 @@ typedef struct gs_tensor {
 int64_t gs_grad_norm_workspace(const gs_tensor* tensors, int64_t count);
 int gs_grad_norm_dev(gs_ctx* ctx, const gs_tensor* tensors, int64_t count, int kind, float* norm,
                      void* workspace, int64_t workspace_bytes, void* stream);
-/* out_k = in_k * min(1, max_norm / (*norm + 1e-6)) for every tensor of a list, the factor
- * and the products in fp32; a NaN norm makes all values NaN. out_k has in_k's rows and
- * cols, or one of the two has its values in one run (rows 1, or stride equal to cols); its
- * dtype and stride are its own. It is in_k itself (all of its description; not written then
- * where the factor is 1), or overlaps no tensor of the lists. max_norm >= 0. */
+/* out_k = in_k * min(1, max_norm / (norm + 1e-6)) for every tensor of a list, the factor
+ * and the products in fp32; a NaN norm makes all values NaN. The norm is the list's own,
+ * written to *norm as gs_grad_norm_dev does (with a workspace of
+ * gs_grad_norm_workspace(in, count)), or with GS_NORM_GIVEN what *norm holds (no workspace).
+ * out_k has in_k's rows and cols, or one of the two has its values in one run (rows 1, or
+ * stride equal to cols); its dtype and stride are its own. It is in_k itself (all of its
+ * description; not written then where the factor is 1), or overlaps no tensor of the lists;
+ * a norm that is written overlaps none either. max_norm >= 0. */
 int gs_grad_clip_dev(gs_ctx* ctx, const gs_tensor* in, const gs_tensor* out, int64_t count,
-                     const float* norm, double max_norm, void* stream);
+                     int kind, float* norm, double max_norm, void* workspace,
+                     int64_t workspace_bytes, void* stream);
 
 /* ---- device memory helpers (for callers without a GPU framework) ------ */
 int gs_dev_alloc(gs_ctx* ctx, int64_t bytes, void** ptr);

@@ -130,13 +130,13 @@ def test_grad_norm_workspace_and_refusals():
         L.GS_E_CAPACITY
 
 
-def _clip(ins, outs, norm=0x1000, max_norm=1.0):
+def _clip(ins, outs, norm=0x1000, max_norm=1.0, kind=-1, ws=None, size=0):
     """What the clipping of these lists says to a null context: b"" where nothing else
     is wrong."""
     lib = L.load_library()
     i, o = _tensors(*ins), _tensors(*outs)
-    assert lib.gs_grad_clip_dev(None, ctypes.addressof(i), ctypes.addressof(o), len(ins), norm,
-                                max_norm, None) == L.GS_E_INVALID
+    assert lib.gs_grad_clip_dev(None, ctypes.addressof(i), ctypes.addressof(o), len(ins), kind,
+                                norm, max_norm, ws, size, None) == L.GS_E_INVALID
     text = lib.gs_last_error()
     return b"" if b"null ctx" in text else text
 
@@ -193,4 +193,10 @@ def test_clip_refusals():
     assert b"norm is null" in _clip([a], [b], norm=None)
     assert b"aligned" in _clip([a], [b], norm=0x1002)
     assert b"shares memory" in _clip([a], [b], norm=0x20010)
-    assert _clip([a], [b], norm=0x10010) == b""  # the norm may lie among the inputs
+    assert _clip([a], [b], norm=0x10010) == b""  # a given norm may lie among the inputs
+    for kind in (0, 1):
+        assert _clip([a], [b], kind=kind, ws=0x100000, size=1 << 20) == b""
+        assert b"shares memory" in _clip([a], [b], norm=0x10010, kind=kind, ws=0x100000, size=1 << 20)
+        assert b"workspace" in _clip([a], [b], kind=kind)
+        assert b"workspace" in _clip([a], [b], kind=kind, ws=0x100010, size=1 << 20)
+    assert b"unknown norm" in _clip([a], [b], kind=2)

@@ -288,7 +288,8 @@ def test_c_boundary(ops):
                  (at, 1, 0, norm.data_ptr(), ws.data_ptr(), size - 1),
                  (at, 1, 0, norm.data_ptr(), ws.data_ptr() + 8, size)):
         assert lib.gs_grad_norm_dev(h, *args, st) == L.GS_E_INVALID
-    assert lib.gs_grad_clip_dev(h, at, at, 1, norm.data_ptr(), -1.0, st) == L.GS_E_INVALID
-    assert lib.gs_grad_clip_dev(h, at, at, 1, None, 1.0, st) == L.GS_E_INVALID
+    assert lib.gs_grad_clip_dev(h, at, at, 1, -1, norm.data_ptr(), -1.0, None, 0, st) == L.GS_E_INVALID
+    assert lib.gs_grad_clip_dev(h, at, at, 1, -1, None, 1.0, None, 0, st) == L.GS_E_INVALID
     two = (L.GsTensor * 1)(L.GsTensor(t.data_ptr(), 2, t.numel(), 5, 0, 0))
-    assert lib.gs_grad_clip_dev(h, at, ctypes.addressof(two), 1, norm.data_ptr(), 1.0, st) == L.GS_E_INVALID
+    assert lib.gs_grad_clip_dev(h, at, ctypes.addressof(two), 1, -1, norm.data_ptr(), 1.0,
+                                None, 0, st) == L.GS_E_INVALID
