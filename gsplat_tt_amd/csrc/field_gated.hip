@@ -12,13 +12,7 @@
 // cut into three bf16 parts, whose six products above 2^-24 are added up (field_tiles.h).
 // For bf16 inputs dgate and dup are rounded to bf16 as operands of the next products; the
 // biases' gradients sum them in fp32.
-#include <algorithm>
-
-#include "field.h"
-
-#include "field_act.h"
-#include "field_device.h"
-#include "field_tiles.h"
+#include "field_gated.h"
 
 namespace gs {
 
@@ -66,27 +60,6 @@ __global__ __launch_bounds__(kThreads) void k_gated_parts(GatedArgs a, int64_t n
         }
 #pragma unroll
         for (int p = 0; p < NP; ++p) out[p * total + e] = part[p];
-    }
-}
-
-// 8 values of a row from column c, zeros past `cols`.
-template <typename T>
-__device__ __forceinline__ void load8(const T* row, int64_t c, int64_t cols, float* v) {
-    if (c + 8 <= cols) {
-        load_any<8>(row + c, v);
-    } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? to_float(row[c + k]) : 0.0f;
-    }
-}
-template <int VEC, typename T>
-__device__ __forceinline__ void store_cols(T* row, int64_t c, int64_t cols, const float* v) {
-    if (c + VEC <= cols) {
-        store_any<VEC>(row + c, v);
-    } else {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k)
-            if (c + k < cols) row[c + k] = from_float<T>(v[k]);
     }
 }
 
@@ -458,11 +431,14 @@ hipError_t gated_act(const GatedArgs& a, bool grad, hipStream_t st) {
 
 size_t gated_linear_ws(const GatedArgs& a, bool grad) {
     if (a.n == 0 || is_few(a, grad)) return 0;
+    if (a.dim <= kShortDim) return gated_short_ws(a, grad);
     return GatedPlan(nullptr, a.n, a.hidden, a.dim, a.dtype == 0 ? 3 : 1, grad).bytes;
 }
 
 hipError_t launch_gated_linear(const GatedArgs& a, bool grad, hipStream_t st) {
     if (a.n == 0 && !grad) return hipSuccess;
+    if (a.n > 0 && a.dim <= kShortDim && !is_few(a, grad))
+        return a.dtype == 0 ? gated_short_f32(a, grad, st) : gated_short_bf16(a, grad, st);
     return a.dtype == 0 ? gated_act<float, 3>(a, grad, st) : gated_act<bf16, 1>(a, grad, st);
 }
 

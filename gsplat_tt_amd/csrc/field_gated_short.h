@@ -1,0 +1,522 @@
+// field_gated_short.h - gated projections of rows of up to 128 values (field_gated.hip
+// says what they are). A source file each for fp32 and bf16, which compile side by side.
+#pragma once
+
+#include "field_gated.h"
+
+namespace gs {
+
+namespace {
+
+constexpr int kThreads = kTileThreads;
+
+// Rows of up to 128 values. Both kernels keep tiles of operands in LDS in the order in
+// which the matrix cores take them: block (16 rows), step of 32 of the row, lane; a lane's
+// quad is row lane % 16, values 8 (lane / 16) .. + 7. Rows of an odd quarter are placed by
+// (row ^ 8), so that the transposing loads, which take 4 rows of 16 values for 16 lanes,
+// touch all banks once for two such groups.
+
+__device__ __forceinline__ uint32_t quad_place(uint32_t row, uint32_t quarter) {
+    return (row ^ ((quarter & 1) << 3)) + 16 * quarter;
+}
+// The operand of 16 rows and 32 values as it lies in LDS.
+__device__ __forceinline__ bf16x8 operand_of(const quad* at) {
+    const uint32_t lane = threadIdx.x & 63;
+    return __builtin_bit_cast(bf16x8, at[quad_place(lane & 15, lane >> 4)]);
+}
+// The transposed operand of the 16 values from 16 c and the 32 rows of two blocks, `step`
+// quads apart: rows 4 (lane / 16) .. + 3 of the first, then of the second.
+__device__ __forceinline__ bf16x8 operand_across(const quad* at, int step, int c) {
+    typedef __attribute__((ext_vector_type(4))) short s16x4;
+    typedef __attribute__((address_space(3))) s16x4* lds4;
+    const uint32_t lane = threadIdx.x & 63, s = lane & 15;
+    const uint32_t row = (lane >> 4) * 4 + (s >> 2), quarter = (c & 1) * 2 + ((s & 3) >> 1);
+    const char* p = reinterpret_cast<const char*>(at + (c >> 1) * 64 + quad_place(row, quarter)) +
+                    (s & 1) * 8;
+    s16x4 half[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+        half[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + u * step * 16));
+    return __builtin_bit_cast(bf16x8,
+                              __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
+}
+template <int NP>
+__device__ __forceinline__ void multiply(const bf16x8* a, const bf16x8* b, f32x4& acc) {
+#pragma unroll
+    for (int q = 0; q < Products<NP>::kCount; ++q)
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[Products<NP>::a(q)], b[Products<NP>::b(q)],
+                                                      acc, 0, 0, 0);
+}
+
+// A chunk of the weights, 32 units, as 4 blocks of 16 rows: gate, gate, up, up. PAIRED:
+// block i of two has the units 8 (s / 4) + 4 i + s % 4, so that a lane's sums are 8 units
+// in a row, else 16 i + s.
+template <typename T, int NP, bool PAIRED>
+__device__ __forceinline__ void load_weights(const GatedArgs& a, int64_t u0, int i, int s, int c,
+                                             quad* out) {
+    const int64_t unit = u0 + (PAIRED ? (s >> 2) * 8 + (i & 1) * 4 + (s & 3) : (i & 1) * 16 + s);
+    const bool on = unit < a.hidden;
+    const T* w = static_cast<const T*>(i >= 2 ? a.w_up : a.w_gate);
+    load_parts<T, NP>(w + (on ? unit : 0) * (i >= 2 ? a.up_stride : a.gate_stride), a.dim, c, on,
+                      out);
+}
+// The chunks' parts laid out as LDS takes them, so that fp32 weights are cut once.
+template <typename T, int NP, int KS>
+__global__ __launch_bounds__(kThreads) void k_gated_chunks(GatedArgs a, int64_t chunks,
+                                                           quad* out) {
+    const int64_t total = chunks * (256 * KS);
+    for (int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x; e < total;
+         e += (int64_t)gridDim.x * kThreads) {
+        const int64_t chunk = e / (256 * KS);
+        const int q = (int)(e - chunk * (256 * KS)), lane = q & 63, b = q >> 6;
+        quad part[NP];
+        load_weights<T, NP, true>(a, chunk * 32, b / KS, lane & 15, (b % KS) * 32 + (lane >> 4) * 8,
+                                  part);
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+            out[(chunk * NP + p) * (256 * KS) + b * 64 + quad_place(lane & 15, lane >> 4)] = part[p];
+    }
+}
+
+// Rows stay with their wave, 16 J of them in registers, and the weights pass through LDS
+// chunk by chunk: h, or with GRAD dx, whose sums stay in registers too. The gradients of
+// gate and up leave the sums in the layout that the next product takes them in.
+template <typename T, int NP, int ACT, int KS, int J, bool GRAD>
+__global__ __launch_bounds__(kThreads, NP == 1 || J * KS < 8 ? 2 : 1) void k_gated_rows(
+    GatedArgs a, const quad* laid, int64_t chunks, int64_t per_share) {
+    __shared__ quad lds[NP * 256 * KS];
+    __shared__ float bias[64];
+    const int lane = threadIdx.x & 63, w = wave_id(), g = lane >> 4, s = lane & 15;
+    const int64_t i0 = ((int64_t)blockIdx.x * (kThreads / 64) + w) * (16 * J);
+    const int64_t c0 = blockIdx.y * per_share, c1 = min(chunks, c0 + per_share);
+    quad next[KS][NP];
+    float next_bias = 0.0f;
+    auto fetch = [&](int64_t chunk) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            if (NP > 1) {
+#pragma unroll
+                for (int p = 0; p < NP; ++p)
+                    next[k][p] = laid[(chunk * NP + p) * (256 * KS) + k * 256 + threadIdx.x];
+            } else {
+                const int b = k * 4 + w;
+                load_weights<T, NP, true>(a, chunk * 32, b / KS, s, (b % KS) * 32 + g * 8, next[k]);
+            }
+        }
+        if (threadIdx.x < 64) {
+            const int i = threadIdx.x >> 4;
+            const int64_t unit = chunk * 32 + (s >> 2) * 8 + (i & 1) * 4 + (s & 3);
+            const float* from = i >= 2 ? a.b_up : a.b_gate;
+            next_bias = from != nullptr && unit < a.hidden ? from[unit] : 0.0f;
+        }
+    };
+    if (c0 < c1) fetch(c0);
+    bf16x8 x[J][KS][NP];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const int64_t i = i0 + j * 16 + s;
+        const T* row = static_cast<const T*>(a.x) + (i < a.n ? i : 0) * a.x_stride;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            quad part[NP];
+            load_parts<T, NP>(row, a.dim, k * 32 + g * 8, i < a.n, part);
+#pragma unroll
+            for (int p = 0; p < NP; ++p) x[j][k][p] = __builtin_bit_cast(bf16x8, part[p]);
+        }
+    }
+    constexpr int DB = GRAD ? 2 * KS : 1;
+    f32x4 dx[DB][J];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int j = 0; j < J; ++j) dx[d][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int64_t chunk = c0; chunk < c1; ++chunk) {
+        __syncthreads();  // the last chunk has been read
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+                const int b = k * 4 + w;
+                if (NP > 1) lds[p * (256 * KS) + k * 256 + threadIdx.x] = next[k][p];
+                else lds[b * 64 + quad_place(s, g)] = next[k][p];
+            }
+        if (threadIdx.x < 64) bias[threadIdx.x] = next_bias;
+        __syncthreads();
+        if (chunk + 1 < c1) fetch(chunk + 1);
+        const int64_t u0 = chunk * 32 + g * 8;
+        float d[J][8];
+        if (GRAD) {
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int64_t i = i0 + j * 16 + s;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) d[j][k] = 0.0f;
+                if (i < a.n)
+                    load8(static_cast<const T*>(a.dh) + i * a.dh_stride, u0, a.hidden, d[j]);
+            }
+        }
+        f32x4 z[4][J];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x4 b = *reinterpret_cast<const f32x4*>(bias + i * 16 + g * 4);
+#pragma unroll
+            for (int j = 0; j < J; ++j) z[i][j] = b;
+        }
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                bf16x8 f[NP];
+#pragma unroll
+                for (int p = 0; p < NP; ++p)
+                    f[p] = operand_of(lds + p * (256 * KS) + (i * KS + k) * 64);
+#pragma unroll
+                for (int j = 0; j < J; ++j) multiply<NP>(f, x[j][k], z[i][j]);
+            }
+        if (!GRAD) {
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int64_t i = i0 + j * 16 + s;
+                float h[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    h[k] = act<ACT>(z[k / 4][j][k % 4]) * z[2 + k / 4][j][k % 4];
+                if (i < a.n) store_cols<8>(static_cast<T*>(a.h) + i * a.h_stride, u0, a.hidden, h);
+            }
+            continue;
+        }
+        bf16x8 dz[2][J][NP];
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            float dg[8], du[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float zg = z[k / 4][j][k % 4], zu = z[2 + k / 4][j][k % 4];
+                dg[k] = plain_input<NP>(d[j][k] * zu * act_slope<ACT>(zg));
+                du[k] = plain_input<NP>(d[j][k] * act<ACT>(zg));
+            }
+            if (chunk * 32 + 32 > a.hidden) {  // an infinite x against no weights is NaN
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (u0 + k >= a.hidden) dg[k] = du[k] = 0.0f;
+            }
+            quad part[NP];
+            split8_input<NP>(dg, part);
+#pragma unroll
+            for (int p = 0; p < NP; ++p) dz[0][j][p] = __builtin_bit_cast(bf16x8, part[p]);
+            split8_input<NP>(du, part);
+#pragma unroll
+            for (int p = 0; p < NP; ++p) dz[1][j][p] = __builtin_bit_cast(bf16x8, part[p]);
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int c = 0; c < DB; ++c) {
+                bf16x8 f[NP];
+#pragma unroll
+                for (int p = 0; p < NP; ++p)
+                    f[p] = operand_across(lds + p * (256 * KS) + t * (2 * KS * 64), KS * 64, c);
+#pragma unroll
+                for (int j = 0; j < J; ++j) multiply<NP>(f, dz[t][j], dx[c][j]);
+            }
+    }
+    if (!GRAD) return;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const int64_t i = i0 + j * 16 + s;
+        if (i >= a.n) continue;
+        T* row = static_cast<T*>(a.dx) + i * a.dx_stride;
+#pragma unroll
+        for (int c = 0; c < DB; ++c) {
+            const float v[4] = {dx[c][j][0], dx[c][j][1], dx[c][j][2], dx[c][j][3]};
+            store_cols<4>(row, c * 16 + g * 4, a.dim, v);
+        }
+    }
+}
+
+// The weights' gradients: the weights stay with their wave, 32 units in registers, and the
+// rows pass through LDS, 64 at a time. Here the sums come out with the unit in the lane, so
+// that they are the next product's operand over the rows as they are. WU waves have units
+// of their own; the others share the tile's rows, and leave sums of their own.
+template <typename T, int NP, int ACT, int KS, int WU>
+__global__ __launch_bounds__(kThreads, NP == 1 && KS <= 2 ? 2 : 1) void k_gated_units(
+    GatedArgs a, int64_t tiles, int64_t per_share, int64_t wr, float* part, float* db) {
+    constexpr int WS = kThreads / 64 / WU;
+    __shared__ quad lds[NP * 256 * KS];
+    const int lane = threadIdx.x & 63, w = wave_id(), g = lane >> 4, s = lane & 15;
+    const int wu = w / WS, ws = w % WS;
+    const int64_t u0 = ((int64_t)blockIdx.x * WU + wu) * 32;
+    const int64_t t0 = blockIdx.y * per_share, t1 = min(tiles, t0 + per_share);
+    const int64_t slot = (int64_t)blockIdx.y * WS + ws;
+    bf16x8 wt[4][KS][NP];
+    float b[4], sum[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t unit = u0 + (i & 1) * 16 + s;
+        const float* from = i >= 2 ? a.b_up : a.b_gate;
+        b[i] = from != nullptr && unit < a.hidden ? from[unit] : 0.0f;
+        sum[i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            quad q[NP];
+            load_weights<T, NP, false>(a, u0, i, s, k * 32 + g * 8, q);
+#pragma unroll
+            for (int p = 0; p < NP; ++p) wt[i][k][p] = __builtin_bit_cast(bf16x8, q[p]);
+        }
+    }
+    f32x4 dw[4][2 * KS];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < 2 * KS; ++c) dw[i][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // the next tile's rows: raw values, cut when they are stored
+    constexpr int RAW = sizeof(T) / 2;
+    quad next[KS][RAW];
+    auto fetch = [&](int64_t tile) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            const int blk = k * 4 + w;
+            const int64_t i = tile * 64 + (blk / KS) * 16 + s;
+            const int c = (blk % KS) * 32 + g * 8;
+            const T* row = static_cast<const T*>(a.x) + (i < a.n ? i : 0) * a.x_stride;
+            T v[8];
+            if (i < a.n && c + 8 <= a.dim) {
+                __builtin_memcpy(v, row + c, sizeof(v));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = i < a.n && c + e < a.dim ? row[c + e] : (T)0.0f;
+            }
+            __builtin_memcpy(next[k], v, sizeof(v));
+        }
+    };
+    if (t0 < t1) fetch(t0);
+    for (int64_t tile = t0; tile < t1; ++tile) {
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            quad q[NP];
+            if constexpr (NP == 1) {
+                q[0] = next[k][0];
+            } else {
+                float v[8];
+                __builtin_memcpy(v, next[k], sizeof(v));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = plain_input<NP>(v[e]);
+                split8_input<NP>(v, q);
+            }
+#pragma unroll
+            for (int p = 0; p < NP; ++p)
+                lds[p * (256 * KS) + (k * 4 + w) * 64 + quad_place(s, g)] = q[p];
+        }
+        __syncthreads();
+        if (tile + 1 < t1) fetch(tile + 1);
+#pragma unroll 1
+        for (int half = ws; half < 2; half += WS) {  // 32 rows at a time
+            const int64_t r0 = tile * 64 + half * 32;
+            float d[2][2][4];  // units u0 + 16 v + s, rows r0 + 16 j + 4 g + r
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                const int64_t unit = u0 + v * 16 + s;
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int64_t i = r0 + j * 16 + g * 4 + r;
+                        d[v][j][r] = i < a.n && unit < a.hidden
+                                         ? to_float(static_cast<const T*>(a.dh)[i * a.dh_stride + unit])
+                                         : 0.0f;
+                    }
+            }
+            const quad* at = lds + half * (2 * KS * 64);
+            f32x4 z[4][2];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) z[i][j] = f32x4{b[i], b[i], b[i], b[i]};
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    bf16x8 f[NP];
+#pragma unroll
+                    for (int p = 0; p < NP; ++p)
+                        f[p] = operand_of(at + p * (256 * KS) + (j * KS + k) * 64);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) multiply<NP>(f, wt[i][k], z[i][j]);
+                }
+            bf16x8 dz[4][NP];
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                float dg[8], du[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float zg = z[v][e / 4][e % 4], zu = z[2 + v][e / 4][e % 4];
+                    const bool on = r0 + (e / 4) * 16 + g * 4 + e % 4 < a.n;
+                    dg[e] = on ? plain_input<NP>(d[v][e / 4][e % 4] * zu * act_slope<ACT>(zg)) : 0.0f;
+                    du[e] = on ? plain_input<NP>(d[v][e / 4][e % 4] * act<ACT>(zg)) : 0.0f;
+                    sum[v] += dg[e];
+                    sum[2 + v] += du[e];
+                }
+                quad q[NP];
+                split8_input<NP>(dg, q);
+#pragma unroll
+                for (int p = 0; p < NP; ++p) dz[v][p] = __builtin_bit_cast(bf16x8, q[p]);
+                split8_input<NP>(du, q);
+#pragma unroll
+                for (int p = 0; p < NP; ++p) dz[2 + v][p] = __builtin_bit_cast(bf16x8, q[p]);
+            }
+#pragma unroll
+            for (int c = 0; c < 2 * KS; ++c) {
+                bf16x8 f[NP];
+#pragma unroll
+                for (int p = 0; p < NP; ++p)
+                    f[p] = operand_across(at + p * (256 * KS), KS * 64, c);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) multiply<NP>(f, dz[i], dw[i][c]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t r = u0 * 2 + i * 16 + s;
+        f32x4* to = reinterpret_cast<f32x4*>(part + (slot * wr + r) * (32 * KS));
+#pragma unroll
+        for (int c = 0; c < 2 * KS; ++c) to[c * 4 + g] = dw[i][c];
+        sum[i] += __shfl_xor(sum[i], 16, 64);
+        sum[i] += __shfl_xor(sum[i], 32, 64);
+        if (g == 0) db[slot * wr + r] = sum[i];
+    }
+}
+
+// The slots' sums as the weights' and biases' gradients: 64 quads of columns a workgroup,
+// 16 runs of slots that are joined in order. Row r of 64 is block r / 16 (gate, gate, up,
+// up) of 32 units.
+template <typename T>
+__global__ __launch_bounds__(1024) void k_gated_join(GatedArgs a, const float* part,
+                                                     const float* db, int slots, int64_t wr, int ld) {
+    __shared__ f32x4 lds[16][64];
+    const int lane = threadIdx.x & 63, run = threadIdx.x >> 6;
+    const int64_t quads = wr * (ld / 4), all = quads + wr / 4;
+    const int64_t e = (int64_t)blockIdx.x * 64 + lane;
+    const int per = (slots + 15) / 16, b0 = min(slots, run * per), b1 = min(slots, b0 + per);
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (e < all) {
+        const f32x4* from = reinterpret_cast<const f32x4*>(e < quads ? part : db);
+        const int64_t at = e < quads ? e : e - quads, step = e < quads ? quads : wr / 4;
+#pragma unroll 8
+        for (int b = b0; b < b1; ++b) v += from[b * step + at];
+    }
+    lds[run][lane] = v;
+    __syncthreads();
+    if (run != 0 || e >= all) return;
+#pragma unroll
+    for (int k = 1; k < 16; ++k) v += lds[k][lane];
+    if (e < quads) {
+        const int64_t r = e / (ld / 4), unit = (r >> 6) * 32 + (r & 31);
+        const bool up = (r & 32) != 0;
+        if (unit >= a.hidden) return;
+        T* row = static_cast<T*>(up ? a.dw_up : a.dw_gate) + unit * (up ? a.dup_stride : a.dgate_stride);
+        const float o[4] = {v[0], v[1], v[2], v[3]};
+        store_cols<4>(row, (int)(e - r * (ld / 4)) * 4, a.dim, o);
+    } else {
+        const int64_t r = (e - quads) * 4, unit = (r >> 6) * 32 + (r & 31);
+        float* out = (r & 32) != 0 ? a.db_up : a.db_gate;
+        if (out == nullptr) return;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (unit + k < a.hidden) out[unit + k] = v[k];
+    }
+}
+
+struct ShortPlan {
+    int64_t chunks, tiles, wr;
+    int ks, wu;
+    unsigned unit_blocks, shares;
+    int64_t per_share;
+    int slots;
+    quad* laid;
+    float *part, *db;
+    size_t bytes;
+    ShortPlan(void* base, int64_t n, int64_t hidden, int dim, int np, bool grad) {
+        ks = (dim + 31) / 32;
+        chunks = (hidden + 31) / 32;
+        Carve c(base);
+        laid = np > 1 ? c.take<quad>((size_t)(chunks * np * 256 * ks)) : nullptr;
+        if (grad) {
+            wu = hidden > 64 ? 4 : 2;
+            unit_blocks = (unsigned)((chunks + wu - 1) / wu);
+            wr = (int64_t)unit_blocks * wu * 64;
+            tiles = (n + 63) / 64;
+            const int64_t want = std::max<int64_t>(1, 512 / unit_blocks);
+            per_share = std::max<int64_t>((tiles + want - 1) / want, 1);
+            shares = (unsigned)std::max<int64_t>(1, (tiles + per_share - 1) / per_share);
+            slots = (int)shares * (4 / wu);
+            part = c.take<float>((size_t)slots * wr * 32 * ks);
+            db = c.take<float>((size_t)slots * wr);
+        }
+        bytes = c.bytes();
+    }
+};
+
+template <typename T, int NP, int ACT, int KS, int J, bool GRAD>
+hipError_t rows_run(const GatedArgs& a, const ShortPlan& w, hipStream_t st) {
+    const int64_t blocks = (a.n + 64 * J - 1) / (64 * J);
+    // dx is the sum over all chunks: they are shared out for h alone
+    const int64_t want = GRAD ? 1 : std::min<int64_t>(w.chunks, std::max<int64_t>(1, 512 / blocks));
+    const int64_t per = (w.chunks + want - 1) / want;
+    const dim3 grid((unsigned)blocks, (unsigned)((w.chunks + per - 1) / per));
+    k_gated_rows<T, NP, ACT, KS, J, GRAD><<<grid, kThreads, 0, st>>>(a, w.laid, w.chunks, per);
+    return hipGetLastError();
+}
+
+template <typename T, int NP, int ACT, int KS>
+hipError_t short_run(const GatedArgs& a, bool grad, hipStream_t st) {
+    const ShortPlan w(a.ws, a.n, a.hidden, a.dim, NP, grad);
+    if (NP > 1) {
+        k_gated_chunks<T, NP, KS><<<blocks_of(w.chunks * 256 * KS, kThreads), kThreads, 0, st>>>(
+            a, w.chunks, w.laid);
+        GS_LAUNCHED();
+    }
+    constexpr int kMost = NP == 1 ? 4 : 2, kMostGrad = NP == 1 ? (KS <= 2 ? 4 : 2) : (KS <= 2 ? 2 : 1);
+    if (!grad)
+        return a.n <= 16384 ? rows_run<T, NP, ACT, KS, 1, false>(a, w, st)
+                            : rows_run<T, NP, ACT, KS, kMost, false>(a, w, st);
+    hipError_t e = a.n <= 32768 ? rows_run<T, NP, ACT, KS, 1, true>(a, w, st)
+                                : rows_run<T, NP, ACT, KS, kMostGrad, true>(a, w, st);
+    if (e != hipSuccess) return e;
+    const dim3 grid(w.unit_blocks, w.shares);
+    if (w.wu == 4)
+        k_gated_units<T, NP, ACT, KS, 4><<<grid, kThreads, 0, st>>>(a, w.tiles, w.per_share, w.wr,
+                                                                   w.part, w.db);
+    else
+        k_gated_units<T, NP, ACT, KS, 2><<<grid, kThreads, 0, st>>>(a, w.tiles, w.per_share, w.wr,
+                                                                   w.part, w.db);
+    GS_LAUNCHED();
+    const int64_t quads = w.wr * (32 * KS / 4) + w.wr / 4;
+    k_gated_join<T><<<(unsigned)((quads + 63) / 64), 1024, 0, st>>>(a, w.part, w.db, w.slots, w.wr,
+                                                                    32 * KS);
+    return hipGetLastError();
+}
+
+template <typename T, int NP, int ACT>
+hipError_t short_steps(const GatedArgs& a, bool grad, hipStream_t st) {
+    switch ((a.dim + 31) / 32) {
+        case 1: return short_run<T, NP, ACT, 1>(a, grad, st);
+        case 2: return short_run<T, NP, ACT, 2>(a, grad, st);
+        case 3: return short_run<T, NP, ACT, 3>(a, grad, st);
+        default: return short_run<T, NP, ACT, 4>(a, grad, st);
+    }
+}
+template <typename T, int NP>
+hipError_t short_act(const GatedArgs& a, bool grad, hipStream_t st) {
+    switch (a.act) {
+        case kActRelu: return short_steps<T, NP, kActRelu>(a, grad, st);
+        case kActSilu: return short_steps<T, NP, kActSilu>(a, grad, st);
+        case kActGelu: return short_steps<T, NP, kActGelu>(a, grad, st);
+        default: return short_steps<T, NP, kActNone>(a, grad, st);
+    }
+}
+
+}  // namespace
+
+}  // namespace gs

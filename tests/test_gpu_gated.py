@@ -289,9 +289,11 @@ def test_gradients_match_differences(ops):
         assert abs((grad.cpu().to(D64) * step).sum() - slope) <= 1e-6 * 10 + 100 * EPS * size, name
 
 
-def test_many_rows_in_pieces(ops):
-    """More rows than one piece of the workspace takes: the weights' sums go over pieces."""
-    n, dim, hidden = 90_001, 24, 2000
+@pytest.mark.parametrize("dim", [24, 140])
+def test_many_rows_in_pieces(ops, dim):
+    """More rows than one piece of the workspace takes (of the longer rows): the weights'
+    sums go over pieces."""
+    n, hidden = 90_001, 2000
     g = torch.Generator(device="cuda").manual_seed(12)
 
     def randn(*s):
