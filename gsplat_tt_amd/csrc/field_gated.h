@@ -27,6 +27,22 @@ __device__ __forceinline__ void load8(const T* row, int64_t c, int64_t cols, flo
         for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? to_float(row[c + k]) : 0.0f;
     }
 }
+// VEC values at any address of a T, past the caches.
+template <int VEC, typename T>
+__device__ __forceinline__ void store_past(T* p, const float* in) {
+    T u[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) u[j] = from_float<T>(in[j]);
+    typedef __attribute__((ext_vector_type(4))) uint32_t words;
+    typedef __attribute__((ext_vector_type(4), aligned(2))) uint32_t words_any;
+    static_assert(sizeof(u) % 16 == 0, "whole quads");
+#pragma unroll
+    for (int q = 0; q < (int)(sizeof(u) / 16); ++q) {
+        words w;
+        __builtin_memcpy(&w, reinterpret_cast<const char*>(u) + q * 16, 16);
+        __builtin_nontemporal_store(w, reinterpret_cast<words_any*>(p) + q);
+    }
+}
 template <int VEC, typename T>
 __device__ __forceinline__ void store_cols(T* row, int64_t c, int64_t cols, const float* v) {
     if (c + VEC <= cols) {

@@ -12,27 +12,28 @@ constexpr int kThreads = kTileThreads;
 
 // Rows of up to 128 values. Both kernels keep tiles of operands in LDS in the order in
 // which the matrix cores take them: block (16 rows), step of 32 of the row, lane; a lane's
-// quad is row lane % 16, values 8 (lane / 16) .. + 7. Rows of an odd quarter are placed by
-// (row ^ 8), so that the transposing loads, which take 4 rows of 16 values for 16 lanes,
-// touch all banks once for two such groups.
+// quad is row lane % 16, values 8 (lane / 16) .. + 7. The last two quarters' rows are placed
+// by (row ^ 8), so that the transposing loads, which take 4 rows of 4 x 4 values for 16
+// lanes, touch all banks once for two such groups.
 
 __device__ __forceinline__ uint32_t quad_place(uint32_t row, uint32_t quarter) {
-    return (row ^ ((quarter & 1) << 3)) + 16 * quarter;
+    return (row ^ ((quarter >> 1) << 3)) + 16 * quarter;
 }
 // The operand of 16 rows and 32 values as it lies in LDS.
 __device__ __forceinline__ bf16x8 operand_of(const quad* at) {
     const uint32_t lane = threadIdx.x & 63;
     return __builtin_bit_cast(bf16x8, at[quad_place(lane & 15, lane >> 4)]);
 }
-// The transposed operand of the 16 values from 16 c and the 32 rows of two blocks, `step`
-// quads apart: rows 4 (lane / 16) .. + 3 of the first, then of the second.
-__device__ __forceinline__ bf16x8 operand_across(const quad* at, int step, int c) {
+// The transposed operand of 16 of the 32 values and the 32 rows of two blocks, `step` quads
+// apart: rows 4 (lane / 16) .. + 3 of the first, then of the second. Of quarter q, half b ^
+// (q & 1): a lane's sums of b = 0 and 1 are 8 values in a row, in turned order where the
+// lane's quarter is odd.
+__device__ __forceinline__ bf16x8 operand_across(const quad* at, int step, int b) {
     typedef __attribute__((ext_vector_type(4))) short s16x4;
     typedef __attribute__((address_space(3))) s16x4* lds4;
-    const uint32_t lane = threadIdx.x & 63, s = lane & 15;
-    const uint32_t row = (lane >> 4) * 4 + (s >> 2), quarter = (c & 1) * 2 + ((s & 3) >> 1);
-    const char* p = reinterpret_cast<const char*>(at + (c >> 1) * 64 + quad_place(row, quarter)) +
-                    (s & 1) * 8;
+    const uint32_t lane = threadIdx.x & 63, s = lane & 15, q = s & 3;
+    const char* p = reinterpret_cast<const char*>(at + quad_place((lane >> 4) * 4 + (s >> 2), q)) +
+                    ((b ^ q) & 1) * 8;
     s16x4 half[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -40,21 +41,51 @@ __device__ __forceinline__ bf16x8 operand_across(const quad* at, int step, int c
     return __builtin_bit_cast(bf16x8,
                               __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7));
 }
-template <int NP>
-__device__ __forceinline__ void multiply(const bf16x8* a, const bf16x8* b, f32x4& acc) {
+// acc(m, n) += a[m] b[n]; neighbouring products go to different sums, which spares the wait
+// of one for the other.
+template <int NP, int M, int N, class Acc>
+__device__ __forceinline__ void multiply(const bf16x8 (&a)[M][NP], const bf16x8 (&b)[N][NP],
+                                         Acc acc) {
 #pragma unroll
     for (int q = 0; q < Products<NP>::kCount; ++q)
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[Products<NP>::a(q)], b[Products<NP>::b(q)],
-                                                      acc, 0, 0, 0);
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                f32x4& c = acc(m, n);
+                c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[m][Products<NP>::a(q)],
+                                                            b[n][Products<NP>::b(q)], c, 0, 0, 0);
+            }
 }
 
-// A chunk of the weights, 32 units, as 4 blocks of 16 rows: gate, gate, up, up. PAIRED:
-// block i of two has the units 8 (s / 4) + 4 i + s % 4, so that a lane's sums are 8 units
-// in a row, else 16 i + s.
-template <typename T, int NP, bool PAIRED>
+// 8 values as they lie in memory, at any address; zeros from column `cols` on.
+template <typename T>
+struct Raw {
+    quad q[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* row, int64_t c, int64_t cols) {
+        T v[8];
+        if (c + 8 <= cols) {
+            __builtin_memcpy(v, row + c, sizeof(v));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? row[c + e] : (T)0.0f;
+        }
+        __builtin_memcpy(q, v, sizeof(v));
+    }
+    __device__ __forceinline__ float operator[](int k) const {
+        if constexpr (sizeof(T) == 2)
+            return __uint_as_float(k & 1 ? q[0][k / 2] & 0xFFFF0000u : q[0][k / 2] << 16);
+        else
+            return __uint_as_float(q[k / 4][k % 4]);
+    }
+};
+
+// A chunk of the weights, 32 units, as 4 blocks of 16 rows: gate, gate, up, up; block i of
+// two has the units 8 (s / 4) + 4 i + s % 4, so that a lane's sums are 8 units in a row.
+template <typename T, int NP>
 __device__ __forceinline__ void load_weights(const GatedArgs& a, int64_t u0, int i, int s, int c,
                                              quad* out) {
-    const int64_t unit = u0 + (PAIRED ? (s >> 2) * 8 + (i & 1) * 4 + (s & 3) : (i & 1) * 16 + s);
+    const int64_t unit = u0 + (s >> 2) * 8 + (i & 1) * 4 + (s & 3);
     const bool on = unit < a.hidden;
     const T* w = static_cast<const T*>(i >= 2 ? a.w_up : a.w_gate);
     load_parts<T, NP>(w + (on ? unit : 0) * (i >= 2 ? a.up_stride : a.gate_stride), a.dim, c, on,
@@ -70,7 +101,7 @@ __global__ __launch_bounds__(kThreads) void k_gated_chunks(GatedArgs a, int64_t 
         const int64_t chunk = e / (256 * KS);
         const int q = (int)(e - chunk * (256 * KS)), lane = q & 63, b = q >> 6;
         quad part[NP];
-        load_weights<T, NP, true>(a, chunk * 32, b / KS, lane & 15, (b % KS) * 32 + (lane >> 4) * 8,
+        load_weights<T, NP>(a, chunk * 32, b / KS, lane & 15, (b % KS) * 32 + (lane >> 4) * 8,
                                   part);
 #pragma unroll
         for (int p = 0; p < NP; ++p)
@@ -90,8 +121,17 @@ __global__ __launch_bounds__(kThreads, NP == 1 || J * KS < 8 ? 2 : 1) void k_gat
     const int64_t i0 = ((int64_t)blockIdx.x * (kThreads / 64) + w) * (16 * J);
     const int64_t c0 = blockIdx.y * per_share, c1 = min(chunks, c0 + per_share);
     quad next[KS][NP];
+    Raw<T> next_d[J];
     float next_bias = 0.0f;
     auto fetch = [&](int64_t chunk) {
+        if (GRAD) {
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int64_t i = i0 + j * 16 + s;
+                next_d[j].load(static_cast<const T*>(a.dh) + (i < a.n ? i : 0) * a.dh_stride,
+                               chunk * 32 + g * 8, i < a.n ? a.hidden : 0);
+            }
+        }
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
             if (NP > 1) {
@@ -100,7 +140,7 @@ __global__ __launch_bounds__(kThreads, NP == 1 || J * KS < 8 ? 2 : 1) void k_gat
                     next[k][p] = laid[(chunk * NP + p) * (256 * KS) + k * 256 + threadIdx.x];
             } else {
                 const int b = k * 4 + w;
-                load_weights<T, NP, true>(a, chunk * 32, b / KS, s, (b % KS) * 32 + g * 8, next[k]);
+                load_weights<T, NP>(a, chunk * 32, b / KS, s, (b % KS) * 32 + g * 8, next[k]);
             }
         }
         if (threadIdx.x < 64) {
@@ -111,7 +151,7 @@ __global__ __launch_bounds__(kThreads, NP == 1 || J * KS < 8 ? 2 : 1) void k_gat
         }
     };
     if (c0 < c1) fetch(c0);
-    bf16x8 x[J][KS][NP];
+    bf16x8 x[KS][J][NP];
 #pragma unroll
     for (int j = 0; j < J; ++j) {
         const int64_t i = i0 + j * 16 + s;
@@ -121,7 +161,7 @@ __global__ __launch_bounds__(kThreads, NP == 1 || J * KS < 8 ? 2 : 1) void k_gat
             quad part[NP];
             load_parts<T, NP>(row, a.dim, k * 32 + g * 8, i < a.n, part);
 #pragma unroll
-            for (int p = 0; p < NP; ++p) x[j][k][p] = __builtin_bit_cast(bf16x8, part[p]);
+            for (int p = 0; p < NP; ++p) x[k][j][p] = __builtin_bit_cast(bf16x8, part[p]);
         }
     }
     constexpr int DB = GRAD ? 2 * KS : 1;
@@ -141,20 +181,14 @@ __global__ __launch_bounds__(kThreads, NP == 1 || J * KS < 8 ? 2 : 1) void k_gat
                 else lds[b * 64 + quad_place(s, g)] = next[k][p];
             }
         if (threadIdx.x < 64) bias[threadIdx.x] = next_bias;
+        Raw<T> d[J];
+        if (GRAD) {
+#pragma unroll
+            for (int j = 0; j < J; ++j) d[j] = next_d[j];
+        }
         __syncthreads();
         if (chunk + 1 < c1) fetch(chunk + 1);
         const int64_t u0 = chunk * 32 + g * 8;
-        float d[J][8];
-        if (GRAD) {
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                const int64_t i = i0 + j * 16 + s;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) d[j][k] = 0.0f;
-                if (i < a.n)
-                    load8(static_cast<const T*>(a.dh) + i * a.dh_stride, u0, a.hidden, d[j]);
-            }
-        }
         f32x4 z[4][J];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -165,13 +199,14 @@ __global__ __launch_bounds__(kThreads, NP == 1 || J * KS < 8 ? 2 : 1) void k_gat
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                bf16x8 f[NP];
+            for (int i = 0; i < 4; i += 2) {
+                bf16x8 f[2][NP];
 #pragma unroll
-                for (int p = 0; p < NP; ++p)
-                    f[p] = operand_of(lds + p * (256 * KS) + (i * KS + k) * 64);
+                for (int m = 0; m < 2; ++m)
 #pragma unroll
-                for (int j = 0; j < J; ++j) multiply<NP>(f, x[j][k], z[i][j]);
+                    for (int p = 0; p < NP; ++p)
+                        f[m][p] = operand_of(lds + p * (256 * KS) + ((i + m) * KS + k) * 64);
+                multiply<NP>(f, x[k], [&](int m, int j) -> f32x4& { return z[i + m][j]; });
             }
         if (!GRAD) {
 #pragma unroll
@@ -181,7 +216,11 @@ __global__ __launch_bounds__(kThreads, NP == 1 || J * KS < 8 ? 2 : 1) void k_gat
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
                     h[k] = act<ACT>(z[k / 4][j][k % 4]) * z[2 + k / 4][j][k % 4];
-                if (i < a.n) store_cols<8>(static_cast<T*>(a.h) + i * a.h_stride, u0, a.hidden, h);
+                if (i < a.n) {
+                    T* row = static_cast<T*>(a.h) + i * a.h_stride;
+                    if (u0 + 8 <= a.hidden) store_past<8>(row + u0, h);
+                    else store_cols<8>(row, u0, a.hidden, h);
+                }
             }
             continue;
         }
@@ -211,13 +250,15 @@ __global__ __launch_bounds__(kThreads, NP == 1 || J * KS < 8 ? 2 : 1) void k_gat
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int c = 0; c < DB; ++c) {
-                bf16x8 f[NP];
+            for (int k = 0; k < KS; ++k) {
+                bf16x8 f[2][NP];
 #pragma unroll
-                for (int p = 0; p < NP; ++p)
-                    f[p] = operand_across(lds + p * (256 * KS) + t * (2 * KS * 64), KS * 64, c);
+                for (int m = 0; m < 2; ++m)
 #pragma unroll
-                for (int j = 0; j < J; ++j) multiply<NP>(f, dz[t][j], dx[c][j]);
+                    for (int p = 0; p < NP; ++p)
+                        f[m][p] = operand_across(
+                            lds + p * (256 * KS) + t * (2 * KS * 64) + k * 64, KS * 64, m);
+                multiply<NP>(f, dz[t], [&](int m, int j) -> f32x4& { return dx[2 * k + m][j]; });
             }
     }
     if (!GRAD) return;
@@ -227,66 +268,87 @@ __global__ __launch_bounds__(kThreads, NP == 1 || J * KS < 8 ? 2 : 1) void k_gat
         if (i >= a.n) continue;
         T* row = static_cast<T*>(a.dx) + i * a.dx_stride;
 #pragma unroll
-        for (int c = 0; c < DB; ++c) {
-            const float v[4] = {dx[c][j][0], dx[c][j][1], dx[c][j][2], dx[c][j][3]};
-            store_cols<4>(row, c * 16 + g * 4, a.dim, v);
+        for (int k = 0; k < KS; ++k) {
+            const int c = k * 32 + g * 8;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                v[e] = (g & 1) != e / 4 ? dx[2 * k + 1][j][e % 4] : dx[2 * k][j][e % 4];
+            if (c + 8 <= a.dim) store_past<8>(row + c, v);
+            else store_cols<8>(row, c, a.dim, v);
         }
     }
 }
 
-// The weights' gradients: the weights stay with their wave, 32 units in registers, and the
-// rows pass through LDS, 64 at a time. Here the sums come out with the unit in the lane, so
-// that they are the next product's operand over the rows as they are. WU waves have units
-// of their own; the others share the tile's rows, and leave sums of their own.
+// The weights' gradients: the weights stay with their wave, 16 VB units in registers, and
+// the rows pass through LDS, 64 at a time. Here the sums come out with the unit in the lane,
+// so that they are the next product's operand over the rows as they are; dh turns on its
+// way through LDS, in a part of its own for each wave. WU waves have units of their own;
+// the others share the tile's rows, and leave sums of their own.
+template <typename T>
+constexpr int kUnitBlocks = sizeof(T) == 2 ? 2 : 1;  // 64 bytes of a row of dh
+
 template <typename T, int NP, int ACT, int KS, int WU>
-__global__ __launch_bounds__(kThreads, NP == 1 && KS <= 2 ? 2 : 1) void k_gated_units(
+__global__ __launch_bounds__(kThreads, KS <= 2 ? 2 : 1) void k_gated_units(
     GatedArgs a, int64_t tiles, int64_t per_share, int64_t wr, float* part, float* db) {
-    constexpr int WS = kThreads / 64 / WU;
+    constexpr int WS = kThreads / 64 / WU, VB = kUnitBlocks<T>, NB = 2 * VB;
+    constexpr int DQ = 4 / WS;  // quads of dh of a lane
     __shared__ quad lds[NP * 256 * KS];
+    __shared__ quad dh_lds[4][64 * DQ];
     const int lane = threadIdx.x & 63, w = wave_id(), g = lane >> 4, s = lane & 15;
     const int wu = w / WS, ws = w % WS;
-    const int64_t u0 = ((int64_t)blockIdx.x * WU + wu) * 32;
+    const int64_t u0 = ((int64_t)blockIdx.x * WU + wu) * (16 * VB);
     const int64_t t0 = blockIdx.y * per_share, t1 = min(tiles, t0 + per_share);
     const int64_t slot = (int64_t)blockIdx.y * WS + ws;
-    bf16x8 wt[4][KS][NP];
-    float b[4], sum[4];
+    bf16x8 wt[KS][NB][NP];
+    float b[NB], sum[NB];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t unit = u0 + (i & 1) * 16 + s;
-        const float* from = i >= 2 ? a.b_up : a.b_gate;
-        b[i] = from != nullptr && unit < a.hidden ? from[unit] : 0.0f;
+    for (int i = 0; i < NB; ++i) {
+        const int64_t unit = u0 + (i % VB) * 16 + s;
+        const bool on = unit < a.hidden;
+        const float* bias = i >= VB ? a.b_up : a.b_gate;
+        const T* row = static_cast<const T*>(i >= VB ? a.w_up : a.w_gate) +
+                       (on ? unit : 0) * (i >= VB ? a.up_stride : a.gate_stride);
+        b[i] = bias != nullptr && on ? bias[unit] : 0.0f;
         sum[i] = 0.0f;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
             quad q[NP];
-            load_weights<T, NP, false>(a, u0, i, s, k * 32 + g * 8, q);
+            load_parts<T, NP>(row, a.dim, k * 32 + g * 8, on, q);
 #pragma unroll
-            for (int p = 0; p < NP; ++p) wt[i][k][p] = __builtin_bit_cast(bf16x8, q[p]);
+            for (int p = 0; p < NP; ++p) wt[k][i][p] = __builtin_bit_cast(bf16x8, q[p]);
         }
     }
-    f32x4 dw[4][2 * KS];
+    f32x4 dw[NB][2 * KS];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < NB; ++i)
 #pragma unroll
         for (int c = 0; c < 2 * KS; ++c) dw[i][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    // the next tile's rows: raw values, cut when they are stored
-    constexpr int RAW = sizeof(T) / 2;
-    quad next[KS][RAW];
+    // the next tile's x and dh, cut when they are stored
+    Raw<T> next[KS];
+    quad next_d[DQ];
     auto fetch = [&](int64_t tile) {
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
             const int blk = k * 4 + w;
             const int64_t i = tile * 64 + (blk / KS) * 16 + s;
-            const int c = (blk % KS) * 32 + g * 8;
-            const T* row = static_cast<const T*>(a.x) + (i < a.n ? i : 0) * a.x_stride;
-            T v[8];
-            if (i < a.n && c + 8 <= a.dim) {
+            next[k].load(static_cast<const T*>(a.x) + (i < a.n ? i : 0) * a.x_stride,
+                         (blk % KS) * 32 + g * 8, i < a.n ? a.dim : 0);
+        }
+#pragma unroll
+        for (int k = 0; k < DQ; ++k) {
+            constexpr int V = 16 / sizeof(T);
+            const int64_t i = tile * 64 + ws * (64 / WS) + k * 16 + (lane >> 2);
+            const int64_t c = u0 + (lane & 3) * V, cols = i < a.n ? a.hidden : 0;
+            const T* row = static_cast<const T*>(a.dh) + (i < a.n ? i : 0) * a.dh_stride;
+            T v[V];
+            if (c + V <= cols) {
                 __builtin_memcpy(v, row + c, sizeof(v));
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = i < a.n && c + e < a.dim ? row[c + e] : (T)0.0f;
+                for (int e = 0; e < V; ++e) v[e] = c + e < cols ? row[c + e] : (T)0.0f;
             }
-            __builtin_memcpy(next[k], v, sizeof(v));
+            __builtin_memcpy(&next_d[k], v, sizeof(v));
         }
     };
     if (t0 < t1) fetch(t0);
@@ -296,66 +358,87 @@ __global__ __launch_bounds__(kThreads, NP == 1 && KS <= 2 ? 2 : 1) void k_gated_
         for (int k = 0; k < KS; ++k) {
             quad q[NP];
             if constexpr (NP == 1) {
-                q[0] = next[k][0];
+                q[0] = next[k].q[0];
             } else {
                 float v[8];
-                __builtin_memcpy(v, next[k], sizeof(v));
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = plain_input<NP>(v[e]);
+                for (int e = 0; e < 8; ++e) v[e] = plain_input<NP>(next[k][e]);
                 split8_input<NP>(v, q);
             }
 #pragma unroll
             for (int p = 0; p < NP; ++p)
                 lds[p * (256 * KS) + (k * 4 + w) * 64 + quad_place(s, g)] = q[p];
         }
+        // a row's 64 bytes: bf16's 32-byte halves change places every fourth row, fp32's
+        // rows within 4, so that rows 4 apart lie in other banks
+#pragma unroll
+        for (int k = 0; k < DQ; ++k) {
+            const int r = k * 16 + (lane >> 2), q = lane & 3;
+            dh_lds[w][sizeof(T) == 2 ? r * 4 + (q ^ ((r >> 2 & 1) << 1))
+                                     : (r ^ (r >> 2 & 3)) * 4 + q] = next_d[k];
+        }
         __syncthreads();
         if (tile + 1 < t1) fetch(tile + 1);
 #pragma unroll 1
         for (int half = ws; half < 2; half += WS) {  // 32 rows at a time
-            const int64_t r0 = tile * 64 + half * 32;
-            float d[2][2][4];  // units u0 + 16 v + s, rows r0 + 16 j + 4 g + r
-#pragma unroll
-            for (int v = 0; v < 2; ++v) {
-                const int64_t unit = u0 + v * 16 + s;
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int64_t i = r0 + j * 16 + g * 4 + r;
-                        d[v][j][r] = i < a.n && unit < a.hidden
-                                         ? to_float(static_cast<const T*>(a.dh)[i * a.dh_stride + unit])
-                                         : 0.0f;
-                    }
-            }
             const quad* at = lds + half * (2 * KS * 64);
-            f32x4 z[4][2];
+            f32x4 z[NB][2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < NB; ++i)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) z[i][j] = f32x4{b[i], b[i], b[i], b[i]};
 #pragma unroll
-            for (int k = 0; k < KS; ++k)
+            for (int k = 0; k < KS; ++k) {
+                bf16x8 f[2][NP];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    bf16x8 f[NP];
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int p = 0; p < NP; ++p)
-                        f[p] = operand_of(at + p * (256 * KS) + (j * KS + k) * 64);
+                        f[j][p] = operand_of(at + p * (256 * KS) + (j * KS + k) * 64);
+                multiply<NP>(f, wt[k], [&](int j, int i) -> f32x4& { return z[i][j]; });
+            }
+            const int64_t left = a.n - (tile * 64 + half * 32);
+            bf16x8 dz[NB][NP];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) multiply<NP>(f, wt[i][k], z[i][j]);
+            for (int v = 0; v < VB; ++v) {
+                // units u0 + 16 v + s, rows 16 j + 4 g + r of the 32
+                float d[8];
+                const char* from = reinterpret_cast<const char*>(dh_lds[w] + (half - ws) * 128);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    if constexpr (sizeof(T) == 2) {
+                        typedef __attribute__((ext_vector_type(4))) short s16x4;
+                        typedef __attribute__((address_space(3))) s16x4* lds4;
+                        const int r = j * 16 + g * 4 + (s >> 2);
+                        const s16x4 q = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (lds4)(from + r * 64 + ((v ^ (g & 1)) * 32) + (s & 3) * 8));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            d[j * 4 + e] = __uint_as_float((uint32_t)(uint16_t)q[e] << 16);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int r = j * 16 + g * 4 + (e ^ g);
+                            d[j * 4 + e] = *reinterpret_cast<const float*>(from + r * 64 + s * 4);
+                        }
+                    }
                 }
-            bf16x8 dz[4][NP];
-#pragma unroll
-            for (int v = 0; v < 2; ++v) {
                 float dg[8], du[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float zg = z[v][e / 4][e % 4], zu = z[2 + v][e / 4][e % 4];
-                    const bool on = r0 + (e / 4) * 16 + g * 4 + e % 4 < a.n;
-                    dg[e] = on ? plain_input<NP>(d[v][e / 4][e % 4] * zu * act_slope<ACT>(zg)) : 0.0f;
-                    du[e] = on ? plain_input<NP>(d[v][e / 4][e % 4] * act<ACT>(zg)) : 0.0f;
+                    const float zg = z[v][e / 4][e % 4], zu = z[VB + v][e / 4][e % 4];
+                    dg[e] = plain_input<NP>(d[e] * zu * act_slope<ACT>(zg));
+                    du[e] = plain_input<NP>(d[e] * act<ACT>(zg));
+                }
+                if (left < 32) {  // an infinite bias against a dh of 0 is NaN
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if ((e / 4) * 16 + g * 4 + e % 4 >= left) dg[e] = du[e] = 0.0f;
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
                     sum[v] += dg[e];
-                    sum[2 + v] += du[e];
+                    sum[VB + v] += du[e];
                 }
                 quad q[NP];
                 split8_input<NP>(dg, q);
@@ -363,25 +446,28 @@ __global__ __launch_bounds__(kThreads, NP == 1 && KS <= 2 ? 2 : 1) void k_gated_
                 for (int p = 0; p < NP; ++p) dz[v][p] = __builtin_bit_cast(bf16x8, q[p]);
                 split8_input<NP>(du, q);
 #pragma unroll
-                for (int p = 0; p < NP; ++p) dz[2 + v][p] = __builtin_bit_cast(bf16x8, q[p]);
+                for (int p = 0; p < NP; ++p) dz[VB + v][p] = __builtin_bit_cast(bf16x8, q[p]);
             }
 #pragma unroll
-            for (int c = 0; c < 2 * KS; ++c) {
-                bf16x8 f[NP];
+            for (int k = 0; k < KS; ++k) {
+                bf16x8 f[2][NP];
 #pragma unroll
-                for (int p = 0; p < NP; ++p)
-                    f[p] = operand_across(at + p * (256 * KS), KS * 64, c);
+                for (int m = 0; m < 2; ++m)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) multiply<NP>(f, dz[i], dw[i][c]);
+                    for (int p = 0; p < NP; ++p)
+                        f[m][p] = operand_across(at + p * (256 * KS) + k * 64, KS * 64, m);
+                multiply<NP>(f, dz, [&](int m, int i) -> f32x4& { return dw[i][2 * k + m]; });
             }
         }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < NB; ++i) {
         const int64_t r = u0 * 2 + i * 16 + s;
         f32x4* to = reinterpret_cast<f32x4*>(part + (slot * wr + r) * (32 * KS));
 #pragma unroll
-        for (int c = 0; c < 2 * KS; ++c) to[c * 4 + g] = dw[i][c];
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int m = 0; m < 2; ++m) to[k * 8 + g * 2 + (m ^ (g & 1))] = dw[i][2 * k + m];
         sum[i] += __shfl_xor(sum[i], 16, 64);
         sum[i] += __shfl_xor(sum[i], 32, 64);
         if (g == 0) db[slot * wr + r] = sum[i];
@@ -389,11 +475,12 @@ __global__ __launch_bounds__(kThreads, NP == 1 && KS <= 2 ? 2 : 1) void k_gated_
 }
 
 // The slots' sums as the weights' and biases' gradients: 64 quads of columns a workgroup,
-// 16 runs of slots that are joined in order. Row r of 64 is block r / 16 (gate, gate, up,
-// up) of 32 units.
+// 16 runs of slots that are joined in order. The rows are 16 VB gate rows and the same units' up
+// rows by turns.
 template <typename T>
 __global__ __launch_bounds__(1024) void k_gated_join(GatedArgs a, const float* part,
                                                      const float* db, int slots, int64_t wr, int ld) {
+    constexpr int U = 16 * kUnitBlocks<T>;
     __shared__ f32x4 lds[16][64];
     const int lane = threadIdx.x & 63, run = threadIdx.x >> 6;
     const int64_t quads = wr * (ld / 4), all = quads + wr / 4;
@@ -412,15 +499,15 @@ __global__ __launch_bounds__(1024) void k_gated_join(GatedArgs a, const float* p
 #pragma unroll
     for (int k = 1; k < 16; ++k) v += lds[k][lane];
     if (e < quads) {
-        const int64_t r = e / (ld / 4), unit = (r >> 6) * 32 + (r & 31);
-        const bool up = (r & 32) != 0;
+        const int64_t r = e / (ld / 4), unit = r / (2 * U) * U + r % U;
+        const bool up = (r & U) != 0;
         if (unit >= a.hidden) return;
         T* row = static_cast<T*>(up ? a.dw_up : a.dw_gate) + unit * (up ? a.dup_stride : a.dgate_stride);
         const float o[4] = {v[0], v[1], v[2], v[3]};
         store_cols<4>(row, (int)(e - r * (ld / 4)) * 4, a.dim, o);
     } else {
-        const int64_t r = (e - quads) * 4, unit = (r >> 6) * 32 + (r & 31);
-        float* out = (r & 32) != 0 ? a.db_up : a.db_gate;
+        const int64_t r = (e - quads) * 4, unit = r / (2 * U) * U + r % U;
+        float* out = (r & U) != 0 ? a.db_up : a.db_gate;
         if (out == nullptr) return;
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -443,9 +530,10 @@ struct ShortPlan {
         Carve c(base);
         laid = np > 1 ? c.take<quad>((size_t)(chunks * np * 256 * ks)) : nullptr;
         if (grad) {
-            wu = hidden > 64 ? 4 : 2;
-            unit_blocks = (unsigned)((chunks + wu - 1) / wu);
-            wr = (int64_t)unit_blocks * wu * 64;
+            const int64_t units = np > 1 ? 16 : 32;  // of a wave
+            wu = hidden > 2 * units ? 4 : 2;
+            unit_blocks = (unsigned)((hidden + wu * units - 1) / (wu * units));
+            wr = (int64_t)unit_blocks * wu * 2 * units;
             tiles = (n + 63) / 64;
             const int64_t want = std::max<int64_t>(1, 512 / unit_blocks);
             per_share = std::max<int64_t>((tiles + want - 1) / want, 1);
@@ -477,7 +565,7 @@ hipError_t short_run(const GatedArgs& a, bool grad, hipStream_t st) {
             a, w.chunks, w.laid);
         GS_LAUNCHED();
     }
-    constexpr int kMost = NP == 1 ? 4 : 2, kMostGrad = NP == 1 ? (KS <= 2 ? 4 : 2) : (KS <= 2 ? 2 : 1);
+    constexpr int kMost = NP == 1 ? 4 : 2, kMostGrad = NP == 1 ? 2 : (KS <= 2 ? 2 : 1);
     if (!grad)
         return a.n <= 16384 ? rows_run<T, NP, ACT, KS, 1, false>(a, w, st)
                             : rows_run<T, NP, ACT, KS, kMost, false>(a, w, st);
