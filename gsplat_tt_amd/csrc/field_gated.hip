@@ -12,7 +12,10 @@
 // cut into three bf16 parts, whose six products above 2^-24 are added up (field_tiles.h).
 // For bf16 inputs dgate and dup are rounded to bf16 as operands of the next products; the
 // biases' gradients sum them in fp32.
+#include <type_traits>
+
 #include "field_gated.h"
+#include "field_wide.h"
 
 namespace gs {
 
@@ -212,48 +215,233 @@ __global__ __launch_bounds__(kThreads, 2) void k_gated_dw(Mat X, Mat Z, int64_t 
         });
 }
 
-// The shares' sums as the weights' gradients: 4 columns a thread.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void k_gated_dw_sum(GatedArgs a, const float* part,
-                                                           int shares, int64_t wr, int ld) {
-    const int units = ld / 4;
-    const int64_t total = wr * units;
-    for (int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x; e < total;
-         e += (int64_t)gridDim.x * kThreads) {
-        const int64_t r = e / units;
-        const int c = (int)(e - r * units) * 4;
-        const UnitOf u = unit_of(r);
-        if (u.unit >= a.hidden || c >= a.dim) continue;
-        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int k = 0; k < shares; ++k)
-            v += *reinterpret_cast<const f32x4*>(part + (k * wr + r) * ld + c);
+// The shares' sums as the weights' gradients, and the sums over blocks of samples as the
+// biases' (onto what an earlier piece left with `add`): 64 quads of columns a workgroup, 16
+// runs that are joined in order. WIDE: the weights' rows in the wide tiles' order.
+template <typename T, bool WIDE, bool BIASES>
+__global__ __launch_bounds__(1024) void k_gated_sum(GatedArgs a, const float* part, int shares,
+                                                    int64_t wr, int ld, int add) {
+    __shared__ f32x4 lds[16][64];
+    const int lane = threadIdx.x & 63, run = threadIdx.x >> 6;
+    const int64_t quads = BIASES ? wr / 4 : wr * (ld / 4), e = (int64_t)blockIdx.x * 64 + lane;
+    const int per = (shares + 15) / 16, b0 = min(shares, run * per), b1 = min(shares, b0 + per);
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (e < quads) {
+        const f32x4* from = reinterpret_cast<const f32x4*>(part) + e;
+#pragma unroll 8
+        for (int b = b0; b < b1; ++b) v += from[b * quads];
+    }
+    lds[run][lane] = v;
+    __syncthreads();
+    if (run != 0 || e >= quads) return;
+#pragma unroll
+    for (int k = 1; k < 16; ++k) v += lds[k][lane];
+    const int64_t r = BIASES ? e * 4 : e / (ld / 4);
+    // a quad of rows has 4 units in a row, all gate or all up, in either order
+    const UnitOf u = WIDE ? UnitOf{(r >> 4) * 8 + (r & 7), (r & 8) != 0} : unit_of(r);
+    if (u.unit >= a.hidden) return;
+    if (BIASES) {
+        float* out = u.up ? a.db_up : a.db_gate;
+        if (out == nullptr) return;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (u.unit + k < a.hidden) out[u.unit + k] = add ? out[u.unit + k] + v[k] : v[k];
+    } else {
         T* row = static_cast<T*>(u.up ? a.dw_up : a.dw_gate) +
                  u.unit * (u.up ? a.dup_stride : a.dgate_stride);
         const float o[4] = {v[0], v[1], v[2], v[3]};
-        store_cols<4>(row, c, a.dim, o);
+        store_cols<4>(row, (e - r * (ld / 4)) * 4, a.dim, o);
+    }
+}
+unsigned sum_blocks(int64_t quads) { return (unsigned)((quads + 63) / 64); }
+
+// ---------------------------------------------------------------- wide tiles
+// The same products in the tiles of field_wide.h, where there are enough of them to
+// fill the chip. The weights' rows lie in groups of 16, 8 gate and the same 8 up rows, so
+// that with spread blocks a lane's sums are 8 units in a row of both, and its dgate and dup
+// 32 bytes in a row. bf16 rows of x that are aligned are read where they are.
+template <typename T, int NP>
+__global__ __launch_bounds__(kThreads) void k_wide_weights(GatedArgs a, int64_t wr, int ld,
+                                                           quad* out, quad* zero) {
+    const int units = ld / 8;
+    const int64_t total = wr * units;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *zero = quad{0u, 0u, 0u, 0u};
+    for (int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x; e < total;
+         e += (int64_t)gridDim.x * kThreads) {
+        const int64_t r = e / units, unit = (r >> 4) * 8 + (r & 7);
+        const bool on = unit < a.hidden, up = (r & 8) != 0;
+        const T* w = static_cast<const T*>(up ? a.w_up : a.w_gate);
+        quad part[NP];
+        load_parts<T, NP>(w + (on ? unit : 0) * (up ? a.up_stride : a.gate_stride), a.dim,
+                          (int)(e - r * units) * 8, on, part);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) out[p * total + e] = part[p];
     }
 }
 
-// The biases' gradients: sums over the blocks of 64 samples, in 16 runs a row that are
-// joined in order; with `add` onto what an earlier piece left.
-__global__ __launch_bounds__(kThreads) void k_gated_db(GatedArgs a, const float* db,
-                                                       int64_t blocks, int64_t wr, int add) {
-    __shared__ float lds[16][16];
-    const int c = threadIdx.x & 15, k = threadIdx.x >> 4;
-    const int64_t r = (int64_t)blockIdx.x * 16 + c;
-    const int64_t per = (blocks + 15) / 16, b1 = min(blocks, (k + 1) * per);
-    float v = 0.0f;
-    for (int64_t b = k * per; b < b1; ++b) v += db[b * wr + r];
-    lds[k][c] = v;
-    __syncthreads();
-    if (k != 0) return;
-    v = 0.0f;
+template <int NP>
+constexpr int kWideBlocks = NP == 1 ? 8 : 4;  // of 16 rows of A, of a wave
+
+template <typename T, int NP, int ACT, bool GRAD>
+__global__ __launch_bounds__((WideShape<NP, 8>::kThreads), 2) void k_gated_wide(GatedArgs a, WideMat W, WideMat X,
+                                                                int kd, int64_t n0, int64_t nr,
+                                                                int tiles_w, int share, int gy,
+                                                                bf16* dz, float* db) {
+    constexpr int AB = kWideBlocks<NP>;
+    using Shape = WideShape<NP, AB>;
+    __shared__ quad lds[Shape::kQuads];
+    const int lane = threadIdx.x & 63, g = lane >> 4, s = lane & 15;
+    const Spot at = spot((int)(nr / Shape::kCols), gy);
+    const int64_t s0 = (int64_t)at.x * Shape::kCols + Shape::col();
+    const int t0 = at.y * share, t1 = min(tiles_w, t0 + share);
+    if (t0 >= t1) return;
+    const int64_t wr = W.rows;
+    Raw<T> d[AB / 4][GRAD ? 4 : 1];
+    auto row_of = [&](int t) { return (int64_t)(t0 + t) * Shape::kRows + Shape::row(); };
+    wide_products<NP, AB, true, true, true>(
+        W, X, 0, kd, t1 - t0, lds,
+        [&](int t) { return TileRows{(int64_t)(t0 + t) * Shape::kRows, (int64_t)at.x * Shape::kCols}; },
+        [&](int t) {
+            if (!GRAD) return;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v += lds[j][c];
-    const UnitOf u = unit_of(r);
-    float* out = u.up ? a.db_up : a.db_gate;
-    if (out == nullptr || u.unit >= a.hidden) return;
-    out[u.unit] = add ? out[u.unit] + v : v;
+            for (int v = 0; v < AB / 4; ++v)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int64_t i = n0 + s0 + j * 16 + s;
+                    d[v][j].load(static_cast<const T*>(a.dh) + (i < a.n ? i : 0) * a.dh_stride,
+                                 (row_of(t) + v * 64) / 2 + g * 8, i < a.n ? a.hidden : 0);
+                }
+        },
+        [&](int t, f32x4(&acc)[AB][Shape::BB]) {
+#pragma unroll
+            for (int v = 0; v < AB / 4; ++v) {
+                const int64_t r0 = row_of(t) + v * 64, u0 = r0 / 2 + g * 8;
+                const bool whole = r0 / 2 + 32 <= a.hidden;
+                float bg[8], bu[8], sg[8], su[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const bool on = u0 + k < a.hidden;
+                    bg[k] = on && a.b_gate != nullptr ? a.b_gate[u0 + k] : 0.0f;
+                    bu[k] = on && a.b_up != nullptr ? a.b_up[u0 + k] : 0.0f;
+                    sg[k] = su[k] = 0.0f;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int64_t row = s0 + j * 16 + s, i = n0 + row;
+                    float dg[8], du[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float zg = acc[v * 4 + k / 4][j][k % 4] + bg[k];
+                        const float zu = acc[v * 4 + 2 + k / 4][j][k % 4] + bu[k];
+                        if (!GRAD) {
+                            dg[k] = act<ACT>(zg) * zu;
+                        } else {
+                            dg[k] = plain_input<NP>(d[v][j][k] * zu * act_slope<ACT>(zg));
+                            du[k] = plain_input<NP>(d[v][j][k] * act<ACT>(zg));
+                        }
+                    }
+                    if (!GRAD) {
+                        if (i >= a.n) continue;
+                        T* to = static_cast<T*>(a.h) + i * a.h_stride;
+                        store_cols<8>(to, u0, a.hidden, dg);
+                        continue;
+                    }
+                    if (!whole || i >= a.n) {  // what is infinite times a dh of 0 is NaN
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            if (i >= a.n || u0 + k >= a.hidden) dg[k] = du[k] = 0.0f;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        sg[k] += dg[k];
+                        su[k] += du[k];
+                    }
+                    quad pg[NP], pu[NP];
+                    split8_input<NP>(dg, pg);
+                    split8_input<NP>(du, pu);
+#pragma unroll
+                    for (int p = 0; p < NP; ++p) {
+                        quad* to = reinterpret_cast<quad*>(dz + (p * nr + row) * wr + r0 + g * 16);
+                        to[0] = pg[p];
+                        to[1] = pu[p];
+                    }
+                }
+                if (GRAD && db != nullptr) {
+#pragma unroll
+                    for (int o = 1; o < 16; o <<= 1)
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            sg[k] += __shfl_xor(sg[k], o, 64);
+                            su[k] += __shfl_xor(su[k], o, 64);
+                        }
+                    if (s == 0) {
+                        float* to = db + (s0 / 64) * wr + r0 + g * 16;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            to[k] = sg[k];
+                            to[8 + k] = su[k];
+                        }
+                    }
+                }
+            }
+        });
+}
+
+template <typename T, int NP, int AB>
+__global__ __launch_bounds__((WideShape<NP, AB>::kThreads), 2) void k_wide_dx(GatedArgs a, WideMat W, WideMat Z,
+                                                             int64_t n0, int64_t nr, int tiles_c,
+                                                             int gy) {
+    using Shape = WideShape<NP, AB>;
+    __shared__ quad lds[Shape::kQuads];
+    const int lane = threadIdx.x & 63;
+    const Spot at = spot((int)(nr / Shape::kCols), gy);
+    if (at.y >= tiles_c) return;
+    const int64_t c0 = (int64_t)at.y * Shape::kRows, s0 = (int64_t)at.x * Shape::kCols;
+    wide_products<NP, AB, false, true, false>(
+        W, Z, 0, W.rows, 1, lds, [&](int) { return TileRows{c0, s0}; }, [](int) {},
+        [&](int, f32x4(&acc)[AB][Shape::BB]) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int64_t i = n0 + s0 + Shape::col() + j * 16 + (lane & 15);
+                if (i >= a.n) continue;
+                T* row = static_cast<T*>(a.dx) + i * a.dx_stride;
+#pragma unroll
+                for (int k = 0; k < AB; ++k) {
+                    const float v[4] = {acc[k][j][0], acc[k][j][1], acc[k][j][2], acc[k][j][3]};
+                    store_cols<4>(row, c0 + Shape::row() + k * 16 + (lane >> 4) * 4, a.dim, v);
+                }
+            }
+        });
+}
+
+template <int NP, int AB>
+__global__ __launch_bounds__((WideShape<NP, AB>::kThreads), 2) void k_wide_dw(WideMat X, WideMat Z, int64_t nr,
+                                                             int cols, int ldp, int64_t per_share,
+                                                             int add, float* part) {
+    using Shape = WideShape<NP, AB>;
+    __shared__ quad lds[Shape::kQuads];
+    const int lane = threadIdx.x & 63;
+    // a share's tiles run on one XCD, whose L2 gives them its rows of x and dz
+    const int tiles = (int)(Z.cols / Shape::kCols) * cols, tile = (blockIdx.x >> 3) % tiles;
+    const int64_t share = (blockIdx.x >> 3) / tiles * 8 + (blockIdx.x & 7);
+    const int64_t c0 = (int64_t)(tile % cols) * Shape::kRows, r0 = (int64_t)(tile / cols) * Shape::kCols;
+    const int64_t k0 = min(nr, share * per_share), k1 = min(nr, k0 + per_share);
+    wide_products<NP, AB, false, false, false>(
+        X, Z, k0, k1, 1, lds, [&](int) { return TileRows{c0, r0}; }, [](int) {},
+        [&](int, f32x4(&acc)[AB][Shape::BB]) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int64_t r = r0 + Shape::col() + j * 16 + (lane & 15);
+                f32x4* to = reinterpret_cast<f32x4*>(part + (share * Z.cols + r) * ldp + c0 +
+                                                     Shape::row());
+#pragma unroll
+                for (int k = 0; k < AB; ++k) {
+                    f32x4 v = acc[k][j];
+                    if (add) v += to[k * 4 + (lane >> 4)];
+                    to[k * 4 + (lane >> 4)] = v;
+                }
+            }
+        });
 }
 
 // ---------------------------------------------------------------- few rows
@@ -366,9 +554,121 @@ struct GatedPlan {
     }
 };
 
+// Wide tiles pay from about as many as there are CUs (fp32: as fit at a time).
+constexpr int kWideLeast = 192;
+bool is_wide(const GatedArgs& a) {
+    const int64_t tile = a.dtype == 0 ? 128 : 256;
+    return a.dim > kShortDim && ((2 * a.hidden + tile - 1) / tile) * ((a.n + tile - 1) / tile) >=
+                                    (a.dtype == 0 ? 2 * kWideLeast : kWideLeast);
+}
+
+struct WidePlan {
+    int ld, ldp, ab;  // the weights' columns, the partial sums', blocks of A for the gradients
+    int64_t wr, piece, shares, per_share;
+    bool direct;  // x is read where it is
+    quad* zero;
+    bf16 *w, *x, *dz;
+    float *part, *db;
+    size_t bytes;
+    WidePlan(void* base, const GatedArgs& a, int np, bool grad) {
+        ld = (int)pad_to(a.dim, kStep);
+        wr = pad_to(2 * a.hidden, 256);
+        direct = np == 1 && a.dim % 8 == 0 && a.x_stride % 8 == 0 &&
+                 reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_stride < ((int64_t)1 << 24);
+        const int64_t row = (int64_t)np * 2 * ((direct ? 0 : ld) + (grad ? wr : 0));
+        const int cols = np == 1 ? 256 : 128;  // rows of a tile
+        const int64_t all = pad_to(a.n, cols);
+        // a launch takes fewer than 2^32 threads
+        const int64_t most = std::min(row == 0 ? all : kPieceBytes / row,
+                                      ((int64_t)1 << 30) / (wr / 128 * (1 + ld / 1024)));
+        piece = std::min(all, std::max<int64_t>(cols, most / cols * cols));
+        Carve c(base);
+        zero = c.take<quad>(1);
+        w = c.take<bf16>((size_t)(wr * ld) * np);
+        if (!direct) x = c.take<bf16>((size_t)(piece * ld) * np);
+        if (grad) {
+            // tiles of 256 or 128 columns of x for the gradients: what wastes less
+            ab = np == 1 && (a.dim + 127) / 128 % 2 == 0 ? 8 : 4;  // 256 or 128 columns of x
+            ldp = (int)pad_to(a.dim, 32 * ab);
+            const int64_t tiles = (wr / cols) * (ldp / (32 * ab));
+            shares = 8 * std::max<int64_t>(1, (np == 1 ? 32 : 64) / tiles);
+            per_share = pad_to((piece + shares - 1) / shares, kStep);
+            dz = c.take<bf16>((size_t)(piece * wr) * np);
+            part = c.take<float>((size_t)(shares * wr * ldp));
+            db = c.take<float>((size_t)(piece / 64 * wr));
+        }
+        bytes = c.bytes();
+    }
+};
+
+template <typename T, int NP, int ACT>
+hipError_t wide_run(const GatedArgs& a, bool grad, hipStream_t st) {
+    const WidePlan w(a.ws, a, NP, grad);
+    using Shape = WideShape<NP, kWideBlocks<NP>>;
+    constexpr int COLS = Shape::kCols, THREADS = Shape::kThreads;
+    k_wide_weights<T, NP><<<blocks_of(w.wr * (w.ld / 8), kThreads), kThreads, 0, st>>>(
+        a, w.wr, w.ld, reinterpret_cast<quad*>(w.w), w.zero);
+    GS_LAUNCHED();
+    const WideMat W{w.w, w.ld, w.wr * w.ld, w.wr, w.ld, w.zero};
+    const bool biases = a.db_gate != nullptr || a.db_up != nullptr;
+    for (int64_t n0 = 0; n0 < a.n; n0 += w.piece) {
+        const int64_t nr = std::min(w.piece, pad_to(a.n - n0, COLS));
+        WideMat X{w.x, w.ld, nr * w.ld, nr, w.ld, w.zero};
+        if (w.direct) {
+            X = WideMat{static_cast<const bf16*>(a.x) + n0 * a.x_stride, a.x_stride, 0, a.n - n0,
+                        a.dim, w.zero};
+        } else {
+            k_gated_parts<T, NP, false><<<blocks_of(nr * (w.ld / 8), kThreads), kThreads, 0, st>>>(
+                a, n0, nr, w.ld, reinterpret_cast<quad*>(w.x));
+            GS_LAUNCHED();
+        }
+        const int tiles_w = (int)(w.wr / Shape::kRows), share = 2;
+        const SpotGrid sg(nr / COLS, (tiles_w + share - 1) / share, kSpot);
+        if (!grad) {
+            k_gated_wide<T, NP, ACT, false><<<sg.blocks, THREADS, 0, st>>>(
+                a, W, X, w.ld, n0, nr, tiles_w, share, sg.gy, nullptr, nullptr);
+            GS_LAUNCHED();
+            continue;
+        }
+        k_gated_wide<T, NP, ACT, true><<<sg.blocks, THREADS, 0, st>>>(
+            a, W, X, w.ld, n0, nr, tiles_w, share, sg.gy, w.dz, biases ? w.db : nullptr);
+        GS_LAUNCHED();
+        if (biases) {
+            k_gated_sum<T, true, true><<<sum_blocks(w.wr / 4), 1024, 0, st>>>(
+                a, w.db, (int)(nr / 64), w.wr, 4, n0 > 0);
+            GS_LAUNCHED();
+        }
+        const WideMat Z{w.dz, w.wr, nr * w.wr, nr, w.wr, w.zero};
+        const int tiles_c = w.ldp / (32 * w.ab);
+        const SpotGrid xg(nr / COLS, tiles_c, kSpot);
+        const unsigned wg = (unsigned)(w.wr / COLS * tiles_c * w.shares);
+        auto sums = [&](auto ab) {
+            constexpr int AB = decltype(ab)::value;
+            k_wide_dx<T, NP, AB><<<xg.blocks, THREADS, 0, st>>>(a, W, Z, n0, nr, tiles_c, xg.gy);
+            GS_LAUNCHED();
+            k_wide_dw<NP, AB><<<wg, THREADS, 0, st>>>(X, Z, nr, tiles_c, w.ldp, w.per_share, n0 > 0,
+                                                      w.part);
+            return hipGetLastError();
+        };
+        hipError_t e;
+        if constexpr (NP == 1) {
+            e = w.ab == 8 ? sums(std::integral_constant<int, 8>())
+                          : sums(std::integral_constant<int, 4>());
+        } else {
+            e = sums(std::integral_constant<int, 4>());
+        }
+        if (e != hipSuccess) return e;
+    }
+    if (!grad) return hipSuccess;
+    k_gated_sum<T, true, false><<<sum_blocks(w.wr * (w.ldp / 4)), 1024, 0, st>>>(
+        a, w.part, (int)w.shares, w.wr, w.ldp, 0);
+    return hipGetLastError();
+}
+
 template <typename T, int NP, int ACT>
 hipError_t gated_run(const GatedArgs& a, bool grad, hipStream_t st) {
     if (is_few(a, grad)) return few_run<T, NP, ACT>(a, st);
+    if (is_wide(a)) return wide_run<T, NP, ACT>(a, grad, st);
     const GatedPlan w(a.ws, a.n, a.hidden, a.dim, NP, grad);
     const int kd = (int)pad_to(a.dim, kStep);
     const int64_t wu = w.wr * (w.ld / 8);
@@ -396,7 +696,8 @@ hipError_t gated_run(const GatedArgs& a, bool grad, hipStream_t st) {
             a, X, W, kd, n0, nr, w.wr, sg.gy, w.dz, biases ? w.db : nullptr);
         GS_LAUNCHED();
         if (biases) {
-            k_gated_db<<<(unsigned)(w.wr / 16), kThreads, 0, st>>>(a, w.db, nr / 64, w.wr, n0 > 0);
+            k_gated_sum<T, false, true><<<sum_blocks(w.wr / 4), 1024, 0, st>>>(
+                a, w.db, (int)(nr / 64), w.wr, 4, n0 > 0);
             GS_LAUNCHED();
         }
         const SpotGrid xg(nr / kTile, w.ld / kTile, kSpot);
@@ -409,11 +710,11 @@ hipError_t gated_run(const GatedArgs& a, bool grad, hipStream_t st) {
     }
     if (!grad) return hipSuccess;
     if (a.n == 0 && biases) {
-        k_gated_db<<<(unsigned)(w.wr / 16), kThreads, 0, st>>>(a, nullptr, 0, w.wr, 0);
+        k_gated_sum<T, false, true><<<sum_blocks(w.wr / 4), 1024, 0, st>>>(a, nullptr, 0, w.wr, 4, 0);
         GS_LAUNCHED();
     }
-    k_gated_dw_sum<T><<<blocks_of(w.wr * (w.ld / 4), kThreads), kThreads, 0, st>>>(
-        a, w.part, a.n > 0 ? (int)w.shares : 0, w.wr, w.ld);
+    k_gated_sum<T, false, false><<<sum_blocks(w.wr * (w.ld / 4)), 1024, 0, st>>>(
+        a, w.part, a.n > 0 ? (int)w.shares : 0, w.wr, w.ld, 0);
     return hipGetLastError();
 }
 
@@ -432,6 +733,7 @@ hipError_t gated_act(const GatedArgs& a, bool grad, hipStream_t st) {
 size_t gated_linear_ws(const GatedArgs& a, bool grad) {
     if (a.n == 0 || is_few(a, grad)) return 0;
     if (a.dim <= kShortDim) return gated_short_ws(a, grad);
+    if (is_wide(a)) return WidePlan(nullptr, a, a.dtype == 0 ? 3 : 1, grad).bytes;
     return GatedPlan(nullptr, a.n, a.hidden, a.dim, a.dtype == 0 ? 3 : 1, grad).bytes;
 }
 

@@ -58,28 +58,6 @@ __device__ __forceinline__ void multiply(const bf16x8 (&a)[M][NP], const bf16x8 
             }
 }
 
-// 8 values as they lie in memory, at any address; zeros from column `cols` on.
-template <typename T>
-struct Raw {
-    quad q[sizeof(T) / 2];
-    __device__ __forceinline__ void load(const T* row, int64_t c, int64_t cols) {
-        T v[8];
-        if (c + 8 <= cols) {
-            __builtin_memcpy(v, row + c, sizeof(v));
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? row[c + e] : (T)0.0f;
-        }
-        __builtin_memcpy(q, v, sizeof(v));
-    }
-    __device__ __forceinline__ float operator[](int k) const {
-        if constexpr (sizeof(T) == 2)
-            return __uint_as_float(k & 1 ? q[0][k / 2] & 0xFFFF0000u : q[0][k / 2] << 16);
-        else
-            return __uint_as_float(q[k / 4][k % 4]);
-    }
-};
-
 // A chunk of the weights, 32 units, as 4 blocks of 16 rows: gate, gate, up, up; block i of
 // two has the units 8 (s / 4) + 4 i + s % 4, so that a lane's sums are 8 units in a row.
 template <typename T, int NP>

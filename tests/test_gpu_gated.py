@@ -128,6 +128,25 @@ def test_values_and_gradients(ops, n, dim, hidden, dtype):
     assert all(torch.equal(a, b) for a, b in zip(again, (h, *grads)))
 
 
+# 2 hidden / 256 by rows / 256 tiles, at least 192 of them: the wide tiles
+WIDE = [(2500, 136, 2500), (3001, 200, 2050), (2601, 145, 2305), (1900, 520, 3200),
+        (50_001, 131, 40), (49_152, 256, 128), (9000, 320, 700)]
+
+
+@pytest.mark.parametrize("n,dim,hidden", WIDE)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_wide_tiles(ops, n, dim, hidden, dtype):
+    test_values_and_gradients(ops, n, dim, hidden, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_wide_tiles_strides_and_values_that_are_not_finite(ops, dtype):
+    for n, dim, hidden in ((2500, 136, 2500), (2600, 192, 2410)):
+        test_strides_and_alignment(ops, dtype, n, dim, hidden)
+    test_values_that_are_not_finite(ops, dtype, 2600, 136, 2410)
+    test_broadcast_rows(ops, dtype, 2600, 136, 2410)
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("bias", [True, False])
@@ -192,10 +211,9 @@ def test_strides_and_alignment(ops, dtype, n, dim, hidden):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-def test_broadcast_rows(ops, dtype):
+def test_broadcast_rows(ops, dtype, n=700, dim=40, hidden=48):
     """One row of x and of dh for all samples (a stride of 0)."""
-    x, wg, wu, bg, bu, dh = _inputs(1, 40, 48, dtype, seed=6)
-    n = 700
+    x, wg, wu, bg, bu, dh = _inputs(1, dim, hidden, dtype, seed=6)
     many = (x.expand(n, -1), wg, wu, bg, bu, dh.expand(n, -1))
     ref = _reference(*many, "gelu", dtype)
     gx, gd = x.cuda().expand(n, -1), dh.cuda().expand(n, -1)
@@ -321,7 +339,8 @@ def test_many_rows_in_pieces(ops, dim):
 
 @pytest.mark.parametrize("n,dim,hidden,dtype", [(1, 64, 100, F32), (40, 64, 256, BF16),
                                                 (700, 75, 60, F32), (3000, 64, 128, BF16),
-                                                (900, 256, 200, BF16)])
+                                                (900, 256, 200, BF16), (2500, 136, 2500, BF16),
+                                                (2500, 136, 2500, F32)])
 def test_captured_and_replayed(ops, n, dim, hidden, dtype):
     """Two graphs and eager calls between the replays, new inputs in the same buffers."""
     sets = [_cuda(_inputs(n, dim, hidden, dtype, seed=s)) for s in (20, 21, 22)]
