@@ -54,19 +54,59 @@ __device__ __forceinline__ void store_cols(T* row, int64_t c, int64_t cols, cons
     }
 }
 
-// 8 values as they lie in memory, at any address; zeros from column `cols` on.
-template <typename T>
+// N values of a row from column c as they lie in memory, at any address. load() has no
+// branch that lanes could part at: one would hold the program up until the values are there, and
+// they are loaded a step ahead. Past the row's end it reads values that are there; finish(),
+// when they are needed, moves the row's last ones to their places and puts zeros behind.
+template <typename T, int N = 8>
 struct Raw {
-    quad q[sizeof(T) / 2];
+    quad q[N * sizeof(T) / 16];
     __device__ __forceinline__ void load(const T* row, int64_t c, int64_t cols) {
-        T v[8];
-        if (c + 8 <= cols) {
+        if (cols >= N) {
+            __builtin_memcpy(q, row + min(c, cols - N), sizeof(q));
+        } else {  // a short row, the same for all
+            T v[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = row[min((int64_t)e, cols - 1)];
+            __builtin_memcpy(q, v, sizeof(q));
+        }
+    }
+    // Both at once.
+    __device__ __forceinline__ void load_finished(const T* row, int64_t c, int64_t cols) {
+        T v[N];
+        if (c + N <= cols) {
             __builtin_memcpy(v, row + c, sizeof(v));
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? row[c + e] : (T)0.0f;
+            for (int e = 0; e < N; ++e) v[e] = c + e < cols ? row[c + e] : (T)0.0f;
         }
-        __builtin_memcpy(q, v, sizeof(v));
+        __builtin_memcpy(q, v, sizeof(q));
+    }
+    __device__ __forceinline__ void finish(int64_t c, int64_t cols, bool on) {
+        if (on && c + N <= cols) return;
+        T v[N];
+        __builtin_memcpy(v, q, sizeof(q));
+        const int left = on && c < cols ? (int)(cols - c) : 0;  // below N
+        const int by = cols >= N ? N - left : 0;
+#pragma unroll
+        for (int o = N / 2; o > 0; o /= 2)
+#pragma unroll
+            for (int e = 0; e + o < N; ++e) v[e] = by & o ? v[e + o] : v[e];
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[e] = e < left ? v[e] : (T)0.0f;
+        __builtin_memcpy(q, v, sizeof(q));
+    }
+    // As operands.
+    template <int NP>
+    __device__ __forceinline__ void parts(quad (&out)[NP]) const {
+        if constexpr (NP == 1) {
+            out[0] = q[0];
+        } else {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = plain_input<NP>((*this)[e]);
+            split8_input<NP>(v, out);
+        }
     }
     __device__ __forceinline__ float operator[](int k) const {
         if constexpr (sizeof(T) == 2)

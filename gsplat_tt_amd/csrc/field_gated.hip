@@ -308,8 +308,9 @@ __global__ __launch_bounds__((WideShape<NP, 8>::kThreads), 2) void k_gated_wide(
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int64_t i = n0 + s0 + j * 16 + s;
-                    d[v][j].load(static_cast<const T*>(a.dh) + (i < a.n ? i : 0) * a.dh_stride,
-                                 (row_of(t) + v * 64) / 2 + g * 8, i < a.n ? a.hidden : 0);
+                    d[v][j].load_finished(
+                        static_cast<const T*>(a.dh) + (i < a.n ? i : 0) * a.dh_stride,
+                        (row_of(t) + v * 64) / 2 + g * 8, i < a.n ? a.hidden : 0);
                 }
         },
         [&](int t, f32x4(&acc)[AB][Shape::BB]) {

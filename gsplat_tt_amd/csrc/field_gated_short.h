@@ -60,14 +60,14 @@ __device__ __forceinline__ void multiply(const bf16x8 (&a)[M][NP], const bf16x8 
 
 // A chunk of the weights, 32 units, as 4 blocks of 16 rows: gate, gate, up, up; block i of
 // two has the units 8 (s / 4) + 4 i + s % 4, so that a lane's sums are 8 units in a row.
-template <typename T, int NP>
-__device__ __forceinline__ void load_weights(const GatedArgs& a, int64_t u0, int i, int s, int c,
-                                             quad* out) {
-    const int64_t unit = u0 + (s >> 2) * 8 + (i & 1) * 4 + (s & 3);
-    const bool on = unit < a.hidden;
-    const T* w = static_cast<const T*>(i >= 2 ? a.w_up : a.w_gate);
-    load_parts<T, NP>(w + (on ? unit : 0) * (i >= 2 ? a.up_stride : a.gate_stride), a.dim, c, on,
-                      out);
+__device__ __forceinline__ int64_t weight_unit(int64_t u0, int i, int s) {
+    return u0 + (s >> 2) * 8 + (i & 1) * 4 + (s & 3);
+}
+template <typename T>
+__device__ __forceinline__ const T* weight_row(const GatedArgs& a, int64_t u0, int i, int s) {
+    const int64_t unit = weight_unit(u0, i, s);
+    return static_cast<const T*>(i >= 2 ? a.w_up : a.w_gate) +
+           (unit < a.hidden ? unit : 0) * (i >= 2 ? a.up_stride : a.gate_stride);
 }
 // The chunks' parts laid out as LDS takes them, so that fp32 weights are cut once.
 template <typename T, int NP, int KS>
@@ -79,8 +79,9 @@ __global__ __launch_bounds__(kThreads) void k_gated_chunks(GatedArgs a, int64_t 
         const int64_t chunk = e / (256 * KS);
         const int q = (int)(e - chunk * (256 * KS)), lane = q & 63, b = q >> 6;
         quad part[NP];
-        load_weights<T, NP>(a, chunk * 32, b / KS, lane & 15, (b % KS) * 32 + (lane >> 4) * 8,
-                                  part);
+        load_parts<T, NP>(weight_row<T>(a, chunk * 32, b / KS, lane & 15), a.dim,
+                          (b % KS) * 32 + (lane >> 4) * 8,
+                          weight_unit(chunk * 32, b / KS, lane & 15) < a.hidden, part);
 #pragma unroll
         for (int p = 0; p < NP; ++p)
             out[(chunk * NP + p) * (256 * KS) + b * 64 + quad_place(lane & 15, lane >> 4)] = part[p];
@@ -89,16 +90,21 @@ __global__ __launch_bounds__(kThreads) void k_gated_chunks(GatedArgs a, int64_t 
 
 // Rows stay with their wave, 16 J of them in registers, and the weights pass through LDS
 // chunk by chunk: h, or with GRAD dx, whose sums stay in registers too. The gradients of
-// gate and up leave the sums in the layout that the next product takes them in.
-template <typename T, int NP, int ACT, int KS, int J, bool GRAD>
-__global__ __launch_bounds__(kThreads, NP == 1 || J * KS < 8 ? 2 : 1) void k_gated_rows(
+// gate and up leave the sums in the layout that the next product takes them in. LAID: the
+// chunks' parts come from k_gated_chunks. P sets of G waves with the same rows take P chunks
+// at a time, and the first adds up their dx.
+template <typename T, int NP, int ACT, int KS, int J, int G, int P, bool GRAD, bool LAID>
+__global__ __launch_bounds__(64 * G * P, P == 1 && (NP == 1 || J * KS < 8) ? 2 : 1) void k_gated_rows(
     GatedArgs a, const quad* laid, int64_t chunks, int64_t per_share) {
-    __shared__ quad lds[NP * 256 * KS];
-    __shared__ float bias[64];
-    const int lane = threadIdx.x & 63, w = wave_id(), g = lane >> 4, s = lane & 15;
-    const int64_t i0 = ((int64_t)blockIdx.x * (kThreads / 64) + w) * (16 * J);
+    constexpr int SET = NP * 256 * KS, SUMS = P > 1 ? 2 * KS * J * 64 * G : 1, KQ = 4 / G * KS;
+    __shared__ quad lds[P * SET > SUMS ? P * SET : SUMS];
+    __shared__ float bias[P][64];
+    const int lane = threadIdx.x & 63, wave = wave_id(), g = lane >> 4, s = lane & 15;
+    const int w = wave % G, set = wave / G, t = threadIdx.x % (64 * G);
+    const int64_t i0 = ((int64_t)blockIdx.x * G + w) * (16 * J);
     const int64_t c0 = blockIdx.y * per_share, c1 = min(chunks, c0 + per_share);
-    quad next[KS][NP];
+    quad next[KQ][LAID ? NP : 1];
+    Raw<T> next_w[LAID ? 1 : KQ];
     Raw<T> next_d[J];
     float next_bias = 0.0f;
     auto fetch = [&](int64_t chunk) {
@@ -107,37 +113,43 @@ __global__ __launch_bounds__(kThreads, NP == 1 || J * KS < 8 ? 2 : 1) void k_gat
             for (int j = 0; j < J; ++j) {
                 const int64_t i = i0 + j * 16 + s;
                 next_d[j].load(static_cast<const T*>(a.dh) + (i < a.n ? i : 0) * a.dh_stride,
-                               chunk * 32 + g * 8, i < a.n ? a.hidden : 0);
+                               chunk * 32 + g * 8, a.hidden);
             }
         }
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            if (NP > 1) {
+        for (int k = 0; k < KQ; ++k) {
+            if constexpr (LAID) {
 #pragma unroll
                 for (int p = 0; p < NP; ++p)
-                    next[k][p] = laid[(chunk * NP + p) * (256 * KS) + k * 256 + threadIdx.x];
+                    next[k][p] = chunk < c1 ? laid[(chunk * NP + p) * (256 * KS) + k * (64 * G) + t]
+                                            : quad{0u, 0u, 0u, 0u};
             } else {
-                const int b = k * 4 + w;
-                load_weights<T, NP>(a, chunk * 32, b / KS, s, (b % KS) * 32 + g * 8, next[k]);
+                const int blk = k * G + w;
+                next_w[k].load(weight_row<T>(a, chunk * 32, blk / KS, s), (blk % KS) * 32 + g * 8,
+                               a.dim);
             }
         }
-        if (threadIdx.x < 64) {
-            const int i = threadIdx.x >> 4;
-            const int64_t unit = chunk * 32 + (s >> 2) * 8 + (i & 1) * 4 + (s & 3);
+        if (w == 0) {
+            const int i = g;
+            const int64_t unit = weight_unit(chunk * 32, i, s);
             const float* from = i >= 2 ? a.b_up : a.b_gate;
             next_bias = from != nullptr && unit < a.hidden ? from[unit] : 0.0f;
         }
     };
-    if (c0 < c1) fetch(c0);
+    if (c0 < c1) fetch(c0 + set);
     bf16x8 x[KS][J][NP];
 #pragma unroll
     for (int j = 0; j < J; ++j) {
         const int64_t i = i0 + j * 16 + s;
         const T* row = static_cast<const T*>(a.x) + (i < a.n ? i : 0) * a.x_stride;
+        Raw<T> raw[KS];
+#pragma unroll
+        for (int k = 0; k < KS; ++k) raw[k].load(row, k * 32 + g * 8, a.dim);
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
+            raw[k].finish(k * 32 + g * 8, a.dim, i < a.n);
             quad part[NP];
-            load_parts<T, NP>(row, a.dim, k * 32 + g * 8, i < a.n, part);
+            raw[k].parts(part);
 #pragma unroll
             for (int p = 0; p < NP; ++p) x[k][j][p] = __builtin_bit_cast(bf16x8, part[p]);
         }
@@ -148,29 +160,44 @@ __global__ __launch_bounds__(kThreads, NP == 1 || J * KS < 8 ? 2 : 1) void k_gat
     for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int j = 0; j < J; ++j) dx[d][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int64_t chunk = c0; chunk < c1; ++chunk) {
-        __syncthreads();  // the last chunk has been read
+    quad* mine = lds + set * SET;
+    for (int64_t first = c0; first < c1; first += P) {
+        const int64_t chunk = first + set;  // past the last: zeros
+        __syncthreads();  // the last chunks have been read
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
+        for (int k = 0; k < KQ; ++k) {
+            if constexpr (LAID) {
 #pragma unroll
-            for (int p = 0; p < NP; ++p) {
-                const int b = k * 4 + w;
-                if (NP > 1) lds[p * (256 * KS) + k * 256 + threadIdx.x] = next[k][p];
-                else lds[b * 64 + quad_place(s, g)] = next[k][p];
+                for (int p = 0; p < NP; ++p) mine[p * (256 * KS) + k * (64 * G) + t] = next[k][p];
+            } else {
+                const int blk = k * G + w;
+                next_w[k].finish((blk % KS) * 32 + g * 8, a.dim,
+                                 weight_unit(chunk * 32, blk / KS, s) < a.hidden);
+                quad q[NP];
+                next_w[k].parts(q);
+#pragma unroll
+                for (int p = 0; p < NP; ++p)
+                    mine[p * (256 * KS) + (k * G + w) * 64 + quad_place(s, g)] = q[p];
             }
-        if (threadIdx.x < 64) bias[threadIdx.x] = next_bias;
+        }
+        if (w == 0) bias[set][lane] = next_bias;
         Raw<T> d[J];
         if (GRAD) {
 #pragma unroll
             for (int j = 0; j < J; ++j) d[j] = next_d[j];
+            if (chunk * 32 + 32 > a.hidden || i0 + J * 16 > a.n) {
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+                    d[j].finish(chunk * 32 + g * 8, a.hidden, i0 + j * 16 + s < a.n);
+            }
         }
         __syncthreads();
-        if (chunk + 1 < c1) fetch(chunk + 1);
+        if (first + P < c1) fetch(chunk + P);
         const int64_t u0 = chunk * 32 + g * 8;
         f32x4 z[4][J];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const f32x4 b = *reinterpret_cast<const f32x4*>(bias + i * 16 + g * 4);
+            const f32x4 b = *reinterpret_cast<const f32x4*>(bias[set] + i * 16 + g * 4);
 #pragma unroll
             for (int j = 0; j < J; ++j) z[i][j] = b;
         }
@@ -183,7 +210,7 @@ __global__ __launch_bounds__(kThreads, NP == 1 || J * KS < 8 ? 2 : 1) void k_gat
                 for (int m = 0; m < 2; ++m)
 #pragma unroll
                     for (int p = 0; p < NP; ++p)
-                        f[m][p] = operand_of(lds + p * (256 * KS) + ((i + m) * KS + k) * 64);
+                        f[m][p] = operand_of(mine + p * (256 * KS) + ((i + m) * KS + k) * 64);
                 multiply<NP>(f, x[k], [&](int m, int j) -> f32x4& { return z[i + m][j]; });
             }
         if (!GRAD) {
@@ -226,7 +253,7 @@ __global__ __launch_bounds__(kThreads, NP == 1 || J * KS < 8 ? 2 : 1) void k_gat
             for (int p = 0; p < NP; ++p) dz[1][j][p] = __builtin_bit_cast(bf16x8, part[p]);
         }
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 bf16x8 f[2][NP];
@@ -235,11 +262,32 @@ __global__ __launch_bounds__(kThreads, NP == 1 || J * KS < 8 ? 2 : 1) void k_gat
 #pragma unroll
                     for (int p = 0; p < NP; ++p)
                         f[m][p] = operand_across(
-                            lds + p * (256 * KS) + t * (2 * KS * 64) + k * 64, KS * 64, m);
-                multiply<NP>(f, dz[t], [&](int m, int j) -> f32x4& { return dx[2 * k + m][j]; });
+                            mine + p * (256 * KS) + u * (2 * KS * 64) + k * 64, KS * 64, m);
+                multiply<NP>(f, dz[u], [&](int m, int j) -> f32x4& { return dx[2 * k + m][j]; });
             }
     }
     if (!GRAD) return;
+    if constexpr (P > 1) {
+        f32x4* sums = reinterpret_cast<f32x4*>(lds);
+#pragma unroll
+        for (int from = 1; from < P; ++from) {
+            __syncthreads();
+            if (set == from) {
+#pragma unroll
+                for (int c = 0; c < DB; ++c)
+#pragma unroll
+                    for (int j = 0; j < J; ++j) sums[(c * J + j) * (64 * G) + t] = dx[c][j];
+            }
+            __syncthreads();
+            if (set == 0) {
+#pragma unroll
+                for (int c = 0; c < DB; ++c)
+#pragma unroll
+                    for (int j = 0; j < J; ++j) dx[c][j] += sums[(c * J + j) * (64 * G) + t];
+            }
+        }
+        if (set != 0) return;
+    }
 #pragma unroll
     for (int j = 0; j < J; ++j) {
         const int64_t i = i0 + j * 16 + s;
@@ -269,7 +317,7 @@ constexpr int kUnitBlocks = sizeof(T) == 2 ? 2 : 1;  // 64 bytes of a row of dh
 template <typename T, int NP, int ACT, int KS, int WU>
 __global__ __launch_bounds__(kThreads, KS <= 2 ? 2 : 1) void k_gated_units(
     GatedArgs a, int64_t tiles, int64_t per_share, int64_t wr, float* part, float* db) {
-    constexpr int WS = kThreads / 64 / WU, VB = kUnitBlocks<T>, NB = 2 * VB;
+    constexpr int WS = kThreads / 64 / WU, VB = kUnitBlocks<T>;
     constexpr int DQ = 4 / WS;  // quads of dh of a lane
     __shared__ quad lds[NP * 256 * KS];
     __shared__ quad dh_lds[4][64 * DQ];
@@ -278,55 +326,50 @@ __global__ __launch_bounds__(kThreads, KS <= 2 ? 2 : 1) void k_gated_units(
     const int64_t u0 = ((int64_t)blockIdx.x * WU + wu) * (16 * VB);
     const int64_t t0 = blockIdx.y * per_share, t1 = min(tiles, t0 + per_share);
     const int64_t slot = (int64_t)blockIdx.y * WS + ws;
-    bf16x8 wt[KS][NB][NP];
-    float b[NB], sum[NB];
+    bf16x8 wt[KS][VB][2][NP];  // gate, up
+    float b[VB][2], sum[VB][2];
+    f32x4 dw[VB][2][2 * KS];
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-        const int64_t unit = u0 + (i % VB) * 16 + s;
-        const bool on = unit < a.hidden;
-        const float* bias = i >= VB ? a.b_up : a.b_gate;
-        const T* row = static_cast<const T*>(i >= VB ? a.w_up : a.w_gate) +
-                       (on ? unit : 0) * (i >= VB ? a.up_stride : a.gate_stride);
-        b[i] = bias != nullptr && on ? bias[unit] : 0.0f;
-        sum[i] = 0.0f;
+    for (int v = 0; v < VB; ++v)
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            quad q[NP];
-            load_parts<T, NP>(row, a.dim, k * 32 + g * 8, on, q);
+        for (int t = 0; t < 2; ++t) {
+            const int64_t unit = u0 + v * 16 + s;
+            const bool on = unit < a.hidden;
+            const float* bias = t ? a.b_up : a.b_gate;
+            const T* row = static_cast<const T*>(t ? a.w_up : a.w_gate) +
+                           (on ? unit : 0) * (t ? a.up_stride : a.gate_stride);
+            b[v][t] = bias != nullptr && on ? bias[unit] : 0.0f;
+            sum[v][t] = 0.0f;
 #pragma unroll
-            for (int p = 0; p < NP; ++p) wt[k][i][p] = __builtin_bit_cast(bf16x8, q[p]);
+            for (int k = 0; k < KS; ++k) {
+                Raw<T> raw;
+                raw.load(row, k * 32 + g * 8, a.dim);
+                raw.finish(k * 32 + g * 8, a.dim, on);
+                quad q[NP];
+                raw.parts(q);
+#pragma unroll
+                for (int p = 0; p < NP; ++p) wt[k][v][t][p] = __builtin_bit_cast(bf16x8, q[p]);
+            }
+#pragma unroll
+            for (int c = 0; c < 2 * KS; ++c) dw[v][t][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-    }
-    f32x4 dw[NB][2 * KS];
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int c = 0; c < 2 * KS; ++c) dw[i][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     // the next tile's x and dh, cut when they are stored
     Raw<T> next[KS];
-    quad next_d[DQ];
+    constexpr int V = 16 / sizeof(T);
+    Raw<T, V> next_d[DQ];
     auto fetch = [&](int64_t tile) {
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
             const int blk = k * 4 + w;
             const int64_t i = tile * 64 + (blk / KS) * 16 + s;
             next[k].load(static_cast<const T*>(a.x) + (i < a.n ? i : 0) * a.x_stride,
-                         (blk % KS) * 32 + g * 8, i < a.n ? a.dim : 0);
+                         (blk % KS) * 32 + g * 8, a.dim);
         }
 #pragma unroll
         for (int k = 0; k < DQ; ++k) {
-            constexpr int V = 16 / sizeof(T);
             const int64_t i = tile * 64 + ws * (64 / WS) + k * 16 + (lane >> 2);
-            const int64_t c = u0 + (lane & 3) * V, cols = i < a.n ? a.hidden : 0;
-            const T* row = static_cast<const T*>(a.dh) + (i < a.n ? i : 0) * a.dh_stride;
-            T v[V];
-            if (c + V <= cols) {
-                __builtin_memcpy(v, row + c, sizeof(v));
-            } else {
-#pragma unroll
-                for (int e = 0; e < V; ++e) v[e] = c + e < cols ? row[c + e] : (T)0.0f;
-            }
-            __builtin_memcpy(&next_d[k], v, sizeof(v));
+            next_d[k].load(static_cast<const T*>(a.dh) + (i < a.n ? i : 0) * a.dh_stride,
+                           u0 + (lane & 3) * V, a.hidden);
         }
     };
     if (t0 < t1) fetch(t0);
@@ -335,14 +378,9 @@ __global__ __launch_bounds__(kThreads, KS <= 2 ? 2 : 1) void k_gated_units(
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
             quad q[NP];
-            if constexpr (NP == 1) {
-                q[0] = next[k].q[0];
-            } else {
-                float v[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = plain_input<NP>(next[k][e]);
-                split8_input<NP>(v, q);
-            }
+            next[k].finish(((k * 4 + w) % KS) * 32 + g * 8, a.dim,
+                           tile * 64 + ((k * 4 + w) / KS) * 16 + s < a.n);
+            next[k].parts(q);
 #pragma unroll
             for (int p = 0; p < NP; ++p)
                 lds[p * (256 * KS) + (k * 4 + w) * 64 + quad_place(s, g)] = q[p];
@@ -352,33 +390,35 @@ __global__ __launch_bounds__(kThreads, KS <= 2 ? 2 : 1) void k_gated_units(
 #pragma unroll
         for (int k = 0; k < DQ; ++k) {
             const int r = k * 16 + (lane >> 2), q = lane & 3;
+            if (u0 + 16 * VB > a.hidden || tile * 64 + 64 > a.n)
+                next_d[k].finish(u0 + q * V, a.hidden, tile * 64 + ws * (64 / WS) + r < a.n);
             dh_lds[w][sizeof(T) == 2 ? r * 4 + (q ^ ((r >> 2 & 1) << 1))
-                                     : (r ^ (r >> 2 & 3)) * 4 + q] = next_d[k];
+                                     : (r ^ (r >> 2 & 3)) * 4 + q] = next_d[k].q[0];
         }
         __syncthreads();
         if (tile + 1 < t1) fetch(tile + 1);
 #pragma unroll 1
         for (int half = ws; half < 2; half += WS) {  // 32 rows at a time
             const quad* at = lds + half * (2 * KS * 64);
-            f32x4 z[NB][2];
-#pragma unroll
-            for (int i = 0; i < NB; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) z[i][j] = f32x4{b[i], b[i], b[i], b[i]};
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                bf16x8 f[2][NP];
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int p = 0; p < NP; ++p)
-                        f[j][p] = operand_of(at + p * (256 * KS) + (j * KS + k) * 64);
-                multiply<NP>(f, wt[k], [&](int j, int i) -> f32x4& { return z[i][j]; });
-            }
             const int64_t left = a.n - (tile * 64 + half * 32);
-            bf16x8 dz[NB][NP];
+            bf16x8 dz[VB][2][NP];
 #pragma unroll
-            for (int v = 0; v < VB; ++v) {
+            for (int v = 0; v < VB; ++v) {  // one block at a time: the registers do not last for more
+                f32x4 z[2][2];
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) z[t][j] = f32x4{b[v][t], b[v][t], b[v][t], b[v][t]};
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    bf16x8 f[2][NP];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int p = 0; p < NP; ++p)
+                            f[j][p] = operand_of(at + p * (256 * KS) + (j * KS + k) * 64);
+                    multiply<NP>(f, wt[k][v], [&](int j, int t) -> f32x4& { return z[t][j]; });
+                }
                 // units u0 + 16 v + s, rows 16 j + 4 g + r of the 32
                 float d[8];
                 const char* from = reinterpret_cast<const char*>(dh_lds[w] + (half - ws) * 128);
@@ -404,7 +444,7 @@ __global__ __launch_bounds__(kThreads, KS <= 2 ? 2 : 1) void k_gated_units(
                 float dg[8], du[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float zg = z[v][e / 4][e % 4], zu = z[VB + v][e / 4][e % 4];
+                    const float zg = z[0][e / 4][e % 4], zu = z[1][e / 4][e % 4];
                     dg[e] = plain_input<NP>(d[e] * zu * act_slope<ACT>(zg));
                     du[e] = plain_input<NP>(d[e] * act<ACT>(zg));
                 }
@@ -415,16 +455,16 @@ __global__ __launch_bounds__(kThreads, KS <= 2 ? 2 : 1) void k_gated_units(
                 }
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    sum[v] += dg[e];
-                    sum[VB + v] += du[e];
+                    sum[v][0] += dg[e];
+                    sum[v][1] += du[e];
                 }
                 quad q[NP];
                 split8_input<NP>(dg, q);
 #pragma unroll
-                for (int p = 0; p < NP; ++p) dz[v][p] = __builtin_bit_cast(bf16x8, q[p]);
+                for (int p = 0; p < NP; ++p) dz[v][0][p] = __builtin_bit_cast(bf16x8, q[p]);
                 split8_input<NP>(du, q);
 #pragma unroll
-                for (int p = 0; p < NP; ++p) dz[VB + v][p] = __builtin_bit_cast(bf16x8, q[p]);
+                for (int p = 0; p < NP; ++p) dz[v][1][p] = __builtin_bit_cast(bf16x8, q[p]);
             }
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
@@ -434,21 +474,25 @@ __global__ __launch_bounds__(kThreads, KS <= 2 ? 2 : 1) void k_gated_units(
 #pragma unroll
                     for (int p = 0; p < NP; ++p)
                         f[m][p] = operand_across(at + p * (256 * KS) + k * 64, KS * 64, m);
-                multiply<NP>(f, dz, [&](int m, int i) -> f32x4& { return dw[i][2 * k + m]; });
+#pragma unroll
+                for (int v = 0; v < VB; ++v)
+                    multiply<NP>(f, dz[v], [&](int m, int t) -> f32x4& { return dw[v][t][2 * k + m]; });
             }
         }
     }
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
+    for (int i = 0; i < 2 * VB; ++i) {
         const int64_t r = u0 * 2 + i * 16 + s;
         f32x4* to = reinterpret_cast<f32x4*>(part + (slot * wr + r) * (32 * KS));
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
-            for (int m = 0; m < 2; ++m) to[k * 8 + g * 2 + (m ^ (g & 1))] = dw[i][2 * k + m];
-        sum[i] += __shfl_xor(sum[i], 16, 64);
-        sum[i] += __shfl_xor(sum[i], 32, 64);
-        if (g == 0) db[slot * wr + r] = sum[i];
+            for (int m = 0; m < 2; ++m)
+                to[k * 8 + g * 2 + (m ^ (g & 1))] = dw[i % VB][i / VB][2 * k + m];
+        float v = sum[i % VB][i / VB];
+        v += __shfl_xor(v, 16, 64);
+        v += __shfl_xor(v, 32, 64);
+        if (g == 0) db[slot * wr + r] = v;
     }
 }
 
@@ -493,6 +537,11 @@ __global__ __launch_bounds__(1024) void k_gated_join(GatedArgs a, const float* p
     }
 }
 
+// Up to so many rows the kernels do not fill the chip: more waves a row pay, and for h alone a
+// launch less (10007 x 75 to 201 fp32: 16.6 us against 13.0 and 4.1; its dx takes 31 us
+// against 26 with cut weights, and two chunks at a time 21).
+constexpr int64_t kFewerRows = 16384;
+
 struct ShortPlan {
     int64_t chunks, tiles, wr;
     int ks, wu;
@@ -506,14 +555,15 @@ struct ShortPlan {
         ks = (dim + 31) / 32;
         chunks = (hidden + 31) / 32;
         Carve c(base);
-        laid = np > 1 ? c.take<quad>((size_t)(chunks * np * 256 * ks)) : nullptr;
+        laid = np > 1 && (grad || n > kFewerRows) ? c.take<quad>((size_t)(chunks * np * 256 * ks)) : nullptr;
         if (grad) {
             const int64_t units = np > 1 ? 16 : 32;  // of a wave
             wu = hidden > 2 * units ? 4 : 2;
             unit_blocks = (unsigned)((hidden + wu * units - 1) / (wu * units));
             wr = (int64_t)unit_blocks * wu * 2 * units;
             tiles = (n + 63) / 64;
-            const int64_t want = std::max<int64_t>(1, 512 / unit_blocks);
+            // workgroups that run at a time: two a CU, of longer rows one
+            const int64_t want = std::max<int64_t>(1, (ks <= 2 ? 512 : 256) / unit_blocks);
             per_share = std::max<int64_t>((tiles + want - 1) / want, 1);
             shares = (unsigned)std::max<int64_t>(1, (tiles + per_share - 1) / per_share);
             slots = (int)shares * (4 / wu);
@@ -524,31 +574,33 @@ struct ShortPlan {
     }
 };
 
-template <typename T, int NP, int ACT, int KS, int J, bool GRAD>
+template <typename T, int NP, int ACT, int KS, int J, int G, int P, bool GRAD, bool LAID>
 hipError_t rows_run(const GatedArgs& a, const ShortPlan& w, hipStream_t st) {
-    const int64_t blocks = (a.n + 64 * J - 1) / (64 * J);
+    const int64_t blocks = (a.n + 16 * G * J - 1) / (16 * G * J);
     // dx is the sum over all chunks: they are shared out for h alone
     const int64_t want = GRAD ? 1 : std::min<int64_t>(w.chunks, std::max<int64_t>(1, 512 / blocks));
     const int64_t per = (w.chunks + want - 1) / want;
     const dim3 grid((unsigned)blocks, (unsigned)((w.chunks + per - 1) / per));
-    k_gated_rows<T, NP, ACT, KS, J, GRAD><<<grid, kThreads, 0, st>>>(a, w.laid, w.chunks, per);
+    k_gated_rows<T, NP, ACT, KS, J, G, P, GRAD, LAID>
+        <<<grid, 64 * G * P, 0, st>>>(a, w.laid, w.chunks, per);
     return hipGetLastError();
 }
 
 template <typename T, int NP, int ACT, int KS>
 hipError_t short_run(const GatedArgs& a, bool grad, hipStream_t st) {
     const ShortPlan w(a.ws, a.n, a.hidden, a.dim, NP, grad);
-    if (NP > 1) {
+    constexpr bool CUT = NP > 1;
+    if (w.laid != nullptr) {
         k_gated_chunks<T, NP, KS><<<blocks_of(w.chunks * 256 * KS, kThreads), kThreads, 0, st>>>(
             a, w.chunks, w.laid);
         GS_LAUNCHED();
     }
     constexpr int kMost = NP == 1 ? 4 : 2, kMostGrad = NP == 1 ? 2 : (KS <= 2 ? 2 : 1);
     if (!grad)
-        return a.n <= 16384 ? rows_run<T, NP, ACT, KS, 1, false>(a, w, st)
-                            : rows_run<T, NP, ACT, KS, kMost, false>(a, w, st);
-    hipError_t e = a.n <= 32768 ? rows_run<T, NP, ACT, KS, 1, true>(a, w, st)
-                                : rows_run<T, NP, ACT, KS, kMostGrad, true>(a, w, st);
+        return a.n <= kFewerRows ? rows_run<T, NP, ACT, KS, 1, 4, 1, false, false>(a, w, st)
+                                 : rows_run<T, NP, ACT, KS, kMost, 4, 1, false, CUT>(a, w, st);
+    hipError_t e = a.n <= kFewerRows ? rows_run<T, NP, ACT, KS, 1, 4, 2, true, CUT>(a, w, st)
+                                     : rows_run<T, NP, ACT, KS, kMostGrad, 4, 1, true, CUT>(a, w, st);
     if (e != hipSuccess) return e;
     const dim3 grid(w.unit_blocks, w.shares);
     if (w.wu == 4)
