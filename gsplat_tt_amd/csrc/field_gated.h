@@ -16,6 +16,9 @@ constexpr int kShortDim = 128;
 size_t gated_short_ws(const GatedArgs& a, bool grad);
 hipError_t gated_short_f32(const GatedArgs& a, bool grad, hipStream_t st);
 hipError_t gated_short_bf16(const GatedArgs& a, bool grad, hipStream_t st);
+// dx's rows n0 .. + n as sums of `shares` parts (rows, ld).
+hipError_t gated_dx_join(const GatedArgs& a, const float* part, int shares, int64_t rows, int ld,
+                         int64_t n0, int64_t n, hipStream_t st);
 
 // 8 values of a row from column c, zeros past `cols`.
 template <typename T>

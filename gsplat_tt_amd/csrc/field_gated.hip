@@ -38,6 +38,11 @@ __device__ __forceinline__ UnitOf unit_of(int64_t r) {
     return {(r >> 6) * 32 + (s >> 2) * 8 + ((t >> 4) & 1) * 4 + (s & 3), t >= 32};
 }
 
+// The gate row of a unit that is a multiple of 4; its up row is 32 on.
+__device__ __forceinline__ int64_t row_of_unit(int64_t u) {
+    return (u >> 5) * 64 + ((u >> 2) & 1) * 16 + ((u >> 3) & 3) * 4;
+}
+
 // Parts of x's rows from n0 as (nr, ld), or of the weights in the order above; zeros in
 // the padding.
 template <typename T, int NP, bool WEIGHTS>
@@ -158,22 +163,31 @@ __global__ __launch_bounds__(kThreads, 2) void k_gated(GatedArgs a, Mat X, Mat W
         });
 }
 
-// dx of one tile: the weights' columns against the samples' [dgate, dup].
+// dx of one tile: the weights' columns against the samples' [dgate, dup]; of several shares of
+// these (blockIdx.y) each leaves its sums in `part` (share, samples, ld).
 template <typename T, int NP>
 __global__ __launch_bounds__(kThreads, 2) void k_gated_dx(GatedArgs a, Mat W, Mat Z, int64_t n0,
-                                                          int64_t nr, int ld, int64_t wr, int gy) {
+                                                          int64_t nr, int ld, int64_t wr, int gy,
+                                                          int64_t per_share, float* part) {
     GS_TILE_LDS;
+    const int64_t k0 = min(wr, blockIdx.y * per_share), k1 = min(wr, k0 + per_share);
     const int lane = threadIdx.x & 63, w = wave_id();
     const int wm = (w >> 1) * 64, wn = (w & 1) * 64;
     const Spot at = spot((int)(nr / kTile), gy);
     const int64_t c0 = (int64_t)at.y * kTile, s0 = (int64_t)at.x * kTile;
     if (c0 >= ld) return;
     tile_products<NP, false, true>(
-        W, Z, 0, wr, 1, lds, [&](int) { return TileRows{c0, s0}; },
+        W, Z, k0, k1, 1, lds, [&](int) { return TileRows{c0, s0}; },
         [&](int, f32x4(&acc)[4][4]) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int64_t i = n0 + s0 + wn + j * 16 + (lane & 15);
+                const int64_t r = s0 + wn + j * 16 + (lane & 15), i = n0 + r;
+                if (gridDim.y > 1) {
+                    f32x4* to = reinterpret_cast<f32x4*>(part + (blockIdx.y * nr + r) * ld + c0 + wm);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) to[k * 4 + (lane >> 4)] = acc[k][j];
+                    continue;
+                }
                 if (i >= a.n) continue;
                 T* row = static_cast<T*>(a.dx) + i * a.dx_stride;
 #pragma unroll
@@ -183,6 +197,26 @@ __global__ __launch_bounds__(kThreads, 2) void k_gated_dx(GatedArgs a, Mat W, Ma
                 }
             }
         });
+}
+
+// 4 columns of dx a thread, summed over the parts in order.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_gated_dx_join(GatedArgs a, const float* part,
+                                                            int shares, int64_t rows, int ld,
+                                                            int64_t n0, int64_t n) {
+    const int units = (a.dim + 3) / 4;
+    const int64_t total = n * units;
+    for (int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x; e < total;
+         e += (int64_t)gridDim.x * kThreads) {
+        const int64_t i = e / units;
+        const int c = (int)(e - i * units) * 4;
+        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+        for (int k = 0; k < shares; ++k)
+            v += *reinterpret_cast<const f32x4*>(part + (k * rows + i) * ld + c);
+        const float o[4] = {v[0], v[1], v[2], v[3]};
+        store_cols<4>(static_cast<T*>(a.dx) + (n0 + i) * a.dx_stride, c, a.dim, o);
+    }
 }
 
 // One tile of the weights' gradients, over a share of the samples; with `add` onto what an
@@ -446,13 +480,16 @@ __global__ __launch_bounds__((WideShape<NP, AB>::kThreads), 2) void k_wide_dw(Wi
 }
 
 // ---------------------------------------------------------------- few rows
-// Up to 64 rows, without their gradients: every workgroup makes 16 hidden units of all
-// rows, its waves sharing the summed index; the operands come from memory as the matrix
-// cores take them, 8 values of a row a lane, so that nothing is laid out before.
+// Up to 64 rows: every workgroup makes 16 hidden units of all rows, its waves sharing the
+// summed index; the operands come from memory as the matrix cores take them, 8 values of a
+// row a lane, so that nothing is laid out before.
 constexpr int kFewRows = 64;
 
-template <typename T, int NP, int ACT, int J>
-__global__ __launch_bounds__(kThreads) void k_gated_few(GatedArgs a) {
+// With GRAD the rows [dgate, dup] as operands of the tiles below, 128 rows with zeros behind, and
+// the biases' sums over each block of 16 rows.
+template <typename T, int NP, int ACT, int J, bool GRAD>
+__global__ __launch_bounds__(kThreads) void k_gated_few(GatedArgs a, bf16* dz, float* db,
+                                                        int64_t wr) {
     __shared__ f32x4 lds[kThreads / 64][2 * J][64];
     const int lane = threadIdx.x & 63, w = wave_id(), g = lane >> 4, s = lane & 15;
     const int64_t u0 = (int64_t)blockIdx.x * 16;
@@ -499,17 +536,58 @@ __global__ __launch_bounds__(kThreads) void k_gated_few(GatedArgs a) {
             for (int v = 1; v < kThreads / 64; ++v) z[t] += lds[v][t * J + j][lane];
         }
         const int64_t i = j * 16 + s, u = u0 + g * 4;
-        if (i >= a.n) continue;
-        float h[4];
+        if (!GRAD && i >= a.n) continue;
+        float h[4], d[8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const bool in = u + k < a.hidden;
             const float bg = in && a.b_gate != nullptr ? a.b_gate[u + k] : 0.0f;
             const float bu = in && a.b_up != nullptr ? a.b_up[u + k] : 0.0f;
-            h[k] = act<ACT>(z[0][k] + bg) * (z[1][k] + bu);
+            const float zg = z[0][k] + bg, zu = z[1][k] + bu;
+            if (!GRAD) {
+                h[k] = act<ACT>(zg) * zu;
+            } else {
+                const bool on = in && i < a.n;
+                const float v = on ? to_float(static_cast<const T*>(a.dh)[i * a.dh_stride + u + k])
+                                   : 0.0f;
+                d[k] = on ? plain_input<NP>(v * zu * act_slope<ACT>(zg)) : 0.0f;
+                d[4 + k] = on ? plain_input<NP>(v * act<ACT>(zg)) : 0.0f;
+            }
         }
-        store_cols<4>(static_cast<T*>(a.h) + i * a.h_stride, u, a.hidden, h);
+        if (!GRAD) {
+            store_cols<4>(static_cast<T*>(a.h) + i * a.h_stride, u, a.hidden, h);
+            continue;
+        }
+        // 4 units in a row are 4 rows of the weights in a row, gate and 32 on up
+        const int64_t r = row_of_unit(u);
+        quad q[NP];
+        split8_input<NP>(d, q);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            uint2* to = reinterpret_cast<uint2*>(dz + (p * kTile + i) * wr + r);
+            to[0] = make_uint2(q[p][0], q[p][1]);
+            to[8] = make_uint2(q[p][2], q[p][3]);
+        }
+        if (db != nullptr) {
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) d[k] += __shfl_xor(d[k], o, 64);
+            if (s == 0) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) db[j * wr + r + (k / 4) * 32 + k % 4] = d[k];
+            }
+        }
     }
+    if (!GRAD) return;
+    // the rows behind: 4 units a thread and row
+    const int64_t r = row_of_unit(u0 + (threadIdx.x & 3) * 4);
+    for (int i = 16 * J + (int)(threadIdx.x >> 2); i < kTile; i += kThreads / 4)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            uint2* to = reinterpret_cast<uint2*>(dz + (p * kTile + i) * wr + r);
+            to[0] = to[8] = make_uint2(0u, 0u);
+        }
 }
 
 bool is_few(const GatedArgs& a, bool grad) { return !grad && a.n <= kFewRows; }
@@ -517,9 +595,18 @@ bool is_few(const GatedArgs& a, bool grad) { return !grad && a.n <= kFewRows; }
 template <typename T, int NP, int ACT>
 hipError_t few_run(const GatedArgs& a, hipStream_t st) {
     const unsigned blocks = (unsigned)((a.hidden + 15) / 16);
-    if (a.n <= 16) k_gated_few<T, NP, ACT, 1><<<blocks, kThreads, 0, st>>>(a);
-    else if (a.n <= 32) k_gated_few<T, NP, ACT, 2><<<blocks, kThreads, 0, st>>>(a);
-    else k_gated_few<T, NP, ACT, 4><<<blocks, kThreads, 0, st>>>(a);
+    if (a.n <= 16) k_gated_few<T, NP, ACT, 1, false><<<blocks, kThreads, 0, st>>>(a, nullptr, nullptr, 0);
+    else if (a.n <= 32) k_gated_few<T, NP, ACT, 2, false><<<blocks, kThreads, 0, st>>>(a, nullptr, nullptr, 0);
+    else k_gated_few<T, NP, ACT, 4, false><<<blocks, kThreads, 0, st>>>(a, nullptr, nullptr, 0);
+    return hipGetLastError();
+}
+// Every unit of the padded weights has its place in dz.
+template <typename T, int NP, int ACT>
+hipError_t few_grad(const GatedArgs& a, bf16* dz, float* db, int64_t wr, hipStream_t st) {
+    const unsigned blocks = (unsigned)(wr / 32);
+    if (a.n <= 16) k_gated_few<T, NP, ACT, 1, true><<<blocks, kThreads, 0, st>>>(a, dz, db, wr);
+    else if (a.n <= 32) k_gated_few<T, NP, ACT, 2, true><<<blocks, kThreads, 0, st>>>(a, dz, db, wr);
+    else k_gated_few<T, NP, ACT, 4, true><<<blocks, kThreads, 0, st>>>(a, dz, db, wr);
     return hipGetLastError();
 }
 
@@ -530,8 +617,9 @@ constexpr int64_t kPieceBytes = (int64_t)1 << 30;
 struct GatedPlan {
     int ld;            // padded dim
     int64_t wr, piece, shares;  // weight rows, samples of a piece, shares of the weights' sums
-    bf16 *w, *x, *dz;
-    float *part, *db;
+    int64_t dx_shares = 1, dx_per = 0;  // shares of the weights' rows in dx
+    bf16 *w = nullptr, *x = nullptr, *dz = nullptr;
+    float *part = nullptr, *db = nullptr, *dx = nullptr;
     size_t bytes;
     GatedPlan(void* base, int64_t n, int64_t hidden, int dim, int np, bool grad) {
         ld = (int)pad_to(dim, kTile);
@@ -549,7 +637,13 @@ struct GatedPlan {
         if (grad) {
             dz = c.take<bf16>((size_t)(piece * wr) * np);
             part = c.take<float>((size_t)(shares * wr * ld));
-            db = c.take<float>((size_t)(piece / 64 * wr));
+            db = c.take<float>((size_t)(std::max<int64_t>(4, piece / 64) * wr));
+            // one step of the summed index at least, and as many workgroups as run at a time
+            const int64_t of_dx = std::max<int64_t>(1, piece / kTile * (ld / kTile));
+            const int64_t want = std::max<int64_t>(1, std::min(wr / kStep, 512 / of_dx));
+            dx_per = pad_to((wr + want - 1) / want, kStep);
+            dx_shares = (wr + dx_per - 1) / dx_per;
+            dx = dx_shares > 1 ? c.take<float>((size_t)(dx_shares * piece * ld)) : nullptr;
         }
         bytes = c.bytes();
     }
@@ -564,12 +658,12 @@ bool is_wide(const GatedArgs& a) {
 }
 
 struct WidePlan {
-    int ld, ldp, ab;  // the weights' columns, the partial sums', blocks of A for the gradients
-    int64_t wr, piece, shares, per_share;
+    int ld, ldp = 0, ab = 4;  // the weights' columns, the partial sums', blocks of A for the gradients
+    int64_t wr, piece, shares = 0, per_share = 0;
     bool direct;  // x is read where it is
     quad* zero;
-    bf16 *w, *x, *dz;
-    float *part, *db;
+    bf16 *w, *x = nullptr, *dz = nullptr;
+    float *part = nullptr, *db = nullptr;
     size_t bytes;
     WidePlan(void* base, const GatedArgs& a, int np, bool grad) {
         ld = (int)pad_to(a.dim, kStep);
@@ -693,17 +787,30 @@ hipError_t gated_run(const GatedArgs& a, bool grad, hipStream_t st) {
             GS_LAUNCHED();
             continue;
         }
-        k_gated<T, NP, ACT, true><<<sg.blocks, kThreads, 0, st>>>(
-            a, X, W, kd, n0, nr, w.wr, sg.gy, w.dz, biases ? w.db : nullptr);
-        GS_LAUNCHED();
+        const bool few = a.n <= kFewRows;
+        if (few) {
+            const hipError_t e = few_grad<T, NP, ACT>(a, w.dz, biases ? w.db : nullptr, w.wr, st);
+            if (e != hipSuccess) return e;
+        } else {
+            k_gated<T, NP, ACT, true><<<sg.blocks, kThreads, 0, st>>>(
+                a, X, W, kd, n0, nr, w.wr, sg.gy, w.dz, biases ? w.db : nullptr);
+            GS_LAUNCHED();
+        }
         if (biases) {
+            const int64_t blocks = few ? (a.n <= 32 ? (a.n + 15) / 16 : 4) : nr / 64;
             k_gated_sum<T, false, true><<<sum_blocks(w.wr / 4), 1024, 0, st>>>(
-                a, w.db, (int)(nr / 64), w.wr, 4, n0 > 0);
+                a, w.db, (int)blocks, w.wr, 4, n0 > 0);
             GS_LAUNCHED();
         }
         const SpotGrid xg(nr / kTile, w.ld / kTile, kSpot);
-        k_gated_dx<T, NP><<<xg.blocks, kThreads, 0, st>>>(a, W, Z, n0, nr, w.ld, w.wr, xg.gy);
+        k_gated_dx<T, NP><<<dim3(xg.blocks, (unsigned)w.dx_shares), kThreads, 0, st>>>(
+            a, W, Z, n0, nr, w.ld, w.wr, xg.gy, w.dx_per, w.dx);
         GS_LAUNCHED();
+        if (w.dx_shares > 1) {
+            const hipError_t e = gated_dx_join(a, w.dx, (int)w.dx_shares, nr, w.ld, n0,
+                                               std::min(w.piece, a.n - n0), st);
+            if (e != hipSuccess) return e;
+        }
         const int64_t per = pad_to((nr + w.shares - 1) / w.shares, kStep);
         const dim3 grid((unsigned)(w.wr / kTile * (w.ld / kTile)), (unsigned)w.shares);
         k_gated_dw<NP><<<grid, kThreads, 0, st>>>(X, Z, nr, w.ld, w.wr, per, n0 > 0, w.part);
@@ -730,6 +837,16 @@ hipError_t gated_act(const GatedArgs& a, bool grad, hipStream_t st) {
 }
 
 }  // namespace
+
+hipError_t gated_dx_join(const GatedArgs& a, const float* part, int shares, int64_t rows, int ld,
+                         int64_t n0, int64_t n, hipStream_t st) {
+    const unsigned blocks = blocks_of(n * ((a.dim + 3) / 4), kThreads);
+    if (a.dtype == 0)
+        k_gated_dx_join<float><<<blocks, kThreads, 0, st>>>(a, part, shares, rows, ld, n0, n);
+    else
+        k_gated_dx_join<bf16><<<blocks, kThreads, 0, st>>>(a, part, shares, rows, ld, n0, n);
+    return hipGetLastError();
+}
 
 size_t gated_linear_ws(const GatedArgs& a, bool grad) {
     if (a.n == 0 || is_few(a, grad)) return 0;

@@ -91,20 +91,18 @@ __global__ __launch_bounds__(kThreads) void k_gated_chunks(GatedArgs a, int64_t 
 // Rows stay with their wave, 16 J of them in registers, and the weights pass through LDS
 // chunk by chunk: h, or with GRAD dx, whose sums stay in registers too. The gradients of
 // gate and up leave the sums in the layout that the next product takes them in. LAID: the
-// chunks' parts come from k_gated_chunks. P sets of G waves with the same rows take P chunks
-// at a time, and the first adds up their dx.
-template <typename T, int NP, int ACT, int KS, int J, int G, int P, bool GRAD, bool LAID>
-__global__ __launch_bounds__(64 * G * P, P == 1 && (NP == 1 || J * KS < 8) ? 2 : 1) void k_gated_rows(
-    GatedArgs a, const quad* laid, int64_t chunks, int64_t per_share) {
-    constexpr int SET = NP * 256 * KS, SUMS = P > 1 ? 2 * KS * J * 64 * G : 1, KQ = 4 / G * KS;
-    __shared__ quad lds[P * SET > SUMS ? P * SET : SUMS];
-    __shared__ float bias[P][64];
-    const int lane = threadIdx.x & 63, wave = wave_id(), g = lane >> 4, s = lane & 15;
-    const int w = wave % G, set = wave / G, t = threadIdx.x % (64 * G);
-    const int64_t i0 = ((int64_t)blockIdx.x * G + w) * (16 * J);
+// chunks' parts come from k_gated_chunks. Shares of the chunks (blockIdx.y) leave sums of dx
+// of their own in `part` (share, rows, 32 KS), where there are several.
+template <typename T, int NP, int ACT, int KS, int J, bool GRAD, bool LAID>
+__global__ __launch_bounds__(kThreads, NP == 1 || J * KS < 8 ? 2 : 1) void k_gated_rows(
+    GatedArgs a, const quad* laid, int64_t chunks, int64_t per_share, float* part) {
+    __shared__ quad lds[NP * 256 * KS];
+    __shared__ float bias[64];
+    const int lane = threadIdx.x & 63, w = wave_id(), g = lane >> 4, s = lane & 15;
+    const int64_t i0 = ((int64_t)blockIdx.x * (kThreads / 64) + w) * (16 * J);
     const int64_t c0 = blockIdx.y * per_share, c1 = min(chunks, c0 + per_share);
-    quad next[KQ][LAID ? NP : 1];
-    Raw<T> next_w[LAID ? 1 : KQ];
+    quad next[KS][LAID ? NP : 1];
+    Raw<T> next_w[LAID ? 1 : KS];
     Raw<T> next_d[J];
     float next_bias = 0.0f;
     auto fetch = [&](int64_t chunk) {
@@ -117,14 +115,13 @@ __global__ __launch_bounds__(64 * G * P, P == 1 && (NP == 1 || J * KS < 8) ? 2 :
             }
         }
 #pragma unroll
-        for (int k = 0; k < KQ; ++k) {
+        for (int k = 0; k < KS; ++k) {
             if constexpr (LAID) {
 #pragma unroll
                 for (int p = 0; p < NP; ++p)
-                    next[k][p] = chunk < c1 ? laid[(chunk * NP + p) * (256 * KS) + k * (64 * G) + t]
-                                            : quad{0u, 0u, 0u, 0u};
+                    next[k][p] = laid[(chunk * NP + p) * (256 * KS) + k * 256 + threadIdx.x];
             } else {
-                const int blk = k * G + w;
+                const int blk = k * 4 + w;
                 next_w[k].load(weight_row<T>(a, chunk * 32, blk / KS, s), (blk % KS) * 32 + g * 8,
                                a.dim);
             }
@@ -136,7 +133,7 @@ __global__ __launch_bounds__(64 * G * P, P == 1 && (NP == 1 || J * KS < 8) ? 2 :
             next_bias = from != nullptr && unit < a.hidden ? from[unit] : 0.0f;
         }
     };
-    if (c0 < c1) fetch(c0 + set);
+    if (c0 < c1) fetch(c0);
     bf16x8 x[KS][J][NP];
 #pragma unroll
     for (int j = 0; j < J; ++j) {
@@ -160,27 +157,25 @@ __global__ __launch_bounds__(64 * G * P, P == 1 && (NP == 1 || J * KS < 8) ? 2 :
     for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int j = 0; j < J; ++j) dx[d][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    quad* mine = lds + set * SET;
-    for (int64_t first = c0; first < c1; first += P) {
-        const int64_t chunk = first + set;  // past the last: zeros
-        __syncthreads();  // the last chunks have been read
+    for (int64_t chunk = c0; chunk < c1; ++chunk) {
+        __syncthreads();  // the last chunk has been read
 #pragma unroll
-        for (int k = 0; k < KQ; ++k) {
+        for (int k = 0; k < KS; ++k) {
             if constexpr (LAID) {
 #pragma unroll
-                for (int p = 0; p < NP; ++p) mine[p * (256 * KS) + k * (64 * G) + t] = next[k][p];
+                for (int p = 0; p < NP; ++p) lds[p * (256 * KS) + k * 256 + threadIdx.x] = next[k][p];
             } else {
-                const int blk = k * G + w;
+                const int blk = k * 4 + w;
                 next_w[k].finish((blk % KS) * 32 + g * 8, a.dim,
                                  weight_unit(chunk * 32, blk / KS, s) < a.hidden);
                 quad q[NP];
                 next_w[k].parts(q);
 #pragma unroll
                 for (int p = 0; p < NP; ++p)
-                    mine[p * (256 * KS) + (k * G + w) * 64 + quad_place(s, g)] = q[p];
+                    lds[p * (256 * KS) + (k * 4 + w) * 64 + quad_place(s, g)] = q[p];
             }
         }
-        if (w == 0) bias[set][lane] = next_bias;
+        if (w == 0) bias[lane] = next_bias;
         Raw<T> d[J];
         if (GRAD) {
 #pragma unroll
@@ -192,12 +187,12 @@ __global__ __launch_bounds__(64 * G * P, P == 1 && (NP == 1 || J * KS < 8) ? 2 :
             }
         }
         __syncthreads();
-        if (first + P < c1) fetch(chunk + P);
+        if (chunk + 1 < c1) fetch(chunk + 1);
         const int64_t u0 = chunk * 32 + g * 8;
         f32x4 z[4][J];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const f32x4 b = *reinterpret_cast<const f32x4*>(bias[set] + i * 16 + g * 4);
+            const f32x4 b = *reinterpret_cast<const f32x4*>(bias + i * 16 + g * 4);
 #pragma unroll
             for (int j = 0; j < J; ++j) z[i][j] = b;
         }
@@ -210,7 +205,7 @@ __global__ __launch_bounds__(64 * G * P, P == 1 && (NP == 1 || J * KS < 8) ? 2 :
                 for (int m = 0; m < 2; ++m)
 #pragma unroll
                     for (int p = 0; p < NP; ++p)
-                        f[m][p] = operand_of(mine + p * (256 * KS) + ((i + m) * KS + k) * 64);
+                        f[m][p] = operand_of(lds + p * (256 * KS) + ((i + m) * KS + k) * 64);
                 multiply<NP>(f, x[k], [&](int m, int j) -> f32x4& { return z[i + m][j]; });
             }
         if (!GRAD) {
@@ -262,31 +257,21 @@ __global__ __launch_bounds__(64 * G * P, P == 1 && (NP == 1 || J * KS < 8) ? 2 :
 #pragma unroll
                     for (int p = 0; p < NP; ++p)
                         f[m][p] = operand_across(
-                            mine + p * (256 * KS) + u * (2 * KS * 64) + k * 64, KS * 64, m);
+                            lds + p * (256 * KS) + u * (2 * KS * 64) + k * 64, KS * 64, m);
                 multiply<NP>(f, dz[u], [&](int m, int j) -> f32x4& { return dx[2 * k + m][j]; });
             }
     }
     if (!GRAD) return;
-    if constexpr (P > 1) {
-        f32x4* sums = reinterpret_cast<f32x4*>(lds);
+    if (gridDim.y > 1) {
+        const int64_t rows = (int64_t)gridDim.x * (kThreads / 64 * 16 * J);
 #pragma unroll
-        for (int from = 1; from < P; ++from) {
-            __syncthreads();
-            if (set == from) {
+        for (int j = 0; j < J; ++j) {
+            f32x4* to = reinterpret_cast<f32x4*>(
+                part + (blockIdx.y * rows + i0 + j * 16 + s) * (32 * KS));
 #pragma unroll
-                for (int c = 0; c < DB; ++c)
-#pragma unroll
-                    for (int j = 0; j < J; ++j) sums[(c * J + j) * (64 * G) + t] = dx[c][j];
-            }
-            __syncthreads();
-            if (set == 0) {
-#pragma unroll
-                for (int c = 0; c < DB; ++c)
-#pragma unroll
-                    for (int j = 0; j < J; ++j) dx[c][j] += sums[(c * J + j) * (64 * G) + t];
-            }
+            for (int c = 0; c < DB; ++c) to[c / 2 * 8 + g * 2 + ((c ^ g) & 1)] = dx[c][j];
         }
-        if (set != 0) return;
+        return;
     }
 #pragma unroll
     for (int j = 0; j < J; ++j) {
@@ -537,25 +522,36 @@ __global__ __launch_bounds__(1024) void k_gated_join(GatedArgs a, const float* p
     }
 }
 
-// Up to so many rows the kernels do not fill the chip: more waves a row pay, and for h alone a
-// launch less (10007 x 75 to 201 fp32: 16.6 us against 13.0 and 4.1; its dx takes 31 us
-// against 26 with cut weights, and two chunks at a time 21).
+// Up to so many rows the kernels do not fill the chip: 16 rows a wave, chunks in shares, and
+// for h alone no launch to cut the weights before (10007 x 75 to 201 fp32: 16.6 us against
+// 13.0 and 4.1).
 constexpr int64_t kFewerRows = 16384;
 
 struct ShortPlan {
-    int64_t chunks, tiles, wr;
-    int ks, wu;
-    unsigned unit_blocks, shares;
-    int64_t per_share;
-    int slots;
+    int64_t chunks, tiles = 0, wr = 0;
+    int ks, wu = 4;
+    unsigned unit_blocks = 0, shares = 0;
+    int64_t per_share = 0;
+    int slots = 0;
+    int64_t row_blocks, row_shares;  // of k_gated_rows with few rows
     quad* laid;
-    float *part, *db;
+    float *part = nullptr, *db = nullptr, *dx = nullptr;
     size_t bytes;
     ShortPlan(void* base, int64_t n, int64_t hidden, int dim, int np, bool grad) {
         ks = (dim + 31) / 32;
         chunks = (hidden + 31) / 32;
+        // with gradients each share's sums of dx are written and read: at least 2 chunks each
+        row_blocks = (n + 63) / 64;
+        row_shares = 1;
+        if (n <= kFewerRows) {
+            const int64_t want = std::max<int64_t>(1, std::min((grad ? chunks / 2 : chunks),
+                                                               512 / std::max<int64_t>(1, row_blocks)));
+            const int64_t per = (chunks + want - 1) / want;
+            row_shares = (chunks + per - 1) / per;
+        }
         Carve c(base);
-        laid = np > 1 && (grad || n > kFewerRows) ? c.take<quad>((size_t)(chunks * np * 256 * ks)) : nullptr;
+        laid = np > 1 && (grad || n > kFewerRows) ? c.take<quad>((size_t)(chunks * np * 256 * ks))
+                                                  : nullptr;
         if (grad) {
             const int64_t units = np > 1 ? 16 : 32;  // of a wave
             wu = hidden > 2 * units ? 4 : 2;
@@ -569,20 +565,20 @@ struct ShortPlan {
             slots = (int)shares * (4 / wu);
             part = c.take<float>((size_t)slots * wr * 32 * ks);
             db = c.take<float>((size_t)slots * wr);
+            dx = row_shares > 1 ? c.take<float>((size_t)(row_shares * row_blocks * 64 * 32 * ks))
+                                : nullptr;
         }
         bytes = c.bytes();
     }
 };
 
-template <typename T, int NP, int ACT, int KS, int J, int G, int P, bool GRAD, bool LAID>
+template <typename T, int NP, int ACT, int KS, int J, bool GRAD, bool LAID>
 hipError_t rows_run(const GatedArgs& a, const ShortPlan& w, hipStream_t st) {
-    const int64_t blocks = (a.n + 16 * G * J - 1) / (16 * G * J);
-    // dx is the sum over all chunks: they are shared out for h alone
-    const int64_t want = GRAD ? 1 : std::min<int64_t>(w.chunks, std::max<int64_t>(1, 512 / blocks));
-    const int64_t per = (w.chunks + want - 1) / want;
-    const dim3 grid((unsigned)blocks, (unsigned)((w.chunks + per - 1) / per));
-    k_gated_rows<T, NP, ACT, KS, J, G, P, GRAD, LAID>
-        <<<grid, 64 * G * P, 0, st>>>(a, w.laid, w.chunks, per);
+    const int64_t blocks = (a.n + 64 * J - 1) / (64 * J);
+    const int64_t per = (w.chunks + w.row_shares - 1) / w.row_shares;
+    const dim3 grid((unsigned)blocks, (unsigned)w.row_shares);
+    k_gated_rows<T, NP, ACT, KS, J, GRAD, LAID>
+        <<<grid, kThreads, 0, st>>>(a, w.laid, w.chunks, per, w.dx);
     return hipGetLastError();
 }
 
@@ -597,11 +593,15 @@ hipError_t short_run(const GatedArgs& a, bool grad, hipStream_t st) {
     }
     constexpr int kMost = NP == 1 ? 4 : 2, kMostGrad = NP == 1 ? 2 : (KS <= 2 ? 2 : 1);
     if (!grad)
-        return a.n <= kFewerRows ? rows_run<T, NP, ACT, KS, 1, 4, 1, false, false>(a, w, st)
-                                 : rows_run<T, NP, ACT, KS, kMost, 4, 1, false, CUT>(a, w, st);
-    hipError_t e = a.n <= kFewerRows ? rows_run<T, NP, ACT, KS, 1, 4, 2, true, CUT>(a, w, st)
-                                     : rows_run<T, NP, ACT, KS, kMostGrad, 4, 1, true, CUT>(a, w, st);
+        return a.n <= kFewerRows ? rows_run<T, NP, ACT, KS, 1, false, false>(a, w, st)
+                                 : rows_run<T, NP, ACT, KS, kMost, false, CUT>(a, w, st);
+    hipError_t e = a.n <= kFewerRows ? rows_run<T, NP, ACT, KS, 1, true, CUT>(a, w, st)
+                                     : rows_run<T, NP, ACT, KS, kMostGrad, true, CUT>(a, w, st);
     if (e != hipSuccess) return e;
+    if (w.row_shares > 1) {
+        e = gated_dx_join(a, w.dx, (int)w.row_shares, w.row_blocks * 64, 32 * KS, 0, a.n, st);
+        if (e != hipSuccess) return e;
+    }
     const dim3 grid(w.unit_blocks, w.shares);
     if (w.wu == 4)
         k_gated_units<T, NP, ACT, KS, 4><<<grid, kThreads, 0, st>>>(a, w.tiles, w.per_share, w.wr,

@@ -107,7 +107,8 @@ NAMES = ("dx", "dw_gate", "dw_up", "db_gate", "db_up")
 SIZES = [(1, 1, 1), (1, 64, 256), (2, 3, 5), (7, 8, 16), (33, 512, 70), (64, 32, 32),
          (65, 33, 31), (127, 129, 65), (129, 64, 128), (300, 16, 200), (1000, 75, 201),
          (5, 1000, 17), (513, 128, 64), (2000, 40, 24), (4097, 64, 128), (1, 300, 1000),
-         (16, 64, 33), (17, 256, 100), (640, 260, 136)]
+         (16, 64, 33), (17, 256, 100), (640, 260, 136), (7, 512, 512), (31, 200, 333), (48, 140, 1000),
+         (64, 129, 30), (3586, 100, 300), (200, 128, 2000)]
 
 
 @pytest.mark.parametrize("n,dim,hidden", SIZES)
