@@ -22,7 +22,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kVec = 4;
 constexpr int kAhead = 4;  // vectors that a thread loads before it uses them
-constexpr int64_t kChunk = kThreads * kVec * kAhead;
+constexpr int64_t kChunk = 2 * kThreads * kVec * kAhead;  // whole rounds of either type
 constexpr int64_t kMostChunks = 4096;  // of the whole list, about
 
 struct Entry {

@@ -178,6 +178,25 @@ def test_norm_given(ops):
     assert (t - 0.25).abs().max() <= 2 * EPS
 
 
+def test_parameters_and_inference_tensors(ops):
+    """Tensors that are parameters, or made under inference_mode, among others; versions of
+    what is written are counted."""
+    p = torch.nn.Parameter(torch.ones(30, device="cuda"))
+    with torch.inference_mode():
+        i = torch.ones(20, device="cuda")
+    t = torch.ones(50, device="cuda")
+    version = t._version
+    with torch.no_grad():
+        n = ops.clip_grads([p, i, t], 1.0)
+    assert abs(float(n) - 10.0) <= 1e-6 and t._version == version + 1
+    for x in (p, i, t):
+        assert (x.detach() - 0.1).abs().max() <= 4 * EPS
+    with pytest.raises(ValueError, match="requires a gradient"):
+        ops.grad_norm([p])
+    n = ops.grad_norm(x.detach() for x in (p, t))  # any iterable
+    assert abs(float(n) - 80 ** 0.5 / 10) <= 1e-6
+
+
 def test_results_do_not_change_from_run_to_run(ops):
     ts = [torch.randn(n, device="cuda") for n in (5_000_011, 3, 100_003)]
     first = ops.grad_norm(ts)
