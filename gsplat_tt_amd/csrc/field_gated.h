@@ -12,6 +12,9 @@
 
 namespace gs {
 
+// Rows of up to 128 stay in registers (field_gated_short.h); against tiles, h and a training
+// pass: 100000 x 128 to 512 bf16 50 and 249 us, in tiles 78 and 333; 30000 x 128 to 512 fp32
+// 56 and 288, in tiles 62 and 298.
 constexpr int kShortDim = 128;
 size_t gated_short_ws(const GatedArgs& a, bool grad);
 hipError_t gated_short_f32(const GatedArgs& a, bool grad, hipStream_t st);

@@ -10,8 +10,21 @@
 //
 // All products run on the matrix cores with bf16 operands and fp32 sums; fp32 values are
 // cut into three bf16 parts, whose six products above 2^-24 are added up (field_tiles.h).
-// For bf16 inputs dgate and dup are rounded to bf16 as operands of the next products; the
-// biases' gradients sum them in fp32.
+// For bf16 inputs dgate and dup are rounded to bf16 as operands of the next products (100003
+// x 512 to 2048: gradients 0.0024 off, 2-norm, relative, where rounding them alone gives
+// 0.0017); the biases' gradients sum them in fp32.
+//
+// Four ways, by size:
+//   few     up to 64 rows: one launch, operands straight from memory (with gradients of long
+//           rows, their first part).
+//   short   rows of up to 128 (field_gated_short.h): rows in registers, weights through LDS; dx
+//           in a pass over the weights, the weights' gradients in one over the rows, and
+//           [dgate, dup] made in both, which costs 8 n dim hidden operations but not 12 bytes
+//           a value.
+//   wide    longer rows, many tiles: 256 x 256 (fp32 128 x 128), [dgate, dup] of one piece of the
+//           rows at a time in the workspace.
+//   tiles   what is between: 128 x 128, all operands laid out before.
+// All sums are made in an order that depends on the sizes alone.
 #include <type_traits>
 
 #include "field_gated.h"
@@ -294,6 +307,13 @@ unsigned sum_blocks(int64_t quads) { return (unsigned)((quads + 63) / 64); }
 // fill the chip. The weights' rows lie in groups of 16, 8 gate and the same 8 up rows, so
 // that with spread blocks a lane's sums are 8 units in a row of both, and its dgate and dup
 // 32 bytes in a row. bf16 rows of x that are aligned are read where they are.
+//
+// 100003 x 512 to 2048 bf16, 420 GFLOP each: h 487 us (the library's plain product, without
+// activation, 613), dgate and dup 603, dx 472 (483), dW 370 (741); the matrix cores are
+// busy 30 to 50 % of the time at 2.2 GHz. 50021 x 256 to 1024 fp32, 52 GFLOP in six products:
+// 276 (509), 392, 310 (487), 227 (618); busy 35 to 69 %. What bounds them: field_wide.h; h,
+// dgate and dup also by the activation, which a CU's only workgroup does between its
+// products.
 template <typename T, int NP>
 __global__ __launch_bounds__(kThreads) void k_wide_weights(GatedArgs a, int64_t wr, int ld,
                                                            quad* out, quad* zero) {
@@ -482,7 +502,10 @@ __global__ __launch_bounds__((WideShape<NP, AB>::kThreads), 2) void k_wide_dw(Wi
 // ---------------------------------------------------------------- few rows
 // Up to 64 rows: every workgroup makes 16 hidden units of all rows, its waves sharing the
 // summed index; the operands come from memory as the matrix cores take them, 8 values of a
-// row a lane, so that nothing is laid out before.
+// row a lane, so that nothing is laid out before. 64 rows of 512 to 1024 bf16 take 13.5 us
+// a call so and 39 in tiles, with their gradients 58 and 173; 40 of fp32 13.6 and 56, 96
+// and 236. One row of 64 to 256 fp32 is a kernel of 4.1 us, 33 of 512 to 2048 bf16 of 5.9:
+// the way to memory and back, once.
 constexpr int kFewRows = 64;
 
 // With GRAD the rows [dgate, dup] as operands of the tiles below, 128 rows with zeros behind, and
@@ -649,12 +672,14 @@ struct GatedPlan {
     }
 };
 
-// Wide tiles pay from about as many as there are CUs (fp32: as fit at a time).
-constexpr int kWideLeast = 192;
+// Wide tiles pay from about 448 of them: training passes of 512 to 1024, with them and without,
+// 12000 rows of bf16 (376 tiles) 208 and 201 us, 16000 213 and 245; fp32 2000 rows (256)
+// 254 and 210, 4000 282 and 289, 6000 343 and 451.
+constexpr int kWideLeast = 448;
 bool is_wide(const GatedArgs& a) {
     const int64_t tile = a.dtype == 0 ? 128 : 256;
-    return a.dim > kShortDim && ((2 * a.hidden + tile - 1) / tile) * ((a.n + tile - 1) / tile) >=
-                                    (a.dtype == 0 ? 2 * kWideLeast : kWideLeast);
+    return a.dim > kShortDim &&
+           ((2 * a.hidden + tile - 1) / tile) * ((a.n + tile - 1) / tile) >= kWideLeast;
 }
 
 struct WidePlan {

@@ -91,7 +91,12 @@ __global__ __launch_bounds__(kThreads) void k_gated_chunks(GatedArgs a, int64_t 
 // Rows stay with their wave, 16 J of them in registers, and the weights pass through LDS
 // chunk by chunk: h, or with GRAD dx, whose sums stay in registers too. The gradients of
 // gate and up leave the sums in the layout that the next product takes them in. LAID: the
-// chunks' parts come from k_gated_chunks. Shares of the chunks (blockIdx.y) leave sums of dx
+// chunks' parts come from k_gated_chunks (cutting them in the kernel took dx of 10007 x 75 to
+// 201 from 26 to 38 us). bf16 rows are 64 a wave (fp32 32), with gradients half of that: 16
+// took as long, 128 do not fit the registers. 307200 x 64 to 256 bf16: 45 us, 197 MB at 4.4
+// TB/s, bound by them; to 128 with gradients 52, 157 MB, the vector units busy half of the
+// time with silu and its slope. 921600 x 128 to 128 fp32: 360, the matrix cores busy 48 % and
+// the vector units 38 % of the time, at a clock that has come down to 2 GHz. Shares of the chunks (blockIdx.y) leave sums of dx
 // of their own in `part` (share, rows, 32 KS), where there are several.
 template <typename T, int NP, int ACT, int KS, int J, bool GRAD, bool LAID>
 __global__ __launch_bounds__(kThreads, NP == 1 || J * KS < 8 ? 2 : 1) void k_gated_rows(
@@ -295,7 +300,9 @@ __global__ __launch_bounds__(kThreads, NP == 1 || J * KS < 8 ? 2 : 1) void k_gat
 // the rows pass through LDS, 64 at a time. Here the sums come out with the unit in the lane,
 // so that they are the next product's operand over the rows as they are; dh turns on its
 // way through LDS, in a part of its own for each wave. WU waves have units of their own;
-// the others share the tile's rows, and leave sums of their own.
+// the others share the tile's rows, and leave sums of their own. 307200 x 64 to 128 bf16: 48
+// us, 118 MB, the vector units busy 48 % of the time, two waves a SIMD (registers); dh
+// loaded value by value took 100.
 template <typename T>
 constexpr int kUnitBlocks = sizeof(T) == 2 ? 2 : 1;  // 64 bytes of a row of dh
 
@@ -523,8 +530,8 @@ __global__ __launch_bounds__(1024) void k_gated_join(GatedArgs a, const float* p
 }
 
 // Up to so many rows the kernels do not fill the chip: 16 rows a wave, chunks in shares, and
-// for h alone no launch to cut the weights before (10007 x 75 to 201 fp32: 16.6 us against
-// 13.0 and 4.1).
+// for h alone no launch to cut the weights before. 16000 x 64 to 128 fp32 take 12.5 us a call
+// so, a training pass 48; 17.7 and 59 as more rows do. bf16 12.6 and 43.4; 13.6 and 43.4.
 constexpr int64_t kFewerRows = 16384;
 
 struct ShortPlan {

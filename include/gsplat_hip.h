@@ -427,7 +427,8 @@ int gs_train_loss(gs_ctx* ctx, const float* image, const float* target, int heig
  *   row are contiguous. Inputs may overlap each other and themselves (a stride
  *   of 0 repeats a row); an output overlaps nothing, except that
  *   gs_group_norm_dev's y may be x and gs_group_norm_grad_dev's dx may be x or
- *   dy, with the same strides.
+ *   dy, with the same strides, and that gs_grad_clip_dev's outputs may be its
+ *   inputs.
  * - ids and labels: int32 (ids64 0) or int64 (1). One below 0 is masked. One at
  *   or past `rows` is treated as masked too, and bit GS_FLAG_ID_RANGE is set in
  *   *flags (a device word that the caller clears and reads; NULL: not wanted).
@@ -550,7 +551,8 @@ int gs_gated_linear_dev(gs_ctx* ctx, const gs_gated_linear* in, void* h, int64_t
  * dw_up (hidden, dim) of in->dtype, db_gate and db_up (hidden) fp32 (each may be NULL),
  * the weights' and biases' summed over the rows. For bf16 inputs the gradients of gate and
  * up are rounded to bf16 before they are multiplied, as operands of the matrix cores. The
- * workspace is at most about 1 GB beside copies of the weights. */
+ * workspace is at most about 1 GB beside copies of the weights and partial sums of their
+ * gradients. */
 int gs_gated_linear_grad_dev(gs_ctx* ctx, const gs_gated_linear* in, const void* dh,
                              int64_t dh_stride, void* dx, int64_t dx_stride, void* dw_gate,
                              int64_t dw_gate_stride, void* dw_up, int64_t dw_up_stride,

@@ -108,7 +108,7 @@ SIZES = [(1, 1, 1), (1, 64, 256), (2, 3, 5), (7, 8, 16), (33, 512, 70), (64, 32,
          (65, 33, 31), (127, 129, 65), (129, 64, 128), (300, 16, 200), (1000, 75, 201),
          (5, 1000, 17), (513, 128, 64), (2000, 40, 24), (4097, 64, 128), (1, 300, 1000),
          (16, 64, 33), (17, 256, 100), (640, 260, 136), (7, 512, 512), (31, 200, 333), (48, 140, 1000),
-         (64, 129, 30), (3586, 100, 300), (200, 128, 2000)]
+         (64, 129, 30), (3586, 100, 300), (200, 128, 2000), (2500, 136, 2500), (3000, 260, 700)]
 
 
 @pytest.mark.parametrize("n,dim,hidden", SIZES)
@@ -129,9 +129,9 @@ def test_values_and_gradients(ops, n, dim, hidden, dtype):
     assert all(torch.equal(a, b) for a, b in zip(again, (h, *grads)))
 
 
-# 2 hidden / 256 by rows / 256 tiles, at least 192 of them: the wide tiles
-WIDE = [(2500, 136, 2500), (3001, 200, 2050), (2601, 145, 2305), (1900, 520, 3200),
-        (50_001, 131, 40), (49_152, 256, 128), (9000, 320, 700)]
+# 2 hidden / 256 by rows / 256 tiles, at least 448 of them: the wide tiles
+WIDE = [(4900, 136, 3000), (3801, 200, 4100), (2601, 145, 5700), (1900, 520, 7400),
+        (115_001, 131, 40), (114_944, 256, 128), (23_000, 320, 700)]
 
 
 @pytest.mark.parametrize("n,dim,hidden", WIDE)
@@ -142,10 +142,10 @@ def test_wide_tiles(ops, n, dim, hidden, dtype):
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_wide_tiles_strides_and_values_that_are_not_finite(ops, dtype):
-    for n, dim, hidden in ((2500, 136, 2500), (2600, 192, 2410)):
+    for n, dim, hidden in ((4900, 136, 3000), (4700, 192, 3100)):
         test_strides_and_alignment(ops, dtype, n, dim, hidden)
-    test_values_that_are_not_finite(ops, dtype, 2600, 136, 2410)
-    test_broadcast_rows(ops, dtype, 2600, 136, 2410)
+    test_values_that_are_not_finite(ops, dtype, 4900, 136, 3000)
+    test_broadcast_rows(ops, dtype, 4900, 136, 3000)
 
 
 @pytest.mark.parametrize("act", ACTS)
@@ -340,8 +340,8 @@ def test_many_rows_in_pieces(ops, dim):
 
 @pytest.mark.parametrize("n,dim,hidden,dtype", [(1, 64, 100, F32), (40, 64, 256, BF16),
                                                 (700, 75, 60, F32), (3000, 64, 128, BF16),
-                                                (900, 256, 200, BF16), (2500, 136, 2500, BF16),
-                                                (2500, 136, 2500, F32)])
+                                                (900, 256, 200, BF16), (4900, 136, 3000, BF16),
+                                                (4900, 136, 3000, F32)])
 def test_captured_and_replayed(ops, n, dim, hidden, dtype):
     """Two graphs and eager calls between the replays, new inputs in the same buffers."""
     sets = [_cuda(_inputs(n, dim, hidden, dtype, seed=s)) for s in (20, 21, 22)]
