@@ -23,6 +23,11 @@ hipError_t gated_short_bf16(const GatedArgs& a, bool grad, hipStream_t st);
 hipError_t gated_dx_join(const GatedArgs& a, const float* part, int shares, int64_t rows, int ld,
                          int64_t n0, int64_t n, hipStream_t st);
 
+// Workgroups of the kernels that join sums, 64 quads each and walking over the rest.
+inline unsigned sum_blocks(int64_t quads) {
+    return (unsigned)std::min<int64_t>((quads + 63) / 64, (int64_t)1 << 20);
+}
+
 // 8 values of a row from column c, zeros past `cols`.
 template <typename T>
 __device__ __forceinline__ void load8(const T* row, int64_t c, int64_t cols, float* v) {

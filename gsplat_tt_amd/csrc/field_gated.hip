@@ -270,37 +270,40 @@ __global__ __launch_bounds__(1024) void k_gated_sum(GatedArgs a, const float* pa
                                                     int64_t wr, int ld, int add) {
     __shared__ f32x4 lds[16][64];
     const int lane = threadIdx.x & 63, run = threadIdx.x >> 6;
-    const int64_t quads = BIASES ? wr / 4 : wr * (ld / 4), e = (int64_t)blockIdx.x * 64 + lane;
+    const int64_t quads = BIASES ? wr / 4 : wr * (ld / 4);
     const int per = (shares + 15) / 16, b0 = min(shares, run * per), b1 = min(shares, b0 + per);
-    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (e < quads) {
-        const f32x4* from = reinterpret_cast<const f32x4*>(part) + e;
+    for (int64_t e0 = (int64_t)blockIdx.x * 64; e0 < quads; e0 += (int64_t)gridDim.x * 64) {
+        const int64_t e = e0 + lane;
+        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (e < quads) {
+            const f32x4* from = reinterpret_cast<const f32x4*>(part) + e;
 #pragma unroll 8
-        for (int b = b0; b < b1; ++b) v += from[b * quads];
-    }
-    lds[run][lane] = v;
-    __syncthreads();
-    if (run != 0 || e >= quads) return;
+            for (int b = b0; b < b1; ++b) v += from[b * quads];
+        }
+        __syncthreads();  // what was there has been read
+        lds[run][lane] = v;
+        __syncthreads();
+        if (run != 0 || e >= quads) continue;
 #pragma unroll
-    for (int k = 1; k < 16; ++k) v += lds[k][lane];
-    const int64_t r = BIASES ? e * 4 : e / (ld / 4);
-    // a quad of rows has 4 units in a row, all gate or all up, in either order
-    const UnitOf u = WIDE ? UnitOf{(r >> 4) * 8 + (r & 7), (r & 8) != 0} : unit_of(r);
-    if (u.unit >= a.hidden) return;
-    if (BIASES) {
-        float* out = u.up ? a.db_up : a.db_gate;
-        if (out == nullptr) return;
+        for (int k = 1; k < 16; ++k) v += lds[k][lane];
+        const int64_t r = BIASES ? e * 4 : e / (ld / 4);
+        // a quad of rows has 4 units in a row, all gate or all up, in either order
+        const UnitOf u = WIDE ? UnitOf{(r >> 4) * 8 + (r & 7), (r & 8) != 0} : unit_of(r);
+        if (u.unit >= a.hidden) continue;
+        if (BIASES) {
+            float* out = u.up ? a.db_up : a.db_gate;
+            if (out == nullptr) continue;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (u.unit + k < a.hidden) out[u.unit + k] = add ? out[u.unit + k] + v[k] : v[k];
-    } else {
-        T* row = static_cast<T*>(u.up ? a.dw_up : a.dw_gate) +
-                 u.unit * (u.up ? a.dup_stride : a.dgate_stride);
-        const float o[4] = {v[0], v[1], v[2], v[3]};
-        store_cols<4>(row, (e - r * (ld / 4)) * 4, a.dim, o);
+            for (int k = 0; k < 4; ++k)
+                if (u.unit + k < a.hidden) out[u.unit + k] = add ? out[u.unit + k] + v[k] : v[k];
+        } else {
+            T* row = static_cast<T*>(u.up ? a.dw_up : a.dw_gate) +
+                     u.unit * (u.up ? a.dup_stride : a.dgate_stride);
+            const float o[4] = {v[0], v[1], v[2], v[3]};
+            store_cols<4>(row, (e - r * (ld / 4)) * 4, a.dim, o);
+        }
     }
 }
-unsigned sum_blocks(int64_t quads) { return (unsigned)((quads + 63) / 64); }
 
 // ---------------------------------------------------------------- wide tiles
 // The same products in the tiles of field_wide.h, where there are enough of them to
@@ -471,14 +474,16 @@ __global__ __launch_bounds__((WideShape<NP, AB>::kThreads), 2) void k_wide_dx(Ga
 
 template <int NP, int AB>
 __global__ __launch_bounds__((WideShape<NP, AB>::kThreads), 2) void k_wide_dw(WideMat X, WideMat Z, int64_t nr,
-                                                             int cols, int ldp, int64_t per_share,
+                                                             int cols, int ldp, int spread,
+                                                             int64_t per_share,
                                                              int add, float* part) {
     using Shape = WideShape<NP, AB>;
     __shared__ quad lds[Shape::kQuads];
     const int lane = threadIdx.x & 63;
-    // a share's tiles run on one XCD, whose L2 gives them its rows of x and dz
-    const int tiles = (int)(Z.cols / Shape::kCols) * cols, tile = (blockIdx.x >> 3) % tiles;
-    const int64_t share = (blockIdx.x >> 3) / tiles * 8 + (blockIdx.x & 7);
+    // with `spread` 8 a share's tiles run on one XCD, whose L2 gives them its rows of x and dz
+    const int tiles = (int)(Z.cols / Shape::kCols) * cols;
+    const int k = (int)blockIdx.x / spread, tile = k % tiles;
+    const int64_t share = k / tiles * spread + (int)blockIdx.x % spread;
     const int64_t c0 = (int64_t)(tile % cols) * Shape::kRows, r0 = (int64_t)(tile / cols) * Shape::kCols;
     const int64_t k0 = min(nr, share * per_share), k1 = min(nr, k0 + per_share);
     wide_products<NP, AB, false, false, false>(
@@ -684,6 +689,7 @@ bool is_wide(const GatedArgs& a) {
 
 struct WidePlan {
     int ld, ldp = 0, ab = 4;  // the weights' columns, the partial sums', blocks of A for the gradients
+    int spread = 8;  // XCDs that the shares of the weights' sums go over
     int64_t wr, piece, shares = 0, per_share = 0;
     bool direct;  // x is read where it is
     quad* zero;
@@ -694,7 +700,8 @@ struct WidePlan {
         ld = (int)pad_to(a.dim, kStep);
         wr = pad_to(2 * a.hidden, 256);
         direct = np == 1 && a.dim % 8 == 0 && a.x_stride % 8 == 0 &&
-                 reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_stride < ((int64_t)1 << 24);
+                 reinterpret_cast<uintptr_t>(a.x) % 16 == 0 &&
+                 a.x_stride < ((int64_t)1 << 22);  // 256 rows within a lane's 32-bit offset
         const int64_t row = (int64_t)np * 2 * ((direct ? 0 : ld) + (grad ? wr : 0));
         const int cols = np == 1 ? 256 : 128;  // rows of a tile
         const int64_t all = pad_to(a.n, cols);
@@ -711,7 +718,9 @@ struct WidePlan {
             ab = np == 1 && (a.dim + 127) / 128 % 2 == 0 ? 8 : 4;  // 256 or 128 columns of x
             ldp = (int)pad_to(a.dim, 32 * ab);
             const int64_t tiles = (wr / cols) * (ldp / (32 * ab));
-            shares = 8 * std::max<int64_t>(1, (np == 1 ? 32 : 64) / tiles);
+            // of weights whose tiles alone fill the chip, one
+            spread = tiles >= 256 ? 1 : 8;
+            shares = spread * std::max<int64_t>(1, (np == 1 ? 32 : 64) / tiles);
             per_share = pad_to((piece + shares - 1) / shares, kStep);
             dz = c.take<bf16>((size_t)(piece * wr) * np);
             part = c.take<float>((size_t)(shares * wr * ldp));
@@ -766,8 +775,8 @@ hipError_t wide_run(const GatedArgs& a, bool grad, hipStream_t st) {
             constexpr int AB = decltype(ab)::value;
             k_wide_dx<T, NP, AB><<<xg.blocks, THREADS, 0, st>>>(a, W, Z, n0, nr, tiles_c, xg.gy);
             GS_LAUNCHED();
-            k_wide_dw<NP, AB><<<wg, THREADS, 0, st>>>(X, Z, nr, tiles_c, w.ldp, w.per_share, n0 > 0,
-                                                      w.part);
+            k_wide_dw<NP, AB><<<wg, THREADS, 0, st>>>(X, Z, nr, tiles_c, w.ldp, w.spread, w.per_share,
+                                                      n0 > 0, w.part);
             return hipGetLastError();
         };
         hipError_t e;

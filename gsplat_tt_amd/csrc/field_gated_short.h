@@ -100,11 +100,11 @@ __global__ __launch_bounds__(kThreads) void k_gated_chunks(GatedArgs a, int64_t 
 // of their own in `part` (share, rows, 32 KS), where there are several.
 template <typename T, int NP, int ACT, int KS, int J, bool GRAD, bool LAID>
 __global__ __launch_bounds__(kThreads, NP == 1 || J * KS < 8 ? 2 : 1) void k_gated_rows(
-    GatedArgs a, const quad* laid, int64_t chunks, int64_t per_share, float* part) {
+    GatedArgs a, const quad* laid, int64_t block0, int64_t chunks, int64_t per_share, float* part) {
     __shared__ quad lds[NP * 256 * KS];
     __shared__ float bias[64];
     const int lane = threadIdx.x & 63, w = wave_id(), g = lane >> 4, s = lane & 15;
-    const int64_t i0 = ((int64_t)blockIdx.x * (kThreads / 64) + w) * (16 * J);
+    const int64_t i0 = ((block0 + blockIdx.x) * (kThreads / 64) + w) * (16 * J);
     const int64_t c0 = blockIdx.y * per_share, c1 = min(chunks, c0 + per_share);
     quad next[KS][LAID ? NP : 1];
     Raw<T> next_w[LAID ? 1 : KS];
@@ -498,34 +498,38 @@ __global__ __launch_bounds__(1024) void k_gated_join(GatedArgs a, const float* p
     __shared__ f32x4 lds[16][64];
     const int lane = threadIdx.x & 63, run = threadIdx.x >> 6;
     const int64_t quads = wr * (ld / 4), all = quads + wr / 4;
-    const int64_t e = (int64_t)blockIdx.x * 64 + lane;
     const int per = (slots + 15) / 16, b0 = min(slots, run * per), b1 = min(slots, b0 + per);
-    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (e < all) {
-        const f32x4* from = reinterpret_cast<const f32x4*>(e < quads ? part : db);
-        const int64_t at = e < quads ? e : e - quads, step = e < quads ? quads : wr / 4;
+    for (int64_t e0 = (int64_t)blockIdx.x * 64; e0 < all; e0 += (int64_t)gridDim.x * 64) {
+        const int64_t e = e0 + lane;
+        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (e < all) {
+            const f32x4* from = reinterpret_cast<const f32x4*>(e < quads ? part : db);
+            const int64_t at = e < quads ? e : e - quads, step = e < quads ? quads : wr / 4;
 #pragma unroll 8
-        for (int b = b0; b < b1; ++b) v += from[b * step + at];
-    }
-    lds[run][lane] = v;
-    __syncthreads();
-    if (run != 0 || e >= all) return;
+            for (int b = b0; b < b1; ++b) v += from[b * step + at];
+        }
+        __syncthreads();  // what was there has been read
+        lds[run][lane] = v;
+        __syncthreads();
+        if (run != 0 || e >= all) continue;
 #pragma unroll
-    for (int k = 1; k < 16; ++k) v += lds[k][lane];
-    if (e < quads) {
-        const int64_t r = e / (ld / 4), unit = r / (2 * U) * U + r % U;
-        const bool up = (r & U) != 0;
-        if (unit >= a.hidden) return;
-        T* row = static_cast<T*>(up ? a.dw_up : a.dw_gate) + unit * (up ? a.dup_stride : a.dgate_stride);
-        const float o[4] = {v[0], v[1], v[2], v[3]};
-        store_cols<4>(row, (int)(e - r * (ld / 4)) * 4, a.dim, o);
-    } else {
-        const int64_t r = (e - quads) * 4, unit = r / (2 * U) * U + r % U;
-        float* out = (r & U) != 0 ? a.db_up : a.db_gate;
-        if (out == nullptr) return;
+        for (int k = 1; k < 16; ++k) v += lds[k][lane];
+        if (e < quads) {
+            const int64_t r = e / (ld / 4), unit = r / (2 * U) * U + r % U;
+            const bool up = (r & U) != 0;
+            if (unit >= a.hidden) continue;
+            T* row = static_cast<T*>(up ? a.dw_up : a.dw_gate) +
+                     unit * (up ? a.dup_stride : a.dgate_stride);
+            const float o[4] = {v[0], v[1], v[2], v[3]};
+            store_cols<4>(row, (int)(e - r * (ld / 4)) * 4, a.dim, o);
+        } else {
+            const int64_t r = (e - quads) * 4, unit = r / (2 * U) * U + r % U;
+            float* out = (r & U) != 0 ? a.db_up : a.db_gate;
+            if (out == nullptr) continue;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (unit + k < a.hidden) out[unit + k] = v[k];
+            for (int k = 0; k < 4; ++k)
+                if (unit + k < a.hidden) out[unit + k] = v[k];
+        }
     }
 }
 
@@ -583,10 +587,13 @@ template <typename T, int NP, int ACT, int KS, int J, bool GRAD, bool LAID>
 hipError_t rows_run(const GatedArgs& a, const ShortPlan& w, hipStream_t st) {
     const int64_t blocks = (a.n + 64 * J - 1) / (64 * J);
     const int64_t per = (w.chunks + w.row_shares - 1) / w.row_shares;
-    const dim3 grid((unsigned)blocks, (unsigned)w.row_shares);
-    k_gated_rows<T, NP, ACT, KS, J, GRAD, LAID>
-        <<<grid, kThreads, 0, st>>>(a, w.laid, w.chunks, per, w.dx);
-    return hipGetLastError();
+    for (int64_t at = 0; at < blocks; at += kMostBlocks) {
+        const dim3 grid((unsigned)std::min(blocks - at, kMostBlocks), (unsigned)w.row_shares);
+        k_gated_rows<T, NP, ACT, KS, J, GRAD, LAID>
+            <<<grid, kThreads, 0, st>>>(a, w.laid, at, w.chunks, per, w.dx);
+        GS_LAUNCHED();
+    }
+    return hipSuccess;
 }
 
 template <typename T, int NP, int ACT, int KS>
@@ -618,7 +625,7 @@ hipError_t short_run(const GatedArgs& a, bool grad, hipStream_t st) {
                                                                    w.part, w.db);
     GS_LAUNCHED();
     const int64_t quads = w.wr * (32 * KS / 4) + w.wr / 4;
-    k_gated_join<T><<<(unsigned)((quads + 63) / 64), 1024, 0, st>>>(a, w.part, w.db, w.slots, w.wr,
+    k_gated_join<T><<<sum_blocks(quads), 1024, 0, st>>>(a, w.part, w.db, w.slots, w.wr,
                                                                     32 * KS);
     return hipGetLastError();
 }

@@ -466,3 +466,33 @@ def test_closed_context_and_c_boundary(ops):
             ptr[3], ptr[4], ws.data_ptr(), size, ops._stream()) == 0
         assert all(torch.equal(a, b) for k, (a, b) in enumerate(zip(outs, want)) if k != skip)
     del keep
+
+
+# ------------------------------------------------------------------ far apart
+@pytest.mark.parametrize("stride", [(1 << 22) - 8, 1 << 22, (1 << 23) + 8])
+def test_rows_far_apart(ops, stride):
+    """300 rows some megabytes apart, offsets past 32 bits: wide tiles whose rows of x are
+    read where they are, or laid out before."""
+    n, dim, hidden = 300, 136, 30_000
+    x, wg, wu, bg, bu, dh = _inputs(n, dim, hidden, BF16, seed=40)
+    room = torch.empty(n * stride, dtype=BF16, device="cuda")
+    far = torch.as_strided(room, (n, dim), (stride, 1))
+    far.copy_(x)
+    near = _cuda((x, wg, wu, bg, bu))
+    dh = dh.cuda()
+    h = ops.gated_linear(far, *near[1:])
+    want = ops.gated_linear(*near)
+    assert torch.equal(h, want)
+    for a, b in zip(ops.gated_linear_grad(dh, far, *near[1:]), ops.gated_linear_grad(dh, *near)):
+        assert torch.equal(a, b)
+    ref = _reference(x[:40], wg, wu, bg, bu, dh[:40].cpu(), "silu", BF16)
+    _check(h[:40], ref["h"], "h")
+    del room, far
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("n,dim,hidden,dtype", [(700, 72, 33_000, BF16), (400, 600, 25_000, BF16),
+                                                (300, 40, 9000, F32), (150, 140, 20_000, F32)])
+def test_many_units(ops, n, dim, hidden, dtype):
+    """More units than rows: the weights' tiles alone fill the chip."""
+    test_values_and_gradients(ops, n, dim, hidden, dtype)
