@@ -243,6 +243,32 @@ def test_no_rows(ops, dtype):
     assert rest[0].shape == (30, 20) and rest[2].shape == (30,)
 
 
+@pytest.mark.parametrize("n,dim,hidden", [(1, 136, 57_400), (3, 131, 57_500), (70, 136, 57_400)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_few_rows_of_many_units(ops, n, dim, hidden, dtype):
+    """The units alone fill the wide tiles, whose rows are nearly all past the last one."""
+    ins = _inputs(n, dim, hidden, dtype)
+    ref = _reference(*ins, "silu", dtype)
+    *args, dh = _cuda(ins)
+    _check(ops.gated_linear(*args), ref["h"], "h")
+    for name, g in zip(NAMES, ops.gated_linear_grad(dh, *args)):
+        _check(g, ref[name], name)
+
+
+@pytest.mark.parametrize("dim,hidden", [(200, 30), (136, 57_400)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_no_rows_of_long_features(ops, dim, hidden, dtype):
+    """The weights' gradients are zeros, written over what was there; nothing around them is."""
+    x, wg, wu, bg, bu, dh = _cuda(_inputs(0, dim, hidden, dtype))
+    assert ops.gated_linear(x, wg, wu, bg, bu).shape == (0, hidden)
+    rooms = [torch.full((hidden + 2, dim + 8), 3.0, dtype=dtype, device="cuda") for _ in range(2)]
+    outs = [r[1:-1, :dim] for r in rooms]
+    dx, *rest = ops.gated_linear_grad(dh, x, wg, wu, bg, bu, dw_gate=outs[0], dw_up=outs[1])
+    assert dx.shape == (0, dim) and not any(t.any() for t in rest)
+    for r in rooms:
+        assert (r[0] == 3).all() and (r[-1] == 3).all() and (r[:, dim:] == 3).all()
+
+
 @pytest.mark.parametrize("n,dim,hidden", [(4, 40, 24), (300, 32, 64), (300, 72, 130), (200, 300, 40)])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_values_that_are_not_finite(ops, dtype, n, dim, hidden):
