@@ -19,7 +19,9 @@ the context's device and nothing waits; outputs and workspaces come from torch's
 allocator on that stream. A tensor made on another stream must be ordered before
 the call by the caller, as for any torch operation. The operators are not part of
 torch's graph: in grad mode a tensor that requires a gradient is refused, and the
-gradients are calls of their own. There is no CPU fallback.
+gradients are calls of their own. Tensors are taken by their memory: one with torch's
+lazy negation (an imaginary part of a conjugate) is refused, its resolve_neg() is not.
+There is no CPU fallback.
 """
 from __future__ import annotations
 
@@ -109,6 +111,8 @@ class FieldOps:
             if t.requires_grad and torch.is_grad_enabled():
                 raise ValueError(f"{name} requires a gradient, which these operators do not "
                                  "record: detach() it or call under torch.no_grad()")
+            if t.is_neg():  # its memory holds the values with the other sign
+                raise ValueError(f"{name} is negated when it is read: give its resolve_neg()")
             return t
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a torch tensor")
@@ -374,7 +378,8 @@ class FieldOps:
         if plain:
             types = set(map(_get_dtype, tensors))
             plain = types <= _DTYPES.keys() and set(map(_get_device, tensors)) <= {self._index} and \
-                not (torch.is_grad_enabled() and any(map(_get_requires_grad, tensors)))
+                not (torch.is_grad_enabled() and any(map(_get_requires_grad, tensors))) and \
+                not any(map(torch.Tensor.is_neg, tensors))
         if not plain:
             for t in tensors:
                 self._own(t, name)
