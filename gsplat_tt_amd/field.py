@@ -18,10 +18,10 @@ The reference has no counterpart. Work is enqueued on torch's current stream of
 the context's device and nothing waits; outputs and workspaces come from torch's
 allocator on that stream. A tensor made on another stream must be ordered before
 the call by the caller, as for any torch operation. The operators are not part of
-torch's graph: in grad mode a tensor that requires a gradient is refused, and the
-gradients are calls of their own. Tensors are taken by their memory: one with torch's
-lazy negation (an imaginary part of a conjugate) is refused, its resolve_neg() is not.
-There is no CPU fallback.
+torch's graph: in grad mode a tensor that requires a gradient is refused, and at any
+time one with a tangent of the forward mode; the gradients are calls of their own.
+Tensors are taken by their memory: one with torch's lazy negation (an imaginary part
+of a conjugate) is refused, its resolve_neg() is not. There is no CPU fallback.
 """
 from __future__ import annotations
 
@@ -31,6 +31,7 @@ import math
 import operator
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -82,6 +83,12 @@ def _collapse(t):
     return rows, cols, stride if rows > 1 else cols
 
 
+def _in_forward_mode():
+    """Whether there can be tensors with tangents: unpack_dual() of each takes longer than
+    all other checks."""
+    return forward_ad._current_level >= 0
+
+
 def _written(out):
     """Counts a given output as changed in place, for graphs that have saved it."""
     if not out.is_inference():
@@ -111,6 +118,9 @@ class FieldOps:
             if t.requires_grad and torch.is_grad_enabled():
                 raise ValueError(f"{name} requires a gradient, which these operators do not "
                                  "record: detach() it or call under torch.no_grad()")
+            if _in_forward_mode() and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{name} has a tangent (torch's forward mode), which these "
+                                 "operators do not carry on: detach() it")
             if t.is_neg():  # its memory holds the values with the other sign
                 raise ValueError(f"{name} is negated when it is read: give its resolve_neg()")
             return t
@@ -379,7 +389,7 @@ class FieldOps:
             types = set(map(_get_dtype, tensors))
             plain = types <= _DTYPES.keys() and set(map(_get_device, tensors)) <= {self._index} and \
                 not (torch.is_grad_enabled() and any(map(_get_requires_grad, tensors))) and \
-                not any(map(torch.Tensor.is_neg, tensors))
+                not any(map(torch.Tensor.is_neg, tensors)) and not _in_forward_mode()
         if not plain:
             for t in tensors:
                 self._own(t, name)

@@ -4,6 +4,7 @@ import ctypes
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from gsplat_tt_amd import field
 
@@ -106,3 +107,20 @@ def test_imaginary_parts_of_conjugates_are_refused(ops):
         with pytest.raises(ValueError, match="resolve_neg"):
             call(t)
         call(z.imag)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_forward_mode_tensors_are_refused(ops, name):
+    """Their tangents would be dropped: each tensor of each call."""
+    call, tensors = _calls(ops)[name]
+    with fwd.dual_level():
+        call(*tensors)  # no dual tensor among them
+        for k, t in enumerate(tensors):
+            dual = fwd.make_dual(t, torch.ones_like(t))
+            ops._L.launched.clear()
+            for mode in (torch.enable_grad, torch.no_grad):  # which is for the reverse mode alone
+                with mode(), pytest.raises(ValueError, match="forward mode"):
+                    call(*tensors[:k], dual, *tensors[k + 1:])
+            assert not ops._L.launched
+            call(*tensors[:k], dual.detach(), *tensors[k + 1:])
+    call(*tensors[:-1], dual)  # its level has ended, and with it the tangent
