@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <utility>
 #include <vector>
 
 #include "../../include/gsplat_hip.h"
@@ -227,11 +228,15 @@ struct Span {
     size_t row, stride;  // bytes of a row and between rows; stride 0: one row
     bool written;
 };
+Span span_of(const void* data, int64_t rows, int64_t cols, int64_t stride, int dtype,
+             bool written) {
+    const size_t e = (size_t)gs::elem_bytes(dtype);
+    const uintptr_t p = reinterpret_cast<uintptr_t>(data);
+    return {p, p + ((size_t)(rows - 1) * (size_t)stride + (size_t)cols) * e, (size_t)cols * e,
+            rows > 1 ? (size_t)stride * e : 0, written};
+}
 Span span_of(const gs::TensorRef& t, bool written) {
-    const size_t e = (size_t)gs::elem_bytes(t.dtype);
-    const uintptr_t p = reinterpret_cast<uintptr_t>(t.data);
-    return {p, p + ((size_t)(t.rows - 1) * (size_t)t.stride + (size_t)t.cols) * e,
-            (size_t)t.cols * e, t.rows > 1 ? (size_t)t.stride * e : 0, written};
+    return span_of(t.data, t.rows, t.cols, t.stride, t.dtype, written);
 }
 // Whether two spans that overlap have no byte in common all the same: columns of one
 // matrix.
@@ -244,7 +249,7 @@ bool apart(const Span& a, const Span& b) {
                                          : (stride - (a.begin - b.begin) % stride) % stride;
     return at >= a.row && at + b.row <= stride;
 }
-void check_apart(std::vector<Span>& spans) {
+void check_apart(std::vector<Span>& spans, const char* what) {
     std::sort(spans.begin(), spans.end(),
               [](const Span& a, const Span& b) { return a.begin < b.begin; });
     // `open`: earlier spans that reach past the present one's begin
@@ -254,12 +259,30 @@ void check_apart(std::vector<Span>& spans) {
         for (const Span& o : open) {
             if (o.end <= s.begin) continue;
             REQUIRE(!(o.written || s.written) || apart(o, s),
-                    "grad_clip: an output shares memory with another tensor");
+                    std::string(what) + ": an output shares memory with another tensor");
             open[kept++] = o;
         }
         open.resize(kept);
         open.push_back(s);
     }
+}
+
+// The memory of a gated call: `spans` beside what the description names and the workspace;
+// without rows `spans` alone.
+void check_gated_apart(const gs::GatedArgs& a, std::vector<Span> spans, const void* ws,
+                       size_t ws_bytes, const char* what) {
+    if (a.n > 0) {
+        spans.push_back(span_of(a.x, a.n, a.dim, a.x_stride, a.dtype, false));
+        spans.push_back(span_of(a.w_gate, a.hidden, a.dim, a.gate_stride, a.dtype, false));
+        spans.push_back(span_of(a.w_up, a.hidden, a.dim, a.up_stride, a.dtype, false));
+        for (const float* b : {a.b_gate, a.b_up})
+            if (b != nullptr) spans.push_back(span_of(b, 1, a.hidden, 0, GS_F32, false));
+        if (ws_bytes > 0) {
+            const uintptr_t at = reinterpret_cast<uintptr_t>(ws);
+            spans.push_back({at, at + ws_bytes, ws_bytes, 0, true});
+        }
+    }
+    check_apart(spans, what);
 }
 
 }  // namespace
@@ -469,7 +492,10 @@ int gs_gated_linear_dev(gs_ctx* ctx, const gs_gated_linear* in, void* h, int64_t
         if (a.n > 0) {
             check_ptr(h, a.dtype, "gated_linear: h");
             check_rows(a.n, h_stride, (int)a.hidden, "gated_linear: h", true);
-            check_ws(workspace, workspace_bytes, gs::gated_linear_ws(a, false), "gated_linear");
+            const size_t need = gs::gated_linear_ws(a, false);
+            check_ws(workspace, workspace_bytes, need, "gated_linear");
+            check_gated_apart(a, {span_of(h, a.n, a.hidden, h_stride, a.dtype, true)}, workspace,
+                              need, "gated_linear");
         }
         a.h = h;
         a.h_stride = h_stride;
@@ -487,13 +513,14 @@ int gs_gated_linear_grad_dev(gs_ctx* ctx, const gs_gated_linear* in, const void*
                              int64_t workspace_bytes, void* stream) {
     return guard([&] {
         gs::GatedArgs a = gated_args(in, true);
+        size_t need = 0;
         if (a.n > 0) {
             check_ptr(dh, a.dtype, "gated_linear_grad: dh");
             check_rows(a.n, dh_stride, (int)a.hidden, "gated_linear_grad: dh");
             check_ptr(dx, a.dtype, "gated_linear_grad: dx");
             check_rows(a.n, dx_stride, a.dim, "gated_linear_grad: dx", true);
-            check_ws(workspace, workspace_bytes, gs::gated_linear_ws(a, true),
-                     "gated_linear_grad");
+            need = gs::gated_linear_ws(a, true);
+            check_ws(workspace, workspace_bytes, need, "gated_linear_grad");
         }
         check_ptr(dw_gate, a.dtype, "gated_linear_grad: dw_gate");
         check_rows(a.hidden, dw_gate_stride, a.dim, "gated_linear_grad: dw_gate", true);
@@ -501,6 +528,17 @@ int gs_gated_linear_grad_dev(gs_ctx* ctx, const gs_gated_linear* in, const void*
         check_rows(a.hidden, dw_up_stride, a.dim, "gated_linear_grad: dw_up", true);
         check_words(db_gate, "gated_linear_grad: db_gate");
         check_words(db_up, "gated_linear_grad: db_up");
+        std::vector<Span> outputs;
+        outputs.reserve(12);
+        outputs.push_back(span_of(dw_gate, a.hidden, a.dim, dw_gate_stride, a.dtype, true));
+        outputs.push_back(span_of(dw_up, a.hidden, a.dim, dw_up_stride, a.dtype, true));
+        for (const float* b : {db_gate, db_up})
+            if (b != nullptr) outputs.push_back(span_of(b, 1, a.hidden, 0, GS_F32, true));
+        if (a.n > 0) {
+            outputs.push_back(span_of(dh, a.n, a.hidden, dh_stride, a.dtype, false));
+            outputs.push_back(span_of(dx, a.n, a.dim, dx_stride, a.dtype, true));
+        }
+        check_gated_apart(a, std::move(outputs), workspace, need, "gated_linear_grad");
         a.dh = dh;
         a.dh_stride = dh_stride;
         a.dx = dx;
@@ -578,7 +616,7 @@ int gs_grad_clip_dev(gs_ctx* ctx, const gs_tensor* in, const gs_tensor* out, int
         }
         const uintptr_t at = reinterpret_cast<uintptr_t>(norm);
         spans.push_back({at, at + 4, 4, 0, kind != GS_NORM_GIVEN});
-        check_apart(spans);
+        check_apart(spans, "grad_clip");
         REQUIRE(ctx, "null ctx");  // last: the other checks need no device
         const OnDevice on(ctx);
         HIPCHK(gs::launch_grad_clip(from.data(), to.data(), (int64_t)from.size(), kind, norm,

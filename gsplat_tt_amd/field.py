@@ -21,7 +21,10 @@ the call by the caller, as for any torch operation. The operators are not part o
 torch's graph: in grad mode a tensor that requires a gradient is refused, and at any
 time one with a tangent of the forward mode; the gradients are calls of their own.
 Tensors are taken by their memory: one with torch's lazy negation (an imaginary part
-of a conjugate) is refused, its resolve_neg() is not. There is no CPU fallback.
+of a conjugate) is refused, its resolve_neg() is not. Outputs that are given share no
+memory with another tensor of the call, but for group_norm's `out` = x,
+group_norm_grad's = x or dy, and clip_grads() in place; the gated projections and
+clip_grads() refuse such outputs. There is no CPU fallback.
 """
 from __future__ import annotations
 

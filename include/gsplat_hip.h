@@ -428,7 +428,9 @@ int gs_train_loss(gs_ctx* ctx, const float* image, const float* target, int heig
  *   of 0 repeats a row); an output overlaps nothing, except that
  *   gs_group_norm_dev's y may be x and gs_group_norm_grad_dev's dx may be x or
  *   dy, with the same strides, and that gs_grad_clip_dev's outputs may be its
- *   inputs.
+ *   inputs. The gated projections and gs_grad_clip_dev refuse outputs (and a
+ *   workspace of the former) that do; of two tensors of rows that reach over each
+ *   other they take columns of one matrix (equal strides) and refuse the rest.
  * - ids and labels: int32 (ids64 0) or int64 (1). One below 0 is masked. One at
  *   or past `rows` is treated as masked too, and bit GS_FLAG_ID_RANGE is set in
  *   *flags (a device word that the caller clears and reads; NULL: not wanted).

@@ -200,3 +200,73 @@ def test_clip_refusals():
         assert b"workspace" in _clip([a], [b], kind=kind)
         assert b"workspace" in _clip([a], [b], kind=kind, ws=0x100010, size=1 << 20)
     assert b"unknown norm" in _clip([a], [b], kind=2)
+
+
+# ------------------------------------------------------------------ shared memory
+X, WG, WU, BG, BU = 0x10000, 0x20000, 0x30000, 0x40000, 0x50000  # of _gated()
+NO_CTX = b"null ctx"
+
+
+def _forward(d=None, h=0x60000, stride=32, ws=0x100000):
+    lib = L.load_library()
+    assert lib.gs_gated_linear_dev(None, ctypes.byref(d or _gated()), h, stride, ws, 1 << 20,
+                                   None) == L.GS_E_INVALID
+    return lib.gs_last_error()
+
+
+def _backward(d=None, dh=(0x60000, 32), dx=(0x70000, 16), dwg=(0x80000, 16), dwu=(0x90000, 16),
+              db=(0xa0000, 0xb0000), ws=0x100000):
+    lib = L.load_library()
+    assert lib.gs_gated_linear_grad_dev(None, ctypes.byref(d or _gated()), *dh, *dx, *dwg, *dwu, *db,
+                                        ws, 1 << 40, None) == L.GS_E_INVALID
+    return lib.gs_last_error()
+
+
+@pytest.mark.parametrize("h", [X, X + 4, X + 4 * 16 * 99, WG, WU + 32 * 16 * 4 - 4, BG, BU + 4 * 31,
+                               WG - 4 * 32 * 100 + 4])
+def test_gated_linear_output_over_an_input(h):
+    assert b"shares memory" in _forward(h=h)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(dx=(X, 16)), dict(dx=(0x60000, 32)), dict(dx=(0x60000, 16)), dict(dx=(WG, 16)),
+    dict(dx=(BU, 16)), dict(dwg=(0x90000, 16)), dict(dwu=(0x80000 + 4 * 16 * 31, 16)),
+    dict(dwg=(WG, 16)), dict(dwu=(WG, 16)), dict(dwu=(0x70000, 16)), dict(dwg=(0x60000 + 64, 16)),
+    dict(db=(0xa0000, 0xa0000)), dict(db=(0xa0000, 0xa0000 + 124)), dict(db=(BG, 0xb0000)),
+    dict(db=(0xa0000, 0x80000)), dict(db=(0x60000 + 4, None)),
+])
+def test_gated_linear_grad_outputs_over_others(bad):
+    assert b"shares memory" in _backward(**bad)
+
+
+def test_gated_linear_workspace_over_others():
+    """Calls that have a workspace (forward: of more rows than one launch takes)."""
+    d = _gated(n=200, dim=144, x_stride=144, gate_stride=144, up_stride=144, w_gate=0x400000,
+               w_up=0x500000, x=0x600000)
+    assert NO_CTX in _forward(d)
+    for ws in (0x400000, 0x500100, 0x600000, 0x60000, 0x60100):
+        assert b"shares memory" in _forward(d, ws=ws), hex(ws)
+    for ws in (X, WG, BU, 0x60000, 0x70000, 0x80000, 0x90000, 0xa0000, 0xb0000):
+        assert b"shares memory" in _backward(ws=ws), hex(ws)
+
+
+def test_gated_linear_takes_what_shares_no_memory():
+    assert NO_CTX in _forward() and NO_CTX in _backward()
+    # inputs may share: one weight for both, rows of x and of dh repeated
+    d = _gated(w_up=WG, b_up=BG, x_stride=0)
+    assert NO_CTX in _forward(d) and NO_CTX in _backward(d, dh=(0x60000, 0))
+    # end to end, and columns of one matrix of 64 columns
+    assert NO_CTX in _forward(h=X + 4 * 16 * 100) and NO_CTX in _forward(h=X - 4 * 32 * 100)
+    d = _gated(n=100, x_stride=64)
+    assert NO_CTX in _forward(d, h=X + 64, stride=64) and NO_CTX in _forward(d, h=X + 128, stride=64)
+    assert b"shares memory" in _forward(d, h=X + 60, stride=64)
+    assert NO_CTX in _backward(d, dh=(X + 64, 64), dx=(X + 192, 64))
+    assert b"shares memory" in _backward(d, dh=(X + 64, 64), dx=(X + 180, 64))
+    # both weights' gradients in one matrix, row by row in turn
+    assert NO_CTX in _backward(dwg=(0x80000, 32), dwu=(0x80000 + 64, 32))
+    # without rows nothing is read, and x, dh and dx need not be there
+    d = _gated(n=0, x=None, w_gate=None, w_up=None)
+    assert NO_CTX in _forward(d, h=None)
+    assert NO_CTX in _backward(d, dh=(None, 32), dx=(None, 16))
+    assert NO_CTX in _backward(_gated(n=0), dwg=(WG, 16), dwu=(X, 16))
+    assert b"shares memory" in _backward(d, dh=(None, 32), dx=(None, 16), dwu=(0x80000, 16))

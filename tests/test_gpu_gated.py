@@ -522,3 +522,34 @@ def test_rows_far_apart(ops, stride):
 def test_many_units(ops, n, dim, hidden, dtype):
     """More units than rows: the weights' tiles alone fill the chip."""
     test_values_and_gradients(ops, n, dim, hidden, dtype)
+
+
+def test_outputs_over_other_tensors_are_refused(ops):
+    """They would be read and written at once, or written twice."""
+    n = 90
+    x, wg, wu, bg, bu, dh = _cuda(_inputs(n, 24, 24, F32, seed=50))
+    before = [t.clone() for t in (x, wg, wu, bg, bu, dh)]
+    args = (x, wg, wu, bg, bu)
+    both = torch.full((48, 24), 3.0, device="cuda")
+    for call in (lambda: ops.gated_linear(*args, out=x),
+                 lambda: ops.gated_linear(x[:24], wg, wu, out=wu),
+                 lambda: ops.gated_linear(*args, out=both[:1].expand(n, 24)),
+                 lambda: ops.gated_linear_grad(dh, *args, dx=x),
+                 lambda: ops.gated_linear_grad(dh, *args, dx=dh),
+                 lambda: ops.gated_linear_grad(dh, *args, dw_gate=wg),
+                 lambda: ops.gated_linear_grad(dh, *args, dw_gate=both[:24], dw_up=both[:24]),
+                 lambda: ops.gated_linear_grad(dh, *args, dw_gate=both[:24], dw_up=both[23:47])):
+        with pytest.raises(ValueError, match="shares memory|overlap"):
+            call()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip((x, wg, wu, bg, bu, dh), before))
+    assert (both == 3.0).all()
+    # beside each other they are taken, in one matrix by turns of rows too
+    want = ops.gated_linear_grad(dh, *args)
+    for dw_gate, dw_up in ((both[:24], both[24:]), (both[::2], both[1::2])):
+        got = ops.gated_linear_grad(dh, *args, dw_gate=dw_gate, dw_up=dw_up)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    room = torch.zeros(n, 48, device="cuda")
+    room[:, :24] = x
+    ops.gated_linear(room[:, :24], wg, wu, bg, bu, out=room[:, 24:])
+    assert torch.equal(room[:, 24:], ops.gated_linear(*args)) and torch.equal(room[:, :24], x)
