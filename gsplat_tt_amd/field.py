@@ -18,8 +18,8 @@ The reference has no counterpart. Work is enqueued on torch's current stream of
 the context's device and nothing waits; outputs and workspaces come from torch's
 allocator on that stream. A tensor made on another stream must be ordered before
 the call by the caller, as for any torch operation. The operators are not part of
-torch's graph: in grad mode a tensor that requires a gradient is refused, and at any
-time one with a tangent of the forward mode; the gradients are calls of their own.
+torch's graph: in grad mode a tensor that requires a gradient is refused, and where the
+forward mode is on one with a tangent; the gradients are calls of their own.
 Tensors are taken by their memory: one with torch's lazy negation (an imaginary part
 of a conjugate) is refused, its resolve_neg() is not. Outputs that are given share no
 memory with another tensor of the call, but for group_norm's `out` = x,

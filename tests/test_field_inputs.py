@@ -124,3 +124,30 @@ def test_forward_mode_tensors_are_refused(ops, name):
             assert not ops._L.launched
             call(*tensors[:k], dual.detach(), *tensors[k + 1:])
     call(*tensors[:-1], dual)  # its level has ended, and with it the tangent
+
+
+def test_functions_with_a_rule_for_tangents(ops):
+    """A Function's forward gets its inputs with their tangents, which are its jvp's work:
+    torch has the forward mode off there, as it has the reverse mode."""
+    class Norm(torch.autograd.Function):
+        @staticmethod
+        def forward(x):
+            ops.grad_norm([x])
+            return ops.lookup(x, torch.zeros(2, dtype=torch.int64)) * 0
+
+        @staticmethod
+        def setup_context(ctx, inputs, output):
+            pass
+
+        @staticmethod
+        def jvp(ctx, t):
+            return torch.full((2, DIM), 5.0)
+
+    x = torch.ones(N, DIM)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        out = Norm.apply(dual)
+        assert (fwd.unpack_dual(out).tangent == 5).all()
+        assert ops._L.launched == ["gs_grad_norm_dev", "gs_lookup_dev"]
+        with pytest.raises(ValueError, match="forward mode"):
+            ops.grad_norm([dual])
