@@ -161,7 +161,7 @@ gs::LossArgs loss_args(const gs_label_loss* d, float* loss, float* lse, void* ws
 
 
 // The description alone, and its pointers if there is a row to compute.
-gs::GatedArgs gated_args(const gs_gated_linear* d, bool grad) {
+gs::GatedArgs gated_args(const gs_gated_linear* d) {
     REQUIRE(d != nullptr, "gated_linear: null description");
     REQUIRE(d->n >= 0, "gated_linear: n must not be negative");
     REQUIRE(d->hidden >= 1, "gated_linear: hidden must be at least 1");
@@ -478,7 +478,7 @@ int gs_label_loss_grad_dev(gs_ctx* ctx, const gs_label_loss* in, const float* ro
 
 int64_t gs_gated_linear_workspace(const gs_gated_linear* in, int grad) {
     try {
-        return (int64_t)gs::gated_linear_ws(gated_args(in, grad != 0), grad != 0);
+        return (int64_t)gs::gated_linear_ws(gated_args(in), grad != 0);
     } catch (const std::exception& e) {
         gs::g_err = e.what();
         return -1;
@@ -488,7 +488,7 @@ int64_t gs_gated_linear_workspace(const gs_gated_linear* in, int grad) {
 int gs_gated_linear_dev(gs_ctx* ctx, const gs_gated_linear* in, void* h, int64_t h_stride,
                         void* workspace, int64_t workspace_bytes, void* stream) {
     return guard([&] {
-        gs::GatedArgs a = gated_args(in, false);
+        gs::GatedArgs a = gated_args(in);
         if (a.n > 0) {
             check_ptr(h, a.dtype, "gated_linear: h");
             check_rows(a.n, h_stride, (int)a.hidden, "gated_linear: h", true);
@@ -512,7 +512,7 @@ int gs_gated_linear_grad_dev(gs_ctx* ctx, const gs_gated_linear* in, const void*
                              float* db_gate, float* db_up, void* workspace,
                              int64_t workspace_bytes, void* stream) {
     return guard([&] {
-        gs::GatedArgs a = gated_args(in, true);
+        gs::GatedArgs a = gated_args(in);
         size_t need = 0;
         if (a.n > 0) {
             check_ptr(dh, a.dtype, "gated_linear_grad: dh");
