@@ -225,3 +225,31 @@ def test_wide_bf16_tiles_in_pieces(ops):  # noqa: F811
     *weights, dh = rest
     for name, t in zip(NAMES, ops.gated_linear_grad(dh, room[:, 1:dim + 1], *weights, act="gelu")):
         _within(t, ref[name], name)
+
+
+# ------------------------------------------------------------------ very many rows
+@pytest.mark.parametrize("n,dtype", [((1 << 29) + 12_345, F32), ((1 << 30) + 12_345, BF16)])
+def test_more_rows_than_a_launch_takes(ops, n, dtype):  # noqa: F811
+    """Rows of one value: h in two launches (2^22 workgroups in each), the gradients in two and
+    four. Few rows have a dh that is not 0, so that the weights' gradients are theirs."""
+    some = torch.tensor([0, 1, n // 2 - 1, (1 << 29) - 1, 1 << 29, n - 12_346, n - 2, n - 1], device="cuda")
+    x = torch.arange(n, dtype=torch.int32, device="cuda").remainder_(7).sub_(3).to(dtype)[:, None]
+    x.mul_(0.375)
+    dh = torch.zeros(n, 1, dtype=dtype, device="cuda")
+    dh[some] = (torch.arange(8, device="cuda")[:, None] * 0.25 - 0.8).to(dtype)
+    some = some.unique()  # two of them are one row of the fp32 case, which is summed once
+    _, wg, wu, bg, bu, _ = _inputs(1, 1, 1, dtype, seed=66)
+    args = _cuda((wg, wu, bg, bu))
+    ref = _reference(x[some].cpu(), wg, wu, bg, bu, dh[some].cpu(), "silu", dtype)
+    h = ops.gated_linear(x, *args)
+    _within(h[some].cpu(), ref["h"], "h")
+    ends = torch.cat([torch.arange(5000, device="cuda"), torch.arange(n - 20_000, n, device="cuda")])
+    assert torch.equal(h[ends], ops.gated_linear(x[ends], *args))
+    del h
+    dx, *rest = ops.gated_linear_grad(dh, x, *args)
+    _within(dx[some].cpu(), ref["dx"], "dx")
+    assert int(dx.count_nonzero()) <= 8
+    for name, t in zip(NAMES[1:], rest):
+        _within(t.cpu(), ref[name], name)
+    del x, dh, dx, rest
+    torch.cuda.empty_cache()
