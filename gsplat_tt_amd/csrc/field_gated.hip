@@ -6,13 +6,17 @@
 //   dx = dgate Wg + dup Wu;  dWg = dgate^T x;  dWu = dup^T x;  db = column sums.
 //
 // The backward pass makes gate and up again: keeping them would cost 2 n hidden values
-// written and read against 4 n dim hidden operations.
+// written and read against 4 n dim hidden operations (in fp32 50021 x 256 to 1024 820 MB, 160
+// us at a copy's rate, against 276 of products; such a form was not built).
 //
 // All products run on the matrix cores with bf16 operands and fp32 sums; fp32 values are
-// cut into three bf16 parts, whose six products above 2^-24 are added up (field_tiles.h).
-// For bf16 inputs dgate and dup are rounded to bf16 as operands of the next products (100003
-// x 512 to 2048: gradients 0.0024 off, 2-norm, relative, where rounding them alone gives
-// 0.0017); the biases' gradients sum them in fp32.
+// cut into three bf16 parts, whose six largest products are added up (field_tiles.h).
+// For bf16 inputs dgate and dup are rounded to bf16 as operands of the next products, as they
+// are where gate and up are bf16 tensors with gradients of their own: 100003 x 512 to 2048 the
+// gradients are 0.0024 off (2-norm, relative), where rounding them alone gives 0.0017. A
+// second part of them would take that away for twice the products of dx and dW, 840 of 1950
+// us there, and twice the bytes of [dgate, dup]. The biases' gradients sum what was not
+// rounded, in fp32.
 //
 // Four ways, by size:
 //   few     up to 64 rows: one launch, operands straight from memory (with gradients of long
@@ -677,9 +681,15 @@ struct GatedPlan {
     }
 };
 
-// Wide tiles pay from about 448 of them: training passes of 512 to 1024, with them and without,
-// 12000 rows of bf16 (376 tiles) 208 and 201 us, 16000 213 and 245; fp32 2000 rows (256)
-// 254 and 210, 4000 282 and 289, 6000 343 and 451.
+// Wide tiles pay from about 448 of them. h and a training pass in tiles, then in wide ones, us:
+//   bf16 512 to 1024, 12000 rows (376 tiles): 44 and 203, 42 and 210; 15000 (472): 52 and
+//   246, 43 and 222; 256 to 512, 20000 (316): 30 and 134, 28 and 144; 30000 (472): 38 and 181,
+//   30 and 154; fp32 512 to 1024, 3000 (384): 54 and 252, 63 and 273; 4000 (512): 59 and 297,
+//   65 and 287; 6000 (752): 95 and 455, 86 and 352; 256 to 512, 8000 (504): 39 and 195, 44
+//   and 179; 12000 (752): 55 and 290, 54 and 214.
+// Of wider weights a training pass needs more of them: bf16 1024 to 4096, 4000 rows (512): 83
+// and 518, 77 and 643; 7000 (896): 134 and 753, 128 and 805; fp32 1200 (640): 188 and 982, 163
+// and 924.
 constexpr int kWideLeast = 448;
 bool is_wide(const GatedArgs& a) {
     const int64_t tile = a.dtype == 0 ? 128 : 256;

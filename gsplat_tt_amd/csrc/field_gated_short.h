@@ -92,12 +92,14 @@ __global__ __launch_bounds__(kThreads) void k_gated_chunks(GatedArgs a, int64_t 
 // chunk by chunk: h, or with GRAD dx, whose sums stay in registers too. The gradients of
 // gate and up leave the sums in the layout that the next product takes them in. LAID: the
 // chunks' parts come from k_gated_chunks (cutting them in the kernel took dx of 10007 x 75 to
-// 201 from 26 to 38 us). bf16 rows are 64 a wave (fp32 32), with gradients half of that: 16
-// took as long, 128 do not fit the registers. 307200 x 64 to 256 bf16: 45 us, 197 MB at 4.4
-// TB/s, bound by them; to 128 with gradients 52, 157 MB, the vector units busy half of the
-// time with silu and its slope. 921600 x 128 to 128 fp32: 360, the matrix cores busy 48 % and
-// the vector units 38 % of the time, at a clock that has come down to 2 GHz. Shares of the chunks (blockIdx.y) leave sums of dx
-// of their own in `part` (share, rows, 32 KS), where there are several.
+// 201 from 26 to 38 us). bf16 rows are 64 a wave, with gradients 32; fp32 rows 32, with
+// gradients of more than 64 values 16: 16 took as long, 128 do not fit the registers. 307200 x
+// 64 to 256 bf16: 45 us a call, 197 MB at 4.4 TB/s, bound by them; to 128 with gradients 52,
+// 157 MB, the vector units busy half of the time with silu and its slope. 921600 x 128 to 128
+// fp32: 365 a call (355 to 416 in kernel traces), the matrix cores busy 48 % and the vector
+// units 38 % of the time, at a clock that has come down to 2 GHz. Shares of the chunks
+// (blockIdx.y) leave sums of dx of their own in `part` (share, rows, 32 KS), where there are
+// several.
 template <typename T, int NP, int ACT, int KS, int J, bool GRAD, bool LAID>
 __global__ __launch_bounds__(kThreads, NP == 1 || J * KS < 8 ? 2 : 1) void k_gated_rows(
     GatedArgs a, const quad* laid, int64_t block0, int64_t chunks, int64_t per_share, float* part) {
@@ -534,8 +536,12 @@ __global__ __launch_bounds__(1024) void k_gated_join(GatedArgs a, const float* p
 }
 
 // Up to so many rows the kernels do not fill the chip: 16 rows a wave, chunks in shares, and
-// for h alone no launch to cut the weights before. 16000 x 64 to 128 fp32 take 12.5 us a call
-// so, a training pass 48; 17.7 and 59 as more rows do. bf16 12.6 and 43.4; 13.6 and 43.4.
+// for h alone no launch to cut the weights before. h and a training pass so, then as more rows
+// do, us: 16000 x 64 to 128 fp32 15 and 53, 18 and 59; 75 to 201 17 and 86, 24 and 96; 128 to
+// 512 37 and 179, 54 and 209, bf16 15 and 76, 35 and 105. 24000 x 75 to 201 fp32 26 and 119,
+// 25 and 118; 128 to 512 64 and 274, 54 and 263; bf16 of long rows goes over later (24000 24
+// and 97, 35 and 118). bf16 x 64 to 128 does not gain: 16000 15 and 48, 14 and 44, by the
+// launch that joins dx.
 constexpr int64_t kFewerRows = 16384;
 
 struct ShortPlan {

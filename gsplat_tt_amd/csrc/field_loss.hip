@@ -8,8 +8,9 @@
 //
 // All products run on the matrix cores with bf16 operands and fp32 sums. fp32
 // inputs are cut into three bf16 parts of 8 bits each (exact: 24 bits; for infinite
-// values see split8_input) and the six products whose weight is above 2^-24 are added up, which keeps fp32's
-// precision at 6/16 of the cost of the fp32 matrix instructions. Bf16 inputs are
+// and very small values see split8_input) and the six largest of their products are added
+// up (what the others add: Products), which keeps fp32's precision at 6/16 of the cost of
+// the fp32 matrix instructions. Bf16 inputs are
 // the operands as they are; their G is rounded to bf16, as their gradients are in
 // the end, since parts of G would double the products that it enters: 30011 x 32003 of
 // 512 the gradients are 0.0023 off (2-norm, relative), where rounding them alone gives

@@ -532,7 +532,8 @@ int gs_label_loss_grad_dev(gs_ctx* ctx, const gs_label_loss* in, const float* ro
  * block: h = act(gate) * up, gate = x Wg^T + bg, up = x Wu^T + bu. x (n, dim), w_gate and
  * w_up (hidden, dim), h (n, hidden) of one dtype; b_gate and b_up (hidden) fp32 or NULL
  * (0). dim at most 65536, hidden 1 .. 2^20, n at most 2^31 - 256. Infinite values and NaN
- * act as in plain arithmetic. */
+ * act as in plain arithmetic. Of fp32 operands, x, weights and the gradients of gate and up,
+ * bits below 2^-133 are left out: a value below that counts as 0. */
 typedef struct gs_gated_linear {
     const void* x;
     const void* w_gate;
